@@ -8,6 +8,8 @@ Modules:
   ops        reshape_and_cache_flash, gather_kv, merge_attention_states,
              compute_slot_mapping, copy_page_indices, block gather/scatter, swap
   decode     BatchDecodeWithPagedKVCacheWrapper (plan / run)
+  prompt     BatchPromptAttentionWrapper: new prompts over their own K/V
+  eviction   BatchAttentionWeightsWrapper: attention weight per cached token
   kv_cache   PagedKVCache: caches, block table, page pool, step setup, swap
   allocator  PageAllocator protocol, PagePool, pages_needed
   workloads  seeded synthetic workloads of the benchmark configurations
@@ -21,7 +23,8 @@ __version__ = "0.1.0"
 def __getattr__(name):
     # Lazy imports keep `import gpu_offloading_amd` cheap (no torch) for the
     # allocator-only users, e.g. CPU scheduler tests.
-    if name in ("ops", "decode", "kv_cache", "workloads", "build", "_lib"):
+    if name in ("ops", "decode", "prompt", "eviction", "kv_cache", "workloads", "build",
+                "_lib"):
         import importlib
         return importlib.import_module(f".{name}", __name__)
     if name == "PagedKVCache":

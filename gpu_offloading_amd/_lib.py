@@ -90,6 +90,44 @@ class KvcPrefillSplit(ctypes.Structure):
     ]
 
 
+class KvcPromptSchedule(ctypes.Structure):
+    """Mirror of ``kvc_prompt_schedule`` (include/kvc.h)."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("num_qo_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("causal", c_int32),
+        ("tile_tokens", c_int32),
+        ("num_units", c_int32),
+        ("num_workgroups", c_int32),
+        ("total_q", c_int32),
+        ("total_kv", c_int32),
+        ("max_key_tiles", c_int32),
+        ("reserved", c_int32),
+        ("plan_ints", c_int64),
+    ]
+
+
+class KvcWeightsSchedule(ctypes.Structure):
+    """Mirror of ``kvc_weights_schedule`` (include/kvc.h)."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("num_qo_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("page_size", c_int32),
+        ("causal", c_int32),
+        ("shared_keys", c_int32),
+        ("num_units", c_int32),
+        ("num_workgroups", c_int32),
+        ("total_q", c_int32),
+        ("plan_ints", c_int64),
+    ]
+
+
 class KvcDecodeStepLayout(ctypes.Structure):
     """Mirror of ``kvc_decode_step_layout`` (include/kvc.h)."""
 
@@ -189,6 +227,26 @@ SIGNATURES = {
     "kvc_decode_step_setup": (c_int, [
         _I32P, _I32P, POINTER(KvcDecodeStepLayout), _I32P, c_int64, c_int32, c_int32,
         _I32P, _P, c_int32, _I32P, c_int64, _P]),
+    "kvc_prompt_plan": (c_int, [
+        c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
+        POINTER(KvcPromptSchedule), c_void_p, c_int64]),
+    "kvc_prompt_run": (c_int, [
+        POINTER(KvcPromptSchedule), _I32P, _P, c_int64, _P, c_int64, _P, c_int64, c_int32,
+        c_float, _P, c_int64, _P, _P]),
+    "kvc_weights_plan": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
+        c_int32, POINTER(KvcWeightsSchedule), c_void_p, c_int64]),
+    "kvc_batch_attention_weights_run": (c_int, [
+        POINTER(KvcWeightsSchedule), _I32P, _P, c_int64, _P, _P, c_int64, c_int64, c_int64,
+        _I32P, c_int64, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),
+    "kvc_decode_attention_weights": (c_int, [
+        _P, c_int64, _P, _P, c_int64, c_int64, c_int64, _I32P, _I32P, c_int64, _I32P, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),
+    "kvc_evict_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
+    "kvc_evict_kv": (c_int, [
+        _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, _P, _I32P,
+        _I32P, c_int64, c_int32, c_int32, _I32P, _I32P, _I32P, _I32P, _I32P, c_int32, c_int32,
+        _P, c_int64, _P]),
 }
 
 _lock = threading.Lock()

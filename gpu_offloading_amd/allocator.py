@@ -113,6 +113,14 @@ class PagePool:
         self.seq_page_list[seq_id] = []
         return pages
 
+    def trim(self, seq_id: int, n_pages: int) -> list[int]:
+        """Return the pages of ``seq_id`` past its first ``n_pages`` to the free
+        list; returns them."""
+        pages = self.seq_page_list[seq_id][n_pages:]
+        del self.seq_page_list[seq_id][n_pages:]
+        self.free_pages.extend(pages)
+        return pages
+
     def detach(self, seq_id: int) -> list[int]:
         """Take the page list of ``seq_id`` away without freeing the pages
         (used while a swap-out still reads them)."""

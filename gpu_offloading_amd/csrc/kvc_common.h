@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <exception>
 #include <string>
 
 #include "kvc.h"
@@ -31,6 +32,14 @@ inline int ok() { return KVC_OK; }
   } while (0)
 
 #define KVC_LAUNCH_CHECK() KVC_HIP_CHECK(hipGetLastError())
+
+// Body of a C entry whose host code allocates: no exception leaves it.
+#define KVC_NO_THROW(...)                                                    \
+  try {                                                                      \
+    __VA_ARGS__;                                                             \
+  } catch (const std::exception& e_) {                                       \
+    return ::kvc::set_error(KVC_ERR_INVALID_ARG, e_.what());                 \
+  }
 
 inline bool aligned(const void* p, uintptr_t a) {
   return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;

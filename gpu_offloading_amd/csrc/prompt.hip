@@ -1,0 +1,431 @@
+// Attention of whole prompts over their own contiguous K/V (MFMA, gfx950):
+// sequences packed one after another, causal or full, grouped heads.
+//
+//   s_ij = scale q_i . k_j   (j <= i + kv_len - q_len where causal)
+//   out_i = sum_j e^(s_ij - m_i) v_j / l_i,   l_i = sum_j e^(s_ij - m_i),   lse_i = m_i + ln l_i
+// in one pass over the keys with a running maximum m and sum l (online softmax).
+//
+// Work unit = (sequence, tile of query rows) x one KV head.  A query row is a
+// (token, query head) pair: the `group` query heads of a KV head are packed into
+// the rows of a tile, so that each K/V tile staged in LDS serves all of them and
+// the causal edge is as narrow as the tile has tokens.  Any group: row r is token
+// r / group, head r % group.
+#include "kvc_common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "unit_plan.h"
+
+namespace kvc {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+
+constexpr int kThreads = 256;
+constexpr int kWaveRows = 32;
+constexpr int kTileRows = kThreads / 64 * kWaveRows;
+constexpr int kKeys = 64;                     // keys per tile
+constexpr int kMaxGroup = kTileRows;
+constexpr float kRescaleLog2 = 8.f;           // lazy-rescale threshold (base 2)
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct PromptArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_stride, k_stride, v_stride;   // elements between tokens
+  const int2* wg_units;                   // [workgroups]: (first unit, units)
+  const int4* units;                      // [units][2]: (KV head, first query, q_len, kv_len),
+                                          //             (q offset, k offset, key tiles, 0)
+  int32_t num_kv_heads, group, tile_tokens, causal;
+  uint32_t inv_group;                     // 65536 / group, rounded up
+  float scale_log2;                       // sm_scale * log2(e)
+  uint16_t* out;
+  int64_t out_stride;
+  float* lse;                             // [total_q][Hq] natural log, may be null
+};
+
+// The element types: bf16 and fp16 through the same kernel.
+struct Bf16 {
+  typedef __bf16 e;
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kExp = 0x7f80u;   // exponent bits: all set is inf or NaN
+  static __device__ __forceinline__ f32x16_t mfma(x8 a, x8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+struct Fp16 {
+  typedef _Float16 e;
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr uint32_t kExp = 0x7c00u;
+  static __device__ __forceinline__ f32x16_t mfma(x8 a, x8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// Two floats as a pair of the element type, round to nearest even.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const typename T::x2 v = {static_cast<typename T::e>(lo), static_cast<typename T::e>(hi)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// A word with its elements that are inf or NaN made 0; *found is set if there was one.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w, bool* found) {
+  const bool lo = (w & T::kExp) == T::kExp, hi = ((w >> 16) & T::kExp) == T::kExp;
+  *found |= lo | hi;
+  return (lo ? 0u : w & 0xffffu) | (hi ? 0u : w & 0xffff0000u);
+}
+
+// LDS tiles hold [key][dim] rows whose 16-byte chunks are XOR-swizzled by key,
+// so that MFMA operand reads hit distinct banks: K is read as 16 bytes of one
+// key's dims, 16 consecutive keys at a time; V^T through the transposing
+// ds_read_b64_tr_b16, 64 bytes of four consecutive keys at a time.  Rows of 128
+// bytes (D = 64) put two keys into the 256 bytes of all banks.
+template <int D>
+__device__ __forceinline__ int k_slot(int key, int chunk) {
+  return D == 64 ? chunk ^ ((key >> 1) & 7) : chunk ^ (key & 15);
+}
+template <int D>
+__device__ __forceinline__ int v_slot(int key, int chunk) {
+  return D == 64 ? chunk ^ (4 * ((key >> 1) & 1)) : chunk ^ (4 * (key & 3));
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(PromptArgs a) {
+  constexpr int kRow = 2 * D;                 // bytes per K or V row
+  constexpr int kChunks = kRow / 16;
+  constexpr int kSteps = D / 16;              // MFMA k-steps of K Q^T
+  constexpr int kBlocks = D / 32;             // 32-dim blocks of O
+  constexpr int kLoads = kKeys * kChunks / kThreads;
+  typedef typename T::x8 x8;
+  __shared__ struct alignas(16) {
+    uint8_t k[kKeys * kRow], v[kKeys * kRow];
+    int bad[2];
+  } lds;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 31, half = lane >> 5;
+  const int row = wave * kWaveRows + r;
+  const int row_tok = int(row * a.inv_group >> 16);     // row / group
+  const int row_head = row - row_tok * a.group;
+  const int Hq = a.num_kv_heads * a.group;
+  uint32_t v_rd[kBlocks];
+  {
+    const int e = (lane >> 2) & 3, q = lane & 3, gp = (lane >> 4) & 1;
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db)
+      v_rd[db] = (4 * half + e) * kRow +
+                 (v_slot<D>(4 * half + e, 4 * db + 2 * gp + (q >> 1)) << 4) + ((q & 1) << 3);
+  }
+
+  const int2 span = a.wg_units[blockIdx.x];
+  for (int u = span.x; u < span.x + span.y; ++u) {
+    const int4 x = a.units[2 * u], y = a.units[2 * u + 1];
+    const int h = x.x, tok0 = x.y, q_len = x.z, kv_len = x.w, ntiles = y.z;
+    const int tok = tok0 + row_tok;
+    const bool row_ok = row_tok < a.tile_tokens && tok < q_len;
+    const int limit = !row_ok ? -1 : a.causal ? min(tok + kv_len - q_len, kv_len - 1) : kv_len - 1;
+    // Tiles [0, n_full) are seen whole by every row of the unit.
+    const int lim_lo = a.causal ? min(tok0 + kv_len - q_len, kv_len - 1) : kv_len - 1;
+    const int n_full = max(0, min(ntiles, (lim_lo + 1) / kKeys));
+    const uint16_t* kb = a.k + int64_t(y.y) * a.k_stride + h * D;
+    const uint16_t* vb = a.v + int64_t(y.y) * a.v_stride + h * D;
+
+    x8 qb[kSteps];
+    {
+      // Rows of no token read the unit's first one; they are never stored.
+      const uint16_t* qp = a.q + int64_t(y.x + (row_ok ? tok : tok0)) * a.q_stride +
+                           (h * a.group + (row_ok ? row_head : 0)) * D + 8 * half;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks)
+        qb[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
+    }
+    f32x16_t o[kBlocks];
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+    float m_run = -INFINITY, l_half = 0.f;
+    if (threadIdx.x == 0) lds.bad[u & 1] = 0;
+
+    for (int j = 0; j < ntiles; ++j) {
+      __syncthreads();   // the tiles are free (and `bad` of this unit is set to 0)
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int id = i * kThreads + threadIdx.x, key = id / kChunks, c = id % kChunks;
+        const int t = j * kKeys + key;
+        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+        if (t < kv_len) {
+          kx = *reinterpret_cast<const uint4*>(kb + int64_t(t) * a.k_stride + 8 * c);
+          vx = *reinterpret_cast<const uint4*>(vb + int64_t(t) * a.v_stride + 8 * c);
+        }
+        if (j >= n_full) {
+          // Some row does not see this key: 0 times an inf or NaN must not reach it.
+          vx.x = finite2<T>(vx.x, &bad);
+          vx.y = finite2<T>(vx.y, &bad);
+          vx.z = finite2<T>(vx.z, &bad);
+          vx.w = finite2<T>(vx.w, &bad);
+        }
+        *reinterpret_cast<uint4*>(lds.k + key * kRow + k_slot<D>(key, c) * 16) = kx;
+        *reinterpret_cast<uint4*>(lds.v + key * kRow + v_slot<D>(key, c) * 16) = vx;
+      }
+      if (bad) lds.bad[u & 1] = 1;
+      __syncthreads();
+
+      // S^T = K Q^T: accumulator entry e of key block b is key 32b + 8(e/4) + 4half + e%4
+      // of the tile, for the row of this lane.
+      f32x16_t s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+          const int key = 32 * b + r;
+          s[b] = T::mfma(__builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
+                             lds.k + key * kRow + k_slot<D>(key, 2 * ks + half) * 16)),
+                         qb[ks], s[b]);
+        }
+      }
+      if (j >= n_full) {
+        const int rel = limit - j * kKeys - 4 * half;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) <= rel ? s[b][e] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      // The running maximum moves when it grew by more than 2^8; p stays below that.
+      const float cand = fmaxf(m_run, mx * a.scale_log2);
+      if (cand > m_run + kRescaleLog2) {
+        const float alpha = fast_exp2(m_run - cand);
+        m_run = cand;
+        l_half *= alpha;
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db) o[db] *= alpha;
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
+      uint32_t pw[2][8];
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = fast_exp2(fmaf(s[b][e], a.scale_log2, -m_use));
+          const float p1 = fast_exp2(fmaf(s[b][e + 1], a.scale_log2, -m_use));
+          sum += p0 + p1;
+          pw[b][e >> 1] = pack2<T>(p0, p1);
+        }
+      l_half += sum;
+      // O^T += V^T P^T: key step st covers keys 16st..+15 in the order that S^T left P in.
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const uint32_t* pp = &pw[st >> 1][4 * (st & 1)];
+        const x8 pb = __builtin_bit_cast(x8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db) {
+          const uint8_t* p = lds.v + v_rd[db] + st * 16 * kRow;
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 8 * kRow));
+          o[db] = T::mfma(__builtin_bit_cast(
+                              x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)),
+                          pb, o[db]);
+        }
+      }
+    }
+
+    const float l = l_half + __shfl_xor(l_half, 32);
+    const float inv = l == 0.f ? 0.f : 1.f / l;    // a row that sees no key: 0
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db) o[db] *= inv;
+    __syncthreads();
+    if (ntiles > 0 && lds.bad[u & 1]) {
+      // Rows that do see an inf or NaN of the boundary tiles get it: p > 0 times it.
+      for (int t = n_full * kKeys; t < min(ntiles * kKeys, kv_len); ++t) {
+        const uint16_t* vr = vb + int64_t(t) * a.v_stride + 4 * half;
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint16_t w = vr[32 * db + 8 * (e >> 2) + (e & 3)];
+            if (t <= limit && (w & T::kExp) == T::kExp)
+              o[db][e] += float(__builtin_bit_cast(typename T::e, w));
+          }
+      }
+    }
+    if (row_ok) {
+      // O^T entry (db, 4i+j) is head dim 32db + 8i + 4half + j of this lane's row.
+      uint16_t* op = a.out + int64_t(y.x + tok) * a.out_stride +
+                     (h * a.group + row_head) * D + 4 * half;
+#pragma unroll
+      for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint2*>(op + 32 * db + 8 * i) =
+              make_uint2(pack2<T>(o[db][4 * i], o[db][4 * i + 1]),
+                         pack2<T>(o[db][4 * i + 2], o[db][4 * i + 3]));
+      if (a.lse && half == 0)
+        a.lse[int64_t(y.x + tok) * Hq + h * a.group + row_head] =
+            l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
+    }
+  }
+}
+
+constexpr int64_t kMaxWorkgroups = 512;
+int64_t plan_workgroups(int64_t units) { return std::min(kMaxWorkgroups, units); }
+
+int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batch, int32_t hq,
+                int32_t hkv, int32_t head_dim, int32_t causal, kvc_prompt_schedule* sched,
+                int32_t* plan_host, int64_t plan_capacity) {
+  KVC_REQUIRE(sched, KVC_ERR_INVALID_ARG, "null schedule");
+  KVC_REQUIRE(batch >= 0, KVC_ERR_INVALID_ARG, "negative batch");
+  KVC_REQUIRE(batch == 0 || (qo_indptr && kv_indptr), KVC_ERR_INVALID_ARG, "null indptr");
+  KVC_REQUIRE(hkv > 0 && hq > 0 && hq % hkv == 0, KVC_ERR_INVALID_ARG,
+              "num_qo_heads must be a positive multiple of num_kv_heads");
+  const int group = hq / hkv;
+  KVC_REQUIRE((head_dim == 64 || head_dim == 128 || head_dim == 256) && group <= kMaxGroup,
+              KVC_ERR_UNSUPPORTED,
+              "prompt attention supports head_dim 64, 128, 256 and groups up to 128");
+  const int tile_tokens = kTileRows / group;
+  std::vector<int32_t> rec;
+  int max_tiles = 0;
+  int64_t end_q = 0, end_kv = 0, items = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int64_t q_len = int64_t(qo_indptr[b + 1]) - qo_indptr[b];
+    const int64_t kv_len = int64_t(kv_indptr[b + 1]) - kv_indptr[b];
+    KVC_REQUIRE(q_len >= 0 && kv_len >= 0 && qo_indptr[b] >= 0 && kv_indptr[b] >= 0,
+                KVC_ERR_INVALID_ARG, "qo_indptr and kv_indptr must be non-negative and "
+                                     "non-decreasing");
+    KVC_REQUIRE(kv_len < (int64_t(1) << 30) && q_len < (int64_t(1) << 30), KVC_ERR_INVALID_ARG,
+                "sequence too long");
+    items += (q_len + tile_tokens - 1) / tile_tokens;
+    KVC_REQUIRE(items * hkv < (int64_t(1) << 27), KVC_ERR_INVALID_ARG,
+                "too many (query tile, KV head) units");
+    end_q = qo_indptr[b + 1];
+    end_kv = kv_indptr[b + 1];
+    for (int64_t t0 = 0; t0 < q_len; t0 += tile_tokens) {
+      const int64_t last = std::min<int64_t>(t0 + tile_tokens, q_len) - 1;
+      int64_t keys = causal ? last + kv_len - q_len + 1 : kv_len;
+      keys = std::max<int64_t>(0, std::min<int64_t>(keys, kv_len));
+      const int tiles = int((keys + kKeys - 1) / kKeys);
+      max_tiles = std::max(max_tiles, tiles);
+      const int32_t r8[kUnitInts] = {b, int32_t(t0), int32_t(q_len), int32_t(kv_len),
+                                     qo_indptr[b], kv_indptr[b], tiles, 0};
+      rec.insert(rec.end(), r8, r8 + kUnitInts);
+    }
+  }
+  const int64_t n = int64_t(rec.size()) / kUnitInts;
+  const int64_t W = plan_workgroups(n * hkv);
+  sched->batch = batch;
+  sched->num_qo_heads = hq;
+  sched->num_kv_heads = hkv;
+  sched->head_dim = head_dim;
+  sched->causal = causal ? 1 : 0;
+  sched->tile_tokens = tile_tokens;
+  sched->num_units = int32_t(n * hkv);
+  sched->num_workgroups = int32_t(W);
+  sched->total_q = int32_t(end_q);
+  sched->total_kv = int32_t(end_kv);
+  sched->max_key_tiles = max_tiles;
+  sched->reserved = 0;
+  sched->plan_ints = unit_table_ints(W) + n * hkv * kUnitInts;
+  KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
+              KVC_ERR_WORKSPACE,
+              "plan buffer too small: need " + std::to_string(sched->plan_ints) + " int32");
+  write_unit_plan(rec, n, hkv, W, plan_host);
+  return ok();
+}
+
+template <typename T>
+void launch(const PromptArgs& a, int head_dim, unsigned workgroups, hipStream_t s) {
+  if (head_dim == 64) prompt_kernel<T, 64><<<dim3(workgroups), kThreads, 0, s>>>(a);
+  else if (head_dim == 128) prompt_kernel<T, 128><<<dim3(workgroups), kThreads, 0, s>>>(a);
+  else prompt_kernel<T, 256><<<dim3(workgroups), kThreads, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace kvc
+
+using namespace kvc;
+
+extern "C" int kvc_prompt_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
+                               int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                               int32_t head_dim, int32_t causal, kvc_prompt_schedule* schedule,
+                               int32_t* plan_host, int64_t plan_capacity) {
+  KVC_NO_THROW(return prompt_plan(qo_indptr_host, kv_indptr_host, batch, num_qo_heads,
+                                  num_kv_heads, head_dim, causal, schedule, plan_host,
+                                  plan_capacity));
+}
+
+extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* plan,
+                              const void* q, int64_t q_token_stride, const void* key,
+                              int64_t key_token_stride, const void* value,
+                              int64_t value_token_stride, int32_t dtype, float sm_scale,
+                              void* out, int64_t out_token_stride, float* lse, void* stream) {
+  KVC_REQUIRE(sched, KVC_ERR_INVALID_ARG, "null schedule");
+  const int Hq = sched->num_qo_heads, Hkv = sched->num_kv_heads, D = sched->head_dim;
+  KVC_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= kMaxGroup &&
+                  (D == 64 || D == 128 || D == 256) && sched->num_units >= 0 &&
+                  sched->tile_tokens == kTileRows / (Hq / Hkv) &&
+                  sched->num_workgroups == plan_workgroups(sched->num_units) &&
+                  sched->plan_ints == unit_table_ints(sched->num_workgroups) +
+                                          int64_t(sched->num_units) * kUnitInts,
+              KVC_ERR_INVALID_ARG, "schedule not produced by kvc_prompt_plan");
+  KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
+              "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
+  KVC_REQUIRE(sm_scale > 0.f && std::isfinite(sm_scale), KVC_ERR_INVALID_ARG,
+              "sm_scale must be positive and finite");
+  if (sched->num_units == 0) return ok();
+  KVC_REQUIRE(plan && q && out && (sched->total_kv == 0 || (key && value)), KVC_ERR_INVALID_ARG,
+              "null pointer");
+  const int64_t qw = int64_t(Hq) * D, kw = int64_t(Hkv) * D;
+  KVC_REQUIRE(q_token_stride >= qw && out_token_stride >= qw && key_token_stride >= kw &&
+                  value_token_stride >= kw,
+              KVC_ERR_INVALID_ARG, "token stride smaller than the token's heads");
+  KVC_REQUIRE(key_token_stride < (int64_t(1) << 24) && value_token_stride < (int64_t(1) << 24),
+              KVC_ERR_INVALID_ARG, "K/V tokens 32 MiB or more apart");
+  KVC_REQUIRE(aligned(q, 16) && aligned(key, 16) && aligned(value, 16) && aligned(out, 16) &&
+                  aligned(plan, 16) && q_token_stride % 8 == 0 && key_token_stride % 8 == 0 &&
+                  value_token_stride % 8 == 0 && out_token_stride % 8 == 0,
+              KVC_ERR_ALIGNMENT,
+              "q/key/value/out/plan must be 16-byte aligned and token strides multiples of 8");
+  PromptArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(key);
+  a.v = static_cast<const uint16_t*>(value);
+  a.q_stride = q_token_stride;
+  a.k_stride = key_token_stride;
+  a.v_stride = value_token_stride;
+  a.wg_units = reinterpret_cast<const int2*>(plan);
+  a.units = reinterpret_cast<const int4*>(plan + unit_table_ints(sched->num_workgroups));
+  a.num_kv_heads = Hkv;
+  a.group = Hq / Hkv;
+  a.tile_tokens = sched->tile_tokens;
+  a.causal = sched->causal;
+  a.inv_group = (65536u + unsigned(a.group) - 1) / unsigned(a.group);
+  a.scale_log2 = sm_scale * kLog2e;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_stride = out_token_stride;
+  a.lse = lse;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == KVC_DTYPE_BF16) launch<Bf16>(a, D, unsigned(sched->num_workgroups), s);
+  else launch<Fp16>(a, D, unsigned(sched->num_workgroups), s);
+  KVC_LAUNCH_CHECK();
+  return ok();
+}

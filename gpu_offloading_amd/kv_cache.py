@@ -9,7 +9,8 @@ mapping and decode planning of a step (:1896-1955, 3475-3556), the
 continuation-prefill planning (:1678-1751, 3649-3727) and the kernels called
 per layer: the KV append (:2343-2347), decode attention (:3907-3909) and
 paged prefill attention (:3939-3941).  It also adds the swap API the engine lacks (block eviction to
-pinned host memory and restore, on a side stream).
+pinned host memory and restore, on a side stream), the new prompts' own attention
+(:2081, 3776) and the eviction of single tokens by the attention they received.
 
 All arithmetic runs in libkvc.so; this module only does host bookkeeping,
 small H2D copies of metadata, and stream/event ordering.
@@ -27,7 +28,9 @@ import torch
 from . import _lib, hostmem, ops
 from .allocator import PagePool, pages_needed
 from .decode import BatchDecodeWithPagedKVCacheWrapper
+from .eviction import BatchAttentionWeightsWrapper
 from .prefill import BatchPrefillWithPagedKVCacheWrapper
+from .prompt import BatchPromptAttentionWrapper
 from .swap_ledger import SwapLedger
 
 __all__ = ["PagedKVCache", "SwapHandle"]
@@ -49,6 +52,11 @@ class SwapHandle:
     dst_block_ids: Optional[torch.Tensor] = None
     restored: bool = False
     num_bytes: int = 0                   # bytes over the host link each way
+    # of a cache that tracks attention: the sequences' evicted tokens, and per
+    # layer the pages' (scores, positions), which stay on the device
+    evicted: Optional[list] = None
+    tracked: Optional[list] = None
+    tracked_event: Optional[torch.cuda.Event] = None
     _keepalive: list = field(default_factory=list)
 
     @property
@@ -168,6 +176,16 @@ class PagedKVCache:
         self._swap_warm = False   # reserve_swap's copy-path warm-up done
         self._swaps = SwapLedger()   # swap-outs / restores still in flight
 
+        # Attention tracking (track_attention): per layer each cached token's
+        # accumulated weight and position, and per sequence the tokens evicted.
+        self.scores: Optional[list[torch.Tensor]] = None
+        self.positions: Optional[list[torch.Tensor]] = None
+        self._evicted = np.zeros(max_seqs, dtype=np.int32)
+        self._evicted_dev: Optional[torch.Tensor] = None
+        self._evicted_dirty = False
+        self._decode_ids: Optional[torch.Tensor] = None   # the decode plan's sequences
+        self._weights_ids: Optional[torch.Tensor] = None  # the chunk weights plan's
+
     def _init_step_buffers(self) -> None:
         """Decode workspace + wrapper and the device page-index buffer
         (moe_engine.py:541-575).  Only a GPU cache has them; a CPU-resident
@@ -186,6 +204,8 @@ class PagedKVCache:
                                                                     kv_layout="NHD")
         self._prefill_indices_gpu = torch.zeros(self.max_seqs * self.max_pages_per_seq,
                                                 dtype=torch.int32, device=self.device)
+        self._prompt_wrapper = BatchPromptAttentionWrapper(self._workspace_buf)
+        self._weights_wrapper = BatchAttentionWeightsWrapper(self._workspace_buf)
 
     def _to_device(self, arr) -> torch.Tensor:
         """Async H2D of a small host array through a fresh pinned buffer."""
@@ -314,6 +334,7 @@ class PagedKVCache:
             self._swaps.on_free(seq_id, torch.cuda.current_stream(self.device))
         self._seq_lens_cpu[seq_id] = 0
         self.seq_lens[seq_id] = 0
+        self._set_evicted(seq_id, 0)
         if self._dynamic_pages:
             self.free_seq_pages(seq_id)
 
@@ -331,6 +352,11 @@ class PagedKVCache:
             self._bt_pending.clear()
             self._bt.fill_(-1)
         self._swaps.clear()
+        self._evicted[:] = 0
+        if self.scores is not None:
+            self._evicted_dirty = True
+            for t in self.scores + self.positions:
+                t.zero_()
 
     # ----------------------------------------------------- snapshot / fill
     def fill_kv_random(self, std: float = 0.01, generator: Optional[torch.Generator] = None) -> None:
@@ -415,6 +441,7 @@ class PagedKVCache:
         if b == 0:
             return
         self._sync_seqs(seq_ids)
+        self._upload_evicted()
         lens = self._seq_lens_cpu.numpy()[ids].astype(np.int32)
         nblk = (lens + self.page_size - 1) // self.page_size
         indptr = np.zeros(b + 1, dtype=np.int32)
@@ -424,6 +451,7 @@ class PagedKVCache:
         self._check_page_counts(nblk)
         indptr_d = self._to_device(indptr)
         ids_d = self._to_device(ids.astype(np.int32))
+        self._decode_ids = ids_d
         ops.copy_page_indices(self.block_table, indptr_d, self._plan_indices_gpu, seq_ids=ids_d)
         total = int(indptr[b])
         self._decode_wrapper.plan(
@@ -511,6 +539,7 @@ class PagedKVCache:
             return slots
         ids = self._check_seq_ids(seq_ids)
         self._sync_seqs(seq_ids)
+        self._upload_evicted()
         lens_all = self._seq_lens_cpu.numpy()
         ms, ps = self.max_seqs, self.page_size
         lens = lens_all[ids].astype(np.int32) + 1
@@ -577,8 +606,9 @@ class PagedKVCache:
         if self._step_views is None or self._step_views[0] != vk:
             dm = self._step_dev
             self._step_views = (vk, dm[0:cap], dm[o_ip:o_lpl], dm[o_lpl:o_lpl + b],
-                                self._slots_dev[:graph_n], self._slots_dev[:b])
-        _, plan_v, indptr_v, lpl_v, slots, step_slots = self._step_views
+                                self._slots_dev[:graph_n], self._slots_dev[:b],
+                                dm[o_ids:o_ids + b])
+        _, plan_v, indptr_v, lpl_v, slots, step_slots, self._decode_ids = self._step_views
         lay = self._step_layout
         lay.plan_ints = int(sched.plan_ints)   # the plan's unused capacity is not sent
         lay.tail_begin, lay.tail_end = cap, n
@@ -655,10 +685,13 @@ class PagedKVCache:
         # Without the fused append, append_and_decode may make a separate append,
         # which reads the step's slot tensor (a new one when a step outgrows it).
         slots = 0 if w.fused_append_supported else self._step_slots.data_ptr()
-        return (self._step_dev.data_ptr(), w._indices.data_ptr(), w._num_indices, slots,
-                s.batch, s.small_batch, s.num_segments,
-                s.num_head_groups, s.heads_per_group, s.max_partitions, s.num_empty > 0,
-                s.pieces_offset, s.nparts_offset, s.append_pieces)
+        key = (self._step_dev.data_ptr(), w._indices.data_ptr(), w._num_indices, slots,
+               s.batch, s.small_batch, s.num_segments,
+               s.num_head_groups, s.heads_per_group, s.max_partitions, s.num_empty > 0,
+               s.pieces_offset, s.nparts_offset, s.append_pieces)
+        if self.scores is not None:   # decode_weights reads the step's lengths and ids, too
+            key += (w._indptr.data_ptr(), w._lpl.data_ptr(), self._decode_ids.data_ptr())
+        return key
 
     def prepare_step(self, decode_seq_ids: Sequence[int] = (),
                      prefill_seq_ids: Sequence[int] = (), prefill_lens: Sequence[int] = (),
@@ -680,7 +713,7 @@ class PagedKVCache:
         ``decode_seq_ids`` order) and the prefill wrapper over the
         continuations (``prefill``: their q rows, chunk after chunk).  New
         prompts attend over their own contiguous K/V outside the paged cache,
-        as in the engine.  Pages must already cover every new token."""
+        as in the engine (``plan_prompt`` and ``prompt``).  Pages must already cover every new token."""
         self._require_gpu()
         dec = [int(s) for s in decode_seq_ids]
         pre = [int(s) for s in prefill_seq_ids]
@@ -703,6 +736,7 @@ class PagedKVCache:
         if R == 0:
             return torch.full((graph_n,), -1, dtype=torch.int64, device=self.device)
         self._sync_seqs(ids.tolist())
+        self._upload_evicted()
         lens_all = self._seq_lens_cpu.numpy()
         ms, ps = self.max_seqs, self.page_size
         before = lens_all[ids].astype(np.int64)
@@ -808,6 +842,7 @@ class PagedKVCache:
             pw._sched = None
         if D:
             total = int(dip[-1])
+            self._decode_ids = ids_d[:D]
             ops.copy_page_indices(self._bt, dm[o_dip:o_dlpl], self._plan_indices_gpu,
                                   seq_ids=ids_d[:D])
             dw._install(dsched, dm[o_dplan:o_dplan + dcap], dm[o_dip:o_dlpl],
@@ -864,6 +899,181 @@ class PagedKVCache:
         return self._decode_wrapper._launch(q, None, out, None, return_lse,
                                             self._step_stream_for_call(), None, None,
                                             self._layer_kv[layer])
+
+    # --------------------------------------------------- new prompts' attention
+    def plan_prompt(self, prompt_lens: Sequence[int]) -> None:
+        """Plan the attention of new prompts of these lengths over their own
+        K/V, packed in order (the tokens of ``prepare_step``'s prefills)."""
+        self._require_gpu()
+        lens = np.asarray(prompt_lens, dtype=np.int64).reshape(-1)
+        if (lens < 0).any() or lens.sum() > np.iinfo(np.int32).max:
+            raise ValueError("prompt lengths must not be negative")
+        indptr = np.zeros(len(lens) + 1, dtype=np.int32)
+        np.cumsum(lens, out=indptr[1:])
+        self._prompt_wrapper.plan(torch.from_numpy(indptr), num_qo_heads=self.num_heads,
+                                  num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
+                                  causal=True, q_data_type=self.dtype)
+
+    def prompt(self, q: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+               out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+               return_lse: bool = False):
+        """Causal attention of the planned prompts' ``q [tokens, Hq, D]`` over
+        their own ``key`` / ``value [tokens, Hkv, D]`` (what ``append`` writes to the
+        cache).  Returns ``out`` or ``(out, lse)``."""
+        self._require_gpu()
+        return self._prompt_wrapper.run(q, key, value, out=out, lse=lse, return_lse=return_lse)
+
+    # ---------------------------------------------- attention weights, eviction
+    def track_attention(self) -> None:
+        """Keep each cached token's accumulated attention weight and position:
+        per layer ``scores`` (float32) and ``positions`` (int32), ``[pages, Hkv,
+        16]`` beside the cache (8 bytes per token and KV head).  Call it while no
+        sequence holds tokens.  From then on every step's ``decode_weights`` /
+        ``chunk_weights`` must follow its attention in every layer, as a token
+        gets its position and first score there; ``evict`` needs both.  Swapped
+        sequences keep theirs on the device; ``kv_snapshot`` does not cover them."""
+        self._require_gpu()
+        if self.scores is not None:
+            return
+        if int(self._seq_lens_cpu.max()) > 0:
+            raise RuntimeError("track_attention needs an empty cache (no cached tokens)")
+        shape = (self.total_pages, self.num_kv_heads, self.page_size)
+        self.scores = [torch.zeros(shape, dtype=torch.float32, device=self.device)
+                       for _ in range(self.num_layers)]
+        self.positions = [torch.zeros(shape, dtype=torch.int32, device=self.device)
+                          for _ in range(self.num_layers)]
+        self._evicted_dev = torch.zeros(self.max_seqs, dtype=torch.int32, device=self.device)
+
+    def _require_tracking(self) -> None:
+        self._require_gpu()
+        if self.scores is None:
+            raise RuntimeError("attention is not tracked (track_attention first)")
+
+    def _set_evicted(self, seq_id: int, n: int) -> None:
+        if int(self._evicted[seq_id]) != n:
+            self._evicted[seq_id] = n
+            self._evicted_dirty = True
+
+    def _upload_evicted(self) -> None:
+        """The device's evicted counts, which the weights kernels read, as the
+        host has them (a plan or a step's setup calls this on its stream)."""
+        if self._evicted_dirty and self._evicted_dev is not None:
+            self._evicted_dev.copy_(torch.from_numpy(self._evicted).pin_memory(),
+                                    non_blocking=True)
+            self._evicted_dirty = False
+
+    def next_position(self, seq_id: int) -> int:
+        """Position of the sequence's next token: its cached tokens and those
+        that were evicted (what its rotary phase goes by)."""
+        return int(self._seq_lens_cpu[seq_id]) + int(self._evicted[seq_id])
+
+    def decode_weights(self, layer: int, q: torch.Tensor, lse: torch.Tensor) -> None:
+        """Accumulate the attention weights of the planned decode step in
+        ``layer``: ``q`` as for ``decode``, ``lse`` as ``decode(...,
+        return_lse=True)`` returned it."""
+        self._require_tracking()
+        w = self._decode_wrapper
+        if w.schedule is None or w._indptr is None:
+            raise RuntimeError("decode_weights needs a planned decode step")
+        b = w.schedule.batch
+        if q.dim() != 3 or q.shape[0] < b or lse.dim() != 2 or lse.shape[0] < b:
+            raise RuntimeError(f"q and lse need a row for each of the step's {b} requests")
+        self._step_stream_for_call()
+        ops.decode_attention_weights(q[:b], lse[:b], self.k_cache[layer], w._indptr, w._indices,
+                                     w._lpl, self.scores[layer], self.positions[layer],
+                                     self._evicted_dev, seq_ids=self._decode_ids,
+                                     sm_scale=w._sm_scale)
+
+    def plan_chunk_weights(self, seq_ids: Sequence[int], query_lens: Sequence[int],
+                           new_tokens: Optional[Sequence[int]] = None) -> None:
+        """Plan ``chunk_weights`` for prompts and continuation chunks whose
+        tokens are counted in ``seq_lens``: the queries are the last
+        ``query_lens[i]`` tokens of each sequence, the last ``new_tokens[i]``
+        (default: the same) get their first score.  A prompt of which only the
+        last tokens vote passes its whole length as new."""
+        self._require_tracking()
+        ids = self._check_seq_ids(seq_ids)
+        b = len(ids)
+        qlen = np.asarray(query_lens, dtype=np.int64).reshape(-1)
+        new = qlen if new_tokens is None else np.asarray(new_tokens, dtype=np.int64).reshape(-1)
+        if len(qlen) != b or len(new) != b:
+            raise ValueError("one length per sequence")
+        self._sync_seqs(seq_ids)
+        self._upload_evicted()
+        lens = self._seq_lens_cpu.numpy()[ids].astype(np.int64)
+        if (qlen < 0).any() or (qlen > lens).any() or (new < 0).any() or (new > lens).any():
+            raise ValueError("queries and new tokens must be among a sequence's cached tokens")
+        nblk = (lens + self.page_size - 1) // self.page_size
+        self._check_page_counts(nblk)
+        indptr = np.zeros(b + 1, dtype=np.int32)
+        np.cumsum(nblk, out=indptr[1:])
+        qo = np.zeros(b + 1, dtype=np.int32)
+        np.cumsum(qlen, out=qo[1:])
+        lpl = np.where(lens > 0, (lens - 1) % self.page_size + 1, 0).astype(np.int32)
+        indices = torch.empty(max(int(indptr[b]), 1), dtype=torch.int32, device=self.device)
+        self._weights_ids = self._to_device(ids.astype(np.int32))
+        if b:
+            ops.copy_page_indices(self.block_table, self._to_device(indptr), indices,
+                                  seq_ids=self._weights_ids)
+        self._weights_wrapper.plan(
+            torch.from_numpy(qo), torch.from_numpy(indptr), indices, torch.from_numpy(lpl),
+            self.num_heads, self.num_kv_heads, self.head_dim, self.page_size, causal=True,
+            q_data_type=self.dtype, new_tokens=torch.from_numpy(new.astype(np.int32)))
+
+    def chunk_weights(self, layer: int, q: torch.Tensor, lse: torch.Tensor) -> None:
+        """Accumulate the attention weights of the planned chunks in ``layer``:
+        ``q [sum(query_lens), Hq, D]`` with ``lse`` as ``prompt`` or ``prefill``
+        returned it for these rows."""
+        self._require_tracking()
+        self._weights_wrapper.run(q, lse, self.k_cache[layer], self.scores[layer],
+                                  self.positions[layer], self._evicted_dev, self._weights_ids)
+
+    def evict(self, seq_ids: Sequence[int], keep: Sequence[int] | int,
+              recent: Sequence[int] | int = 0) -> None:
+        """Cut each sequence to ``keep`` cached tokens in every layer and KV
+        head: the ``recent`` last ones stay, and of the others those of the
+        largest ``scores`` (which the caller may have smoothed before).  Sets the
+        lengths, frees the pages that are no longer needed and drops the current
+        plans.  Sequences of at most ``keep`` tokens are left alone; the lists
+        are one entry per sequence."""
+        self._require_tracking()
+        ids = self._check_seq_ids(seq_ids)
+        b = len(ids)
+        keeps = np.broadcast_to(np.asarray(keep, dtype=np.int64), (b,))
+        recents = np.broadcast_to(np.asarray(recent, dtype=np.int64), (b,))
+        if (recents < 0).any() or (recents > keeps).any():
+            raise ValueError("need 0 <= recent <= keep")
+        lens = self._seq_lens_cpu.numpy()[ids].astype(np.int64)
+        cut = lens > keeps
+        if not cut.any():
+            return
+        ids, keeps, recents, lens = ids[cut], keeps[cut], recents[cut], lens[cut]
+        self._sync_seqs(ids.tolist())
+        meta = self._to_device(np.stack([ids, lens, keeps, recents,
+                                         self._evicted[ids]]).astype(np.int32))
+        top = int(lens.max())
+        work = torch.empty(ops.evict_workspace_bytes(len(ids), self.num_kv_heads, top),
+                           dtype=torch.uint8, device=self.device)
+        table = self.block_table
+        for layer in range(self.num_layers):
+            ops.evict_kv(self.k_cache[layer], self.v_cache[layer], self.scores[layer],
+                         table, meta[1], meta[2], meta[3], top,
+                         self.positions[layer], meta[4], seq_ids=meta[0], workspace=work)
+        # A plan made before would attend over slots that are gone.
+        self._step_slots = None
+        self._decode_wrapper._sched = None
+        self._prefill_wrapper._sched = None
+        self._weights_wrapper._sched = None
+        for sid, n, k in zip(ids.tolist(), lens.tolist(), keeps.tolist()):
+            self._seq_lens_cpu[sid] = k
+            self._set_evicted(sid, int(self._evicted[sid]) + n - k)
+            if self._dynamic_pages:
+                first = pages_needed(k, self.page_size)
+                gone = self._pool.trim(sid, first)
+                if gone:
+                    self._bt_write(sid, first, [-1] * len(gone))
+        self._lens_to_device()
+        self._upload_evicted()
 
     def gather(self, layer: int, seq_ids: Sequence[int], out_key: Optional[torch.Tensor] = None,
                out_value: Optional[torch.Tensor] = None):
@@ -1140,6 +1350,10 @@ class PagedKVCache:
             self._seq_lens_cpu[sid] = 0
         self._lens_to_device()
         n = len(ids)
+        evicted = []
+        for sid in seq_ids:
+            evicted.append(int(self._evicted[sid]))
+            self._set_evicted(sid, 0)
         bb = ops.block_bytes(self.k_cache[0])
         nbytes = self.num_layers * n * 2 * bb
         if host is None:
@@ -1147,11 +1361,18 @@ class PagedKVCache:
         elif host.is_cuda or not host.is_pinned() or host.numel() * host.element_size() < nbytes:
             raise RuntimeError(f"host buffer must be pinned CPU memory of >= {nbytes} bytes")
         ids_t = self._to_device(np.asarray(ids, dtype=np.int32))
+        tracked = tracked_event = None
+        if self.scores is not None:
+            tracked = [(s.index_select(0, ids_t), p.index_select(0, ids_t))
+                       for s, p in zip(self.scores, self.positions)]
+            tracked_event = torch.cuda.Event()
+            tracked_event.record(cur)
         self._side_stream().wait_stream(cur)
         start, ev = self._pipelined_swap(True, ids_t, n, host)
         # The host buffer must outlive the D2H copy even if the handle is dropped.
         self._swaps.add_swap_out(ev, ids, [ids_t, host])
-        return SwapHandle(seq_ids, lens, npages, ids_t, host, ev, out_start=start, num_bytes=nbytes)
+        return SwapHandle(seq_ids, lens, npages, ids_t, host, ev, out_start=start, num_bytes=nbytes,
+                          evicted=evicted, tracked=tracked, tracked_event=tracked_event)
 
     def swap_in(self, handle: SwapHandle, wait: bool = False,
                 seq_ids: Optional[Sequence[int]] = None) -> None:
@@ -1171,6 +1392,8 @@ class PagedKVCache:
         targets = list(handle.seq_ids) if seq_ids is None else [int(s) for s in seq_ids]
         if len(targets) != len(handle.seq_ids) or len(set(targets)) != len(targets):
             raise ValueError("seq_ids must name one distinct slot per evicted sequence")
+        if self.scores is not None and handle.tracked is None:
+            raise RuntimeError("the sequences were swapped out before track_attention")
         cur = torch.cuda.current_stream(self.device)
         dst = []
         for sid, n, ln in zip(targets, handle.num_pages, handle.seq_lens):
@@ -1181,6 +1404,18 @@ class PagedKVCache:
             self._seq_lens_cpu[sid] = ln
         self._lens_to_device()
         dst_t = self._to_device(np.asarray(dst, dtype=np.int32))
+        if handle.evicted is not None:
+            for sid, e in zip(targets, handle.evicted):
+                self._set_evicted(sid, e)
+        if self.scores is not None:
+            cur.wait_event(handle.tracked_event)
+            at = dst_t.long()
+            for s, p, (hs, hp) in zip(self.scores, self.positions, handle.tracked):
+                s.index_copy_(0, at, hs)
+                p.index_copy_(0, at, hp)
+                hs.record_stream(cur)
+                hp.record_stream(cur)
+            handle.tracked = []
         side = self._side_stream()
         side.wait_stream(cur)
         side.wait_event(handle.out_event)

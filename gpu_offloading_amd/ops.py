@@ -11,6 +11,7 @@ Reference call sites (aojsd/GPU_Offloading):
   compute_slot_mapping      src/MoE/moe_engine.py:3514-3541 (eager :1308-1316)
   copy_page_indices         src/MoE/moe_engine.py:1937-1946
   stage_from_host           src/MoE/moe_engine.py:3493-3494, 3506-3507
+  decode_attention_weights, evict_kv  new API (the engine never evicts single tokens)
   gather_kv / *_blocks / swap_*   new API (the engine has no gather or swap;
                             precedents moe_engine.py:4163-4183 and
                             src/dense/include/paged_offload_transformer.py:111-134, 394-418)
@@ -38,6 +39,9 @@ __all__ = [
     "reshape_and_cache",
     "paged_attention_v1",
     "paged_attention_v2",
+    "decode_attention_weights",
+    "evict_kv",
+    "evict_workspace_bytes",
 ]
 
 
@@ -624,3 +628,155 @@ def paged_attention_v2(out: torch.Tensor, exp_sums: torch.Tensor, max_logits: to
                      alibi_slopes, kv_cache_dtype, k_scale, v_scale,
                      (blocksparse_local_blocks, blocksparse_vert_stride, blocksparse_block_size,
                       blocksparse_head_sliding_step), stream)
+
+
+# --------------------------------------------------------------------------
+# Attention weights and eviction of single tokens
+# --------------------------------------------------------------------------
+_WDTYPES = {torch.float16: 0, torch.bfloat16: 1}     # KVC_DTYPE_* of include/kvc.h
+
+
+def _check_state(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, blocks: int,
+                 heads: int) -> None:
+    if t is not None and (t.dtype is not dtype or tuple(t.shape) != (blocks, heads, 16)
+                          or not t.is_contiguous()):
+        _fail(f"{name} must be contiguous {dtype} [{blocks}, {heads}, 16]")
+
+
+def _check_ints(name: str, t: Optional[torch.Tensor], n: int) -> None:
+    if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.numel() < n
+                          or not t.is_contiguous()):
+        _fail(f"{name} must be a contiguous 1-D int32 tensor of at least {n} entries")
+
+
+def check_scores(q: torch.Tensor, lse: torch.Tensor, rows: int, hq: int, k_cache: torch.Tensor,
+                 hkv: int, dim: int, scores: torch.Tensor, positions: Optional[torch.Tensor],
+                 position_offsets: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor],
+                 batch: int) -> torch.device:
+    """The checks that the chunk and decode forms of the attention weights share."""
+    dev = _check_cuda(q, lse, k_cache, scores, positions, position_offsets, seq_ids)
+    shape, _ = _check_cache(k_cache, "k_cache")
+    if tuple(shape[1:]) != (16, hkv, dim):
+        _fail(f"k_cache must be [blocks, 16, {hkv}, {dim}], got {tuple(shape)}")
+    if k_cache.dtype is not q.dtype:
+        _fail(f"dtype mismatch: q {q.dtype} vs cache {k_cache.dtype}")
+    if lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.dim() != 2 \
+            or lse.shape[0] < rows or lse.shape[1] != hq:
+        _fail(f"lse must be contiguous float32 [{rows}, {hq}]")
+    _check_state("scores", scores, torch.float32, shape[0], hkv)
+    _check_state("positions", positions, torch.int32, shape[0], hkv)
+    _check_ints("seq_ids", seq_ids, batch)
+    _check_ints("position_offsets", position_offsets, 0 if seq_ids is not None else batch)
+    return dev
+
+
+def decode_attention_weights(q: torch.Tensor, lse: torch.Tensor, key_cache: torch.Tensor,
+                             indptr: torch.Tensor, indices: torch.Tensor,
+                             last_page_len: torch.Tensor, scores: torch.Tensor,
+                             positions: Optional[torch.Tensor] = None,
+                             position_offsets: Optional[torch.Tensor] = None, *,
+                             seq_ids: Optional[torch.Tensor] = None,
+                             sm_scale: Optional[float] = None,
+                             stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+    """Attention weight that each cached token gets from a decode step, added up
+    over the query heads of its KV head: ``scores[block, head, slot] +=
+    sum exp(sm_scale q.k - lse)``; the request's last token, the query's own,
+    starts from it instead.
+
+    ``q [B, num_qo_heads, head_dim]`` and ``lse [B, num_qo_heads]`` (float32,
+    natural log) are the decode attention's query and log-sum-exp; ``indptr [B +
+    1]``, ``indices`` and ``last_page_len [B]`` its pages, int32 on the device (read
+    by the kernel: the launch can be captured and replayed).  ``scores`` is float32
+    ``[blocks, num_kv_heads, 16]``, beside ``key_cache``.  ``positions`` (int32,
+    as ``scores``) gets the last token's position, its slot in the sequence plus
+    ``position_offsets[seq_ids[b]]`` (``seq_ids`` defaults to b).  Returns
+    ``scores``."""
+    if q.dim() != 3:
+        _fail(f"q must be [requests, num_qo_heads, head_dim], got {tuple(q.shape)}")
+    if q.dtype not in _WDTYPES:
+        _fail(f"only bfloat16 and float16 are supported, got {q.dtype}")
+    if key_cache.dim() != 4:
+        _fail(f"key_cache must be [blocks, 16, heads, dim], got {tuple(key_cache.shape)}")
+    batch, hq, d = q.shape
+    hkv = key_cache.shape[2]
+    if d > 0 and (q.stride(2) != 1 or (hq > 1 and q.stride(1) != d)):
+        _fail("q: the heads of a request must be contiguous")
+    _check_ints("indptr", indptr, batch + 1)
+    _check_ints("indices", indices, 0)
+    _check_ints("last_page_len", last_page_len, batch)
+    check_scores(q, lse, batch, hq, key_cache, hkv, d, scores, positions, position_offsets,
+                 seq_ids, batch)
+    dev = _check_cuda(q, indptr, indices, last_page_len)
+    scale = float(sm_scale) if sm_scale is not None else d ** -0.5
+    with torch.cuda.device(dev):
+        _lib.call("kvc_decode_attention_weights", q.data_ptr(),
+                  q.stride(0) if batch > 1 else hq * d, lse.data_ptr(),
+                  key_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1),
+                  key_cache.shape[0], indptr.data_ptr(), indices.data_ptr(), indices.numel(),
+                  last_page_len.data_ptr(), batch, hq, hkv, d, key_cache.shape[1],
+                  _WDTYPES[q.dtype], scale, scores.data_ptr(), _ptr(positions),
+                  _ptr(position_offsets), _ptr(seq_ids), _stream_handle(dev, stream))
+    return scores
+
+
+def evict_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: torch.Tensor,
+             block_table: torch.Tensor, seq_lens: torch.Tensor, keep: torch.Tensor,
+             recent: torch.Tensor, max_seq_len: int,
+             positions: Optional[torch.Tensor] = None,
+             position_offsets: Optional[torch.Tensor] = None, *,
+             seq_ids: Optional[torch.Tensor] = None,
+             workspace: Optional[torch.Tensor] = None,
+             stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Cut each sequence's cache to ``keep[b]`` tokens, in place and per KV head:
+    its ``recent[b]`` last ones stay and of the others those of the largest
+    ``scores`` (equal ones by the lower slot; NaN ranks above inf).
+
+    Tokens that stay in slots at or above ``keep[b]`` move into the slots of
+    those that go, in order; the others keep their slots.  Afterwards the
+    sequence is its slots ``[0, keep[b])``: the caller sets its length and frees
+    its other pages (``PagedKVCache.evict`` does).  Sequences of at most ``keep[b]``
+    tokens are left alone.  ``scores`` float32 and ``positions`` int32 are ``[blocks,
+    heads, 16]`` and move along; with ``positions`` the last tokens are those
+    of positions ``>= seq_lens[b] + position_offsets[b] - recent[b]``, without
+    those of the last slots.  ``seq_lens``, ``keep``, ``recent``, ``position_offsets``
+    are int32 per sequence, on the device; sequence b's pages are row
+    ``seq_ids[b]`` (default b) of ``block_table``.  ``max_seq_len`` (host int) must
+    bound every length.  ``workspace`` (uint8, ``evict_workspace_bytes``) is
+    allocated if not given."""
+    dev = _check_cuda(key_cache, value_cache, scores, block_table, seq_lens, keep, recent,
+                      positions, position_offsets, seq_ids, workspace)
+    shape, cs = _check_cache(key_cache, "key_cache")
+    if (shape, cs) != _check_cache(value_cache, "value_cache") \
+            or key_cache.dtype is not value_cache.dtype:
+        _fail("key_cache and value_cache must have the same shape, strides and dtype")
+    nb, bs, h, d = shape
+    _check_state("scores", scores, torch.float32, nb, h)
+    _check_state("positions", positions, torch.int32, nb, h)
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 \
+            or block_table.stride(1) != 1:
+        _fail("block_table must be a 2-D int32 tensor with contiguous rows")
+    batch = seq_lens.numel()
+    for name, t in (("seq_lens", seq_lens), ("keep", keep), ("recent", recent),
+                    ("position_offsets", position_offsets), ("seq_ids", seq_ids)):
+        _check_ints(name, t, batch)
+    if seq_ids is None and block_table.shape[0] < batch:
+        _fail(f"block_table has {block_table.shape[0]} rows for {batch} sequences")
+    need = evict_workspace_bytes(batch, h, max_seq_len)
+    if workspace is None:
+        with torch.cuda.stream(stream):
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        _fail(f"workspace must be a contiguous tensor of at least {need} bytes")
+    with torch.cuda.device(dev):
+        _lib.call("kvc_evict_kv", key_cache.data_ptr(), value_cache.data_ptr(), nb, h, d, bs,
+                  key_cache.element_size(), cs[0], cs[1], scores.data_ptr(), _ptr(positions),
+                  block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                  block_table.shape[0], _ptr(seq_ids), seq_lens.data_ptr(), keep.data_ptr(),
+                  recent.data_ptr(), _ptr(position_offsets), batch, int(max_seq_len),
+                  workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                  _stream_handle(dev, stream))
+
+
+def evict_workspace_bytes(batch: int, num_kv_heads: int, max_seq_len: int) -> int:
+    """Device memory that ``evict_kv`` needs for its move lists."""
+    return int(_lib.load().kvc_evict_workspace_bytes(batch, num_kv_heads, max_seq_len))

@@ -1,0 +1,182 @@
+"""Attention of whole prompts over their own contiguous K/V.
+
+``BatchPromptAttentionWrapper`` covers the attention that the reference engine
+runs for new prompts outside the paged cache (src/MoE/moe_engine.py:2081,
+3776): packed sequences, causal or full, grouped heads, bf16 or fp16, head_dim
+64, 128 or 256.  It has the ``plan`` / ``run`` form of the paged wrappers:
+``plan`` reads the host index pointers, cuts every prompt's queries into tiles
+and stages the work list with one small H2D copy; ``run`` launches the kernel of
+csrc/prompt.hip once per layer.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Union
+
+import numpy as np
+import torch
+
+from . import _lib
+from .prefill import _fail, _host_int32
+
+__all__ = ["BatchPromptAttentionWrapper"]
+
+# KVC_DTYPE_* of include/kvc.h
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_DTYPE_NAMES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
+                "float16": torch.float16, "fp16": torch.float16, "half": torch.float16}
+
+
+def _dtype(dt: Union[str, torch.dtype]) -> torch.dtype:
+    got = _DTYPE_NAMES.get(dt, dt) if isinstance(dt, str) else dt
+    if got not in _DTYPES:
+        _fail(f"only bfloat16 and float16 are supported, got {dt}")
+    return got
+
+
+def _scale(sm_scale: Optional[float], head_dim: int) -> float:
+    s = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(head_dim)
+    if not (math.isfinite(s) and s > 0.0):
+        _fail(f"sm_scale must be positive and finite, got {s}")
+    return s
+
+
+def stage_plan(name: str, sched, args: tuple, capacity: int, device: torch.device) -> torch.Tensor:
+    """The host plan function ``name(*args, sched, image, capacity)``, run again
+    with the capacity it asks for where ``capacity`` int32 are too few, and its
+    image's device copy."""
+    lib = _lib.load()
+    while True:
+        image = torch.empty(max(capacity, 8), dtype=torch.int32, pin_memory=True)
+        st = getattr(lib, name)(*args, sched, image.data_ptr(), image.numel())
+        if st == _lib.KVC_ERR_WORKSPACE and sched.plan_ints > image.numel():
+            capacity = int(sched.plan_ints)
+            continue
+        _lib.check(name, st)
+        return image[:max(int(sched.plan_ints), 8)].to(device, non_blocking=True)
+
+
+class PlannedRuns:
+    """A wrapper whose runs read device memory that its plan staged.  A run on
+    another stream than the plan's is ordered after the plan's copies, and their
+    memory is kept for it; under graph capture the order is the caller's, and
+    the graph may be replayed until the next plan."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor):
+        if not float_workspace_buffer.is_cuda:
+            _fail("float_workspace_buffer must be a GPU tensor")
+        self._device = float_workspace_buffer.device
+        self._sched = None
+        self._staged: tuple = ()
+        self._plan_stream: Optional[int] = None
+        self._plan_event: Optional[torch.cuda.Event] = None
+        self._ordered: set = set()
+        self._dtype = torch.bfloat16
+        self._sm_scale = 0.0
+
+    def _set_staged(self, *tensors: torch.Tensor) -> None:
+        self._staged = tensors
+        self._plan_stream = _lib.current_stream_handle(self._device)
+        self._plan_event = torch.cuda.Event()
+        self._plan_event.record(torch.cuda.current_stream(self._device))
+        self._ordered = set()
+
+    def _run_stream(self, stream: Optional[torch.cuda.Stream]) -> int:
+        sh = stream.cuda_stream if stream is not None else _lib.current_stream_handle(self._device)
+        if sh != self._plan_stream and sh not in self._ordered \
+                and not torch.cuda.is_current_stream_capturing():
+            st = stream if stream is not None else torch.cuda.current_stream(self._device)
+            st.wait_event(self._plan_event)
+            for t in self._staged:
+                t.record_stream(st)
+            self._ordered.add(sh)
+        return sh
+
+
+class BatchPromptAttentionWrapper(PlannedRuns):
+    """Self-attention of packed prompts.  ``float_workspace_buffer`` only fixes
+    the device (interface parity with the paged wrappers)."""
+
+    def plan(self, qo_indptr: torch.Tensor, kv_indptr: Optional[torch.Tensor] = None, *,
+             num_qo_heads: int, num_kv_heads: int, head_dim: int, causal: bool = True,
+             sm_scale: Optional[float] = None,
+             q_data_type: Union[str, torch.dtype] = torch.bfloat16) -> None:
+        """Stage the work list for ``run``.  Sequence b's queries are rows
+        ``qo_indptr[b]:qo_indptr[b+1]``, its keys rows
+        ``kv_indptr[b]:kv_indptr[b+1]`` (default: the same rows); with
+        ``causal`` query i sees keys ``j <= i + kv_len - q_len``.  The index
+        pointers are int32 and may live on the host or the device (the
+        schedule is computed from host copies)."""
+        dt = _dtype(q_data_type)
+        scale = _scale(sm_scale, head_dim)
+        batch = qo_indptr.numel() - 1
+        if batch < 0:
+            _fail("qo_indptr must have at least one entry")
+        qo = _host_int32(qo_indptr, batch + 1, "qo_indptr")
+        if kv_indptr is None:
+            kv = qo
+        elif kv_indptr.numel() != batch + 1:
+            _fail("qo_indptr and kv_indptr must have the same length")
+        else:
+            kv = _host_int32(kv_indptr, batch + 1, "kv_indptr")
+        sched = _lib.KvcPromptSchedule()
+        group = max(1, num_qo_heads // max(1, num_kv_heads))
+        tokens = int(max(0, int(qo[-1]) - int(qo[0])))
+        guess = 1024 + 8 * max(1, num_kv_heads) * (tokens * group // 256 + batch)
+        plan = stage_plan("kvc_prompt_plan", sched,
+                          (qo.ctypes.data, kv.ctypes.data, batch, num_qo_heads, num_kv_heads,
+                           head_dim, 1 if causal else 0), guess, self._device)
+        self._set_staged(plan)
+        self._sched, self._dtype, self._sm_scale = sched, dt, scale
+
+    @property
+    def schedule(self) -> Optional[_lib.KvcPromptSchedule]:
+        return self._sched
+
+    def run(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+            return_lse: bool = False, stream: Optional[torch.cuda.Stream] = None):
+        """Attention of ``q [tokens, num_qo_heads, head_dim]`` over ``k``/``v
+        [tokens, num_kv_heads, head_dim]`` (rows past the planned ones are left
+        alone; slices of one fused tensor will do).  Returns ``out`` or ``(out,
+        lse)``, ``lse`` float32 ``[tokens, num_qo_heads]``, natural log, -inf for
+        a query that sees no key."""
+        s = self._sched
+        if s is None:
+            _fail("run() called before plan()")
+        hq, hkv, d = s.num_qo_heads, s.num_kv_heads, s.head_dim
+        for name, t, n, h in (("q", q, s.total_q, hq), ("k", k, s.total_kv, hkv),
+                              ("v", v, s.total_kv, hkv)):
+            _check_rows(name, t, n, h, d, self._dtype, self._device)
+        if out is not None:
+            _check_rows("out", out, s.total_q, hq, d, self._dtype, self._device)
+        with torch.cuda.stream(stream):     # the memory of the stream that writes it
+            if out is None:
+                out = torch.empty(s.total_q, hq, d, dtype=self._dtype, device=self._device)
+            if return_lse and lse is None:
+                lse = torch.empty(s.total_q, hq, dtype=torch.float32, device=self._device)
+        if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous()
+                                or lse.numel() < s.total_q * hq or lse.device != self._device):
+            _fail("lse must be contiguous float32 [tokens, num_qo_heads] on the wrapper's device")
+        sh = self._run_stream(stream)
+        with torch.cuda.device(self._device):
+            _lib.call("kvc_prompt_run", s, self._staged[0].data_ptr(), q.data_ptr(),
+                      _token_stride(q), k.data_ptr(), _token_stride(k), v.data_ptr(),
+                      _token_stride(v), _DTYPES[self._dtype], self._sm_scale, out.data_ptr(),
+                      _token_stride(out), lse.data_ptr() if lse is not None else None, sh)
+        return (out, lse) if return_lse else out
+
+
+def _check_rows(name: str, t: torch.Tensor, rows: int, heads: int, dim: int, dtype: torch.dtype,
+                device: torch.device) -> None:
+    if t.dim() != 3 or t.shape[0] < rows or tuple(t.shape[1:]) != (heads, dim):
+        _fail(f"{name} must be [{rows}, {heads}, {dim}], got {tuple(t.shape)}")
+    if t.dtype != dtype or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        _fail(f"{name} must be {dtype} with the heads of a token contiguous")
+    if t.device != device:
+        _fail(f"{name} on {t.device}, the wrapper's device is {device}")
+
+
+def _token_stride(t: torch.Tensor) -> int:
+    """Elements between tokens (of a single token: any valid stride)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]

@@ -557,6 +557,153 @@ int kvc_decode_step_setup(const int32_t* host_image, int32_t* dev_image,
                           int32_t* seq_lens, int64_t* slot_mapping, int32_t num_slots,
                           int32_t* indices, int64_t indices_capacity, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Attention of whole prompts over their own contiguous K/V (a new prompt's
+ * self-attention, before or beside the append into the cache), sequences
+ * packed one after another.  Sequence b's queries are rows
+ * qo_indptr[b] .. qo_indptr[b+1] of q, its keys rows kv_indptr[b] ..
+ * kv_indptr[b+1] of key and value (the same array as qo_indptr for whole
+ * prompts).  Query i (0-based in the sequence) sees key j when
+ * j <= i + kv_len - q_len (causal) or always (causal = 0):
+ *   out[i][hq] = softmax_j(sm_scale q[i][hq] . key[j][hq/group]) . value[j][hq/group]
+ * A query that sees no key gets 0 (lse -inf).  What a query does not see has
+ * no effect on it, inf and NaN included.  Optional lse[row][hq] is the
+ * natural-log log-sum-exp of the scaled logits, from fp32 sums of the
+ * unrounded exponentials; the exponentials are rounded to the element type for
+ * the value product.
+ *
+ * kvc_prompt_plan is host-only: one work unit per (tile of tile_tokens query
+ * tokens, KV head), longest first, dealt to num_workgroups workgroups.  If
+ * plan_capacity is too small it fills schedule->plan_ints and returns
+ * KVC_ERR_WORKSPACE.  The caller copies the image (16-byte aligned) to the
+ * device for kvc_prompt_run.  head_dim 64, 128 or 256, groups up to 128.
+ *
+ * kvc_prompt_run: q/out [rows][num_qo_heads][head_dim], key/value
+ * [rows][num_kv_heads][head_dim], each with a token stride (elements, a
+ * multiple of 8; slices of one fused projection output will do), 16-byte
+ * aligned; q, key and value hold at least schedule->total_q and total_kv rows.
+ * dtype is KVC_DTYPE_BF16 or KVC_DTYPE_FP16, for all four.
+ * ---------------------------------------------------------------------- */
+typedef struct kvc_prompt_schedule {
+  int32_t batch;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t causal;
+  int32_t tile_tokens;      /* query tokens per work unit                  */
+  int32_t num_units;
+  int32_t num_workgroups;
+  int32_t total_q;          /* qo_indptr[batch]                            */
+  int32_t total_kv;         /* kv_indptr[batch]                            */
+  int32_t max_key_tiles;    /* most 64-key tiles one unit visits           */
+  int32_t reserved;
+  int64_t plan_ints;        /* int32 entries of the plan image             */
+} kvc_prompt_schedule;
+
+int kvc_prompt_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
+                    int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t causal, kvc_prompt_schedule* schedule,
+                    int32_t* plan_host, int64_t plan_capacity);
+
+int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
+                   const void* q, int64_t q_token_stride,
+                   const void* key, int64_t key_token_stride,
+                   const void* value, int64_t value_token_stride,
+                   int32_t dtype, float sm_scale, void* out, int64_t out_token_stride,
+                   float* lse, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention weight that each cached token receives, accumulated per KV head:
+ *   w[t][h] = sum over query rows (i, hq in h's group) that see t of
+ *             exp(sm_scale q[i][hq] . K[t][h] - lse[i][hq])
+ *   scores[block][h][slot] = w (a new token) or += w (an older one)
+ * where lse is the natural-log log-sum-exp that the attention over the same
+ * keys returned (decode, prefill or prompt run).  A row whose lse is -inf saw no
+ * key and adds nothing.  scores is fp32 [num_blocks][num_kv_heads][16], beside
+ * the cache.  positions (int32, the same shape, may be null) gets each new
+ * token's position, its slot in the sequence + position_offsets[seq_ids[b]]
+ * (the tokens evicted from the sequence before; null: 0; seq_ids null: b).  A
+ * page belongs to one request of a call.  Other slots of the last page and
+ * other blocks are left as they are; page ids outside [0, num_blocks) are
+ * skipped.
+ *
+ * Chunk form: request b's queries are the last q_len tokens of its kv_len
+ * cached ones (rows qo_indptr[b] .. of q and lse), causal as the prefill's or
+ * not; its last new_tokens[b] tokens (null: q_len) are new.  kvc_weights_plan is
+ * host-only, as kvc_prompt_plan; kvc_batch_attention_weights_run runs it.
+ * Decode form: one query token per request, its last cached token, which is
+ * new; indptr, indices and last_page_len are device arrays as the decode's
+ * (at most num_indices pages are read), so that the launch can be captured and
+ * replayed.  Every sum has a fixed order.  head_dim 64, 128 or 256,
+ * page_size 16, groups up to 128; q and the cache are 16-byte aligned with
+ * strides that are multiples of 8 elements.
+ * ---------------------------------------------------------------------- */
+typedef struct kvc_weights_schedule {
+  int32_t batch;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t causal;
+  int32_t shared_keys;      /* a workgroup's waves share keys, not rows    */
+  int32_t num_units;
+  int32_t num_workgroups;
+  int32_t total_q;          /* qo_indptr[batch]                            */
+  int64_t plan_ints;        /* int32 entries of the plan image             */
+} kvc_weights_schedule;
+
+int kvc_weights_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
+                     const int32_t* last_page_len_host, const int32_t* new_tokens_host,
+                     int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                     int32_t head_dim, int32_t page_size, int32_t causal,
+                     kvc_weights_schedule* schedule, int32_t* plan_host,
+                     int64_t plan_capacity);
+
+int kvc_batch_attention_weights_run(
+    const kvc_weights_schedule* schedule, const int32_t* plan,
+    const void* q, int64_t q_token_stride, const float* lse,
+    const void* key_cache, int64_t cache_block_stride, int64_t cache_token_stride,
+    int64_t num_blocks, const int32_t* indices, int64_t num_indices,
+    int32_t dtype, float sm_scale, float* scores, int32_t* positions,
+    const int32_t* position_offsets, const int32_t* seq_ids, void* stream);
+
+int kvc_decode_attention_weights(
+    const void* q, int64_t q_token_stride, const float* lse,
+    const void* key_cache, int64_t cache_block_stride, int64_t cache_token_stride,
+    int64_t num_blocks, const int32_t* indptr, const int32_t* indices, int64_t num_indices,
+    const int32_t* last_page_len, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t page_size, int32_t dtype, float sm_scale, float* scores,
+    int32_t* positions, const int32_t* position_offsets, const int32_t* seq_ids, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Eviction of single tokens: of sequence b's seq_lens[b] cached tokens,
+ * keep[b] stay in each KV head -- its recent[b] last ones (by position:
+ * positions >= seq_lens[b] + position_offsets[b] - recent[b]; without
+ * positions by slot) and of the others those of the largest scores, equal ones
+ * by the lower slot (NaN counts as larger than inf).  Tokens that stay in slots
+ * at or above keep[b] move, ascending, into the slots below it whose tokens
+ * go: K and V rows, scores and positions.  Afterwards the sequence's cache is
+ * its slots [0, keep[b]); what the slots above hold is unspecified but was
+ * not written.  A sequence of at most keep[b] tokens is left alone.
+ * block_table rows are picked by seq_ids (null: row b); max_seq_len bounds every
+ * seq_lens[b] (tokens past it, or past the table's row, are not considered);
+ * tokens of pages outside [0, num_blocks) rank last and do not move.
+ * Rows (head_dim * elem_bytes) are multiples of 16 bytes; the caches 16-byte
+ * aligned.  workspace: kvc_evict_workspace_bytes(...) of device memory, not
+ * kept between calls.
+ * ---------------------------------------------------------------------- */
+int64_t kvc_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t max_seq_len);
+
+int kvc_evict_kv(
+    void* key_cache, void* value_cache, int64_t num_blocks, int32_t num_kv_heads,
+    int32_t head_dim, int32_t block_size, int32_t elem_bytes,
+    int64_t cache_block_stride, int64_t cache_token_stride,
+    float* scores, int32_t* positions,
+    const int32_t* block_table, int64_t block_table_row_stride, int32_t block_table_width,
+    int32_t block_table_rows, const int32_t* seq_ids, const int32_t* seq_lens,
+    const int32_t* keep, const int32_t* recent, const int32_t* position_offsets,
+    int32_t batch, int32_t max_seq_len, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,360 @@
+"""GPU tests of the attention weights per cached token (csrc/weights.hip) and of
+the eviction by them (csrc/evict.hip), against 64 bits and a plain ranking.
+The tolerances of the weights are the error bounds of attention_ref.weights."""
+import math
+import random
+
+import pytest
+import torch
+
+import attention_ref as ref
+from gpu_offloading_amd import ops
+from gpu_offloading_amd.eviction import BatchAttentionWeightsWrapper
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _randn(gpu, *shape, seed, dtype, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype).to(gpu)
+
+
+class Pool:
+    """A permuted page pool, K/V and the tracked state of sequences of these lengths."""
+
+    def __init__(self, gpu, lens, hkv, d, dtype, seed, spare=3):
+        self.lens, self.hkv, self.d = lens, hkv, d
+        counts = [(n + 15) // 16 for n in lens]
+        total = sum(counts) + spare
+        order = list(range(total))
+        random.Random(seed).shuffle(order)
+        at = ref.cumulative(counts)
+        self.rows = [order[a:b] for a, b in zip(at, at[1:])]
+        width = max(counts + [1])
+        self.table = torch.tensor([r + [-1] * (width - len(r)) for r in self.rows],
+                                  dtype=torch.int32, device=gpu).reshape(len(lens), width)
+        cache = _randn(gpu, total, 2, 16, hkv, d, seed=seed, dtype=dtype)
+        self.kc, self.vc = cache[:, 0], cache[:, 1]
+        g = torch.Generator().manual_seed(seed + 5)
+        self.scores = torch.rand(total, hkv, 16, generator=g).to(gpu)
+        self.positions = torch.randint(-50, -1, (total, hkv, 16), generator=g).int().to(gpu)
+        self.indptr = torch.tensor(at, dtype=torch.int32, device=gpu)
+        self.indices = torch.tensor(sum(self.rows, []) or [0], dtype=torch.int32, device=gpu)
+        self.lpl = torch.tensor([(n - 1) % 16 + 1 if n else 0 for n in lens], dtype=torch.int32,
+                                device=gpu)
+
+    def keys(self, b):
+        """K [n, Hkv, D] of sequence b."""
+        n = self.lens[b]
+        return self.kc[torch.tensor(self.rows[b], dtype=torch.int64, device=self.kc.device)
+                       ].flatten(0, 1)[:n]
+
+    def at(self, x, b):
+        """A state array's [Hkv, n] of sequence b, on the host."""
+        n = self.lens[b]
+        return x.cpu()[torch.tensor(self.rows[b], dtype=torch.int64)].transpose(0, 1).flatten(1)[:, :n]
+
+
+def _lse(gpu, rows, hq, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.rand(rows, hq, generator=g) * 4 + 1).to(gpu)
+
+
+def _check_weights(pool, before, q, lse, qlens, new, causal, offsets, scale):
+    scores, positions = before
+    used = torch.zeros_like(scores, dtype=torch.bool)
+    qa = ref.cumulative(qlens)
+    for b, n in enumerate(pool.lens):
+        if qlens[b] == 0 and new[b] == 0:
+            continue
+        w, tol = ref.weights(q[qa[b]:qa[b + 1]], lse[qa[b]:qa[b + 1]], pool.keys(b),
+                             n - qlens[b], causal, scale)
+        old = pool.at(scores, b).double()
+        fresh = torch.arange(n) >= n - new[b]
+        want = torch.where(fresh, w, old + w)
+        ref.assert_within(pool.at(pool.scores, b), want, tol + 2.0 ** -23 * want.abs() + 1e-30,
+                          f"request {b}")
+        place = torch.arange(n, dtype=torch.int32) + offsets[b]
+        assert torch.equal(pool.at(pool.positions, b),
+                           torch.where(fresh, place, pool.at(positions, b)))
+        for t in range(n):
+            used[pool.rows[b][t // 16], :, t % 16] = True
+    # nothing else was written
+    assert torch.equal(pool.scores[~used], scores[~used])
+    assert torch.equal(pool.positions[~used], positions[~used])
+
+
+def _chunk(gpu, lens, qlens, hkv, group, d, dtype, causal=True, new=None, seed=0, std=1.0):
+    print("weights", lens, qlens, hkv, group, d, dtype, causal, new, flush=True)
+    pool = Pool(gpu, lens, hkv, d, dtype, seed)
+    hq = hkv * group
+    q = _randn(gpu, sum(qlens) + 1, hq, d, seed=seed + 1, dtype=dtype, std=std)
+    lse = _lse(gpu, sum(qlens) + 1, hq, seed + 2)
+    offsets = [7 * b for b in range(len(lens))]
+    w = BatchAttentionWeightsWrapper(torch.empty(16, dtype=torch.uint8, device=gpu))
+    w.plan(torch.tensor(ref.cumulative(qlens), dtype=torch.int32), pool.indptr.cpu(), pool.indices,
+           pool.lpl.cpu(), hq, hkv, d, 16, causal=causal, q_data_type=dtype,
+           new_tokens=None if new is None else torch.tensor(new, dtype=torch.int32))
+    before = pool.scores.clone(), pool.positions.clone()
+    w.run(q, lse, pool.kc, pool.scores, pool.positions,
+          torch.tensor(offsets, dtype=torch.int32, device=gpu))
+    torch.cuda.synchronize()
+    _check_weights(pool, before, q, lse, qlens, qlens if new is None else new, causal, offsets,
+                   d ** -0.5)
+    return pool, q, lse, w
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("causal", [True, False])
+def test_chunk_dims_and_types(gpu, d, dtype, causal):
+    _chunk(gpu, [1, 16, 17, 200, 65, 31], [1, 3, 17, 40, 1, 31], 2, 4, d, dtype, causal, seed=d)
+
+
+@pytest.mark.parametrize("hkv,group", [(1, 1), (3, 2), (1, 3), (2, 7), (1, 16), (1, 33), (1, 128)])
+def test_chunk_groups(gpu, hkv, group):
+    _chunk(gpu, [70, 5, 140], [20, 5, 3], hkv, group, 64, BF, seed=group)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("qlens", [[260, 600], [8, 30]])
+def test_chunk_waves_that_share_keys_and_that_do_not(gpu, d, qlens):
+    *_, w = _chunk(gpu, [700, 600], qlens, 1, 2, d, BF, seed=9)
+    assert w.schedule.shared_keys == (qlens[1] == 600)
+
+
+def test_prompt_whose_last_tokens_vote(gpu):
+    """Every token is new, and the tokens that no query row may add to, too."""
+    _chunk(gpu, [300, 40, 64], [32, 32, 0], 2, 4, 128, BF, new=[300, 40, 64], seed=4)
+    _chunk(gpu, [300, 40, 64], [32, 8, 0], 2, 4, 128, BF, new=[0, 20, 5], seed=5)
+
+
+def test_rows_that_saw_no_key_add_nothing(gpu):
+    pool, q, lse, w = _chunk(gpu, [50, 33], [20, 33], 1, 2, 128, BF, seed=6)
+    lse[3:30, 0] = -math.inf
+    before = pool.scores.clone(), pool.positions.clone()
+    w.run(q, lse, pool.kc, pool.scores, pool.positions, torch.tensor([0, 7], dtype=torch.int32,
+                                                                     device=gpu))
+    _check_weights(pool, before, q, lse, [20, 33], [20, 33], True, [0, 7], 128 ** -0.5)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_key_that_is_not_finite_stays_alone(gpu, bad):
+    """Other tokens' weights are as without it."""
+    lens, qlens = [100, 40], [50, 40]
+    pool, q, lse, w = _chunk(gpu, lens, qlens, 2, 2, 128, BF, seed=7)
+    w.run(q, lse, pool.kc, pool.scores)     # all queries' tokens: their first score again
+    clean = pool.scores.clone()
+    pool.scores.copy_(pool.scores)
+    blk, off = pool.rows[0][60 // 16], 60 % 16
+    pool.kc[blk, off] = bad
+    base = pool.scores.clone()
+    w.run(q, lse, pool.kc, pool.scores)
+    keep = torch.ones_like(clean, dtype=torch.bool)
+    keep[blk, :, off] = False
+    new = torch.zeros_like(keep)
+    for b in range(2):
+        for t in range(lens[b] - qlens[b], lens[b]):
+            new[pool.rows[b][t // 16], :, t % 16] = True
+    assert torch.equal(pool.scores[keep & new], base[keep & new])
+    assert torch.isfinite(pool.scores[keep]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hkv,group", [(8, 4), (1, 1), (3, 3), (2, 8), (1, 16), (2, 17), (1, 128)])
+def test_decode(gpu, d, dtype, hkv, group):
+    lens = [1, 16, 17, 0, 129, 64, 300, 15, 48]
+    print("decode weights", hkv, group, d, dtype, flush=True)
+    pool = Pool(gpu, lens, hkv, d, dtype, seed=d + group)
+    hq = hkv * group
+    q = _randn(gpu, len(lens), hq, d, seed=3, dtype=dtype)
+    lse = _lse(gpu, len(lens), hq, 4)
+    lse[4, 0] = -math.inf
+    seq_ids = torch.randperm(20, generator=torch.Generator().manual_seed(1))[:len(lens)].int()
+    offsets = torch.arange(20, dtype=torch.int32) * 3
+    before = pool.scores.clone(), pool.positions.clone()
+    ops.decode_attention_weights(q, lse, pool.kc, pool.indptr, pool.indices, pool.lpl, pool.scores,
+                                 pool.positions, offsets.to(gpu), seq_ids=seq_ids.to(gpu))
+    torch.cuda.synchronize()
+    one = [min(n, 1) for n in lens]
+    rows = torch.tensor([b for b, n in enumerate(lens) if n], device=gpu)
+    _check_weights(pool, before, q[rows], lse[rows], one, one, True,
+                   offsets[seq_ids.long()].tolist(), d ** -0.5)
+
+
+def test_decode_of_many_requests_and_strided_queries(gpu):
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(1, 90, (150,), generator=g).tolist()
+    pool = Pool(gpu, lens, 2, 128, BF, seed=12)
+    wide = _randn(gpu, 150, 12, 128, seed=5, dtype=BF)
+    q, lse = wide[:, 2:10], _lse(gpu, 150, 8, 6)
+    before = pool.scores.clone(), pool.positions.clone()
+    ops.decode_attention_weights(q, lse, pool.kc, pool.indptr, pool.indices, pool.lpl, pool.scores,
+                                 pool.positions)
+    _check_weights(pool, before, q, lse, [1] * 150, [1] * 150, True, [0] * 150, 128 ** -0.5)
+    # the same sums in the same order every time
+    scores = pool.scores.clone()
+    pool.scores.copy_(before[0])
+    ops.decode_attention_weights(q, lse, pool.kc, pool.indptr, pool.indices, pool.lpl, pool.scores)
+    assert torch.equal(pool.scores, scores)
+
+
+def test_missing_pages_are_skipped(gpu):
+    lens = [40, 100]
+    pool = Pool(gpu, lens, 2, 64, BF, seed=2)
+    q, lse = _randn(gpu, 2, 4, 64, seed=1, dtype=BF), _lse(gpu, 2, 4, 2)
+    good = pool.scores.clone()
+    ops.decode_attention_weights(q, lse, pool.kc, pool.indptr, pool.indices, pool.lpl, good)
+    bad = pool.indices.clone()
+    bad[1], bad[4] = -1, pool.kc.shape[0]
+    got = pool.scores.clone()
+    ops.decode_attention_weights(q, lse, pool.kc, pool.indptr, bad, pool.lpl, got)
+    for i in (1, 4):
+        p = int(pool.indices[i])
+        good[p] = pool.scores[p]
+    assert torch.equal(got, good)
+    w = BatchAttentionWeightsWrapper(torch.empty(16, dtype=torch.uint8, device=gpu))
+    for idx, keep in ((pool.indices, False), (bad, True)):
+        w.plan(torch.tensor([0, 2, 4], dtype=torch.int32), pool.indptr.cpu(), idx, pool.lpl.cpu(),
+               4, 2, 64, 16)
+        q4, lse4 = _randn(gpu, 4, 4, 64, seed=1, dtype=BF), _lse(gpu, 4, 4, 2)
+        s = pool.scores.clone()
+        w.run(q4, lse4, pool.kc, s)
+        if keep:
+            for i in (1, 4):
+                p = int(pool.indices[i])
+                assert torch.equal(s[p], pool.scores[p])
+                first[p] = pool.scores[p]
+            assert torch.equal(s, first)
+        first = s.clone()
+
+
+# ------------------------------------------------------------------ eviction
+def _evict(gpu, pool, keep, recent, positions, offsets, max_len=None, seq_ids=None, **kw):
+    lens = pool.lens
+    kc, vc = pool.kc.clone(), pool.vc.clone()
+    sc, ps = pool.scores.clone(), pool.positions.clone()
+    table, ids = pool.table, None
+    if seq_ids is not None:   # the sequences' rows elsewhere in a larger table
+        table = torch.full((max(seq_ids) + 2, pool.table.shape[1]), -1, dtype=torch.int32,
+                           device=gpu)
+        table[torch.tensor(seq_ids, device=gpu)] = pool.table
+        ids = torch.tensor(seq_ids, dtype=torch.int32, device=gpu)
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device=gpu)
+    ops.evict_kv(pool.kc, pool.vc, pool.scores, table, ints(lens), ints(keep), ints(recent),
+                 max(lens) if max_len is None else max_len, pool.positions if positions else None,
+                 ints(offsets) if offsets is not None else None, seq_ids=ids, **kw)
+    torch.cuda.synchronize()
+    moved = 0
+    for b, n in enumerate(lens):
+        off = 0 if offsets is None else offsets[b]
+        blk = pool.rows[b]
+        for h in range(pool.hkv):
+            score = [float(sc[blk[t // 16], h, t % 16]) for t in range(n)] if n > keep[b] else []
+            place = [int(ps[blk[t // 16], h, t % 16]) if positions else t for t in range(n)]
+            end = n + (off if positions else 0)
+            dst, src = ref.evict(score, place, n, keep[b], recent[b], end)
+            assert len(dst) == len(src)
+            moved += len(dst)
+            for d, s in zip(dst, src):
+                to, frm = (blk[d // 16], d % 16), (blk[s // 16], s % 16)
+                for x, was in ((kc, pool.kc), (vc, pool.vc)):
+                    x[to[0], to[1], h] = x[frm[0], frm[1], h]
+                sc[to[0], h, to[1]] = sc[frm[0], h, frm[1]]
+                if positions:
+                    ps[to[0], h, to[1]] = ps[frm[0], h, frm[1]]
+    assert torch.equal(pool.kc.view(torch.int16), kc.view(torch.int16))
+    assert torch.equal(pool.vc.view(torch.int16), vc.view(torch.int16))
+    assert torch.equal(torch.nan_to_num(pool.scores, 1e30), torch.nan_to_num(sc, 1e30))
+    assert torch.equal(pool.positions, ps)
+    return moved
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("positions", [False, True])
+def test_evict_keeps_recent_and_largest(gpu, d, positions):
+    lens = [0, 1, 15, 16, 17, 100, 333, 64, 200, 700]
+    pool = Pool(gpu, lens, 3, d, BF, seed=d)
+    offsets = [4 * b for b in range(len(lens))]
+    # positions in any order, as after an eviction
+    for b, n in enumerate(lens):
+        for h in range(3):
+            place = torch.randperm(n, generator=torch.Generator().manual_seed(b * 3 + h)) + offsets[b]
+            for t in range(n):
+                pool.positions[pool.rows[b][t // 16], h, t % 16] = int(place[t])
+    keep = [3, 1, 7, 16, 16, 40, 100, 0, 199, 650]
+    recent = [0, 1, 7, 2, 16, 10, 1, 0, 30, 0]
+    assert _evict(gpu, pool, keep, recent, positions, offsets if positions else None) > 0
+
+
+@pytest.mark.parametrize("dtype", [HF, torch.float32])
+def test_evict_other_types_sequence_ids_and_a_larger_bound(gpu, dtype):
+    lens = [90, 40, 130]
+    pool = Pool(gpu, lens, 2, 64, HF, seed=3)
+    if dtype is torch.float32:
+        pool.kc, pool.vc = pool.kc.float(), pool.vc.float()
+    ws = torch.empty(ops.evict_workspace_bytes(3, 2, 1000), dtype=torch.uint8, device=gpu)
+    assert _evict(gpu, pool, [50, 45, 20], [10, 5, 20], False, None, max_len=1000,
+                  seq_ids=[5, 0, 3], workspace=ws) > 0
+
+
+def test_evict_ties_infinities_and_nan(gpu):
+    """Equal scores go by slot, -0 equals 0, NaN ranks above inf."""
+    lens = [120, 120, 60]
+    pool = Pool(gpu, lens, 2, 64, BF, seed=8)
+    pool.scores[:] = torch.randint(0, 3, pool.scores.shape,
+                                   generator=torch.Generator().manual_seed(1)).float().to(gpu) - 1
+    zero = pool.scores == 0
+    pool.scores[zero & (torch.rand(zero.shape, generator=torch.Generator().manual_seed(2)).to(gpu)
+                        < 0.5)] = -0.0
+    for t, s in ((100, math.nan), (101, math.inf), (110, math.nan), (5, -math.inf), (117, 1e-40)):
+        pool.scores[pool.rows[1][t // 16], :, t % 16] = s
+    assert _evict(gpu, pool, [60, 4, 30], [3, 1, 30], False, None) > 0
+
+
+def test_evict_long_sequences(gpu):
+    """More tokens than one pass of the ranking holds, and thousands of moves."""
+    lens = [9000, 2049]
+    pool = Pool(gpu, lens, 1, 64, BF, seed=5)
+    assert _evict(gpu, pool, [3001, 2048], [100, 1], False, None) > 1000
+
+
+def test_evict_missing_pages_rank_last_and_do_not_move(gpu):
+    lens = [64]
+    pool = Pool(gpu, lens, 1, 64, BF, seed=6)
+    pool.table[0, 1] = -1
+    pool.table[0, 3] = pool.kc.shape[0]
+    k0, s0 = pool.kc.clone(), pool.scores.clone()
+    ops.evict_kv(pool.kc, pool.vc, pool.scores, pool.table,
+                 *(torch.tensor([x], dtype=torch.int32, device=gpu) for x in (64, 32, 0)), 64)
+    # all 32 tokens of pages 0 and 2 stay; page 1's slots cannot take page 2's tokens
+    assert torch.equal(pool.kc, k0) and torch.equal(pool.scores, s0)
+
+
+def test_evict_captured_and_replayed(gpu):
+    lens = [200, 90]
+    pool = Pool(gpu, lens, 2, 128, BF, seed=9)
+    ints = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([200, 90], [64, 50], [8, 8])]
+    ws = torch.empty(ops.evict_workspace_bytes(2, 2, 200), dtype=torch.uint8, device=gpu)
+    kc, vc, sc = pool.kc.clone(), pool.vc.clone(), pool.scores.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.evict_kv(pool.kc, pool.vc, pool.scores, pool.table, *ints, 200, workspace=ws)
+    for seed in (1, 2, 3):
+        fresh = torch.rand(sc.shape, generator=torch.Generator().manual_seed(seed)).to(gpu)
+        pool.kc.copy_(kc)
+        pool.vc.copy_(vc)
+        pool.scores.copy_(fresh)
+        g.replay()
+        k2, v2, s2 = kc.clone(), vc.clone(), fresh.clone()
+        cache = torch.stack([k2, v2], 1)
+        k2, v2 = cache[:, 0], cache[:, 1]
+        ops.evict_kv(k2, v2, s2, pool.table, *ints, 200)
+        torch.cuda.synchronize()
+        assert torch.equal(pool.kc, k2) and torch.equal(pool.vc, v2)
+        assert torch.equal(pool.scores, s2)
