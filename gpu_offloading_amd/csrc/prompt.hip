@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "unit_plan.h"
@@ -25,11 +26,21 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
-constexpr int kThreads = 256;
-constexpr int kWaveRows = 32;
-constexpr int kTileRows = kThreads / 64 * kWaveRows;
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+constexpr int kWaveRows = 32;                 // query rows per wave
 constexpr int kKeys = 64;                     // keys per tile
-constexpr int kMaxGroup = kTileRows;
+constexpr int kMaxGroup = 128;
+// Waves of a workgroup: two per SIMD, or one with the whole register file
+// (head_dim 256: O alone is 128 registers).
+constexpr int kWaves(int head_dim) { return head_dim == 256 ? 4 : 8; }
+constexpr int tile_rows(int head_dim) { return kWaves(head_dim) * kWaveRows; }
+// Word 3 of a raw buffer resource (32-bit data, no swizzle): loads past
+// num_records return zeros.
+constexpr int kBufferRsrcWord3 = 0x00020000;
+// s_waitcnt vmcnt(0) with the other counters unconstrained (gfx9 encoding).
+constexpr int kWaitVmcnt0 = 0x0F70;
 constexpr float kRescaleLog2 = 8.f;           // lazy-rescale threshold (base 2)
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -99,8 +110,460 @@ __device__ __forceinline__ int v_slot(int key, int chunk) {
   return D == 64 ? chunk ^ (4 * ((key >> 1) & 1)) : chunk ^ (4 * (key & 3));
 }
 
+// A work unit's record.
+struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles; };
+
+// head_dim 64 and 128: eight waves in two teams of four, one workgroup per CU,
+// two waves per SIMD: wave w of team 0 and wave w of team 1 share SIMD w.  Each
+// team owns 128 query rows and both read the same K/V tiles.  Per 64-key tile a
+// wave has an MFMA phase M_j (O^T += V_{j-1}^T P_{j-1}^T, then S_j^T = K_j Q^T,
+// operands read ahead) and a VALU phase X_j (softmax of S_j into P_j).  Team 1
+// runs one phase behind team 0 and every phase (slot) ends on a workgroup barrier,
+// so that on each SIMD one wave's matrix instructions run beside the other's
+// exponentials:
+//   slot 2j: team 0 M_j, team 1 X_{j-1};   slot 2j+1: team 0 X_j, team 1 M_j.
+// Team 1 also stages: at the start of slot 2j each of its waves issues the
+// direct-to-LDS loads of its 16 keys of K_{j+1} and V_j (the buffers were last
+// read in slot 2j-1) and waits for them before the barrier that ends slot 2j+1.
+// A workgroup runs a list of units: while one runs, the next one's record and Q
+// are loaded, and its first K tile is staged in the slot 2n of this one.
+//
+// S^T tiles come from v_mfma_f32_32x32x16 (A: lane l = row l%32, k =
+// 8(l/32)..+7; B: column l%32, same k; C: acc[4i+j] = row 8i+4(l/32)+j, column
+// l%32) with K as A: a lane owns ONE query row (column l%32) and 32 of the tile's
+// keys, lane l^32 the other 32.  Its P values are then laid out as the B operand
+// of O^T += V^T P^T, keys in the order {4h..4h+3, 8+4h..8+4h+3} for lane half h,
+// and O^T's columns are query rows too.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
+  constexpr int kRow = 2 * D;                  // bytes per K or V row
+  constexpr int kChunks = kRow / 16;
+  constexpr int kSteps = D / 16;               // k-steps of S^T
+  constexpr int kBlocks = D / 32;              // 32-dim blocks of O^T
+  constexpr int kTile = kKeys * kRow;
+  constexpr int kORow = kRow + 16;             // bytes per staged output row
+  constexpr int kDma = 16 * kRow / 1024;       // loads per wave, 16 keys each
+  constexpr int kLaneKeys = 1024 / kRow;       // keys per load
+  typedef typename T::x8 x8;
+  // One LDS object with the tiles first: operand reads then use immediate
+  // offsets.  ostage: each wave's finished rows on their way out, padded so that
+  // one instruction's pieces spread over the banks.  bad: the last unit (by its
+  // parity) whose boundary tiles held an inf or NaN in V.
+  struct Lds {
+    uint8_t k[2][kTile];
+    uint8_t v[2][kTile];
+    uint8_t ostage[8][kWaveRows * kORow];
+    int bad[2];
+  };
+  __shared__ alignas(16) Lds lds;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = wave >> 2;
+  const int sw = wave & 3;                     // team 1: the 16 keys of a tile it stages
+  const int lane = threadIdx.x & 63;
+  const int r = lane & 31;
+  const int half = lane >> 5;
+  const int row = wave * kWaveRows + r;
+  const int row_tok = int(row * a.inv_group >> 16);     // row / group
+  const int row_head = row - row_tok * a.group;
+  const int Hq = a.num_kv_heads * a.group;
+  if (threadIdx.x < 2) lds.bad[threadIdx.x] = -1;
+
+  const int2 span = a.wg_units[blockIdx.x];
+  const int u_first = __builtin_amdgcn_readfirstlane(span.x);
+  const int u_count = __builtin_amdgcn_readfirstlane(span.y);
+  // A unit's record as loaded (VGPRs, no wait) and as used (SGPRs).
+  struct RawUnit { int4 x, y; };
+  auto fetch_unit = [&](int u) __attribute__((always_inline)) {
+    return RawUnit{a.units[2 * u], a.units[2 * u + 1]};
+  };
+  auto to_unit = [](const RawUnit& t) __attribute__((always_inline)) {
+    auto rfl = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    return Unit{rfl(t.x.x), rfl(t.x.y), rfl(t.x.z), rfl(t.x.w), rfl(t.y.x), rfl(t.y.y),
+                rfl(t.y.z)};
+  };
+  // Rows of no token read the unit's first one; they are never stored.
+  auto load_q = [&](const Unit& U, x8 (&dst)[kSteps]) __attribute__((always_inline)) {
+    const bool there = row_tok < a.tile_tokens && U.tok0 + row_tok < U.q_len;
+    const uint16_t* qp = a.q + int64_t(U.q_off + U.tok0 + (there ? row_tok : 0)) * a.q_stride +
+                         int64_t(U.h * a.group + (there ? row_head : 0)) * D + 8 * half;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks)
+      dst[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
+  };
+
+  Unit cu = to_unit(fetch_unit(u_first));
+  int limit = -1, n_full = 0;
+  bool row_ok = false;
+  auto set_unit = [&](const Unit& U) __attribute__((always_inline)) {
+    cu = U;
+    const int tok = U.tok0 + row_tok;
+    row_ok = row_tok < a.tile_tokens && tok < U.q_len;
+    // Last key this row may see (inclusive); tiles [0, n_full) are seen whole by
+    // every row of the unit.
+    limit = !row_ok ? -1 : a.causal ? min(tok + U.kv_len - U.q_len, U.kv_len - 1) : U.kv_len - 1;
+    const int lim_lo = a.causal ? min(U.tok0 + U.kv_len - U.q_len, U.kv_len - 1) : U.kv_len - 1;
+    n_full = max(0, min(U.ntiles, (lim_lo + 1) / kKeys));
+  };
+  set_unit(cu);
+  x8 qb[kSteps];
+  load_q(cu, qb);
+
+  // Direct-to-LDS staging: load i of a wave fetches keys kLaneKeys i .. of its 16,
+  // lane L key kLaneKeys i + L / kChunks, the chunk whose swizzled slot is
+  // L % kChunks, at these byte offsets from the wave's first key.
+  const uint32_t k_bytes = uint32_t(a.k_stride * 2), v_bytes = uint32_t(a.v_stride * 2);
+  uint32_t lane_k[kDma], lane_v[kDma];
+#pragma unroll
+  for (int i = 0; i < kDma; ++i) {
+    const int key = kLaneKeys * i + lane / kChunks;
+    lane_k[i] = key * k_bytes + k_slot<D>(key, lane % kChunks) * 16;
+    lane_v[i] = key * v_bytes + v_slot<D>(key, lane % kChunks) * 16;
+  }
+  auto wait_dma = []() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    asm volatile("" ::: "memory");
+  };
+  auto lds_addr = [](const void* p) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)p));
+  };
+  // buffer_load_dwordx4 ... lds: 16 bytes per lane, lane L at LDS offset 16 L
+  // from the wave-uniform address in M0; inline assembly, so that the compiler
+  // does not make every later LDS read wait for it (each wave waits for its own
+  // before the barrier that publishes the tiles).  The resource is bounded to the
+  // sequence's last row: rows past it are not read.  No compiler-generated code
+  // here uses M0 (tests/test_prompt_m0.py checks the built assembly).
+  auto dma = [&](uint8_t* tile, const uint16_t* base, int64_t stride, uint32_t row_bytes,
+                 const uint32_t (&lane_off)[kDma], const Unit& U, int j)
+      __attribute__((always_inline)) {
+    const int key0 = j * kKeys + sw * 16;
+    const int rows = max(0, min(16, U.kv_len - key0));
+    const uint64_t p = reinterpret_cast<uint64_t>(base + (int64_t(U.k_off) + key0) * stride +
+                                                  U.h * D);
+    const int bytes = rows > 0 ? int(uint32_t(rows - 1) * row_bytes + kRow) : 0;
+    const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane(int(uint32_t(p))),
+                          __builtin_amdgcn_readfirstlane(int(uint32_t(p >> 32) & 0xFFFF)),
+                          __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3};
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile + sw * 16 * kRow));
+#pragma unroll
+    for (int i = 0; i < kDma; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to + 1024 * i), "v"(lane_off[i]), "s"(rsrc) : "memory");
+  };
+  auto dma_k = [&](const Unit& U, int j) __attribute__((always_inline)) {
+    dma(lds.k[j & 1], a.k, a.k_stride, k_bytes, lane_k, U, j);
+  };
+  auto dma_v = [&](const Unit& U, int j) __attribute__((always_inline)) {
+    dma(lds.v[j & 1], a.v, a.v_stride, v_bytes, lane_v, U, j);
+  };
+  // A boundary tile's V in LDS (this wave's 16 keys, just staged): inf and NaN
+  // and rows past the sequence become 0, as 0 times them must not reach the rows
+  // that do not see them; finish_unit gives them to those that do.
+  auto clean_v = [&](int j, int stamp) __attribute__((always_inline)) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) {
+      const int key = kLaneKeys * i + lane / kChunks;
+      uint4* at = reinterpret_cast<uint4*>(lds.v[j & 1] + sw * 16 * kRow + 1024 * i + 16 * lane);
+      uint4 x = *at;
+      if (j * kKeys + sw * 16 + key >= cu.kv_len) {
+        x = make_uint4(0, 0, 0, 0);
+      } else {
+        x.x = finite2<T>(x.x, &bad);
+        x.y = finite2<T>(x.y, &bad);
+        x.z = finite2<T>(x.z, &bad);
+        x.w = finite2<T>(x.w, &bad);
+      }
+      *at = x;
+    }
+    if (bad) lds.bad[stamp & 1] = stamp;
+  };
+
+  uint32_t v_rd[kBlocks];
+  {
+    const int e = (lane >> 2) & 3, q = lane & 3, gp = (lane >> 4) & 1;
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db)
+      v_rd[db] = (4 * half + e) * kRow +
+                 (v_slot<D>(4 * half + e, 4 * db + 2 * gp + (q >> 1)) << 4) + ((q & 1) << 3);
+  }
+  // Score MFMA i of a tile: k-step i/2 of key block i%2.  Output MFMA i: key step
+  // i / kBlocks, head-dim block i % kBlocks; its V^T operand through two transposing
+  // reads (ds_read_b64_tr_b16: within 16 lanes, lane j supplies the address of 4
+  // consecutive elements and lane i receives element i%4 of the rows supplied
+  // by lanes i/4 + {0,4,8,12}).
+  auto k_operand = [&](const uint8_t* buf, int i) __attribute__((always_inline)) {
+    return __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
+        buf + (32 * (i & 1) + r) * kRow + (k_slot<D>(r, 2 * (i >> 1) + half) << 4)));
+  };
+  auto v_operand = [&](const uint8_t* buf, int i) __attribute__((always_inline)) {
+    const uint8_t* p = buf + v_rd[i % kBlocks] + (i / kBlocks) * 16 * kRow;
+    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
+    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 8 * kRow));
+    return __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x16_t o[kBlocks], s[2];
+#pragma unroll
+  for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
+  uint32_t pw[2][8];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pw[b][e] = 0u;
+  // m_run: the row's running maximum (base 2, scaled); l_half: the running sum of
+  // p over this lane's half of the keys (fp32, before p is rounded).
+  float m_run = -INFINITY, l_half = 0.f;
+
+  auto mfma_phase = [&](int j, auto do_o_c, auto do_s_c) __attribute__((always_inline)) {
+    if constexpr (decltype(do_o_c)::value) {
+      const uint8_t* vb = lds.v[(j - 1) & 1];
+      constexpr int N = 4 * kBlocks;
+      x8 vop[N];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) vop[i] = v_operand(vb, i);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + 3 < N) vop[i + 3] = v_operand(vb, i + 3);
+        const int st = i / kBlocks;
+        const uint32_t* pp = &pw[st >> 1][4 * (st & 1)];
+        const x8 pb = __builtin_bit_cast(x8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
+        o[i % kBlocks] = T::mfma(vop[i], pb, o[i % kBlocks]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (decltype(do_s_c)::value) {
+      const uint8_t* kb = lds.k[j & 1];
+      constexpr int N = 2 * kSteps;
+      const f32x16_t zero = {};
+      x8 kop[N];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) kop[i] = k_operand(kb, i);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + 3 < N) kop[i + 3] = k_operand(kb, i + 3);
+        s[i & 1] = T::mfma(kop[i], qb[i >> 1], i < 2 ? zero : s[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // X_j.  Accumulator entry e of key block b holds key 32b + 8(e/4) + 4half + e%4
+  // of the tile; on boundary tiles the scores of keys the row does not see become
+  // -inf, in place.  The running maximum of a row moves only when it grew by more
+  // than kRescaleLog2 (base 2); otherwise it stays, p < 2^8, and O and l need no
+  // rescaling.  Each row decides for itself, so a row's result does not depend
+  // on which others share its wave.
+  auto valu_phase = [&](int j) __attribute__((always_inline)) {
+    if (j >= n_full) {
+      const int rel = limit - j * kKeys - 4 * half;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) <= rel ? s[b][e] : -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
+    const auto sw2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
+                                                      false, false);
+    mx = fmaxf(__uint_as_float(sw2[0]), __uint_as_float(sw2[1]));
+    const float cand = fmaxf(m_run, mx * a.scale_log2);
+    const bool grow = cand > m_run + kRescaleLog2;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+      const float alpha = grow ? fast_exp2(m_run - cand) : 1.f;
+      m_run = grow ? cand : m_run;
+      l_half *= alpha;
+#pragma unroll
+      for (int db = 0; db < kBlocks; ++db) o[db] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
+    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int b = i >> 3, e = 2 * (i & 7);
+      const float p0 = fast_exp2(fmaf(s[b][e], a.scale_log2, -m_use));
+      const float p1 = fast_exp2(fmaf(s[b][e + 1], a.scale_log2, -m_use));
+      sum0 += p0;
+      sum1 += p1;
+      pw[b][e >> 1] = pack2<T>(p0, p1);
+      if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    l_half += sum0 + sum1;
+  };
+
+  // The unit's rows leave through the wave's LDS staging: a lane holds 8-byte
+  // pieces of one row; read back, kChunks lanes hold a whole row.  Non-temporal
+  // stores: the output is not read again here, and the caches keep K and V.
+  auto finish_unit = [&](int k) __attribute__((always_inline)) {
+    const float l = l_half + __shfl_xor(l_half, 32);
+    const float inv = l == 0.f ? 0.f : 1.f / l;    // a row that sees no key: 0
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db) o[db] *= inv;
+    if (cu.ntiles > 0 && lds.bad[k & 1] == k) {
+      // p > 0 times an inf or NaN that the row sees.
+      for (int t = n_full * kKeys; t < min(cu.ntiles * kKeys, cu.kv_len); ++t) {
+        const uint16_t* vr = a.v + (int64_t(cu.k_off) + t) * a.v_stride + cu.h * D + 4 * half;
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint16_t w = vr[32 * db + 8 * (e >> 2) + (e & 3)];
+            if (t <= limit && (w & T::kExp) == T::kExp)
+              o[db][e] += float(__builtin_bit_cast(typename T::e, w));
+          }
+      }
+    }
+    uint8_t* stg = lds.ostage[wave];
+    // O^T entry (db, 4i+j) is head dim 32db + 8i + 4half + j: (db, i) is the row's
+    // 16-byte chunk 4db + i and half its 8-byte half.
+    uint8_t* wr = stg + r * kORow + 8 * half;
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint2*>(wr + 16 * (4 * db + i)) =
+            make_uint2(pack2<T>(o[db][4 * i], o[db][4 * i + 1]),
+                       pack2<T>(o[db][4 * i + 2], o[db][4 * i + 3]));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int kStoreRows = 64 / kChunks;      // rows per store
+    const int c = lane % kChunks;
+#pragma unroll
+    for (int t0 = 0; t0 < kWaveRows / kStoreRows; t0 += 4) {
+      uint4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = *reinterpret_cast<const uint4*>(
+            stg + ((t0 + i) * kStoreRows + lane / kChunks) * kORow + 16 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int rr = wave * kWaveRows + (t0 + i) * kStoreRows + lane / kChunks;
+        const int tt = int(rr * a.inv_group >> 16);
+        if (tt < a.tile_tokens && cu.tok0 + tt < cu.q_len)
+          store_stream(a.out + int64_t(cu.q_off + cu.tok0 + tt) * a.out_stride +
+                           int64_t(cu.h * a.group + rr - tt * a.group) * D + 8 * c,
+                       v[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (row_ok && a.lse && half == 0)
+      a.lse[int64_t(cu.q_off + cu.tok0 + row_tok) * Hq + cu.h * a.group + row_head] =
+          l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+    m_run = -INFINITY;
+    l_half = 0.f;
+  };
+
+  // Each team has its own copy of the unit loop (the team is a compile-time
+  // constant), first and last tiles peeled; they only meet the same barriers.  A
+  // unit whose first K tile was not staged during the one before (the
+  // workgroup's first, or one after a unit without keys) starts with a staging
+  // step of its own.
+  using yes = std::true_type;
+  using no = std::false_type;
+  auto run = [&](auto team_c) __attribute__((always_inline)) {
+    constexpr int kTeam = decltype(team_c)::value;
+    auto mfma = [&](int j, auto do_o_c, auto do_s_c) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_setprio(1);
+      mfma_phase(j, do_o_c, do_s_c);
+      __builtin_amdgcn_s_setprio(0);
+    };
+    auto staged_all = [&](int j, int k) __attribute__((always_inline)) {   // team 1, slot 2j+1
+      wait_dma();
+      if (j >= n_full) clean_v(j, k);
+    };
+    Unit nu = u_count > 1 ? to_unit(fetch_unit(u_first + 1)) : cu;  // the next unit
+    RawUnit nnu{};                                                   // the one after
+    bool staged = false;
+    for (int k = 0; k < u_count; ++k) {
+      const bool has_next = k + 1 < u_count;
+      const int n = cu.ntiles;
+      if (k + 2 < u_count) nnu = fetch_unit(u_first + k + 2);
+      if (n > 0) {
+        if (kTeam == 0) {
+          if (!staged) __syncthreads();
+          mfma(0, no{}, yes{});
+          __syncthreads();
+          valu_phase(0);
+          __syncthreads();
+          for (int j = 1; j < n; ++j) {
+            mfma(j, yes{}, yes{});
+            __syncthreads();
+            valu_phase(j);
+            __syncthreads();
+          }
+          // Q is not read again in this unit.
+          if (has_next) load_q(nu, qb);
+          mfma(n, yes{}, no{});
+          __syncthreads();
+          finish_unit(k);
+          __syncthreads();
+        } else {
+          if (!staged) {
+            dma_k(cu, 0);
+            wait_dma();
+            __syncthreads();
+          }
+          if (1 < n) dma_k(cu, 1);
+          dma_v(cu, 0);
+          __syncthreads();
+          mfma(0, no{}, yes{});
+          staged_all(0, k);
+          __syncthreads();
+          for (int j = 1; j < n; ++j) {
+            if (j + 1 < n) dma_k(cu, j + 1);
+            dma_v(cu, j);
+            valu_phase(j - 1);
+            __syncthreads();
+            mfma(j, yes{}, yes{});
+            staged_all(j, k);
+            __syncthreads();
+          }
+          valu_phase(n - 1);
+          // The next unit's Q, and its first K tile into lds.k[0], last read in slot
+          // 2n-1 or earlier.
+          if (has_next) load_q(nu, qb);
+          if (has_next && nu.ntiles > 0) dma_k(nu, 0);
+          __syncthreads();
+          mfma(n, yes{}, no{});
+          wait_dma();
+          __syncthreads();
+          finish_unit(k);
+        }
+      } else {
+        if (has_next) load_q(nu, qb);
+        finish_unit(k);
+      }
+      if (has_next) {
+        staged = n > 0 && nu.ntiles > 0;
+        set_unit(nu);
+        if (k + 2 < u_count) nu = to_unit(nnu);
+      }
+    }
+  };
+  if (team == 0) run(std::integral_constant<int, 0>{});
+  else run(std::integral_constant<int, 1>{});
+}
+
+// head_dim 256: four waves, one per SIMD, registers for a row's whole O.
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves(D), 1) void prompt_wide_kernel(PromptArgs a) {
+  constexpr int kThreads = 64 * kWaves(D);
   constexpr int kRow = 2 * D;                 // bytes per K or V row
   constexpr int kChunks = kRow / 16;
   constexpr int kSteps = D / 16;              // MFMA k-steps of K Q^T
@@ -287,7 +750,8 @@ __global__ __launch_bounds__(kThreads, 1) void prompt_kernel(PromptArgs a) {
   }
 }
 
-constexpr int64_t kMaxWorkgroups = 512;
+// Persistent workgroups: one per CU of an MI355X.
+constexpr int64_t kMaxWorkgroups = 256;
 int64_t plan_workgroups(int64_t units) { return std::min(kMaxWorkgroups, units); }
 
 int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batch, int32_t hq,
@@ -302,7 +766,7 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
   KVC_REQUIRE((head_dim == 64 || head_dim == 128 || head_dim == 256) && group <= kMaxGroup,
               KVC_ERR_UNSUPPORTED,
               "prompt attention supports head_dim 64, 128, 256 and groups up to 128");
-  const int tile_tokens = kTileRows / group;
+  const int tile_tokens = tile_rows(head_dim) / group;
   std::vector<int32_t> rec;
   int max_tiles = 0;
   int64_t end_q = 0, end_kv = 0, items = 0;
@@ -354,9 +818,10 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
 
 template <typename T>
 void launch(const PromptArgs& a, int head_dim, unsigned workgroups, hipStream_t s) {
-  if (head_dim == 64) prompt_kernel<T, 64><<<dim3(workgroups), kThreads, 0, s>>>(a);
-  else if (head_dim == 128) prompt_kernel<T, 128><<<dim3(workgroups), kThreads, 0, s>>>(a);
-  else prompt_kernel<T, 256><<<dim3(workgroups), kThreads, 0, s>>>(a);
+  const dim3 grid(workgroups), block(unsigned(64 * kWaves(head_dim)));
+  if (head_dim == 64) prompt_kernel<T, 64><<<grid, block, 0, s>>>(a);
+  else if (head_dim == 128) prompt_kernel<T, 128><<<grid, block, 0, s>>>(a);
+  else prompt_wide_kernel<T, 256><<<grid, block, 0, s>>>(a);
 }
 
 }  // namespace
@@ -382,7 +847,7 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
   const int Hq = sched->num_qo_heads, Hkv = sched->num_kv_heads, D = sched->head_dim;
   KVC_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= kMaxGroup &&
                   (D == 64 || D == 128 || D == 256) && sched->num_units >= 0 &&
-                  sched->tile_tokens == kTileRows / (Hq / Hkv) &&
+                  sched->tile_tokens == tile_rows(D) / (Hq / Hkv) &&
                   sched->num_workgroups == plan_workgroups(sched->num_units) &&
                   sched->plan_ints == unit_table_ints(sched->num_workgroups) +
                                           int64_t(sched->num_units) * kUnitInts,
