@@ -120,11 +120,12 @@ class KvcWeightsSchedule(ctypes.Structure):
         ("head_dim", c_int32),
         ("page_size", c_int32),
         ("causal", c_int32),
-        ("shared_keys", c_int32),
         ("num_units", c_int32),
-        ("num_workgroups", c_int32),
+        ("num_parts", c_int32),
+        ("num_joins", c_int32),
         ("total_q", c_int32),
         ("plan_ints", c_int64),
+        ("workspace_bytes", c_int64),
     ]
 
 
@@ -237,8 +238,8 @@ SIGNATURES = {
         c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
         c_int32, POINTER(KvcWeightsSchedule), c_void_p, c_int64]),
     "kvc_batch_attention_weights_run": (c_int, [
-        POINTER(KvcWeightsSchedule), _I32P, _P, c_int64, _P, _P, c_int64, c_int64, c_int64,
-        _I32P, c_int64, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),
+        POINTER(KvcWeightsSchedule), _I32P, _P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64,
+        c_int64, _I32P, c_int64, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),
     "kvc_decode_attention_weights": (c_int, [
         _P, c_int64, _P, _P, c_int64, c_int64, c_int64, _I32P, _I32P, c_int64, _I32P, c_int32,
         c_int32, c_int32, c_int32, c_int32, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),

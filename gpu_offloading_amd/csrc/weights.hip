@@ -16,8 +16,8 @@
 #include "kvc_common.h"
 
 #include <algorithm>
+#include <array>
 #include <cmath>
-#include <type_traits>
 #include <vector>
 
 #include "unit_plan.h"
@@ -82,136 +82,214 @@ __device__ __forceinline__ void store_weight(const WeightsArgs& a, int32_t block
     a.positions[at] = key + (a.offsets ? a.offsets[a.seq_ids ? a.seq_ids[b] : b] : 0);
 }
 
+// A work unit: kUnitKeys keys of one request and KV head, against a run of the
+// row blocks that see them.  Record (kRecInts int32):
+//   KV head, first key, q_len, kv_len | q offset, page offset, request, first new key |
+//   first block, blocks, partial (-1: the unit's sums are the keys' weights), 0
+constexpr int kRecInts = 12;
+constexpr int kRows = 32;                          // query rows per block
+constexpr int kKeyBlocks = 2;                      // 32-key blocks per wave
+constexpr int kWaveKeys = 32 * kKeyBlocks;
+constexpr int kChunkThreads = 256;
+constexpr int kUnitKeys = kChunkThreads / 64 * kWaveKeys;
+constexpr int kRing = 3;                           // row blocks in LDS
+
 struct ChunkArgs {
   WeightsArgs w;
-  const int2* wg_units;            // [workgroups]: (first unit, units)
-  const int4* units;               // [units][2]: (KV head, first key, q_len, kv_len),
-                                   //   (q offset, page offset, request, first new key)
+  const int4* units;               // [units][3]
+  float* parts;                    // [partials][kUnitKeys]
   int32_t causal;
 };
 
-constexpr int kChunkThreads = 256;
-constexpr int kWaves = kChunkThreads / 64;
-constexpr int kRows = 32;          // query rows per MFMA block
-template <int D> constexpr int kKeyBlocks = D == 256 ? 2 : 4;   // 32-key blocks per wave
+typedef __attribute__((address_space(3))) void lds_void_t;
 
-// kShare: the four waves hold the same keys and take every fourth block of
-// rows; else they hold consecutive keys and each takes all the rows.
-template <typename T, int D, bool kShare>
-__global__ __launch_bounds__(kChunkThreads, 2) void weights_chunk_kernel(ChunkArgs c) {
-  constexpr int KB = kKeyBlocks<D>, kSteps = D / 16;
+// The first query token of a unit (causal: the first that sees one of its keys).
+__host__ __device__ inline int first_token(int key0, int q_len, int kv_len, int causal) {
+  const int t = key0 - (kv_len - q_len);
+  return causal && t > 0 ? t : 0;
+}
+
+// A workgroup per unit.  Its four waves hold kWaveKeys keys each, K in registers for
+// the whole unit (B operands), and walk the same row blocks, which arrive in LDS
+// two blocks ahead (global_load_lds, each wave a quarter of a block, waited for by
+// count).  Bound by the exponentials: per 32 rows x 64 keys a wave issues 32 of 16
+// cycles and 64 other vector instructions of 4 beside 16 matrix instructions of 32
+// (head_dim 128), so three waves per SIMD keep the vector unit busy.
+template <typename T, int D>
+__global__ __launch_bounds__(kChunkThreads, D == 256 ? 2 : 3) void weights_chunk_kernel(ChunkArgs c) {
+  constexpr int KB = kKeyBlocks, kSteps = D / 16, kRow = 2 * D, kChunks = kRow / 16;
+  constexpr int kDma = kRows * kRow / 1024 / 4;    // row loads per wave and block
+  constexpr int kLoadRows = 1024 / kRow;           // rows per load
   typedef typename T::x8 x8;
   const WeightsArgs& a = c.w;
-  __shared__ float lse_s[kWaves][kRows];
-  __shared__ int limit_s[kWaves][kRows];
-  __shared__ float part[kShare ? kWaves : 1][32 * KB];
+  __shared__ struct alignas(16) {
+    uint8_t q[kRing][kRows * kRow];                // 16-byte chunks XOR-swizzled by row
+    float lse[kRing][4][64];                       // each wave's own copy, rows twice
+  } lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r = lane & 31, half = lane >> 5;
   const int Hq = a.num_kv_heads * a.group;
-  const int step_rows = kShare ? kRows * kWaves : kRows;
-  const int step_tok = step_rows / a.group, step_head = step_rows % a.group;
+  const int4 x = c.units[3 * blockIdx.x], y = c.units[3 * blockIdx.x + 1],
+             z = c.units[3 * blockIdx.x + 2];
+  auto rfl = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int h = rfl(x.x), key_first = rfl(x.y), q_len = rfl(x.z), kv_len = rfl(x.w);
+  const int first_block = rfl(z.x), blocks = rfl(z.y);
+  const int key0 = key_first + wave * kWaveKeys;
+  const int ahead = kv_len - q_len;                // keys before the first query token
+  const int tok0 = first_token(key_first, q_len, kv_len, c.causal);
 
-  const int2 span = c.wg_units[blockIdx.x];
-  for (int u = span.x; u < span.x + span.y; ++u) {
-    const int4 x = c.units[2 * u], y = c.units[2 * u + 1];
-    const int h = x.x, q_len = x.z, kv_len = x.w;
-    const int key0 = x.y + (kShare ? 0 : wave * 32 * KB);
-    if (key0 < kv_len) {     // (the same for all waves where they share keys)
-      int32_t block[KB];
-      x8 kop[KB][kSteps];
+  // Row blocks on their way: row (32 block + i) of the unit is token tok0 + row /
+  // group, head row % group; the rows past the last repeat it.  Each lane keeps the
+  // (token, head) of its row in every load and steps it by 32 rows per block.
+  struct Place { int tok, head; };
+  auto place_of = [&](int row) __attribute__((always_inline)) {
+    return Place{row / a.group, row % a.group};
+  };
+  const int step_tok = kRows / a.group, step_head = kRows % a.group;
+  auto step = [&](Place& p) __attribute__((always_inline)) {
+    p.tok += step_tok;
+    p.head += step_head;
+    if (p.head >= a.group) {
+      p.head -= a.group;
+      ++p.tok;
+    }
+  };
+  const int last_tok = q_len - 1 - tok0;
+  Place qrow[kDma], lrow = place_of(first_block * kRows + r);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const int key = key0 + 32 * kb + r;
-        block[kb] = key < kv_len ? block_of(a, int64_t(y.y) + key / kPage) : -1;
-        // A key that is not there reads block 0; its column is not stored.
-        const uint16_t* kp = a.k_cache + int64_t(max(block[kb], 0)) * a.block_stride +
-                             (key % kPage) * a.token_stride + h * D + 8 * half;
+  for (int i = 0; i < kDma; ++i)
+    qrow[i] = place_of(first_block * kRows + (wave * kDma + i) * kLoadRows + lane / kChunks);
+  auto lds_addr = [](const void* p) __attribute__((always_inline)) {
+    return __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)p)));
+  };
+  // kDma + 1 loads into ring slot `slot` (inline assembly: the compiler would wait
+  // for all of them at every LDS read; it uses M0 nowhere itself).
+  auto stage = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks)
-          kop[kb][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 16 * ks));
+    for (int i = 0; i < kDma; ++i) {
+      const Place p = qrow[i];
+      const bool past = p.tok > last_tok;
+      const int row = (wave * kDma + i) * kLoadRows + lane / kChunks;
+      const int chunk = D == 64 ? (lane % kChunks) ^ ((row >> 1) & 7) : (lane % kChunks) ^ (row & 15);
+      const uint16_t* src = a.q + (int64_t(y.x) + tok0 + (past ? last_tok : p.tok)) * a.q_stride +
+                            (h * a.group + (past ? a.group - 1 : p.head)) * D + 8 * chunk;
+      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+                   :: "s"(lds_addr(lds.q[slot] + (wave * kDma + i) * 1024)), "v"(src) : "memory");
+      step(qrow[i]);
+    }
+    const bool past = lrow.tok > last_tok;
+    const float* src = a.lse + (int64_t(y.x) + tok0 + (past ? last_tok : lrow.tok)) * Hq +
+                       h * a.group + (past ? a.group - 1 : lrow.head);
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(lds_addr(lds.lse[slot][wave])), "v"(src) : "memory");
+    step(lrow);
+  };
+
+  x8 kop[KB][kSteps];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    const int key = key0 + 32 * kb + r;
+    const int32_t block = key < kv_len ? block_of(a, int64_t(y.y) + key / kPage) : -1;
+    // A key that is not there reads block 0; its column is not stored.
+    const uint16_t* kp = a.k_cache + int64_t(max(block, 0)) * a.block_stride +
+                         (key % kPage) * a.token_stride + h * D + 8 * half;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks)
+      kop[kb][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 16 * ks));
+  }
+  float acc[KB];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) acc[kb] = 0.f;
+  if (blocks > 0) stage(0);
+  if (blocks > 1) stage(1);
+  Place mine = place_of(first_block * kRows + r);   // this lane's row of the current block
+
+  int slot = 0;
+  for (int i = 0; i < blocks; ++i) {
+    // This block's loads are done, the next one's may run.
+    if (i + 1 < blocks) {
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kDma + 1) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    const int next2 = slot == 0 ? 2 : slot - 1;     // (slot + 2) % 3, read two blocks ago
+    if (i + 2 < blocks) stage(next2);
+
+    const float lse = lds.lse[slot][wave][r];
+    // The last key that this lane's row sees; a row of no key (lse -inf) gives nothing.
+    const bool there = mine.tok <= last_tok && lse != -INFINITY;
+    const int limit = !there ? -1 : c.causal ? ahead + tok0 + mine.tok : kv_len;
+    step(mine);
+    if (__builtin_amdgcn_ballot_w64(limit >= key0) != 0 && key0 < kv_len) {
+      const bool whole = __builtin_amdgcn_ballot_w64(limit < key0 + kWaveKeys - 1) == 0;
+      f32x16_t s[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const int chunk = 2 * ks + half;
+        const x8 qop = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
+            lds.q[slot] + r * kRow +
+            (D == 64 ? chunk ^ ((r >> 1) & 7) : chunk ^ (r & 15)) * 16));
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = T::mfma32(qop, kop[kb][ks], s[kb]);
       }
-      // Rows from the first token that sees key0 on.
-      const int ahead = kv_len - q_len;        // keys before the first query token
-      const int tok0 = c.causal ? max(0, key0 - ahead) : 0;
-      const int rows = max(0, q_len - tok0) * a.group;
-      const int row0 = kShare ? wave * kRows : 0;
-      int tok = tok0 + (row0 + r) / a.group, head = (row0 + r) % a.group;
-      float acc[KB];
+      // Accumulator entry 4i+j is row 8i + 4half + j, the lane's column key r.
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) acc[kb] = 0.f;
-
-      for (int rb = row0; rb < rows; rb += step_rows) {
-        const bool there = rb + r < rows;
-        const int64_t qt = int64_t(y.x) + (there ? tok : q_len - 1);
-        const int qh = h * a.group + (there ? head : 0);
-        x8 qop[kSteps];
-        const uint16_t* qp = a.q + qt * a.q_stride + qh * D + 8 * half;
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 l4 = *reinterpret_cast<const float4*>(&lds.lse[slot][wave][8 * q4 + 4 * half]);
+        const float nl[4] = {l4.x * -kLog2e, l4.y * -kLog2e, l4.z * -kLog2e, l4.w * -kLog2e};
+        if (whole) {
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks)
-          qop[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
-        const float lse = a.lse[qt * Hq + qh];
-        // The last key that this row sees; a row of no key (lse -inf) gives nothing.
-        const int limit = !there || lse == -INFINITY ? -1 : c.causal ? ahead + tok : kv_len;
-        lse_s[wave][r] = lse * -kLog2e;
-        limit_s[wave][r] = limit;
-        const bool whole = __builtin_amdgcn_ballot_w64(limit < key0 + 32 * KB - 1) == 0;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        float4 nl[4];
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          nl[i] = *reinterpret_cast<const float4*>(&lse_s[wave][8 * i + 4 * half]);
+            for (int kb = 0; kb < KB; ++kb)
+              acc[kb] += fast_exp2(fmaf(s[kb][4 * q4 + j], a.scale_log2, nl[j]));
+        } else {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          f32x16_t s;
+          for (int j = 0; j < 4; ++j) {
+            const int lim = __shfl(limit, 8 * q4 + 4 * half + j);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < kSteps; ++ks) s = T::mfma32(qop[ks], kop[kb][ks], s);
-          const int key = key0 + 32 * kb + r;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float n4[4] = {nl[i].x, nl[i].y, nl[i].z, nl[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float p = fast_exp2(fmaf(s[4 * i + j], a.scale_log2, n4[j]));
-              acc[kb] += whole || key <= limit_s[wave][8 * i + 4 * half + j] ? p : 0.f;
+            for (int kb = 0; kb < KB; ++kb) {
+              const float p = fast_exp2(fmaf(s[kb][4 * q4 + j], a.scale_log2, nl[j]));
+              acc[kb] += key0 + 32 * kb + r <= lim ? p : 0.f;
             }
           }
         }
-        __builtin_amdgcn_wave_barrier();
-        tok += step_tok;
-        head += step_head;
-        if (head >= a.group) {
-          head -= a.group;
-          ++tok;
-        }
-      }
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) acc[kb] += __shfl_xor(acc[kb], 32);
-      if (kShare) {
-        if (half == 0)
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) part[wave][32 * kb + r] = acc[kb];
-        __syncthreads();
-        const int i = threadIdx.x;
-        const int key = key0 + i;
-        if (i < 32 * KB && key < kv_len) {
-          const float w = (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
-          const int32_t blk = block_of(a, int64_t(y.y) + key / kPage);
-          if (blk >= 0) store_weight(a, blk, h, key, y.z, w, key >= y.w);
-        }
-        __syncthreads();
-      } else if (half == 0) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const int key = key0 + 32 * kb + r;
-          if (block[kb] >= 0) store_weight(a, block[kb], h, key, y.z, acc[kb], key >= y.w);
-        }
       }
     }
+    slot = slot == kRing - 1 ? 0 : slot + 1;
   }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    const float w = acc[kb] + __shfl_xor(acc[kb], 32);
+    const int key = key0 + 32 * kb + r;
+    if (half != 0 || key >= kv_len) continue;
+    if (z.z >= 0) {
+      c.parts[int64_t(z.z) * kUnitKeys + key - key_first] = w;
+      continue;
+    }
+    const int32_t block = block_of(a, int64_t(y.y) + key / kPage);
+    if (block >= 0) store_weight(a, block, h, key, y.z, w, key >= y.w);
+  }
+}
+
+// Sums of the units whose rows were cut: a workgroup per (key tile, KV head), a
+// thread per key, the partials in order.  Record: KV head, first key, partials, kv_len |
+// first partial, page offset, request, first new key.
+__global__ __launch_bounds__(kUnitKeys) void weights_join_kernel(ChunkArgs c, const int4* joins) {
+  const int4 x = joins[2 * blockIdx.x], y = joins[2 * blockIdx.x + 1];
+  const int key = x.y + threadIdx.x;
+  if (key >= x.w) return;
+  const float* p = c.parts + int64_t(y.x) * kUnitKeys + threadIdx.x;
+  float w = 0.f;
+  for (int i = 0; i < x.z; ++i) w += p[int64_t(i) * kUnitKeys];
+  const int32_t block = block_of(c.w, int64_t(y.y) + key / kPage);
+  if (block >= 0) store_weight(c.w, block, x.x, key, y.z, w, key >= y.w);
 }
 
 struct TokenArgs {
@@ -297,13 +375,12 @@ __global__ __launch_bounds__(kTokenThreads) void weights_token_kernel(TokenArgs 
   }
 }
 
-constexpr int64_t kMaxWorkgroups = 512;
-constexpr int kShareBlocks = 16;   // row blocks of a request from which waves share keys
-int64_t plan_workgroups(int64_t units) { return std::min(kMaxWorkgroups, units); }
-int unit_keys(int head_dim, int share) {
-  return 32 * (head_dim == 256 ? 2 : 4) * (share ? 1 : kWaves);
-}
 constexpr int kMaxGroup = 128;
+// Rows are cut where a unit would be longer than this many blocks, and than a half
+// of what each of the chip's 768 resident workgroups has to do: the last ones to
+// end then leave a quarter of the chip idle for a quarter of the time at most.
+constexpr int64_t kMinSegment = 16;
+constexpr int64_t kSegments = 2 * 768;
 
 int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* lpl,
                  const int32_t* new_tokens, int32_t batch, int32_t hq, int32_t hkv,
@@ -320,7 +397,7 @@ int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32
                   group <= kMaxGroup,
               KVC_ERR_UNSUPPORTED, "attention weights support head_dim 64, 128, 256, page_size "
                                    "16 and groups up to 128");
-  int64_t most = 0, n = 0, total_kv = 0;
+  int64_t total_kv = 0;
   for (int b = 0; b < batch; ++b) {
     const int64_t q_len = int64_t(qo_indptr[b + 1]) - qo_indptr[b];
     const int64_t pages = int64_t(kv_indptr[b + 1]) - kv_indptr[b];
@@ -335,54 +412,98 @@ int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32
                 "queries must be a request's last cached tokens");
     KVC_REQUIRE(!new_tokens || (new_tokens[b] >= 0 && new_tokens[b] <= kv_len),
                 KVC_ERR_INVALID_ARG, "new_tokens outside the request");
-    most = std::max(most, (q_len * group + kRows - 1) / kRows);
     total_kv += kv_len;
   }
-  const int share = most >= kShareBlocks;
-  const int keys = unit_keys(head_dim, share);
-  KVC_REQUIRE((total_kv / keys + batch) * hkv < (int64_t(1) << 27), KVC_ERR_INVALID_ARG,
+  KVC_REQUIRE((total_kv / kUnitKeys + batch) * hkv < (int64_t(1) << 24), KVC_ERR_INVALID_ARG,
               "too many (key tile, KV head) units");
-  std::vector<int32_t> rec;
+  // Key tiles: (request, first key, row blocks that see it).
+  struct Tile { int b, key0, blocks, new_from; };
+  std::vector<Tile> tiles;
+  int64_t total = 0;
   for (int b = 0; b < batch; ++b) {
     const int q_len = qo_indptr[b + 1] - qo_indptr[b];
     const int pages = kv_indptr[b + 1] - kv_indptr[b];
     const int kv_len = pages > 0 ? (pages - 1) * kPage + lpl[b] : 0;
-    const int nnew = new_tokens ? new_tokens[b] : q_len;
-    if (q_len == 0 && nnew == 0) continue;
+    const int fresh = new_tokens ? new_tokens[b] : q_len;
+    if (q_len == 0 && fresh == 0) continue;
     // Without queries only the new tokens change (to 0).
-    for (int k0 = q_len ? 0 : (kv_len - nnew) / keys * keys; k0 < kv_len; k0 += keys) {
-      const int64_t t0 = causal ? std::max(0, k0 - (kv_len - q_len)) : 0;
-      const int64_t blocks = (std::max<int64_t>(0, q_len - t0) * group + kRows - 1) / kRows;
-      const int32_t r8[kUnitInts] = {b, k0, q_len, kv_len, qo_indptr[b], kv_indptr[b],
-                                     int32_t(blocks), kv_len - nnew};
-      rec.insert(rec.end(), r8, r8 + kUnitInts);
-      ++n;
+    for (int k0 = q_len ? 0 : (kv_len - fresh) / kUnitKeys * kUnitKeys; k0 < kv_len;
+         k0 += kUnitKeys) {
+      const int64_t n = int64_t(q_len - first_token(k0, q_len, kv_len, causal)) * group;
+      const int blocks = q_len ? int((n + kRows - 1) / kRows) : 0;
+      tiles.push_back(Tile{b, k0, blocks, kv_len - fresh});
+      total += blocks;
     }
   }
-  const int64_t W = plan_workgroups(n * hkv);
+  const int64_t seg = std::max(kMinSegment, (total * hkv + kSegments - 1) / kSegments);
+  int64_t n_units = 0, n_parts = 0, n_joins = 0;
+  for (const Tile& t : tiles) {
+    const int64_t k = std::max<int64_t>(1, (t.blocks + seg - 1) / seg);
+    n_units += k * hkv;
+    if (k > 1) {
+      n_parts += k * hkv;
+      n_joins += hkv;
+    }
+  }
+  KVC_REQUIRE(n_units < (int64_t(1) << 26), KVC_ERR_INVALID_ARG, "too many units");
   sched->batch = batch;
   sched->num_qo_heads = hq;
   sched->num_kv_heads = hkv;
   sched->head_dim = head_dim;
   sched->page_size = page_size;
   sched->causal = causal ? 1 : 0;
-  sched->shared_keys = share;
-  sched->num_units = int32_t(n * hkv);
-  sched->num_workgroups = int32_t(W);
+  sched->num_units = int32_t(n_units);
+  sched->num_parts = int32_t(n_parts);
+  sched->num_joins = int32_t(n_joins);
   sched->total_q = batch ? qo_indptr[batch] : 0;
-  sched->plan_ints = unit_table_ints(W) + n * hkv * kUnitInts;
+  sched->plan_ints = n_units * kRecInts + n_joins * kUnitInts;
+  sched->workspace_bytes = n_parts * kUnitKeys * 4;
   KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
               KVC_ERR_WORKSPACE,
               "plan buffer too small: need " + std::to_string(sched->plan_ints) + " int32");
-  write_unit_plan(rec, n, hkv, W, plan_host);
-  // Entry 6, the planner's cost, becomes the request (a unit has keys, so it is the
-  // last one whose pages start at the unit's).
-  int32_t* units = plan_host + unit_table_ints(W);
-  for (int64_t u = 0; u < n * hkv; ++u) {
-    const int32_t off = units[u * kUnitInts + 5];
-    const int32_t* p = std::upper_bound(kv_indptr, kv_indptr + batch, off);
-    units[u * kUnitInts + 6] = int32_t(p - kv_indptr) - 1;
+  // Workgroup w runs on XCD w % 8: a request's units of one head, which read the
+  // same Q and K, go to one XCD (to the one with the least work so far), longest
+  // first in each.
+  typedef std::array<int32_t, kRecInts> Rec;
+  std::vector<Rec> list[8];
+  int64_t load[8] = {0};
+  int32_t* join = plan_host + n_units * kRecInts;
+  int64_t part = 0;
+  for (size_t t0 = 0; t0 < tiles.size();) {
+    size_t t1 = t0;
+    while (t1 < tiles.size() && tiles[t1].b == tiles[t0].b) ++t1;
+    for (int h = 0; h < hkv; ++h) {
+      const int xcd = int(std::min_element(load, load + 8) - load);
+      for (size_t i = t0; i < t1; ++i) {
+        const Tile& t = tiles[i];
+        const int q_len = qo_indptr[t.b + 1] - qo_indptr[t.b];
+        const int kv_len = (kv_indptr[t.b + 1] - kv_indptr[t.b] - 1) * kPage + lpl[t.b];
+        const int k = int(std::max<int64_t>(1, (t.blocks + seg - 1) / seg));
+        for (int j = 0; j < k; ++j) {
+          const int from = int(int64_t(t.blocks) * j / k), to = int(int64_t(t.blocks) * (j + 1) / k);
+          list[xcd].push_back(Rec{h, t.key0, q_len, kv_len, qo_indptr[t.b], kv_indptr[t.b], t.b,
+                                  t.new_from, from, to - from, k > 1 ? int32_t(part + j) : -1, 0});
+          load[xcd] += to - from + 4;
+        }
+        if (k > 1) {
+          const int32_t r8[kUnitInts] = {h, t.key0, k, kv_len, int32_t(part), kv_indptr[t.b], t.b,
+                                         t.new_from};
+          join = std::copy_n(r8, kUnitInts, join);
+          part += k;
+        }
+      }
+    }
+    t0 = t1;
   }
+  size_t most = 0;
+  for (auto& l : list) {
+    std::stable_sort(l.begin(), l.end(), [](const Rec& p, const Rec& q) { return p[9] > q[9]; });
+    most = std::max(most, l.size());
+  }
+  int32_t* dst = plan_host;
+  for (size_t i = 0; i < most; ++i)
+    for (auto& l : list)
+      if (i < l.size()) dst = std::copy_n(l[i].begin(), kRecInts, dst);
   return ok();
 }
 
@@ -421,7 +542,8 @@ extern "C" int kvc_weights_plan(const int32_t* qo_indptr_host, const int32_t* kv
 }
 
 extern "C" int kvc_batch_attention_weights_run(
-    const kvc_weights_schedule* sched, const int32_t* plan, const void* q,
+    const kvc_weights_schedule* sched, const int32_t* plan, void* workspace,
+    int64_t workspace_bytes, const void* q,
     int64_t q_token_stride, const float* lse, const void* key_cache,
     int64_t cache_block_stride, int64_t cache_token_stride, int64_t num_blocks,
     const int32_t* indices, int64_t num_indices, int32_t dtype, float sm_scale, float* scores,
@@ -430,10 +552,10 @@ extern "C" int kvc_batch_attention_weights_run(
   const int Hq = sched->num_qo_heads, Hkv = sched->num_kv_heads, D = sched->head_dim;
   KVC_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= kMaxGroup &&
                   (D == 64 || D == 128 || D == 256) && sched->page_size == kPage &&
-                  sched->num_units >= 0 &&
-                  sched->num_workgroups == plan_workgroups(sched->num_units) &&
-                  sched->plan_ints == unit_table_ints(sched->num_workgroups) +
-                                          int64_t(sched->num_units) * kUnitInts,
+                  sched->num_units >= 0 && sched->num_parts >= 0 && sched->num_joins >= 0 &&
+                  sched->workspace_bytes == int64_t(sched->num_parts) * kUnitKeys * 4 &&
+                  sched->plan_ints == int64_t(sched->num_units) * kRecInts +
+                                          int64_t(sched->num_joins) * kUnitInts,
               KVC_ERR_INVALID_ARG, "schedule not produced by kvc_weights_plan");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
               "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
@@ -441,32 +563,35 @@ extern "C" int kvc_batch_attention_weights_run(
   if (sched->num_units == 0) return ok();
   KVC_REQUIRE(plan && (sched->total_q == 0 || (q && lse)), KVC_ERR_INVALID_ARG, "null pointer");
   KVC_REQUIRE(aligned(plan, 16), KVC_ERR_ALIGNMENT, "plan must be 16-byte aligned");
+  KVC_REQUIRE(sched->num_parts == 0 || (workspace && workspace_bytes >= sched->workspace_bytes),
+              KVC_ERR_WORKSPACE,
+              "workspace too small: need " + std::to_string(sched->workspace_bytes) + " bytes");
+  KVC_REQUIRE(aligned(workspace, 4), KVC_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
   ChunkArgs c;
   c.w = WeightsArgs{static_cast<const uint16_t*>(q), q_token_stride, lse,
                     static_cast<const uint16_t*>(key_cache), cache_block_stride,
                     cache_token_stride, num_blocks, indices, num_indices, Hkv, Hq / Hkv,
                     sm_scale * kLog2e, scores, positions, position_offsets, seq_ids};
   if (const int st = check_common(c.w, Hq, Hkv, D, "kvc_batch_attention_weights_run")) return st;
-  c.wg_units = reinterpret_cast<const int2*>(plan);
-  c.units = reinterpret_cast<const int4*>(plan + unit_table_ints(sched->num_workgroups));
+  c.units = reinterpret_cast<const int4*>(plan);
+  c.parts = static_cast<float*>(workspace);
   c.causal = sched->causal;
-  const dim3 grid(static_cast<unsigned>(sched->num_workgroups));
+  const dim3 grid(static_cast<unsigned>(sched->num_units));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto t, auto share) {
+  auto launch = [&](auto t) {
     typedef decltype(t) T;
-    constexpr bool kS = decltype(share)::value;
-    if (D == 64) weights_chunk_kernel<T, 64, kS><<<grid, kChunkThreads, 0, s>>>(c);
-    else if (D == 128) weights_chunk_kernel<T, 128, kS><<<grid, kChunkThreads, 0, s>>>(c);
-    else weights_chunk_kernel<T, 256, kS><<<grid, kChunkThreads, 0, s>>>(c);
+    if (D == 64) weights_chunk_kernel<T, 64><<<grid, kChunkThreads, 0, s>>>(c);
+    else if (D == 128) weights_chunk_kernel<T, 128><<<grid, kChunkThreads, 0, s>>>(c);
+    else weights_chunk_kernel<T, 256><<<grid, kChunkThreads, 0, s>>>(c);
   };
-  if (dtype == KVC_DTYPE_BF16) {
-    if (sched->shared_keys) launch(Bf16{}, std::true_type{});
-    else launch(Bf16{}, std::false_type{});
-  } else {
-    if (sched->shared_keys) launch(Fp16{}, std::true_type{});
-    else launch(Fp16{}, std::false_type{});
-  }
+  if (dtype == KVC_DTYPE_BF16) launch(Bf16{});
+  else launch(Fp16{});
   KVC_LAUNCH_CHECK();
+  if (sched->num_joins > 0) {
+    weights_join_kernel<<<dim3(unsigned(sched->num_joins)), kUnitKeys, 0, s>>>(
+        c, reinterpret_cast<const int4*>(plan + int64_t(sched->num_units) * kRecInts));
+    KVC_LAUNCH_CHECK();
+  }
   return ok();
 }
 

@@ -60,7 +60,7 @@ class BatchAttentionWeightsWrapper(PlannedRuns):
         elif idx.device != self._device:
             _fail("paged_kv_indices on a different device than the workspace")
         sched = _lib.KvcWeightsSchedule()
-        guess = 1024 + 8 * max(1, num_kv_heads) * (total // 4 + batch)
+        guess = 1024 + 12 * max(1, num_kv_heads) * (total // 16 + 2 * batch)
         plan = stage_plan("kvc_weights_plan", sched,
                           (qo.ctypes.data, kv.ctypes.data, lpl.ctypes.data,
                            None if new is None else new.ctypes.data, batch, num_qo_heads,
@@ -94,8 +94,12 @@ class BatchAttentionWeightsWrapper(PlannedRuns):
             return scores
         sh = self._run_stream(stream)
         plan, indices = self._staged
+        nbytes = int(s.workspace_bytes)
+        with torch.cuda.stream(stream):     # the memory of the stream that uses it
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with torch.cuda.device(dev):
             _lib.call("kvc_batch_attention_weights_run", s, plan.data_ptr(),
+                      ws.data_ptr() if nbytes else None, nbytes,
                       q.data_ptr(), _token_stride(q), lse.data_ptr(), k_cache.data_ptr(),
                       k_cache.stride(0), k_cache.stride(1), k_cache.shape[0],
                       indices.data_ptr(), indices.numel(), _DTYPES[self._dtype],

@@ -630,7 +630,10 @@ int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
  * Chunk form: request b's queries are the last q_len tokens of its kv_len
  * cached ones (rows qo_indptr[b] .. of q and lse), causal as the prefill's or
  * not; its last new_tokens[b] tokens (null: q_len) are new.  kvc_weights_plan is
- * host-only, as kvc_prompt_plan; kvc_batch_attention_weights_run runs it.
+ * host-only, as kvc_prompt_plan; kvc_batch_attention_weights_run runs it with
+ * workspace_bytes of device memory (4-byte aligned, not kept between calls): where
+ * few key tiles have many rows, the rows are cut and the sums joined by a second
+ * kernel.
  * Decode form: one query token per request, its last cached token, which is
  * new; indptr, indices and last_page_len are device arrays as the decode's
  * (at most num_indices pages are read), so that the launch can be captured and
@@ -645,11 +648,12 @@ typedef struct kvc_weights_schedule {
   int32_t head_dim;
   int32_t page_size;
   int32_t causal;
-  int32_t shared_keys;      /* a workgroup's waves share keys, not rows    */
   int32_t num_units;
-  int32_t num_workgroups;
+  int32_t num_parts;        /* partial sums of units whose rows are cut    */
+  int32_t num_joins;
   int32_t total_q;          /* qo_indptr[batch]                            */
   int64_t plan_ints;        /* int32 entries of the plan image             */
+  int64_t workspace_bytes;  /* the partial sums                            */
 } kvc_weights_schedule;
 
 int kvc_weights_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
@@ -661,7 +665,7 @@ int kvc_weights_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_hos
 
 int kvc_batch_attention_weights_run(
     const kvc_weights_schedule* schedule, const int32_t* plan,
-    const void* q, int64_t q_token_stride, const float* lse,
+    void* workspace, int64_t workspace_bytes, const void* q, int64_t q_token_stride, const float* lse,
     const void* key_cache, int64_t cache_block_stride, int64_t cache_token_stride,
     int64_t num_blocks, const int32_t* indices, int64_t num_indices,
     int32_t dtype, float sm_scale, float* scores, int32_t* positions,

@@ -120,9 +120,15 @@ def test_chunk_groups(gpu, hkv, group):
 
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("qlens", [[260, 600], [8, 30]])
-def test_chunk_waves_that_share_keys_and_that_do_not(gpu, d, qlens):
-    *_, w = _chunk(gpu, [700, 600], qlens, 1, 2, d, BF, seed=9)
-    assert w.schedule.shared_keys == (qlens[1] == 600)
+def test_chunk_rows_in_one_piece_and_in_several(gpu, d, qlens):
+    pool, q, lse, w = _chunk(gpu, [700, 600], qlens, 1, 2, d, BF, seed=9)
+    assert (w.schedule.num_parts > 0) == (qlens[1] == 600)
+    # the pieces are joined in the same order every time
+    got = []
+    for _ in range(2):
+        s = torch.zeros_like(pool.scores)
+        got.append(w.run(q, lse, pool.kc, s))
+    assert torch.equal(*got)
 
 
 def test_prompt_whose_last_tokens_vote(gpu):

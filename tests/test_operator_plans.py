@@ -129,27 +129,54 @@ def _weights(lib, qlens, lens, hq, hkv, d, new=None, causal=1, page=16, lpl=None
     return st, s, img, qo, kv
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (6, 2, 64), (7, 1, 256)])
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (6, 2, 64), (7, 1, 256), (128, 1, 64)])
+@pytest.mark.parametrize("causal", [0, 1])
 @pytest.mark.parametrize("qlens,new", [([1, 0, 300, 64, 0, 0, 17], None),
+                                       ([1, 0, 900, 3, 0, 0, 1], [1, 0, 1000, 0, 33, 0, 17]),
                                        ([1, 0, 2, 3, 0, 0, 1], [1, 0, 300, 0, 33, 0, 17])])
-def test_weights_units_cover_every_key_once(lib, hq, hkv, d, qlens, new):
+def test_weights_units_cover_every_key_and_row_once(lib, hq, hkv, d, causal, qlens, new):
+    """Key tiles of 256, their row blocks of 32 in one run or in several, whose
+    partials a join record lists in order."""
     lens = [1, 0, 1000, 64, 200, 0, 17]
-    st, s, img, qo, kv = _weights(lib, qlens, lens, hq, hkv, d, new)
+    st, s, img, qo, kv = _weights(lib, qlens, lens, hq, hkv, d, new, causal)
     assert st == 0
-    tile = 32 * (2 if d == 256 else 4) * (1 if s.shared_keys else 4)
-    seen = set()
-    for h, k0, m, n, q0, p0, b, fresh in _units(s, img).tolist():
-        assert (m, n, q0, p0) == (qlens[b], lens[b], qo[b], kv[b])
-        assert fresh == n - (qlens[b] if new is None else new[b])
-        seen.add((h, b, k0))
-    want = set()
+    n = s.num_units
+    assert s.plan_ints == 12 * n + 8 * s.num_joins
+    assert s.workspace_bytes == s.num_parts * 256 * 4
+    runs, part_of = {}, {}
+    for h, k0, m, ln, q0, p0, b, fresh, first, blocks, part, _ in img[:12 * n].reshape(-1, 12).tolist():
+        assert (m, ln, q0, p0) == (qlens[b], lens[b], qo[b], kv[b])
+        assert fresh == ln - (qlens[b] if new is None else new[b])
+        runs.setdefault((h, b, k0), []).append((first, blocks, part))
+        if part >= 0:
+            assert part not in part_of
+            part_of[part] = (h, b, k0, first)
+    assert sorted(part_of) == list(range(s.num_parts))
+    want = {}
     for h in range(hkv):
-        for b, n in enumerate(lens):
+        for b, ln in enumerate(lens):
             f = qlens[b] if new is None else new[b]
             if qlens[b] or f:
-                want |= {(h, b, k) for k in range(0, n, tile)
-                         if qlens[b] or k + tile > n - f}
-    assert seen == want and s.num_units == len(want)
+                for k in range(0, ln, 256):
+                    if qlens[b] or k + 256 > ln - f:
+                        t = max(0, k - (ln - qlens[b])) if causal else 0
+                        want[h, b, k] = -(-(qlens[b] - t) * (hq // hkv) // 32) if qlens[b] else 0
+    assert set(runs) == set(want)
+    for key, pieces in runs.items():
+        pieces.sort()
+        at = 0
+        for first, blocks, part in pieces:
+            assert first == at and (part >= 0) == (len(pieces) > 1)
+            assert blocks > 0 or len(pieces) == 1
+            at += blocks
+        assert at == want[key]
+    joins = img[12 * n:s.plan_ints].reshape(-1, 8).tolist()
+    assert len(joins) == sum(len(p) > 1 for p in runs.values())
+    for h, k0, k, ln, first, p0, b, fresh in joins:
+        pieces = runs[h, b, k0]
+        assert k == len(pieces) and [p[2] for p in pieces] == list(range(first, first + k))
+        assert ln == lens[b] and p0 == kv[b]
+        assert fresh == ln - (qlens[b] if new is None else new[b])
 
 
 @pytest.mark.parametrize("kw,want", [
@@ -179,8 +206,8 @@ def test_weights_run_refuses(lib):
     def chunk(**kw):
         a = {**ok, **kw}
         return lib.kvc_batch_attention_weights_run(
-            ctypes.byref(s), a["plan"], a["q"], a["qs"], a["lse"], a["k"], a["bs"], a["ts"],
-            a["nb"], a["idx"], a["ni"], a["dt"], ctypes.c_float(a["scale"]), a["sc"], None, None,
+            ctypes.byref(s), a["plan"], None, 0, a["q"], a["qs"], a["lse"], a["k"], a["bs"],
+            a["ts"], a["nb"], a["idx"], a["ni"], a["dt"], ctypes.c_float(a["scale"]), a["sc"], None, None,
             None, None)
 
     def decode(**kw):
@@ -204,6 +231,9 @@ def test_weights_run_refuses(lib):
     assert decode(b=0) == 0 and decode(ni=0) == 0     # nothing to do
     s.plan_ints += 8
     assert chunk() == 1
+    _, s, *_ = _weights(lib, [900], [900], 128, 1, 64)
+    assert s.num_parts > 0 and s.workspace_bytes > 0
+    assert chunk(qs=8192, bs=1024, ts=64) == 4        # no workspace
 
 
 def test_evict_refuses(lib):

@@ -1,5 +1,5 @@
-"""Build-time check of the prompt attention's AMD assembly (built here with
-hipcc): its direct-to-LDS loads take their LDS address from M0, which the inline
+"""Build-time check of the prompt attention's and the attention weights' AMD
+assembly (built here with hipcc): their direct-to-LDS loads take their LDS address from M0, which the inline
 assembly writes and cannot declare clobbered (hipcc reserves M0).  So nothing the
 compiler generates may use M0: every instruction naming M0 is one of the kernel's
 own `s_mov_b32 m0, sN`, directly followed by a direct-to-LDS load, every such load
@@ -15,14 +15,15 @@ from test_prefill_m0 import HIPCC, IMPLICIT_M0, LDS_DMA, ROOT, _instructions
 
 
 @pytest.mark.skipif(not os.access(HIPCC, os.X_OK), reason="hipcc not available")
-def test_only_the_direct_lds_loads_use_m0(tmp_path):
-    out = tmp_path / "prompt.s"
+@pytest.mark.parametrize("source", ["prompt", "weights"])
+def test_only_the_direct_lds_loads_use_m0(tmp_path, source):
+    out = tmp_path / (source + ".s")
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang",
                     "-target-feature", "-Xclang", "-packed-fp32-ops",
                     "-I" + os.path.join(ROOT, "include"),
                     "-I" + os.path.join(ROOT, "gpu_offloading_amd", "csrc"),
                     "--cuda-device-only", "-S",
-                    os.path.join(ROOT, "gpu_offloading_amd", "csrc", "prompt.hip"),
+                    os.path.join(ROOT, "gpu_offloading_amd", "csrc", source + ".hip"),
                     "-o", str(out)], check=True, capture_output=True)
     ins = list(_instructions(out.read_text()))
     set_m0 = re.compile(r"^s_mov_b32 m0, s\d+$")
