@@ -9,7 +9,8 @@
 //
 // evict_select_kernel: a workgroup per (sequence, KV head) ranks its tokens by
 // (recent, score, lower slot first) with a radix select over 32-bit keys and
-// writes the move list.  evict_move_kernel: K, V, score and position of each move.
+// writes the move list.  evict_move_kernel: K, V, score and position of each move,
+// bound by memory (rows of one head, 256 bytes at head_dim 128, from anywhere).
 #include "kvc_common.h"
 
 #include <algorithm>
@@ -17,10 +18,14 @@
 namespace kvc {
 namespace {
 
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
 constexpr int kPage = 16;
-constexpr int kSelectThreads = 512;
-constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kBins = 256;
+constexpr int kBins = 2048;              // 11 bits of the key at a time, then 11 and 10
+// Tokens whose keys are kept in LDS beside the histogram, by the kernel's size;
+// longer sequences read them from memory in every pass.
+constexpr int kShortKeys = 2048, kMiddleKeys = 8192, kLongKeys = 32768;
 constexpr uint32_t kRecentKey = 0xffffffffu, kNanKey = 0xfffffffeu;
 
 struct EvictArgs {
@@ -41,8 +46,8 @@ struct EvictArgs {
   const int32_t* offsets;                         // may be null
   int32_t batch, max_len, max_moves;
   int32_t* counts;                                // [batch][Hkv] moves
-  int32_t* dst;                                   // [batch][Hkv][max_moves] slots
-  int32_t* src;
+  int32_t* dst;                                   // [batch][Hkv][max_moves] token rows of the
+  int32_t* src;                                   // cache (block * 16 + slot), -1: missing
 };
 
 __device__ __forceinline__ const int32_t* table_row(const EvictArgs& a, int b) {
@@ -50,12 +55,13 @@ __device__ __forceinline__ const int32_t* table_row(const EvictArgs& a, int b) {
   return row >= 0 && row < a.table_rows ? a.table + row * a.table_stride : nullptr;
 }
 
-// Index of (slot, head) in the scores, or -1 where the slot's page is missing.
-__device__ __forceinline__ int64_t score_at(const EvictArgs& a, const int32_t* row, int slot,
-                                            int h) {
+// The cache's token row of a slot, or -1 where its page is missing.
+__device__ __forceinline__ int32_t token_row(const EvictArgs& a, const int32_t* row, int slot) {
   const int32_t id = row[slot / kPage];
-  return id >= 0 && id < a.num_blocks
-             ? (int64_t(id) * a.num_kv_heads + h) * kPage + slot % kPage : -1;
+  return id >= 0 && id < a.num_blocks ? id * kPage + slot % kPage : -1;
+}
+__device__ __forceinline__ int64_t score_at(const EvictArgs& a, int32_t token, int h) {
+  return (int64_t(token / kPage) * a.num_kv_heads + h) * kPage + token % kPage;
 }
 
 // Scores as unsigned keys of the same order; -0 is 0, every NaN ranks above inf.
@@ -65,8 +71,9 @@ __device__ __forceinline__ uint32_t score_key(float s) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of v over the workgroup's threads before this one, and over all.
-__device__ __forceinline__ int2 block_scan(int v, int* wave_sums) {
+// Sum of v over the workgroup's threads before this one.
+template <int kThreads>
+__device__ __forceinline__ int block_scan(int v, int* wave_sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
 #pragma unroll
@@ -74,117 +81,313 @@ __device__ __forceinline__ int2 block_scan(int v, int* wave_sums) {
     const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
-  __syncthreads();
   if (lane == 63) wave_sums[wave] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  int before = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) {
-    before += w < wave ? wave_sums[w] : 0;
-    all += wave_sums[w];
-  }
-  return make_int2(before + x - v, all);
+  for (int w = 0; w < kThreads / 64; ++w) before += w < wave ? wave_sums[w] : 0;
+  return before + x - v;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
+// kKeys: tokens whose keys fit in LDS (0: none are kept).  Bound by latency: the loads, the
+// histogram (its atomics meet in few bins where scores are alike; with 11 bits
+// rather than 8 in the first pass a bin is a quarter of a power of two) and three
+// scans of the keys in which each wave counts its own run of slots by ballots.
+template <int kThreads, int kKeys>
+__global__ __launch_bounds__(kThreads) void evict_select_kernel(EvictArgs a) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr bool kLds = kKeys > 0;
+  __shared__ alignas(16) uint32_t lds_keys[kLds ? kKeys : 4];
   __shared__ int hist[kBins];
-  __shared__ int wave_sums[kSelectWaves];
-  __shared__ int found[2];
+  __shared__ int sums[3][kWaves];
+  __shared__ int found[3];
   const int h = blockIdx.x, b = blockIdx.y;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* row = table_row(a, b);
   const int n = row ? min(min(a.seq_lens[b], a.max_len), a.table_width * kPage) : 0;
   const int keep = min(max(a.keep[b], 0), n);
   int* count = a.counts + int64_t(b) * a.num_kv_heads + h;
-  if (n <= keep) {
+  if (n <= keep || keep == 0) {
     if (threadIdx.x == 0) *count = 0;
     return;
   }
   const int offset = a.positions && a.offsets ? a.offsets[b] : 0;
-  const int64_t recent_from = int64_t(n) + offset - max(a.recent[b], 0);
-  auto key_of = [&](int slot) __attribute__((always_inline)) -> uint32_t {
-    const int64_t at = score_at(a, row, slot, h);
-    if (at < 0) return 0u;   // ranks last
-    const int64_t place = a.positions ? a.positions[at] : slot;
-    return place >= recent_from ? kRecentKey : score_key(a.scores[at]);
+  const int32_t recent_from = int32_t(min(max(int64_t(n) + offset - max(a.recent[b], 0),
+                                              int64_t(INT32_MIN)), int64_t(INT32_MAX)));
+  // Keys of four slots of one page from s on (the states' rows of 16 are 64-byte
+  // aligned), given the token row of the first.  Slots at or past n get 0.
+  auto keys_of = [&](int s, int32_t token, f32x4_t f, i32x4_t p) __attribute__((always_inline)) {
+    u32x4_t k;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int32_t place = a.positions ? p[e] : s + e;
+      k[e] = token < 0 || s + e >= n ? 0u   // a missing page's tokens rank last
+             : place >= recent_from  ? kRecentKey : score_key(f[e]);
+    }
+    return k;
+  };
+  auto scores_at = [&](int32_t token) __attribute__((always_inline)) {   // (block 0 if missing)
+    return *reinterpret_cast<const f32x4_t*>(a.scores + score_at(a, max(token, 0), h));
+  };
+  auto places_at = [&](int32_t token) __attribute__((always_inline)) {
+    return a.positions ? *reinterpret_cast<const i32x4_t*>(a.positions +
+                                                           score_at(a, max(token, 0), h))
+                       : i32x4_t{0, 0, 0, 0};
+  };
+  // The pages' first token rows, which the histogram's LDS holds after the selection.
+  constexpr int kPages = kLds ? (kKeys / kPage + kThreads - 1) / kThreads : 1;
+  static_assert(kKeys / kPage <= kBins, "the pages fit where the histogram was");
+  int32_t page[kPages];
+  if (kLds) {
+#pragma unroll
+    for (int i = 0; i < kPages; ++i) {
+      const int s = (i * kThreads + int(threadIdx.x)) * kPage;
+      page[i] = s < n ? token_row(a, row, s) : -1;
+    }
+    constexpr int kBatch = 4;   // page ids, then scores, in flight per thread
+    for (int s0 = 4 * threadIdx.x; s0 < n; s0 += 4 * kThreads * kBatch) {
+      int32_t token[kBatch];
+      f32x4_t f[kBatch];
+      i32x4_t p[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + 4 * kThreads * i;
+        token[i] = s < n ? token_row(a, row, s) : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        f[i] = scores_at(token[i]);
+        p[i] = places_at(token[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + 4 * kThreads * i;
+        if (s < n) *reinterpret_cast<u32x4_t*>(lds_keys + s) = keys_of(s, token[i], f[i], p[i]);
+      }
+    }
+  }
+  auto key4 = [&](int s) __attribute__((always_inline)) {   // s a multiple of 4, below n
+    if (kLds) return *reinterpret_cast<const u32x4_t*>(lds_keys + s);
+    const int32_t token = token_row(a, row, s);
+    return keys_of(s, token, scores_at(token), places_at(token));
+  };
+  auto key = [&](int s) __attribute__((always_inline)) -> uint32_t {
+    if (kLds) return lds_keys[s];
+    const int32_t token = token_row(a, row, s);
+    if (token < 0) return 0u;
+    const int64_t at = score_at(a, token, h);
+    return (a.positions ? a.positions[at] : s) >= recent_from ? kRecentKey
+                                                              : score_key(a.scores[at]);
   };
 
-  // Radix select of the keep-th largest key, 8 bits at a time: `prefix` holds
-  // the key's bits found so far, `want` how many keys with that prefix stay.
+  // Radix select of the keep-th largest key: `prefix` holds its bits found so far,
+  // `want` how many keys with that prefix stay.
   uint32_t prefix = 0;
   int want = keep;
-  for (int shift = 24; want > 0 && shift >= 0; shift -= 8) {
-    if (threadIdx.x < kBins) hist[threadIdx.x] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+    const int shift = kShift[pass];
+    for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
-    for (int s = threadIdx.x; s < n; s += kSelectThreads) {
-      const uint32_t k = key_of(s);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(k >> shift) & 255], 1);
+    const uint32_t mask = (1u << kBits[pass]) - 1;
+    for (int s = 4 * threadIdx.x; s < n; s += 4 * kThreads) {
+      const u32x4_t k = key4(s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // With the prefix taken off, the keys that have it are at most the mask.
+        const uint32_t d = pass == 0 ? k[e] >> shift : (k[e] - prefix) >> shift;
+        if (d <= mask && s + e < n) atomicAdd(&hist[d], 1);
+      }
     }
     __syncthreads();
-    // Keys in larger bins than this thread's: bins are scanned from the top.
-    const int bin = kBins - 1 - int(threadIdx.x);
-    const int c = threadIdx.x < kBins ? hist[bin] : 0;
-    const int above = block_scan(c, wave_sums).x;
-    if (threadIdx.x < kBins && above < want && want <= above + c) {
-      found[0] = bin;
-      found[1] = want - above;
+    // Bins from the top, kBins / kThreads consecutive ones a thread.
+    constexpr int kPer = kBins / kThreads;
+    int c[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      c[i] = hist[kBins - 1 - (kPer * int(threadIdx.x) + i)];
+      mine += c[i];
+    }
+    int above = block_scan<kThreads>(mine, sums[0]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (above < want && want <= above + c[i]) {
+        found[0] = kBins - 1 - (kPer * int(threadIdx.x) + i);
+        found[1] = want - above;
+        found[2] = c[i];
+      }
+      above += c[i];
     }
     __syncthreads();
     prefix |= uint32_t(found[0]) << shift;
     want = found[1];
   }
-  // Keys above `prefix` stay, and the first `want` equal to it by slot.
-  int ties = 0, holes = 0, sources = 0;   // found so far, over the workgroup
+
+  // Keys above `prefix` stay, and the first `want` equal to it by slot: all of them,
+  // mostly.  Wave w has the slots [w run, (w + 1) run).
+  const bool rank_ties = found[2] != want;
+  const int run = (n + 4 * kThreads - 1) / (4 * kThreads) * 256;
+  const int first = min(n, wave * run), last = min(n, first + run);
+  auto below = [&](uint64_t m) __attribute__((always_inline)) {
+    return int(__builtin_amdgcn_mbcnt_hi(uint32_t(m >> 32),
+                                         __builtin_amdgcn_mbcnt_lo(uint32_t(m), 0)));
+  };
+  auto before = [&](const int* x) __attribute__((always_inline)) {
+    int t = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) t += w < wave ? x[w] : 0;
+    return t;
+  };
+  int ties_before = 0;
+  if (rank_ties) {
+    int ties = 0;
+    for (int s0 = first; s0 < last; s0 += 64) {
+      const int s = s0 + lane;
+      ties += __builtin_popcountll(
+          __builtin_amdgcn_ballot_w64(s < last && key(s) == prefix));
+    }
+    if (lane == 0) sums[0][wave] = ties;
+    __syncthreads();
+    ties_before = before(sums[0]);
+  }
+  // The run's holes and sources, 64 slots at a time and kStep of these in flight:
+  // calls put(list, index, slot, mask) where there are any.
   int32_t* dst = a.dst + (int64_t(b) * a.num_kv_heads + h) * a.max_moves;
   int32_t* src = a.src + (int64_t(b) * a.num_kv_heads + h) * a.max_moves;
-  for (int base = 0; base < n; base += kSelectThreads) {
-    const int s = base + threadIdx.x;
-    const uint32_t k = s < n ? key_of(s) : 0u;
-    const bool tie = keep > 0 && s < n && k == prefix;
-    const int2 t = block_scan(tie, wave_sums);
-    const bool stays = keep > 0 && s < n && (k > prefix || (tie && ties + t.x < want));
-    ties += t.y;
-    const bool hole = s < keep && !stays, source = s >= keep && stays;
-    const int2 m = block_scan(hole | (source << 16), wave_sums);
-    if (hole) {
-      const int i = holes + (m.x & 0xffff);
-      if (i < a.max_moves) dst[i] = s;
+  auto walk = [&](int holes, int sources, auto put) __attribute__((always_inline)) {
+    constexpr int kStep = 4;
+    int ties = ties_before;
+    for (int s1 = first; s1 < last; s1 += 64 * kStep) {
+      uint32_t k[kStep];
+#pragma unroll
+      for (int g = 0; g < kStep; ++g) k[g] = key(min(s1 + 64 * g + lane, last - 1));
+#pragma unroll
+      for (int g = 0; g < kStep; ++g) {
+        const int s0 = s1 + 64 * g, s = s0 + lane;
+        if (s0 >= last) break;
+        bool stays = k[g] >= prefix;
+        if (rank_ties) {
+          const uint64_t tie = __builtin_amdgcn_ballot_w64(s < last && k[g] == prefix);
+          stays = k[g] > prefix || (k[g] == prefix && ties + below(tie) < want);
+          ties += __builtin_popcountll(tie);
+        }
+        if (s0 < keep) {
+          const uint64_t m = __builtin_amdgcn_ballot_w64(!stays && s < min(keep, last));
+          put(dst, holes, s, m);
+          holes += __builtin_popcountll(m);
+        }
+        if (s0 + 63 >= keep) {
+          const uint64_t m = __builtin_amdgcn_ballot_w64(stays && s >= keep && s < last);
+          put(src, sources, s, m);
+          sources += __builtin_popcountll(m);
+        }
+      }
     }
-    if (source) {
-      const int i = sources + (m.x >> 16);
-      if (i < a.max_moves) src[i] = s;
-    }
-    holes += m.y & 0xffff;
-    sources += m.y >> 16;
+    return make_int2(holes, sources);
+  };
+  if (kLds) {
+#pragma unroll
+    for (int i = 0; i < kPages; ++i)
+      if (i * kThreads + threadIdx.x < kBins) hist[i * kThreads + threadIdx.x] = page[i];
   }
-  if (threadIdx.x == 0) *count = min(holes, a.max_moves);
+  int2 mine = make_int2(0, 0);
+  if (rank_ties) {
+    mine = walk(0, 0, [](int32_t*, int, int, uint64_t) {});
+  } else {
+    // Four slots a lane, counted in the lane.
+    int low = 0, high = 0;    // tokens that stay below and above `keep`
+    for (int s0 = first; s0 < last; s0 += 256) {
+      const int s = s0 + 4 * lane;
+      if (s >= last) continue;
+      const u32x4_t k = key4(s);
+      if (s0 + 256 <= min(keep, last)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) low += k[e] >= prefix;
+      } else if (s0 >= keep && s0 + 256 <= last) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) high += k[e] >= prefix;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          low += s + e < min(keep, last) && k[e] >= prefix;
+          high += s + e >= keep && s + e < last && k[e] >= prefix;
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) {
+      low += __shfl_xor(low, x);
+      high += __shfl_xor(high, x);
+    }
+    mine = make_int2(max(0, min(keep, last) - first) - low, high);
+  }
+  if (lane == 0) {
+    sums[1][wave] = mine.x;
+    sums[2][wave] = mine.y;
+  }
+  __syncthreads();
+  const int hole0 = before(sums[1]);
+  walk(hole0, before(sums[2]),
+       [&](int32_t* list, int at, int s, uint64_t m) __attribute__((always_inline)) {
+         if (!(m >> lane & 1)) return;
+         if (kLds) {
+           const int32_t token = hist[s / kPage];
+           list[at + below(m)] = token < 0 ? -1 : token + s % kPage;
+         } else {
+           list[at + below(m)] = token_row(a, row, s);
+         }
+       });
+  if (wave == kWaves - 1 && lane == 0) *count = hole0 + mine.x;
 }
 
 constexpr int kMoveThreads = 256;
+constexpr int64_t kMoveWorkgroups = 4096;   // about; each loops over its share
 
+// 2 * row_bytes / 16 threads per move (K's pieces, then V's), kAhead moves of a
+// thread in flight.
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
+  constexpr int kAhead = 4;
   const int h = blockIdx.y % a.num_kv_heads, b = blockIdx.y / a.num_kv_heads;
   const int64_t list = int64_t(b) * a.num_kv_heads + h;
-  const int32_t* row = table_row(a, b);
   const int count = a.counts[list];
-  const int chunks = a.row_bytes / 16;             // 16-byte pieces of a row
-  const int lanes = 2 * chunks;                    // K's pieces, then V's
-  for (int64_t id = int64_t(blockIdx.x) * kMoveThreads + threadIdx.x;
-       id < int64_t(count) * lanes; id += int64_t(gridDim.x) * kMoveThreads) {
-    const int i = int(id / lanes), c = int(id % lanes);
-    const int d = a.dst[list * a.max_moves + i], s = a.src[list * a.max_moves + i];
-    const int64_t db = row[d / kPage], sb = row[s / kPage];
-    if (db < 0 || db >= a.num_blocks || sb < 0 || sb >= a.num_blocks) continue;
-    uint8_t* cache = c < chunks ? a.k_cache : a.v_cache;
-    const int64_t in = int64_t(h) * a.row_bytes + (c % chunks) * 16;
-    *reinterpret_cast<uint4*>(cache + db * a.block_bytes + (d % kPage) * a.token_bytes + in) =
-        *reinterpret_cast<const uint4*>(cache + sb * a.block_bytes +
-                                        (s % kPage) * a.token_bytes + in);
-    if (c == 0) {
-      const int64_t to = (db * a.num_kv_heads + h) * kPage + d % kPage;
-      const int64_t from = (sb * a.num_kv_heads + h) * kPage + s % kPage;
-      a.scores[to] = a.scores[from];
-      if (a.positions) a.positions[to] = a.positions[from];
+  const int32_t* dst = a.dst + list * a.max_moves;
+  const int32_t* src = a.src + list * a.max_moves;
+  const int chunks = a.row_bytes / 16;
+  const int lanes = 2 * chunks;
+  auto row_at = [&](int32_t token, int piece) __attribute__((always_inline)) {
+    return int64_t(token / kPage) * a.block_bytes + int64_t(token % kPage) * a.token_bytes +
+           int64_t(h) * a.row_bytes + (piece < chunks ? piece : piece - chunks) * 16;
+  };
+  const int64_t all = int64_t(count) * lanes, step = int64_t(gridDim.x) * kMoveThreads;
+  for (int64_t id0 = int64_t(blockIdx.x) * kMoveThreads + threadIdx.x; id0 < all;
+       id0 += kAhead * step) {
+    int32_t to[kAhead], from[kAhead];
+    int piece[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t id = id0 + i * step;
+      const int m = id < all ? int(id / lanes) : 0;
+      piece[i] = int(id % lanes);
+      to[i] = id < all ? dst[m] : -1;
+      from[i] = src[m];
+    }
+    u32x4_t x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      // (a move of a missing page reads row 0 and is not stored)
+      const uint8_t* cache = piece[i] < chunks ? a.k_cache : a.v_cache;
+      x[i] = *reinterpret_cast<const u32x4_t*>(cache + row_at(max(from[i], 0), piece[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (to[i] < 0 || from[i] < 0) continue;
+      uint8_t* cache = piece[i] < chunks ? a.k_cache : a.v_cache;
+      *reinterpret_cast<u32x4_t*>(cache + row_at(to[i], piece[i])) = x[i];
+      if (piece[i] == 0) a.scores[score_at(a, to[i], h)] = a.scores[score_at(a, from[i], h)];
+      if (piece[i] == 1 && a.positions)
+        a.positions[score_at(a, to[i], h)] = a.positions[score_at(a, from[i], h)];
     }
   }
 }
@@ -223,6 +426,10 @@ extern "C" int kvc_evict_kv(
   if (batch == 0 || max_seq_len == 0) return ok();
   KVC_REQUIRE(key_cache && value_cache && scores && block_table && seq_lens && keep && recent,
               KVC_ERR_INVALID_ARG, "null pointer");
+  KVC_REQUIRE(num_blocks < (int64_t(1) << 27), KVC_ERR_UNSUPPORTED,
+              "eviction takes caches of fewer than 2^27 blocks");
+  KVC_REQUIRE(aligned(scores, 16) && aligned(positions, 16), KVC_ERR_ALIGNMENT,
+              "scores and positions must be 16-byte aligned");
   KVC_REQUIRE(num_blocks > 0 && block_table_width >= 0 && block_table_width < (1 << 26) &&
                   block_table_rows > 0 && block_table_row_stride >= block_table_width,
               KVC_ERR_INVALID_ARG, "bad num_blocks or block table");
@@ -264,10 +471,20 @@ extern "C" int kvc_evict_kv(
   a.dst = a.counts + pairs;
   a.src = a.dst + pairs * a.max_moves;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  evict_select_kernel<<<dim3(unsigned(num_kv_heads), unsigned(batch)), kSelectThreads, 0, s>>>(a);
+  const dim3 grid{unsigned(num_kv_heads), unsigned(batch)};
+  // Four waves for sequences of up to 2048 tokens, with more of them per CU; sixteen
+  // for longer ones.
+  if (max_seq_len <= kShortKeys)
+    evict_select_kernel<256, kShortKeys><<<grid, 256, 0, s>>>(a);
+  else if (max_seq_len <= kMiddleKeys)
+    evict_select_kernel<1024, kMiddleKeys><<<grid, 1024, 0, s>>>(a);
+  else if (max_seq_len <= kLongKeys)
+    evict_select_kernel<1024, kLongKeys><<<grid, 1024, 0, s>>>(a);
+  else
+    evict_select_kernel<1024, 0><<<grid, 1024, 0, s>>>(a);
   KVC_LAUNCH_CHECK();
   const int64_t per = (int64_t(a.max_moves) * 2 * (row / 16) + kMoveThreads - 1) / kMoveThreads;
-  const int64_t chunks = std::max<int64_t>(1, std::min(per, (4096 + pairs - 1) / pairs));
+  const int64_t chunks = std::max<int64_t>(1, std::min(per, (kMoveWorkgroups + pairs - 1) / pairs));
   evict_move_kernel<<<dim3(unsigned(chunks), unsigned(pairs)), kMoveThreads, 0, s>>>(a);
   KVC_LAUNCH_CHECK();
   return ok();

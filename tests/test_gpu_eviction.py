@@ -323,11 +323,20 @@ def test_evict_ties_infinities_and_nan(gpu):
     assert _evict(gpu, pool, [60, 4, 30], [3, 1, 30], False, None) > 0
 
 
-def test_evict_long_sequences(gpu):
-    """More tokens than one pass of the ranking holds, and thousands of moves."""
-    lens = [9000, 2049]
+@pytest.mark.parametrize("top", [2048, 8192, 32768, 32769])
+@pytest.mark.parametrize("positions", [False, True])
+def test_evict_long_sequences(gpu, top, positions):
+    """Every size of the ranking, at its limit (a larger bound on the lengths, too),
+    and thousands of moves."""
+    lens = [top, 2047]
     pool = Pool(gpu, lens, 1, 64, BF, seed=5)
-    assert _evict(gpu, pool, [3001, 2048], [100, 1], False, None) > 1000
+    for b, n in enumerate(lens):
+        place = torch.randperm(n, generator=torch.Generator().manual_seed(b)).int()
+        pages = torch.tensor(pool.rows[b], device=gpu)
+        pool.positions[pages] = torch.nn.functional.pad(place, (0, -n % 16), value=-1).to(
+            gpu).reshape(-1, 1, 16)
+    assert _evict(gpu, pool, [top // 3 + 1, 2000], [100, 1], positions,
+                  [0, 0] if positions else None) > 400
 
 
 def test_evict_missing_pages_rank_last_and_do_not_move(gpu):

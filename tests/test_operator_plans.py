@@ -254,6 +254,7 @@ def test_evict_refuses(lib):
                       (dict(e=0), 1), (dict(nb=0), 1), (dict(rs=6), 1), (dict(rows=0), 1),
                       (dict(ts=100), 1), (dict(bs=4000), 1), (dict(page=32), 2), (dict(d=60), 2),
                       (dict(b=30000), 2), (dict(k=72), 3), (dict(bs=4100), 3), (dict(ws=None), 4),
-                      (dict(wb=need - 1), 4), (dict(ws=66), 3)):
+                      (dict(wb=need - 1), 4), (dict(ws=66), 3), (dict(sc=72), 3),
+                      (dict(nb=1 << 27), 2)):
         assert run(**bad) == want, bad
     assert run(b=0) == 0 and run(top=0) == 0
