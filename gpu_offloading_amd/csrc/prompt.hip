@@ -560,27 +560,130 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   else run(std::integral_constant<int, 1>{});
 }
 
-// head_dim 256: four waves, one per SIMD, registers for a row's whole O.
+// head_dim 256: O alone is 128 registers of a wave, so four waves, one per SIMD
+// with the whole register file, and no second wave to fill the matrix pipe's
+// gaps: each wave does that itself, a tile ahead.  While it runs the 32 matrix
+// instructions of S_{j+1}^T = K_{j+1} Q^T it does the softmax of S_j between them
+// (about as many cycles), then the 32 of O^T += V_j^T P_j^T.  One barrier per tile:
+// behind it K_{j+1} and V_j are in LDS for all, and the loads of K_{j+2} and
+// V_{j+1} start into the buffers read last before it.
+//
+// x * alpha of an accumulator register.  In plain code the rare rescaling of O would
+// pull all of it into the ordinary registers and back in every tile (256 moves).  At
+// least eight matrix instructions separate it from those that write O before and read
+// it after, more than the wait states that the assembler cannot see to here.
+__device__ __forceinline__ float scale_acc(float x, float alpha) {
+  float t;
+  asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+               : "+a"(x), "=&v"(t) : "v"(alpha));
+  return x;
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves(D), 1) void prompt_wide_kernel(PromptArgs a) {
-  constexpr int kThreads = 64 * kWaves(D);
-  constexpr int kRow = 2 * D;                 // bytes per K or V row
+__global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
+  constexpr int kRow = 2 * D;                  // bytes per K or V row
   constexpr int kChunks = kRow / 16;
-  constexpr int kSteps = D / 16;              // MFMA k-steps of K Q^T
-  constexpr int kBlocks = D / 32;             // 32-dim blocks of O
-  constexpr int kLoads = kKeys * kChunks / kThreads;
+  constexpr int kSteps = D / 16;               // k-steps of S^T
+  constexpr int kBlocks = D / 32;              // 32-dim blocks of O^T
+  constexpr int kTile = kKeys * kRow;
+  constexpr int kDma = 16 * kRow / 1024;       // loads per wave, 16 keys each
+  constexpr int kLaneKeys = 1024 / kRow;       // keys per load
   typedef typename T::x8 x8;
-  __shared__ struct alignas(16) {
-    uint8_t k[kKeys * kRow], v[kKeys * kRow];
+  struct Lds {
+    uint8_t k[2][kTile];
+    uint8_t v[2][kTile];
     int bad[2];
-  } lds;
+  };
+  __shared__ alignas(16) Lds lds;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, r = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63;
+  const int r = lane & 31;
+  const int half = lane >> 5;
   const int row = wave * kWaveRows + r;
   const int row_tok = int(row * a.inv_group >> 16);     // row / group
   const int row_head = row - row_tok * a.group;
   const int Hq = a.num_kv_heads * a.group;
+  if (threadIdx.x < 2) lds.bad[threadIdx.x] = -1;
+
+  const int2 span = a.wg_units[blockIdx.x];
+  const int u_first = __builtin_amdgcn_readfirstlane(span.x);
+  const int u_count = __builtin_amdgcn_readfirstlane(span.y);
+  auto get_unit = [&](int u) __attribute__((always_inline)) {
+    const int4 x = a.units[2 * u], y = a.units[2 * u + 1];
+    auto rfl = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    return Unit{rfl(x.x), rfl(x.y), rfl(x.z), rfl(x.w), rfl(y.x), rfl(y.y), rfl(y.z)};
+  };
+  x8 qb[kSteps];
+  // Rows of no token read the unit's first one; they are never stored.
+  auto load_q = [&](const Unit& U) __attribute__((always_inline)) {
+    const bool there = row_tok < a.tile_tokens && U.tok0 + row_tok < U.q_len;
+    const uint16_t* qp = a.q + int64_t(U.q_off + U.tok0 + (there ? row_tok : 0)) * a.q_stride +
+                         int64_t(U.h * a.group + (there ? row_head : 0)) * D + 8 * half;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks)
+      qb[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
+  };
+
+  // Direct-to-LDS staging as in prompt_kernel, 16 keys a wave.
+  const uint32_t k_bytes = uint32_t(a.k_stride * 2), v_bytes = uint32_t(a.v_stride * 2);
+  uint32_t lane_k[kDma], lane_v[kDma];
+#pragma unroll
+  for (int i = 0; i < kDma; ++i) {
+    const int key = kLaneKeys * i + lane / kChunks;
+    lane_k[i] = key * k_bytes + k_slot<D>(key, lane % kChunks) * 16;
+    lane_v[i] = key * v_bytes + v_slot<D>(key, lane % kChunks) * 16;
+  }
+  auto wait_dma = []() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    asm volatile("" ::: "memory");
+  };
+  auto lds_addr = [](const void* p) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)p));
+  };
+  auto dma = [&](uint8_t* tile, const uint16_t* base, int64_t stride, uint32_t row_bytes,
+                 const uint32_t (&lane_off)[kDma], const Unit& U, int j)
+      __attribute__((always_inline)) {
+    const int key0 = j * kKeys + wave * 16;
+    const int rows = max(0, min(16, U.kv_len - key0));
+    const uint64_t p = reinterpret_cast<uint64_t>(base + (int64_t(U.k_off) + key0) * stride +
+                                                  U.h * D);
+    const int bytes = rows > 0 ? int(uint32_t(rows - 1) * row_bytes + kRow) : 0;
+    const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane(int(uint32_t(p))),
+                          __builtin_amdgcn_readfirstlane(int(uint32_t(p >> 32) & 0xFFFF)),
+                          __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3};
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile + wave * 16 * kRow));
+#pragma unroll
+    for (int i = 0; i < kDma; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to + 1024 * i), "v"(lane_off[i]), "s"(rsrc) : "memory");
+  };
+  auto dma_k = [&](const Unit& U, int j) __attribute__((always_inline)) {
+    dma(lds.k[j & 1], a.k, a.k_stride, k_bytes, lane_k, U, j);
+  };
+  auto dma_v = [&](const Unit& U, int j) __attribute__((always_inline)) {
+    dma(lds.v[j & 1], a.v, a.v_stride, v_bytes, lane_v, U, j);
+  };
+  auto clean_v = [&](const Unit& U, int j, int stamp) __attribute__((always_inline)) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) {
+      const int key = kLaneKeys * i + lane / kChunks;
+      uint4* at = reinterpret_cast<uint4*>(lds.v[j & 1] + wave * 16 * kRow + 1024 * i + 16 * lane);
+      uint4 x = *at;
+      if (j * kKeys + wave * 16 + key >= U.kv_len) {
+        x = make_uint4(0, 0, 0, 0);
+      } else {
+        x.x = finite2<T>(x.x, &bad);
+        x.y = finite2<T>(x.y, &bad);
+        x.z = finite2<T>(x.z, &bad);
+        x.w = finite2<T>(x.w, &bad);
+      }
+      *at = x;
+    }
+    if (bad) lds.bad[stamp & 1] = stamp;
+  };
+
   uint32_t v_rd[kBlocks];
   {
     const int e = (lane >> 2) & 3, q = lane & 3, gp = (lane >> 4) & 1;
@@ -589,139 +692,160 @@ __global__ __launch_bounds__(64 * kWaves(D), 1) void prompt_wide_kernel(PromptAr
       v_rd[db] = (4 * half + e) * kRow +
                  (v_slot<D>(4 * half + e, 4 * db + 2 * gp + (q >> 1)) << 4) + ((q & 1) << 3);
   }
+  auto k_operand = [&](const uint8_t* buf, int i) __attribute__((always_inline)) {
+    return __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
+        buf + (32 * (i & 1) + r) * kRow + (k_slot<D>(r, 2 * (i >> 1) + half) << 4)));
+  };
+  auto v_operand = [&](const uint8_t* buf, int i) __attribute__((always_inline)) {
+    const uint8_t* p = buf + v_rd[i % kBlocks] + (i / kBlocks) * 16 * kRow;
+    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
+    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 8 * kRow));
+    return __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
 
-  const int2 span = a.wg_units[blockIdx.x];
-  for (int u = span.x; u < span.x + span.y; ++u) {
-    const int4 x = a.units[2 * u], y = a.units[2 * u + 1];
-    const int h = x.x, tok0 = x.y, q_len = x.z, kv_len = x.w, ntiles = y.z;
-    const int tok = tok0 + row_tok;
-    const bool row_ok = row_tok < a.tile_tokens && tok < q_len;
-    const int limit = !row_ok ? -1 : a.causal ? min(tok + kv_len - q_len, kv_len - 1) : kv_len - 1;
+  f32x16_t o[kBlocks], s[2], sn[2];
+  uint32_t pw[2][8];
+  const f32x16_t zero = {};
+  constexpr int kS = 2 * kSteps;               // MFMAs of S^T
+  constexpr int kAhead = 4;                    // operands read ahead
+  static_assert(kS >= 24, "the softmax's pieces fit between the score MFMAs");
+
+  Unit cu = get_unit(u_first);
+  load_q(cu);
+  bool staged = false;
+  for (int k = 0; k < u_count; ++k) {
+    const int n = cu.ntiles;
+    const bool has_next = k + 1 < u_count;
+    const Unit nu = has_next ? get_unit(u_first + k + 1) : cu;
+    const int tok = cu.tok0 + row_tok;
+    const bool row_ok = row_tok < a.tile_tokens && tok < cu.q_len;
+    const int limit = !row_ok ? -1
+                      : a.causal ? min(tok + cu.kv_len - cu.q_len, cu.kv_len - 1) : cu.kv_len - 1;
     // Tiles [0, n_full) are seen whole by every row of the unit.
-    const int lim_lo = a.causal ? min(tok0 + kv_len - q_len, kv_len - 1) : kv_len - 1;
-    const int n_full = max(0, min(ntiles, (lim_lo + 1) / kKeys));
-    const uint16_t* kb = a.k + int64_t(y.y) * a.k_stride + h * D;
-    const uint16_t* vb = a.v + int64_t(y.y) * a.v_stride + h * D;
-
-    x8 qb[kSteps];
-    {
-      // Rows of no token read the unit's first one; they are never stored.
-      const uint16_t* qp = a.q + int64_t(y.x + (row_ok ? tok : tok0)) * a.q_stride +
-                           (h * a.group + (row_ok ? row_head : 0)) * D + 8 * half;
-#pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks)
-        qb[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 16 * ks));
-    }
-    f32x16_t o[kBlocks];
-#pragma unroll
-    for (int db = 0; db < kBlocks; ++db)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+    const int lim_lo = a.causal ? min(cu.tok0 + cu.kv_len - cu.q_len, cu.kv_len - 1) : cu.kv_len - 1;
+    const int n_full = max(0, min(n, (lim_lo + 1) / kKeys));
+    // K_0 of the next unit goes into lds.k[0], which the last tile's S_{n} must not
+    // read meanwhile: n odd.
+    const bool early = n > 0 && has_next && nu.ntiles > 0 && (n & 1);
     float m_run = -INFINITY, l_half = 0.f;
-    if (threadIdx.x == 0) lds.bad[u & 1] = 0;
-
-    for (int j = 0; j < ntiles; ++j) {
-      __syncthreads();   // the tiles are free (and `bad` of this unit is set to 0)
-      bool bad = false;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int id = i * kThreads + threadIdx.x, key = id / kChunks, c = id % kChunks;
-        const int t = j * kKeys + key;
-        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-        if (t < kv_len) {
-          kx = *reinterpret_cast<const uint4*>(kb + int64_t(t) * a.k_stride + 8 * c);
-          vx = *reinterpret_cast<const uint4*>(vb + int64_t(t) * a.v_stride + 8 * c);
-        }
-        if (j >= n_full) {
-          // Some row does not see this key: 0 times an inf or NaN must not reach it.
-          vx.x = finite2<T>(vx.x, &bad);
-          vx.y = finite2<T>(vx.y, &bad);
-          vx.z = finite2<T>(vx.z, &bad);
-          vx.w = finite2<T>(vx.w, &bad);
-        }
-        *reinterpret_cast<uint4*>(lds.k + key * kRow + k_slot<D>(key, c) * 16) = kx;
-        *reinterpret_cast<uint4*>(lds.v + key * kRow + v_slot<D>(key, c) * 16) = vx;
+    for (int db = 0; db < kBlocks; ++db) o[db] = zero;
+
+    if (n > 0) {
+      if (!staged) {
+        __syncthreads();        // (the last unit's reads are done)
+        dma_k(cu, 0);
       }
-      if (bad) lds.bad[u & 1] = 1;
+      wait_dma();
       __syncthreads();
+      if (1 < n) dma_k(cu, 1);
+      dma_v(cu, 0);
+      {
+        x8 kop[kS];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) kop[i] = k_operand(lds.k[0], i);
+#pragma unroll
+        for (int i = 0; i < kS; ++i) {
+          if (i + kAhead < kS) kop[i + kAhead] = k_operand(lds.k[0], i + kAhead);
+          s[i & 1] = T::mfma(kop[i], qb[i >> 1], i < 2 ? zero : s[i & 1]);
+        }
+      }
+      // One tile; S of the next one goes to `sn` (behind the last tile that is a
+      // product of whatever the buffer holds, which nothing reads).
+      auto tile = [&](int j, f32x16_t (&s)[2], f32x16_t (&sn)[2]) __attribute__((always_inline)) {
+        wait_dma();
+        if (j >= n_full) clean_v(cu, j, k);
+        __syncthreads();
+        if (j + 2 < n) dma_k(cu, j + 2);
+        if (j + 1 < n) dma_v(cu, j + 1);
+        // The next unit's first K tile: no K tile of this one is read again but the
+        // one in the other buffer.
+        if (j + 1 == n && early) dma_k(nu, 0);
 
-      // S^T = K Q^T: accumulator entry e of key block b is key 32b + 8(e/4) + 4half + e%4
-      // of the tile, for the row of this lane.
-      f32x16_t s[2];
+        if (j >= n_full) {
+          const int rel = limit - j * kKeys - 4 * half;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
-          const int key = 32 * b + r;
-          s[b] = T::mfma(__builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
-                             lds.k + key * kRow + k_slot<D>(key, 2 * ks + half) * 16)),
-                         qb[ks], s[b]);
+            for (int e = 0; e < 16; ++e)
+              s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) <= rel ? s[b][e] : -INFINITY;
         }
-      }
-      if (j >= n_full) {
-        const int rel = limit - j * kKeys - 4 * half;
+        const uint8_t* kb = lds.k[(j + 1) & 1];
+        float mx = -INFINITY, sum = 0.f;
+        x8 kop[kS];
+        auto score = [&](int i) __attribute__((always_inline)) {
+          if (i + kAhead < kS) kop[i + kAhead] = k_operand(kb, i + kAhead);
+          sn[i & 1] = T::mfma(kop[i], qb[i >> 1], i < 2 ? zero : sn[i & 1]);
+        };
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int i = 0; i < kAhead; ++i) kop[i] = k_operand(kb, i);
+        // The maximum between the first MFMAs, the exponentials, two a step, between the
+        // others.
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) <= rel ? s[b][e] : -INFINITY;
-      }
-      float mx = -INFINITY;
+        for (int i = 0; i < 8; ++i) {
+          score(i);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      // The running maximum moves when it grew by more than 2^8; p stays below that.
-      const float cand = fmaxf(m_run, mx * a.scale_log2);
-      if (cand > m_run + kRescaleLog2) {
-        const float alpha = fast_exp2(m_run - cand);
-        m_run = cand;
-        l_half *= alpha;
-#pragma unroll
-        for (int db = 0; db < kBlocks; ++db) o[db] *= alpha;
-      }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
-      uint32_t pw[2][8];
-      float sum = 0.f;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = fast_exp2(fmaf(s[b][e], a.scale_log2, -m_use));
-          const float p1 = fast_exp2(fmaf(s[b][e + 1], a.scale_log2, -m_use));
-          sum += p0 + p1;
-          pw[b][e >> 1] = pack2<T>(p0, p1);
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[i >> 2][4 * (i & 3) + e]);
+          __builtin_amdgcn_sched_barrier(0);
         }
-      l_half += sum;
-      // O^T += V^T P^T: key step st covers keys 16st..+15 in the order that S^T left P in.
+        const auto sw2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx),
+                                                          __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(sw2[0]), __uint_as_float(sw2[1]));
+        const float cand = fmaxf(m_run, mx * a.scale_log2);
+        const bool grow = cand > m_run + kRescaleLog2;
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+          const float alpha = grow ? fast_exp2(m_run - cand) : 1.f;
+          m_run = grow ? cand : m_run;
+          l_half *= alpha;
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const uint32_t* pp = &pw[st >> 1][4 * (st & 1)];
-        const x8 pb = __builtin_bit_cast(x8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
+          for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
-        for (int db = 0; db < kBlocks; ++db) {
-          const uint8_t* p = lds.v + v_rd[db] + st * 16 * kRow;
-          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p));
-          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 8 * kRow));
-          o[db] = T::mfma(__builtin_bit_cast(
-                              x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)),
-                          pb, o[db]);
+            for (int e = 0; e < 16; ++e) o[db][e] = scale_acc(o[db][e], alpha);
         }
+        const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
+#pragma unroll
+        for (int i = 8; i < kS; ++i) {
+          score(i);
+          if (i < 24) {
+            const int b = (i - 8) >> 3, e = 2 * ((i - 8) & 7);
+            const float p0 = fast_exp2(fmaf(s[b][e], a.scale_log2, -m_use));
+            const float p1 = fast_exp2(fmaf(s[b][e + 1], a.scale_log2, -m_use));
+            sum += p0 + p1;
+            pw[b][e >> 1] = pack2<T>(p0, p1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        l_half += sum;
+        constexpr int kN = 4 * kBlocks;
+        const uint8_t* vb = lds.v[j & 1];
+        x8 vop[kN];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) vop[i] = v_operand(vb, i);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          if (i + kAhead < kN) vop[i + kAhead] = v_operand(vb, i + kAhead);
+          const int st = i / kBlocks;
+          const uint32_t* pp = &pw[st >> 1][4 * (st & 1)];
+          const x8 pb = __builtin_bit_cast(x8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
+          o[i % kBlocks] = T::mfma(vop[i], pb, o[i % kBlocks]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      for (int j = 0; j < n; j += 2) {
+        tile(j, s, sn);
+        if (j + 1 < n) tile(j + 1, sn, s);
       }
     }
+    if (has_next) load_q(nu);
 
     const float l = l_half + __shfl_xor(l_half, 32);
     const float inv = l == 0.f ? 0.f : 1.f / l;    // a row that sees no key: 0
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) o[db] *= inv;
-    __syncthreads();
-    if (ntiles > 0 && lds.bad[u & 1]) {
-      // Rows that do see an inf or NaN of the boundary tiles get it: p > 0 times it.
-      for (int t = n_full * kKeys; t < min(ntiles * kKeys, kv_len); ++t) {
-        const uint16_t* vr = vb + int64_t(t) * a.v_stride + 4 * half;
+    if (n > 0 && lds.bad[k & 1] == k) {
+      // p > 0 times an inf or NaN that the row sees.
+      for (int t = n_full * kKeys; t < min(n * kKeys, cu.kv_len); ++t) {
+        const uint16_t* vr = a.v + (int64_t(cu.k_off) + t) * a.v_stride + cu.h * D + 4 * half;
 #pragma unroll
         for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
@@ -734,8 +858,8 @@ __global__ __launch_bounds__(64 * kWaves(D), 1) void prompt_wide_kernel(PromptAr
     }
     if (row_ok) {
       // O^T entry (db, 4i+j) is head dim 32db + 8i + 4half + j of this lane's row.
-      uint16_t* op = a.out + int64_t(y.x + tok) * a.out_stride +
-                     (h * a.group + row_head) * D + 4 * half;
+      uint16_t* op = a.out + int64_t(cu.q_off + tok) * a.out_stride +
+                     int64_t(cu.h * a.group + row_head) * D + 4 * half;
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
@@ -744,9 +868,11 @@ __global__ __launch_bounds__(64 * kWaves(D), 1) void prompt_wide_kernel(PromptAr
               make_uint2(pack2<T>(o[db][4 * i], o[db][4 * i + 1]),
                          pack2<T>(o[db][4 * i + 2], o[db][4 * i + 3]));
       if (a.lse && half == 0)
-        a.lse[int64_t(y.x + tok) * Hq + h * a.group + row_head] =
+        a.lse[int64_t(cu.q_off + tok) * Hq + cu.h * a.group + row_head] =
             l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
     }
+    staged = early;
+    cu = nu;
   }
 }
 
