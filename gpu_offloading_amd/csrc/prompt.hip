@@ -322,35 +322,33 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   float m_run = -INFINITY, l_half = 0.f;
 
   auto mfma_phase = [&](int j, auto do_o_c, auto do_s_c) __attribute__((always_inline)) {
-    if constexpr (decltype(do_o_c)::value) {
-      const uint8_t* vb = lds.v[(j - 1) & 1];
-      constexpr int N = 4 * kBlocks;
-      x8 vop[N];
+    // One run of MFMAs, each operand read kAhead before its own: the first K operands
+    // come in while the last output MFMAs run.
+    constexpr int NO = decltype(do_o_c)::value ? 4 * kBlocks : 0;
+    constexpr int N = NO + (decltype(do_s_c)::value ? 2 * kSteps : 0);
+    constexpr int kAhead = 3;
+    const uint8_t* vb = lds.v[(j - 1) & 1];
+    const uint8_t* kb = lds.k[j & 1];
+    const f32x16_t zero = {};
+    x8 op[N];
+    auto operand = [&](int i) __attribute__((always_inline)) {
+      return i < NO ? v_operand(vb, i) : k_operand(kb, i - NO);
+    };
 #pragma unroll
-      for (int i = 0; i < 3; ++i) vop[i] = v_operand(vb, i);
+    for (int i = 0; i < kAhead; ++i) op[i] = operand(i);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i + 3 < N) vop[i + 3] = v_operand(vb, i + 3);
+    for (int i = 0; i < N; ++i) {
+      if (i + kAhead < N) op[i + kAhead] = operand(i + kAhead);
+      if (i < NO) {
         const int st = i / kBlocks;
         const uint32_t* pp = &pw[st >> 1][4 * (st & 1)];
         const x8 pb = __builtin_bit_cast(x8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
-        o[i % kBlocks] = T::mfma(vop[i], pb, o[i % kBlocks]);
-        __builtin_amdgcn_sched_barrier(0);
+        o[i % kBlocks] = T::mfma(op[i], pb, o[i % kBlocks]);
+      } else {
+        const int m = i - NO;
+        s[m & 1] = T::mfma(op[i], qb[m >> 1], m < 2 ? zero : s[m & 1]);
       }
-    }
-    if constexpr (decltype(do_s_c)::value) {
-      const uint8_t* kb = lds.k[j & 1];
-      constexpr int N = 2 * kSteps;
-      const f32x16_t zero = {};
-      x8 kop[N];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) kop[i] = k_operand(kb, i);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i + 3 < N) kop[i + 3] = k_operand(kb, i + 3);
-        s[i & 1] = T::mfma(kop[i], qb[i >> 1], i < 2 ? zero : s[i & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // X_j.  Accumulator entry e of key block b holds key 32b + 8(e/4) + 4half + e%4
