@@ -30,7 +30,10 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int kWaveRows = 32;                 // query rows per wave
-constexpr int kKeys = 64;                     // keys per tile
+// Keys per tile: at head_dim 64 a tile of 128, whose phases are as long as those of
+// 64 keys at head_dim 128 (with 64 keys the barriers and the phases' starts are a
+// quarter of them).
+constexpr int tile_keys(int head_dim) { return head_dim == 64 ? 128 : 64; }
 constexpr int kMaxGroup = 128;
 // Waves of a workgroup: two per SIMD, or one with the whole register file
 // (head_dim 256: O alone is 128 registers).
@@ -115,7 +118,7 @@ struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles; };
 
 // head_dim 64 and 128: eight waves in two teams of four, one workgroup per CU,
 // two waves per SIMD: wave w of team 0 and wave w of team 1 share SIMD w.  Each
-// team owns 128 query rows and both read the same K/V tiles.  Per 64-key tile a
+// team owns 128 query rows and both read the same K/V tiles.  Per tile of keys a
 // wave has an MFMA phase M_j (O^T += V_{j-1}^T P_{j-1}^T, then S_j^T = K_j Q^T,
 // operands read ahead) and a VALU phase X_j (softmax of S_j into P_j).  Team 1
 // runs one phase behind team 0 and every phase (slot) ends on a workgroup barrier,
@@ -123,7 +126,7 @@ struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles; };
 // exponentials:
 //   slot 2j: team 0 M_j, team 1 X_{j-1};   slot 2j+1: team 0 X_j, team 1 M_j.
 // Team 1 also stages: at the start of slot 2j each of its waves issues the
-// direct-to-LDS loads of its 16 keys of K_{j+1} and V_j (the buffers were last
+// direct-to-LDS loads of its quarter of K_{j+1} and V_j (the buffers were last
 // read in slot 2j-1) and waits for them before the barrier that ends slot 2j+1.
 // A workgroup runs a list of units: while one runs, the next one's record and Q
 // are loaded, and its first K tile is staged in the slot 2n of this one.
@@ -140,9 +143,12 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   constexpr int kChunks = kRow / 16;
   constexpr int kSteps = D / 16;               // k-steps of S^T
   constexpr int kBlocks = D / 32;              // 32-dim blocks of O^T
+  constexpr int kKeys = tile_keys(D);
+  constexpr int KB = kKeys / 32;               // 32-key blocks of S^T
+  constexpr int kWaveKeys = kKeys / 4;         // keys that a wave of team 1 stages
   constexpr int kTile = kKeys * kRow;
   constexpr int kORow = kRow + 16;             // bytes per staged output row
-  constexpr int kDma = 16 * kRow / 1024;       // loads per wave, 16 keys each
+  constexpr int kDma = kWaveKeys * kRow / 1024;   // loads per wave and tile
   constexpr int kLaneKeys = 1024 / kRow;       // keys per load
   typedef typename T::x8 x8;
   // One LDS object with the tiles first: operand reads then use immediate
@@ -159,7 +165,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int team = wave >> 2;
-  const int sw = wave & 3;                     // team 1: the 16 keys of a tile it stages
+  const int sw = wave & 3;                     // team 1: the quarter of a tile it stages
   const int lane = threadIdx.x & 63;
   const int r = lane & 31;
   const int half = lane >> 5;
@@ -209,7 +215,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   x8 qb[kSteps];
   load_q(cu, qb);
 
-  // Direct-to-LDS staging: load i of a wave fetches keys kLaneKeys i .. of its 16,
+  // Direct-to-LDS staging: load i of a wave fetches keys kLaneKeys i .. of its quarter,
   // lane L key kLaneKeys i + L / kChunks, the chunk whose swizzled slot is
   // L % kChunks, at these byte offsets from the wave's first key.
   const uint32_t k_bytes = uint32_t(a.k_stride * 2), v_bytes = uint32_t(a.v_stride * 2);
@@ -236,15 +242,15 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   auto dma = [&](uint8_t* tile, const uint16_t* base, int64_t stride, uint32_t row_bytes,
                  const uint32_t (&lane_off)[kDma], const Unit& U, int j)
       __attribute__((always_inline)) {
-    const int key0 = j * kKeys + sw * 16;
-    const int rows = max(0, min(16, U.kv_len - key0));
+    const int key0 = j * kKeys + sw * kWaveKeys;
+    const int rows = max(0, min(kWaveKeys, U.kv_len - key0));
     const uint64_t p = reinterpret_cast<uint64_t>(base + (int64_t(U.k_off) + key0) * stride +
                                                   U.h * D);
     const int bytes = rows > 0 ? int(uint32_t(rows - 1) * row_bytes + kRow) : 0;
     const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane(int(uint32_t(p))),
                           __builtin_amdgcn_readfirstlane(int(uint32_t(p >> 32) & 0xFFFF)),
                           __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3};
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile + sw * 16 * kRow));
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile + sw * kWaveKeys * kRow));
 #pragma unroll
     for (int i = 0; i < kDma; ++i)
       asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
@@ -256,7 +262,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   auto dma_v = [&](const Unit& U, int j) __attribute__((always_inline)) {
     dma(lds.v[j & 1], a.v, a.v_stride, v_bytes, lane_v, U, j);
   };
-  // A boundary tile's V in LDS (this wave's 16 keys, just staged): inf and NaN
+  // A boundary tile's V in LDS (this wave's keys, just staged): inf and NaN
   // and rows past the sequence become 0, as 0 times them must not reach the rows
   // that do not see them; finish_unit gives them to those that do.
   auto clean_v = [&](int j, int stamp) __attribute__((always_inline)) {
@@ -264,9 +270,9 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 #pragma unroll
     for (int i = 0; i < kDma; ++i) {
       const int key = kLaneKeys * i + lane / kChunks;
-      uint4* at = reinterpret_cast<uint4*>(lds.v[j & 1] + sw * 16 * kRow + 1024 * i + 16 * lane);
+      uint4* at = reinterpret_cast<uint4*>(lds.v[j & 1] + sw * kWaveKeys * kRow + 1024 * i + 16 * lane);
       uint4 x = *at;
-      if (j * kKeys + sw * 16 + key >= cu.kv_len) {
+      if (j * kKeys + sw * kWaveKeys + key >= cu.kv_len) {
         x = make_uint4(0, 0, 0, 0);
       } else {
         x.x = finite2<T>(x.x, &bad);
@@ -287,14 +293,14 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
       v_rd[db] = (4 * half + e) * kRow +
                  (v_slot<D>(4 * half + e, 4 * db + 2 * gp + (q >> 1)) << 4) + ((q & 1) << 3);
   }
-  // Score MFMA i of a tile: k-step i/2 of key block i%2.  Output MFMA i: key step
+  // Score MFMA i of a tile: k-step i / KB of key block i % KB.  Output MFMA i: key step
   // i / kBlocks, head-dim block i % kBlocks; its V^T operand through two transposing
   // reads (ds_read_b64_tr_b16: within 16 lanes, lane j supplies the address of 4
   // consecutive elements and lane i receives element i%4 of the rows supplied
   // by lanes i/4 + {0,4,8,12}).
   auto k_operand = [&](const uint8_t* buf, int i) __attribute__((always_inline)) {
     return __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
-        buf + (32 * (i & 1) + r) * kRow + (k_slot<D>(r, 2 * (i >> 1) + half) << 4)));
+        buf + (32 * (i % KB) + r) * kRow + (k_slot<D>(r, 2 * (i / KB) + half) << 4)));
   };
   auto v_operand = [&](const uint8_t* buf, int i) __attribute__((always_inline)) {
     const uint8_t* p = buf + v_rd[i % kBlocks] + (i / kBlocks) * 16 * kRow;
@@ -303,18 +309,18 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     return __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  f32x16_t o[kBlocks], s[2];
+  f32x16_t o[kBlocks], s[KB];
 #pragma unroll
   for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < KB; ++b)
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
-  uint32_t pw[2][8];
+  uint32_t pw[KB][8];
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < KB; ++b)
 #pragma unroll
     for (int e = 0; e < 8; ++e) pw[b][e] = 0u;
   // m_run: the row's running maximum (base 2, scaled); l_half: the running sum of
@@ -324,8 +330,8 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   auto mfma_phase = [&](int j, auto do_o_c, auto do_s_c) __attribute__((always_inline)) {
     // One run of MFMAs, each operand read kAhead before its own: the first K operands
     // come in while the last output MFMAs run.
-    constexpr int NO = decltype(do_o_c)::value ? 4 * kBlocks : 0;
-    constexpr int N = NO + (decltype(do_s_c)::value ? 2 * kSteps : 0);
+    constexpr int NO = decltype(do_o_c)::value ? 2 * KB * kBlocks : 0;
+    constexpr int N = NO + (decltype(do_s_c)::value ? KB * kSteps : 0);
     constexpr int kAhead = 3;
     const uint8_t* vb = lds.v[(j - 1) & 1];
     const uint8_t* kb = lds.k[j & 1];
@@ -346,7 +352,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
         o[i % kBlocks] = T::mfma(op[i], pb, o[i % kBlocks]);
       } else {
         const int m = i - NO;
-        s[m & 1] = T::mfma(op[i], qb[m >> 1], m < 2 ? zero : s[m & 1]);
+        s[m % KB] = T::mfma(op[i], qb[m / KB], m < KB ? zero : s[m % KB]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -361,16 +367,23 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     if (j >= n_full) {
       const int rel = limit - j * kKeys - 4 * half;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           s[b][e] = 32 * b + 8 * (e >> 2) + (e & 3) <= rel ? s[b][e] : -INFINITY;
     }
-    float mx = -INFINITY;
+    // Four chains: a dependent instruction waits for the one before.
+    float m4[4];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int c = 0; c < 4; ++c) {
+      m4[c] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
+      for (int i = 0; i < 4 * KB; ++i) {
+        const int e = 4 * KB * c + i;
+        m4[c] = fmaxf(m4[c], s[e >> 4][e & 15]);
+      }
+    }
+    float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
     const auto sw2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
                                                       false, false);
     mx = fmaxf(__uint_as_float(sw2[0]), __uint_as_float(sw2[1]));
@@ -384,18 +397,22 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
       for (int db = 0; db < kBlocks; ++db) o[db] *= alpha;
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
-    float sum0 = 0.f, sum1 = 0.f;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8 * KB; ++i) {
       const int b = i >> 3, e = 2 * (i & 7);
       const float p0 = fast_exp2(fmaf(s[b][e], a.scale_log2, -m_use));
       const float p1 = fast_exp2(fmaf(s[b][e + 1], a.scale_log2, -m_use));
-      sum0 += p0;
-      sum1 += p1;
+      sum[2 * (i & 1)] += p0;
+      sum[2 * (i & 1) + 1] += p1;
       pw[b][e >> 1] = pack2<T>(p0, p1);
-      if ((i & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+      if ((i & 3) == 3) {
+        // (the sums here, not behind all exponentials, which would keep every p)
+        asm volatile("" : "+v"(sum[0]), "+v"(sum[1]), "+v"(sum[2]), "+v"(sum[3]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    l_half += sum0 + sum1;
+    l_half += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
 
   // The unit's rows leave through the wave's LDS staging: a lane holds 8-byte
@@ -583,6 +600,7 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
   constexpr int kChunks = kRow / 16;
   constexpr int kSteps = D / 16;               // k-steps of S^T
   constexpr int kBlocks = D / 32;              // 32-dim blocks of O^T
+  constexpr int kKeys = tile_keys(D);
   constexpr int kTile = kKeys * kRow;
   constexpr int kDma = 16 * kRow / 1024;       // loads per wave, 16 keys each
   constexpr int kLaneKeys = 1024 / kRow;       // keys per load
@@ -890,7 +908,7 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
   KVC_REQUIRE((head_dim == 64 || head_dim == 128 || head_dim == 256) && group <= kMaxGroup,
               KVC_ERR_UNSUPPORTED,
               "prompt attention supports head_dim 64, 128, 256 and groups up to 128");
-  const int tile_tokens = tile_rows(head_dim) / group;
+  const int tile_tokens = tile_rows(head_dim) / group, per_tile = tile_keys(head_dim);
   std::vector<int32_t> rec;
   int max_tiles = 0;
   int64_t end_q = 0, end_kv = 0, items = 0;
@@ -911,7 +929,7 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
       const int64_t last = std::min<int64_t>(t0 + tile_tokens, q_len) - 1;
       int64_t keys = causal ? last + kv_len - q_len + 1 : kv_len;
       keys = std::max<int64_t>(0, std::min<int64_t>(keys, kv_len));
-      const int tiles = int((keys + kKeys - 1) / kKeys);
+      const int tiles = int((keys + per_tile - 1) / per_tile);
       max_tiles = std::max(max_tiles, tiles);
       const int32_t r8[kUnitInts] = {b, int32_t(t0), int32_t(q_len), int32_t(kv_len),
                                      qo_indptr[b], kv_indptr[b], tiles, 0};

@@ -595,7 +595,7 @@ typedef struct kvc_prompt_schedule {
   int32_t num_workgroups;
   int32_t total_q;          /* qo_indptr[batch]                            */
   int32_t total_kv;         /* kv_indptr[batch]                            */
-  int32_t max_key_tiles;    /* most 64-key tiles one unit visits           */
+  int32_t max_key_tiles;    /* most key tiles one unit visits              */
   int32_t reserved;
   int64_t plan_ints;        /* int32 entries of the plan image             */
 } kvc_prompt_schedule;
