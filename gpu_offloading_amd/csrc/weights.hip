@@ -299,79 +299,160 @@ struct TokenArgs {
   int32_t batch;
 };
 
-constexpr int kTokenPages = 4;     // pages of one head per wave and step
 constexpr int kTokenThreads = 256;
-constexpr int64_t kTokenWorkgroups = 4096;   // at most; waves take further tasks in turn
+constexpr int64_t kTokenWorkgroups = 512;   // two per CU: what its registers hold
 
-// A wave takes kTokenPages consecutive entries of the batch's page list for one
-// KV head (heads fastest: neighbouring waves read the same tokens' rows).  S =
-// Q K^T per page with v_mfma_f32_16x16x32 (A: lane l = row l%16, k = 8(l/16)..+7;
-// B: column l%16; C: acc[j] = row 4(l/16)+j, column l%16): rows are the group's
-// query heads, columns the page's tokens.
+// A wave runs a range of tasks; a task is kPages consecutive entries of the batch's
+// page list for one KV head (heads fastest: neighbouring tasks read the same tokens'
+// rows).  Bound by memory: a task's K (16 KB), old scores and query are loaded
+// while the one before is computed, its page ids a task earlier still.  S = Q K^T per
+// page with v_mfma_f32_16x16x32 (A: lane l = row l%16, k = 8(l/16)..+7; B: column
+// l%16; C: acc[j] = row 4(l/16)+j, column l%16): rows are the group's query heads,
+// columns the page's tokens.  Lane 16 i + r then owns token r of page i.
 template <typename T, int D>
-__global__ __launch_bounds__(kTokenThreads) void weights_token_kernel(TokenArgs c) {
+__global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenArgs c) {
   constexpr int kSteps = D / 32;
+  constexpr int kPages = 512 / D;             // 64 registers of K
+  constexpr int kSets = (kPages + 3) / 4;     // of four pages, a quarter wave each
   typedef typename T::x8 x8;
   const WeightsArgs& a = c.w;
   const int lane = threadIdx.x & 63, r = lane & 15, quad = lane >> 4;
   const int Hq = a.num_kv_heads * a.group;
   const int64_t pages = min(int64_t(c.indptr[c.batch]), a.num_indices);
-  const int64_t tasks = (pages + kTokenPages - 1) / kTokenPages * a.num_kv_heads;
+  const int64_t tasks = (pages + kPages - 1) / kPages * a.num_kv_heads;
   const int64_t waves = int64_t(gridDim.x) * (kTokenThreads / 64);
-  for (int64_t task = int64_t(blockIdx.x) * (kTokenThreads / 64) +
-                      __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-       task < tasks; task += waves) {
-    const int h = int(task % a.num_kv_heads);
-    const int64_t p0 = task / a.num_kv_heads * kTokenPages;
-    int32_t block[kTokenPages];
-    x8 kop[kTokenPages][kSteps];
+  const int64_t wave = int64_t(blockIdx.x) * (kTokenThreads / 64) +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t1 = tasks * (wave + 1) / waves;
+  int64_t t = tasks * wave / waves;
+  if (t >= t1) return;
+  // The first 64 requests' ends; others are read where a page may be theirs.
+  const int end0 = lane < c.batch ? c.indptr[lane + 1] : INT32_MAX;
+
+  struct Task { int h; int64_t p0; };
+  auto task_of = [&](int64_t i) __attribute__((always_inline)) {
+    const int64_t g = i / a.num_kv_heads;
+    return Task{int(i - g * a.num_kv_heads), g * kPages};
+  };
+  // Lane i < kPages: page i's id as in the list (the last one's past its end).
+  auto load_ids = [&](const Task& k) __attribute__((always_inline)) {
+    return a.indices[min(k.p0 + lane % kPages, pages - 1)];
+  };
+  // The request of a page: the first whose pages end behind it (uniform).
+  auto request_of = [&](int64_t p) __attribute__((always_inline)) {
+    int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end0 <= p));
+    for (int base = 64; b == base && base < c.batch; base += 64) {
+      const int at = base + lane;
+      b += __builtin_popcountll(
+          __builtin_amdgcn_ballot_w64(at < c.batch && c.indptr[at + 1] <= p));
+    }
+    return b;
+  };
+  struct Loaded {
+    x8 k[kPages][kSteps];
+    x8 q[kSteps];          // the first 16 query heads of the first page's request
+    float lse[4];          // and the lane's four rows' lse
+    float old[kSets];      // the lane's tokens' scores
+    int32_t block[kSets];  // the lane's pages' blocks, -1: missing or past the list
+    int b;                 // request of the first page
+  };
+  auto load_q = [&](int b, int h, int g0, x8 (&q)[kSteps], float (&lse)[4])
+      __attribute__((always_inline)) {
+    const int n = min(16, a.group - g0);
+    const uint16_t* qp = a.q + int64_t(b) * a.q_stride +
+                         (int64_t(h) * a.group + g0 + min(r, n - 1)) * D + 8 * quad;
 #pragma unroll
-    for (int i = 0; i < kTokenPages; ++i) {
-      block[i] = p0 + i < pages ? __builtin_amdgcn_readfirstlane(block_of(a, p0 + i)) : -1;
-      const uint16_t* kp = a.k_cache + int64_t(max(block[i], 0)) * a.block_stride +
-                           r * a.token_stride + h * D + 8 * quad;
+    for (int ks = 0; ks < kSteps; ++ks)
+      q[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 32 * ks));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      lse[j] = a.lse[int64_t(b) * Hq + h * a.group + g0 + min(4 * quad + j, n - 1)];
+  };
+  auto load = [&](const Task& k, int32_t ids, Loaded& x) __attribute__((always_inline)) {
+    const int32_t id = uint64_t(ids) < uint64_t(a.num_blocks) ? ids : -1;
+#pragma unroll
+    for (int i = 0; i < kPages; ++i) {
+      const int32_t blk = max(__builtin_amdgcn_readlane(id, i), 0);   // (block 0 if missing)
+      const uint16_t* kp = a.k_cache + int64_t(blk) * a.block_stride + k.h * D +
+                           r * a.token_stride + 8 * quad;
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks)
-        kop[i][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 32 * ks));
+        x.k[i][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 32 * ks));
     }
 #pragma unroll
-    for (int i = 0; i < kTokenPages; ++i) {
-      if (block[i] < 0) continue;
-      // The request: the last one whose pages start at or before this one.
-      const int64_t p = p0 + i;
-      int b = 0;
-      for (int base = 0; base < c.batch; base += 64) {
-        const int at = base + lane;
-        const bool before = at < c.batch && c.indptr[at + 1] <= p;
-        b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
-      }
-      if (b >= c.batch) continue;
-      const int first = c.indptr[b], last = c.indptr[b + 1] - 1;
-      const int tokens = p < last ? kPage : c.last_page_len[b];
-      float w = 0.f;
-      for (int g0 = 0; g0 < a.group; g0 += 16) {
-        const int n = min(16, a.group - g0);
-        const int64_t qh = int64_t(h) * a.group + g0 + min(r, n - 1);
-        const uint16_t* qp = a.q + b * a.q_stride + qh * D + 8 * quad;
-        f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kSets; ++i) {
+      const int page = 4 * i + quad;
+      const int32_t blk = __shfl(id, page);
+      x.block[i] = page < kPages && k.p0 + page < pages ? blk : -1;
+      x.old[i] = a.scores[(int64_t(max(x.block[i], 0)) * a.num_kv_heads + k.h) * kPage + r];
+    }
+    x.b = min(request_of(k.p0), c.batch - 1);
+    load_q(x.b, k.h, 0, x.q, x.lse);
+  };
+
+  Task now = task_of(t), next = task_of(min(t + 1, t1 - 1));
+  Loaded x;
+  load(now, load_ids(now), x);
+  int32_t ids = load_ids(next);
+  for (; t < t1; ++t) {
+    Loaded y;
+    Task after = next;
+    if (t + 1 < t1) {
+      load(next, ids, y);
+      after = task_of(min(t + 2, t1 - 1));
+      ids = load_ids(after);
+    }
+    int b = x.b;
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks)
-          s = T::mfma16(__builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(qp + 32 * ks)),
-                        kop[i][ks], s);
+    for (int set = 0; set < kSets; ++set) {
+      float mine = 0.f;
+      bool fresh = false, in = false;
+      int key = 0, request = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = 4 * quad + j;
-          const float lse = a.lse[int64_t(b) * Hq + h * a.group + g0 + min(row, n - 1)];
-          const float e = fast_exp2(fmaf(s[j], a.scale_log2, lse * -kLog2e));
-          w += row < n && lse != -INFINITY ? e : 0.f;
+      for (int i = 4 * set; i < min(kPages, 4 * set + 4); ++i) {
+        const int64_t p = now.p0 + i;
+        if (p >= pages) continue;
+        if (p >= c.indptr[b + 1]) {       // this page is another request's
+          b = request_of(p);
+          if (b >= c.batch) break;
+          load_q(b, now.h, 0, x.q, x.lse);
+        }
+        const int first = c.indptr[b], last = c.indptr[b + 1] - 1;
+        const int tokens = p < last ? kPage : c.last_page_len[b];
+        float w = 0.f;
+        for (int g0 = 0; g0 < a.group; g0 += 16) {
+          if (g0 > 0) load_q(b, now.h, g0, x.q, x.lse);
+          f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < kSteps; ++ks) s = T::mfma16(x.q[ks], x.k[i][ks], s);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = fast_exp2(fmaf(s[j], a.scale_log2, x.lse[j] * -kLog2e));
+            w += 4 * quad + j < a.group - g0 && x.lse[j] != -INFINITY ? e : 0.f;
+          }
+        }
+        if (a.group > 16) load_q(b, now.h, 0, x.q, x.lse);   // for the next page
+        w += __shfl_xor(w, 16);
+        w += __shfl_xor(w, 32);
+        if (quad == i - 4 * set) {
+          mine = w;
+          in = r < tokens;
+          fresh = p == last && r == tokens - 1;
+          key = int(p - first) * kPage + r;
+          request = b;
         }
       }
-      w += __shfl_xor(w, 16);
-      w += __shfl_xor(w, 32);
-      const int key = int(p - first) * kPage + r;
-      if (quad == 0 && r < tokens)
-        store_weight(a, block[i], h, key, b, w, p == last && r == tokens - 1);
+      if (in && x.block[set] >= 0) {
+        const int64_t at = (int64_t(x.block[set]) * a.num_kv_heads + now.h) * kPage + r;
+        a.scores[at] = fresh ? mine : x.old[set] + mine;
+        if (fresh && a.positions)
+          a.positions[at] =
+              key + (a.offsets ? a.offsets[a.seq_ids ? a.seq_ids[request] : request] : 0);
+      }
     }
+    x = y;
+    now = next;
+    next = after;
   }
 }
 
@@ -623,7 +704,7 @@ extern "C" int kvc_decode_attention_weights(
   c.indptr = indptr;
   c.last_page_len = last_page_len;
   c.batch = batch;
-  const int64_t tasks = (num_indices + kTokenPages - 1) / kTokenPages * Hkv;
+  const int64_t tasks = (num_indices + 512 / D - 1) / (512 / D) * Hkv;
   const int64_t wgs = (tasks + kTokenThreads / 64 - 1) / (kTokenThreads / 64);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(wgs, kTokenWorkgroups)));
   hipStream_t s = static_cast<hipStream_t>(stream);
