@@ -324,6 +324,23 @@ def call(name: str, *args) -> int:
     return st
 
 
+def call_on(index: int, name: str, *args) -> int:
+    """``call`` with GPU ``index`` current (a kernel is launched on the current
+    one), which it is already in nearly every call."""
+    global _get_device
+    if _get_device is None:
+        import torch
+        _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    if _get_device() == index:
+        return call(name, *args)
+    import torch
+    with torch.cuda.device(index):
+        return call(name, *args)
+
+
+_get_device = None
+
+
 def current_stream_handle(device) -> int:
     """hipStream_t (as an int) of torch's current stream on ``device``:
     torch's raw-stream query when it has one (no Stream object is built),

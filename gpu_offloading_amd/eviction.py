@@ -14,10 +14,9 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .ops import check_scores
+from .ops import _ptr, check_scores
 from .prefill import _fail, _host_int32
-from .prompt import (_DTYPES, PlannedRuns, _check_rows, _dtype, _scale, _token_stride,
-                     stage_plan)
+from .prompt import _DTYPES, PlannedRuns, _dtype, _empty, _scale, check_rows, stage_plan
 
 __all__ = ["BatchAttentionWeightsWrapper"]
 
@@ -87,24 +86,19 @@ class BatchAttentionWeightsWrapper(PlannedRuns):
         s = self._sched
         if s is None:
             _fail("run() called before plan()")
-        _check_rows("q", q, s.total_q, s.num_qo_heads, s.head_dim, self._dtype, self._device)
-        dev = check_scores(q, lse, s.total_q, s.num_qo_heads, k_cache, s.num_kv_heads, s.head_dim,
-                           scores, positions, position_offsets, seq_ids, s.batch)
+        dev = self._index
+        qs = check_rows("q", q, s.total_q, s.num_qo_heads, s.head_dim, self._dtype, dev)
+        cs = check_scores(dev, q.dtype, lse, s.total_q, s.num_qo_heads, k_cache, s.num_kv_heads,
+                          s.head_dim, scores, positions, position_offsets, seq_ids, s.batch)
         if s.num_units == 0:
             return scores
         sh = self._run_stream(stream)
-        plan, indices = self._staged
-        nbytes = int(s.workspace_bytes)
-        with torch.cuda.stream(stream):     # the memory of the stream that uses it
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with torch.cuda.device(dev):
-            _lib.call("kvc_batch_attention_weights_run", s, plan.data_ptr(),
-                      ws.data_ptr() if nbytes else None, nbytes,
-                      q.data_ptr(), _token_stride(q), lse.data_ptr(), k_cache.data_ptr(),
-                      k_cache.stride(0), k_cache.stride(1), k_cache.shape[0],
-                      indices.data_ptr(), indices.numel(), _DTYPES[self._dtype],
-                      self._sm_scale, scores.data_ptr(),
-                      None if positions is None else positions.data_ptr(),
-                      None if position_offsets is None else position_offsets.data_ptr(),
-                      None if seq_ids is None else seq_ids.data_ptr(), sh)
+        indices, nbytes, ws = self._staged[1], s.workspace_bytes, None
+        if nbytes:
+            ws = _empty(nbytes, torch.uint8, self._device, stream)
+        _lib.call_on(dev, "kvc_batch_attention_weights_run", s, self._plan_ptr,
+                     None if ws is None else ws.data_ptr(), nbytes, q.data_ptr(), qs,
+                     lse.data_ptr(), k_cache.data_ptr(), cs[0], cs[1], k_cache.shape[0],
+                     indices.data_ptr(), indices.numel(), _DTYPES[self._dtype], self._sm_scale,
+                     scores.data_ptr(), _ptr(positions), _ptr(position_offsets), _ptr(seq_ids), sh)
         return scores

@@ -636,38 +636,45 @@ def paged_attention_v2(out: torch.Tensor, exp_sums: torch.Tensor, max_logits: to
 _WDTYPES = {torch.float16: 0, torch.bfloat16: 1}     # KVC_DTYPE_* of include/kvc.h
 
 
-def _check_state(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, blocks: int,
-                 heads: int) -> None:
-    if t is not None and (t.dtype is not dtype or tuple(t.shape) != (blocks, heads, 16)
-                          or not t.is_contiguous()):
-        _fail(f"{name} must be contiguous {dtype} [{blocks}, {heads}, 16]")
+def _check_state(name: str, t: torch.Tensor, dtype: torch.dtype, blocks: int, heads: int,
+                 device: int) -> None:
+    if t.dtype is not dtype or t.shape != (blocks, heads, 16) or not t.is_contiguous() \
+            or t.get_device() != device:
+        _fail(f"{name} must be contiguous {dtype} [{blocks}, {heads}, 16] on cuda:{device}, got "
+              f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _check_ints(name: str, t: Optional[torch.Tensor], n: int) -> None:
-    if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or t.numel() < n
-                          or not t.is_contiguous()):
-        _fail(f"{name} must be a contiguous 1-D int32 tensor of at least {n} entries")
+def _check_ints(name: str, t: torch.Tensor, n: int, device: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() < n or not t.is_contiguous() \
+            or t.get_device() != device:
+        _fail(f"{name} must be a contiguous 1-D int32 tensor of at least {n} entries on "
+              f"cuda:{device}")
 
 
-def check_scores(q: torch.Tensor, lse: torch.Tensor, rows: int, hq: int, k_cache: torch.Tensor,
-                 hkv: int, dim: int, scores: torch.Tensor, positions: Optional[torch.Tensor],
-                 position_offsets: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor],
-                 batch: int) -> torch.device:
-    """The checks that the chunk and decode forms of the attention weights share."""
-    dev = _check_cuda(q, lse, k_cache, scores, positions, position_offsets, seq_ids)
-    shape, _ = _check_cache(k_cache, "k_cache")
-    if tuple(shape[1:]) != (16, hkv, dim):
+def check_scores(device: int, dtype: torch.dtype, lse: torch.Tensor, rows: int, hq: int,
+                 k_cache: torch.Tensor, hkv: int, dim: int, scores: torch.Tensor,
+                 positions: Optional[torch.Tensor], position_offsets: Optional[torch.Tensor],
+                 seq_ids: Optional[torch.Tensor], batch: int):
+    """The checks that the chunk and decode forms of the attention weights share;
+    returns the cache's strides."""
+    shape, st = _check_cache(k_cache, "k_cache")
+    if shape[1] != 16 or shape[2] != hkv or shape[3] != dim:
         _fail(f"k_cache must be [blocks, 16, {hkv}, {dim}], got {tuple(shape)}")
-    if k_cache.dtype is not q.dtype:
-        _fail(f"dtype mismatch: q {q.dtype} vs cache {k_cache.dtype}")
-    if lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.dim() != 2 \
-            or lse.shape[0] < rows or lse.shape[1] != hq:
-        _fail(f"lse must be contiguous float32 [{rows}, {hq}]")
-    _check_state("scores", scores, torch.float32, shape[0], hkv)
-    _check_state("positions", positions, torch.int32, shape[0], hkv)
-    _check_ints("seq_ids", seq_ids, batch)
-    _check_ints("position_offsets", position_offsets, 0 if seq_ids is not None else batch)
-    return dev
+    if k_cache.dtype is not dtype or k_cache.get_device() != device:
+        _fail(f"k_cache must be {dtype} on cuda:{device} as q, got {k_cache.dtype} on "
+              f"{k_cache.device}")
+    if lse.dtype is not torch.float32 or lse.dim() != 2 or lse.shape[0] < rows \
+            or lse.shape[1] != hq or not lse.is_contiguous() or lse.get_device() != device:
+        _fail(f"lse must be contiguous float32 [{rows}, {hq}] on cuda:{device}")
+    _check_state("scores", scores, torch.float32, shape[0], hkv, device)
+    if positions is not None:
+        _check_state("positions", positions, torch.int32, shape[0], hkv, device)
+    if seq_ids is not None:
+        _check_ints("seq_ids", seq_ids, batch, device)
+    if position_offsets is not None:
+        _check_ints("position_offsets", position_offsets, 0 if seq_ids is not None else batch,
+                    device)
+    return st
 
 
 def decode_attention_weights(q: torch.Tensor, lse: torch.Tensor, key_cache: torch.Tensor,
@@ -691,31 +698,32 @@ def decode_attention_weights(q: torch.Tensor, lse: torch.Tensor, key_cache: torc
     as ``scores``) gets the last token's position, its slot in the sequence plus
     ``position_offsets[seq_ids[b]]`` (``seq_ids`` defaults to b).  Returns
     ``scores``."""
-    if q.dim() != 3:
-        _fail(f"q must be [requests, num_qo_heads, head_dim], got {tuple(q.shape)}")
-    if q.dtype not in _WDTYPES:
+    if not q.is_cuda:
+        _fail(f"expected a GPU tensor, got one on {q.device}")
+    dev, shape, st = q.get_device(), q.shape, q.stride()
+    if len(shape) != 3:
+        _fail(f"q must be [requests, num_qo_heads, head_dim], got {tuple(shape)}")
+    dt = _WDTYPES.get(q.dtype)
+    if dt is None:
         _fail(f"only bfloat16 and float16 are supported, got {q.dtype}")
+    batch, hq, d = shape
+    if d > 0 and (st[2] != 1 or (hq > 1 and st[1] != d)):
+        _fail("q: the heads of a request must be contiguous")
     if key_cache.dim() != 4:
         _fail(f"key_cache must be [blocks, 16, heads, dim], got {tuple(key_cache.shape)}")
-    batch, hq, d = q.shape
     hkv = key_cache.shape[2]
-    if d > 0 and (q.stride(2) != 1 or (hq > 1 and q.stride(1) != d)):
-        _fail("q: the heads of a request must be contiguous")
-    _check_ints("indptr", indptr, batch + 1)
-    _check_ints("indices", indices, 0)
-    _check_ints("last_page_len", last_page_len, batch)
-    check_scores(q, lse, batch, hq, key_cache, hkv, d, scores, positions, position_offsets,
-                 seq_ids, batch)
-    dev = _check_cuda(q, indptr, indices, last_page_len)
-    scale = float(sm_scale) if sm_scale is not None else d ** -0.5
-    with torch.cuda.device(dev):
-        _lib.call("kvc_decode_attention_weights", q.data_ptr(),
-                  q.stride(0) if batch > 1 else hq * d, lse.data_ptr(),
-                  key_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1),
-                  key_cache.shape[0], indptr.data_ptr(), indices.data_ptr(), indices.numel(),
-                  last_page_len.data_ptr(), batch, hq, hkv, d, key_cache.shape[1],
-                  _WDTYPES[q.dtype], scale, scores.data_ptr(), _ptr(positions),
-                  _ptr(position_offsets), _ptr(seq_ids), _stream_handle(dev, stream))
+    _check_ints("indptr", indptr, batch + 1, dev)
+    _check_ints("indices", indices, 0, dev)
+    _check_ints("last_page_len", last_page_len, batch, dev)
+    cs = check_scores(dev, q.dtype, lse, batch, hq, key_cache, hkv, d, scores, positions,
+                      position_offsets, seq_ids, batch)
+    _lib.call_on(dev, "kvc_decode_attention_weights", q.data_ptr(),
+                 st[0] if batch > 1 else hq * d, lse.data_ptr(), key_cache.data_ptr(), cs[0],
+                 cs[1], key_cache.shape[0], indptr.data_ptr(), indices.data_ptr(),
+                 indices.numel(), last_page_len.data_ptr(), batch, hq, hkv, d, 16, dt,
+                 float(sm_scale) if sm_scale is not None else d ** -0.5, scores.data_ptr(),
+                 _ptr(positions), _ptr(position_offsets), _ptr(seq_ids),
+                 _stream_handle(q.device, stream))
     return scores
 
 
@@ -750,31 +758,36 @@ def evict_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: torch.T
             or key_cache.dtype is not value_cache.dtype:
         _fail("key_cache and value_cache must have the same shape, strides and dtype")
     nb, bs, h, d = shape
-    _check_state("scores", scores, torch.float32, nb, h)
-    _check_state("positions", positions, torch.int32, nb, h)
+    index = key_cache.get_device()
+    _check_state("scores", scores, torch.float32, nb, h, index)
+    if positions is not None:
+        _check_state("positions", positions, torch.int32, nb, h, index)
     if block_table.dtype is not torch.int32 or block_table.dim() != 2 \
             or block_table.stride(1) != 1:
         _fail("block_table must be a 2-D int32 tensor with contiguous rows")
     batch = seq_lens.numel()
     for name, t in (("seq_lens", seq_lens), ("keep", keep), ("recent", recent),
                     ("position_offsets", position_offsets), ("seq_ids", seq_ids)):
-        _check_ints(name, t, batch)
+        if t is not None:
+            _check_ints(name, t, batch, index)
     if seq_ids is None and block_table.shape[0] < batch:
         _fail(f"block_table has {block_table.shape[0]} rows for {batch} sequences")
     need = evict_workspace_bytes(batch, h, max_seq_len)
     if workspace is None:
-        with torch.cuda.stream(stream):
+        if stream is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        else:
+            with torch.cuda.stream(stream):     # the memory of the stream that uses it
+                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
         _fail(f"workspace must be a contiguous tensor of at least {need} bytes")
-    with torch.cuda.device(dev):
-        _lib.call("kvc_evict_kv", key_cache.data_ptr(), value_cache.data_ptr(), nb, h, d, bs,
-                  key_cache.element_size(), cs[0], cs[1], scores.data_ptr(), _ptr(positions),
-                  block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                  block_table.shape[0], _ptr(seq_ids), seq_lens.data_ptr(), keep.data_ptr(),
-                  recent.data_ptr(), _ptr(position_offsets), batch, int(max_seq_len),
-                  workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                  _stream_handle(dev, stream))
+    _lib.call_on(index, "kvc_evict_kv", key_cache.data_ptr(), value_cache.data_ptr(), nb, h, d,
+                 bs, key_cache.element_size(), cs[0], cs[1], scores.data_ptr(), _ptr(positions),
+                 block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                 block_table.shape[0], _ptr(seq_ids), seq_lens.data_ptr(), keep.data_ptr(),
+                 recent.data_ptr(), _ptr(position_offsets), batch, int(max_seq_len),
+                 workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                 _stream_handle(dev, stream))
 
 
 def evict_workspace_bytes(batch: int, num_kv_heads: int, max_seq_len: int) -> int:

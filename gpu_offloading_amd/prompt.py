@@ -66,8 +66,10 @@ class PlannedRuns:
         if not float_workspace_buffer.is_cuda:
             _fail("float_workspace_buffer must be a GPU tensor")
         self._device = float_workspace_buffer.device
+        self._index = self._device.index
         self._sched = None
         self._staged: tuple = ()
+        self._plan_ptr = 0
         self._plan_stream: Optional[int] = None
         self._plan_event: Optional[torch.cuda.Event] = None
         self._ordered: set = set()
@@ -76,6 +78,7 @@ class PlannedRuns:
 
     def _set_staged(self, *tensors: torch.Tensor) -> None:
         self._staged = tensors
+        self._plan_ptr = tensors[0].data_ptr()
         self._plan_stream = _lib.current_stream_handle(self._device)
         self._plan_event = torch.cuda.Event()
         self._plan_event.record(torch.cuda.current_stream(self._device))
@@ -83,7 +86,9 @@ class PlannedRuns:
 
     def _run_stream(self, stream: Optional[torch.cuda.Stream]) -> int:
         sh = stream.cuda_stream if stream is not None else _lib.current_stream_handle(self._device)
-        if sh != self._plan_stream and sh not in self._ordered \
+        if sh == self._plan_stream:
+            return sh
+        if sh not in self._ordered \
                 and not torch.cuda.is_current_stream_capturing():
             st = stream if stream is not None else torch.cuda.current_stream(self._device)
             st.wait_event(self._plan_event)
@@ -145,38 +150,45 @@ class BatchPromptAttentionWrapper(PlannedRuns):
         if s is None:
             _fail("run() called before plan()")
         hq, hkv, d = s.num_qo_heads, s.num_kv_heads, s.head_dim
-        for name, t, n, h in (("q", q, s.total_q, hq), ("k", k, s.total_kv, hkv),
-                              ("v", v, s.total_kv, hkv)):
-            _check_rows(name, t, n, h, d, self._dtype, self._device)
-        if out is not None:
-            _check_rows("out", out, s.total_q, hq, d, self._dtype, self._device)
-        with torch.cuda.stream(stream):     # the memory of the stream that writes it
-            if out is None:
-                out = torch.empty(s.total_q, hq, d, dtype=self._dtype, device=self._device)
-            if return_lse and lse is None:
-                lse = torch.empty(s.total_q, hq, dtype=torch.float32, device=self._device)
-        if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous()
-                                or lse.numel() < s.total_q * hq or lse.device != self._device):
+        dt, dev = self._dtype, self._index
+        total = s.total_q
+        qs = check_rows("q", q, total, hq, d, dt, dev)
+        ks = check_rows("k", k, s.total_kv, hkv, d, dt, dev)
+        vs = check_rows("v", v, s.total_kv, hkv, d, dt, dev)
+        if out is None:
+            out = _empty((total, hq, d), dt, self._device, stream)
+            os = hq * d
+        else:
+            os = check_rows("out", out, total, hq, d, dt, dev)
+        if lse is None:
+            if return_lse:
+                lse = _empty((total, hq), torch.float32, self._device, stream)
+        elif (lse.dtype != torch.float32 or not lse.is_contiguous()
+              or lse.numel() < total * hq or lse.device != self._device):
             _fail("lse must be contiguous float32 [tokens, num_qo_heads] on the wrapper's device")
-        sh = self._run_stream(stream)
-        with torch.cuda.device(self._device):
-            _lib.call("kvc_prompt_run", s, self._staged[0].data_ptr(), q.data_ptr(),
-                      _token_stride(q), k.data_ptr(), _token_stride(k), v.data_ptr(),
-                      _token_stride(v), _DTYPES[self._dtype], self._sm_scale, out.data_ptr(),
-                      _token_stride(out), lse.data_ptr() if lse is not None else None, sh)
+        _lib.call_on(dev, "kvc_prompt_run", s, self._plan_ptr, q.data_ptr(), qs, k.data_ptr(), ks,
+                     v.data_ptr(), vs, _DTYPES[dt], self._sm_scale, out.data_ptr(), os,
+                     None if lse is None else lse.data_ptr(), self._run_stream(stream))
         return (out, lse) if return_lse else out
 
 
-def _check_rows(name: str, t: torch.Tensor, rows: int, heads: int, dim: int, dtype: torch.dtype,
-                device: torch.device) -> None:
-    if t.dim() != 3 or t.shape[0] < rows or tuple(t.shape[1:]) != (heads, dim):
-        _fail(f"{name} must be [{rows}, {heads}, {dim}], got {tuple(t.shape)}")
-    if t.dtype != dtype or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+def _empty(shape, dtype, device, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
+    """An output from the memory of the stream that writes it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def check_rows(name: str, t: torch.Tensor, rows: int, heads: int, dim: int, dtype: torch.dtype,
+               device: int) -> int:
+    """Checks ``[rows or more, heads, dim]`` of ``dtype`` on GPU ``device`` with
+    the heads of a token contiguous; returns the elements between tokens."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or sh[0] < rows or sh[1] != heads or sh[2] != dim:
+        _fail(f"{name} must be [{rows}, {heads}, {dim}], got {tuple(sh)}")
+    if t.dtype is not dtype or st[2] != 1 or (st[1] != dim and heads > 1):
         _fail(f"{name} must be {dtype} with the heads of a token contiguous")
-    if t.device != device:
-        _fail(f"{name} on {t.device}, the wrapper's device is {device}")
-
-
-def _token_stride(t: torch.Tensor) -> int:
-    """Elements between tokens (of a single token: any valid stride)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    if t.get_device() != device:
+        _fail(f"{name} on {t.device}, the wrapper's device is cuda:{device}")
+    return st[0] if sh[0] > 1 else heads * dim     # of a single token: any valid stride
