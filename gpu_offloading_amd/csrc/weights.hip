@@ -326,8 +326,18 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
   const int64_t t1 = tasks * (wave + 1) / waves;
   int64_t t = tasks * wave / waves;
   if (t >= t1) return;
-  // The first 64 requests' ends; others are read where a page may be theirs.
+  // The first 64 requests' pages and last pages' tokens, a lane each (a load of them
+  // beside a task would wait for the next one's K); further requests' are read.
+  const int begin0 = lane < c.batch ? c.indptr[lane] : INT32_MAX;
   const int end0 = lane < c.batch ? c.indptr[lane + 1] : INT32_MAX;
+  const int lpl0 = lane < c.batch ? c.last_page_len[lane] : 0;
+  struct Request { int first, end, lpl; };
+  auto request = [&](int b) __attribute__((always_inline)) {
+    if (b < 64)
+      return Request{__builtin_amdgcn_readlane(begin0, b), __builtin_amdgcn_readlane(end0, b),
+                     __builtin_amdgcn_readlane(lpl0, b)};
+    return Request{c.indptr[b], c.indptr[b + 1], c.last_page_len[b]};
+  };
 
   struct Task { int h; int64_t p0; };
   auto task_of = [&](int64_t i) __attribute__((always_inline)) {
@@ -390,35 +400,37 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
     load_q(x.b, k.h, 0, x.q, x.lse);
   };
 
+  // (Ids come before the K loads that were issued last: waiting for them does not
+  // wait for those.)
   Task now = task_of(t), next = task_of(min(t + 1, t1 - 1));
+  int32_t ids0 = load_ids(now), ids = load_ids(next);
   Loaded x;
-  load(now, load_ids(now), x);
-  int32_t ids = load_ids(next);
+  load(now, ids0, x);
   for (; t < t1; ++t) {
     Loaded y;
-    Task after = next;
-    if (t + 1 < t1) {
-      load(next, ids, y);
-      after = task_of(min(t + 2, t1 - 1));
-      ids = load_ids(after);
-    }
+    const Task after = task_of(min(t + 2, t1 - 1));
+    const int32_t ids2 = load_ids(after);
+    if (t + 1 < t1) load(next, ids, y);
+    ids = ids2;
     int b = x.b;
+    Request req = request(b);
 #pragma unroll
     for (int set = 0; set < kSets; ++set) {
       float mine = 0.f;
       bool fresh = false, in = false;
-      int key = 0, request = 0;
+      int key = 0, owner = 0;
 #pragma unroll
       for (int i = 4 * set; i < min(kPages, 4 * set + 4); ++i) {
         const int64_t p = now.p0 + i;
         if (p >= pages) continue;
-        if (p >= c.indptr[b + 1]) {       // this page is another request's
+        if (p >= req.end) {       // this page is another request's
           b = request_of(p);
           if (b >= c.batch) break;
+          req = request(b);
           load_q(b, now.h, 0, x.q, x.lse);
         }
-        const int first = c.indptr[b], last = c.indptr[b + 1] - 1;
-        const int tokens = p < last ? kPage : c.last_page_len[b];
+        const int first = req.first, last = req.end - 1;
+        const int tokens = p < last ? kPage : req.lpl;
         float w = 0.f;
         for (int g0 = 0; g0 < a.group; g0 += 16) {
           if (g0 > 0) load_q(b, now.h, g0, x.q, x.lse);
@@ -439,7 +451,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
           in = r < tokens;
           fresh = p == last && r == tokens - 1;
           key = int(p - first) * kPage + r;
-          request = b;
+          owner = b;
         }
       }
       if (in && x.block[set] >= 0) {
@@ -447,7 +459,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
         a.scores[at] = fresh ? mine : x.old[set] + mine;
         if (fresh && a.positions)
           a.positions[at] =
-              key + (a.offsets ? a.offsets[a.seq_ids ? a.seq_ids[request] : request] : 0);
+              key + (a.offsets ? a.offsets[a.seq_ids ? a.seq_ids[owner] : owner] : 0);
       }
     }
     x = y;
