@@ -302,9 +302,9 @@ struct TokenArgs {
 constexpr int kTokenThreads = 256;
 constexpr int64_t kTokenWorkgroups = 512;   // two per CU: what its registers hold
 
-// A wave runs a range of tasks; a task is kPages consecutive entries of the batch's
-// page list for one KV head (heads fastest: neighbouring tasks read the same tokens'
-// rows).  Bound by memory: a task's K (16 KB), old scores and query are loaded
+// A wave runs every so-manieth task; a task is kPages consecutive entries of the
+// batch's page list for one KV head (heads fastest: neighbouring waves read the same
+// tokens' rows at the same time).  Bound by memory: a task's K (16 KB), old scores and query are loaded
 // while the one before is computed, its page ids a task earlier still.  S = Q K^T per
 // page with v_mfma_f32_16x16x32 (A: lane l = row l%16, k = 8(l/16)..+7; B: column
 // l%16; C: acc[j] = row 4(l/16)+j, column l%16): rows are the group's query heads,
@@ -323,9 +323,8 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
   const int64_t waves = int64_t(gridDim.x) * (kTokenThreads / 64);
   const int64_t wave = int64_t(blockIdx.x) * (kTokenThreads / 64) +
                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t t1 = tasks * (wave + 1) / waves;
-  int64_t t = tasks * wave / waves;
-  if (t >= t1) return;
+  int64_t t = wave;
+  if (t >= tasks) return;
   // The first 64 requests' pages and last pages' tokens, a lane each (a load of them
   // beside a task would wait for the next one's K); further requests' are read.
   const int begin0 = lane < c.batch ? c.indptr[lane] : INT32_MAX;
@@ -402,15 +401,15 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
 
   // (Ids come before the K loads that were issued last: waiting for them does not
   // wait for those.)
-  Task now = task_of(t), next = task_of(min(t + 1, t1 - 1));
+  Task now = task_of(t), next = task_of(min(t + waves, tasks - 1));
   int32_t ids0 = load_ids(now), ids = load_ids(next);
   Loaded x;
   load(now, ids0, x);
-  for (; t < t1; ++t) {
+  for (; t < tasks; t += waves) {
     Loaded y;
-    const Task after = task_of(min(t + 2, t1 - 1));
+    const Task after = task_of(min(t + 2 * waves, tasks - 1));
     const int32_t ids2 = load_ids(after);
-    if (t + 1 < t1) load(next, ids, y);
+    if (t + waves < tasks) load(next, ids, y);
     ids = ids2;
     int b = x.b;
     Request req = request(b);
