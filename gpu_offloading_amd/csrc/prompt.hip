@@ -153,12 +153,15 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   typedef typename T::x8 x8;
   // One LDS object with the tiles first: operand reads then use immediate
   // offsets.  ostage: each wave's finished rows on their way out, padded so that
-  // one instruction's pieces spread over the banks.  bad: the last unit (by its
+  // one instruction's pieces spread over the banks.  out_off: the rows' places in the
+  // output, in bytes from the tile's first (kept in registers, they would spill, and a
+  // reload waits for every load and store in flight).  bad: the last unit (by its
   // parity) whose boundary tiles held an inf or NaN in V.
   struct Lds {
     uint8_t k[2][kTile];
     uint8_t v[2][kTile];
     uint8_t ostage[8][kWaveRows * kORow];
+    uint32_t out_off[8 * kWaveRows];
     int bad[2];
   };
   __shared__ alignas(16) Lds lds;
@@ -174,6 +177,9 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   const int row_head = row - row_tok * a.group;
   const int Hq = a.num_kv_heads * a.group;
   if (threadIdx.x < 2) lds.bad[threadIdx.x] = -1;
+  if (half == 0)
+    lds.out_off[row] = row_tok < a.tile_tokens
+                           ? uint32_t(row_tok * a.out_stride + row_head * D) * 2 : UINT32_MAX;
 
   const int2 span = a.wg_units[blockIdx.x];
   const int u_first = __builtin_amdgcn_readfirstlane(span.x);
@@ -455,22 +461,23 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     constexpr int kStoreRows = 64 / kChunks;      // rows per store
     const int c = lane % kChunks;
+    uint8_t* obase = reinterpret_cast<uint8_t*>(
+        a.out + int64_t(cu.q_off + cu.tok0) * a.out_stride + int64_t(cu.h * a.group) * D);
+    // (a row's place is below that of the first token that is not there)
+    const uint32_t end = uint32_t(min(a.tile_tokens, cu.q_len - cu.tok0) * a.out_stride) * 2;
 #pragma unroll
     for (int t0 = 0; t0 < kWaveRows / kStoreRows; t0 += 4) {
       uint4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = *reinterpret_cast<const uint4*>(
-            stg + ((t0 + i) * kStoreRows + lane / kChunks) * kORow + 16 * c);
+      uint32_t off[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int rr = wave * kWaveRows + (t0 + i) * kStoreRows + lane / kChunks;
-        const int tt = int(rr * a.inv_group >> 16);
-        if (tt < a.tile_tokens && cu.tok0 + tt < cu.q_len)
-          store_stream(a.out + int64_t(cu.q_off + cu.tok0 + tt) * a.out_stride +
-                           int64_t(cu.h * a.group + rr - tt * a.group) * D + 8 * c,
-                       v[i]);
+        const int rr = (t0 + i) * kStoreRows + lane / kChunks;
+        v[i] = *reinterpret_cast<const uint4*>(stg + rr * kORow + 16 * c);
+        off[i] = lds.out_off[wave * kWaveRows + rr];
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (off[i] < end) store_stream(obase + (off[i] + uint32_t(16 * c)), v[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (row_ok && a.lse && half == 0)
@@ -1005,8 +1012,10 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
   KVC_REQUIRE(q_token_stride >= qw && out_token_stride >= qw && key_token_stride >= kw &&
                   value_token_stride >= kw,
               KVC_ERR_INVALID_ARG, "token stride smaller than the token's heads");
-  KVC_REQUIRE(key_token_stride < (int64_t(1) << 24) && value_token_stride < (int64_t(1) << 24),
-              KVC_ERR_INVALID_ARG, "K/V tokens 32 MiB or more apart");
+  // (a tile's tokens are addressed by 32-bit byte offsets)
+  KVC_REQUIRE(key_token_stride < (int64_t(1) << 22) && value_token_stride < (int64_t(1) << 22) &&
+                  out_token_stride < (int64_t(1) << 22),
+              KVC_ERR_INVALID_ARG, "key, value or out tokens 8 MiB or more apart");
   KVC_REQUIRE(aligned(q, 16) && aligned(key, 16) && aligned(value, 16) && aligned(out, 16) &&
                   aligned(plan, 16) && q_token_stride % 8 == 0 && key_token_stride % 8 == 0 &&
                   value_token_stride % 8 == 0 && out_token_stride % 8 == 0,
