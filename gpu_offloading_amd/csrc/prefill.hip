@@ -47,8 +47,6 @@
 #include <type_traits>
 #include <vector>
 
-#include "unit_plan.h"
-
 namespace kvc {
 namespace {
 
@@ -67,7 +65,7 @@ constexpr int kPage = 16;
 constexpr int kD = 128;
 constexpr int kKRow = kD * 2;                // bytes per K or V row in LDS (unpadded)
 constexpr int kORow = kKRow + 16;            // bytes per staged output row
-constexpr int kItemInts = kUnitInts;
+constexpr int kItemInts = 8;
 constexpr float kRescaleLog2 = 8.f;           // lazy-rescale threshold (base 2)
 // Word 3 of a raw buffer resource (32-bit data, no swizzle): loads past
 // num_records return zeros.
@@ -821,7 +819,7 @@ void launch(const PrefillArgs& a, int workgroups, const int4* merges, int num_me
 // table, padded to 4 int32, then the unit records.
 constexpr int64_t kMaxWorkgroups = 256;
 int64_t plan_workgroups(int64_t items, int hkv) { return std::min(kMaxWorkgroups, items * hkv); }
-int64_t plan_table_ints(int64_t workgroups) { return unit_table_ints(workgroups); }
+int64_t plan_table_ints(int64_t workgroups) { return (2 * workgroups + 3) / 4 * 4; }
 int64_t plan_ints_for(int64_t items, int hkv) {
   return plan_table_ints(plan_workgroups(items, hkv)) + items * hkv * kItemInts;
 }
@@ -957,7 +955,49 @@ int64_t split_plan_ints(int64_t workgroups, int64_t units, int64_t merges) {
 
 // The plan of whole units: plan_ints_for(n, hkv) entries.
 void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int32_t* plan_host) {
-  write_unit_plan(rec, n, hkv, plan_workgroups(n, hkv), plan_host);
+  // Longest items first: the causal tail of short tiles fills the gaps.
+  std::vector<int64_t> order(n);
+  for (int64_t i = 0; i < n; ++i) order[i] = i;
+  std::stable_sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
+    return rec[x * kItemInts + 6] > rec[y * kItemInts + 6];
+  });
+  // Units (item, KV head) in the order a grid of (items, heads) workgroups
+  // would be dispatched: head-major, items longest first.  The hardware
+  // hands workgroup w to XCD w % 8 and each XCD's next workgroup to its
+  // first free CU; the plan replays that list scheduling with each unit's
+  // cost taken as its key tiles + 2, assigning unit d to a workgroup of XCD
+  // d % 8 (workgroup b runs on XCD b % 8), so the units of one request and
+  // head still run side by side on one XCD and share its L2.
+  const int64_t units = n * hkv;
+  const int64_t W = plan_workgroups(n, hkv);
+  const int groups = (W % 8 == 0) ? 8 : 1;
+  std::vector<std::vector<int64_t>> lists(W);
+  {
+    typedef std::pair<int64_t, int64_t> Slot;  // (load, workgroup)
+    std::vector<std::priority_queue<Slot, std::vector<Slot>, std::greater<Slot>>> free_at(groups);
+    for (int64_t b = 0; b < W; ++b) free_at[b % groups].push(Slot(0, b));
+    for (int64_t d = 0; d < units; ++d) {
+      auto& q = free_at[d % groups];
+      const Slot sl = q.top();
+      q.pop();
+      lists[sl.second].push_back(d);
+      const int64_t item = order[d % n];
+      q.push(Slot(sl.first + rec[item * kItemInts + 6] + 2, sl.second));
+    }
+  }
+  const int64_t table = plan_table_ints(W);
+  std::fill_n(plan_host, table, 0);
+  int64_t next = 0;
+  for (int64_t b = 0; b < W; ++b) {
+    plan_host[2 * b] = int32_t(next);
+    plan_host[2 * b + 1] = int32_t(lists[b].size());
+    for (const int64_t d : lists[b]) {
+      int32_t* dst = plan_host + table + next * kItemInts;
+      std::copy_n(rec.data() + order[d % n] * kItemInts, kItemInts, dst);
+      dst[0] = int32_t(d / n);  // the KV head
+      ++next;
+    }
+  }
 }
 
 int split_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t share,

@@ -14,10 +14,11 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
+#include <queue>
 #include <type_traits>
+#include <utility>
 #include <vector>
-
-#include "unit_plan.h"
 
 namespace kvc {
 namespace {
@@ -901,7 +902,82 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
 
 // Persistent workgroups: one per CU of an MI355X.
 constexpr int64_t kMaxWorkgroups = 256;
+constexpr int kUnitInts = 8;
+constexpr int kUnitCost = 3;      // a unit's start and end, in tiles
+constexpr int kXcds = 8;
 int64_t plan_workgroups(int64_t units) { return std::min(kMaxWorkgroups, units); }
+int64_t table_ints(int64_t workgroups) { return (2 * workgroups + 3) / 4 * 4; }
+
+// The work list: a table of the workgroups' (first unit, units), then the unit
+// records in workgroup order.  `rec`: a record per item (entry 0 the sequence, 6 its
+// tiles), sequence by sequence; a unit is an item of one KV head.
+//
+// Workgroup w runs on XCD w % 8, whose L2 serves the K and V of its units: the units
+// are lined up sequence by sequence and head by head, and the line is cut into eight
+// parts of equal cost, so that a head's K and V go through one XCD (seven heads at
+// most through two).  In each part units are dealt in line order, a head's longest
+// first, to the least loaded workgroup; the last quarter of a part longest first over
+// all its heads, which evens the ends out.
+void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W,
+                int32_t* plan_host) {
+  struct Line { int64_t item; int head, cost; };
+  std::vector<Line> line;
+  line.reserve(size_t(n) * hkv);
+  int64_t total = 0;
+  for (int64_t i0 = 0; i0 < n;) {
+    int64_t i1 = i0;
+    while (i1 < n && rec[i1 * kUnitInts] == rec[i0 * kUnitInts]) ++i1;
+    for (int h = 0; h < hkv; ++h) {
+      const size_t at = line.size();
+      for (int64_t i = i0; i < i1; ++i) {
+        const int cost = rec[i * kUnitInts + 6] + kUnitCost;
+        line.push_back(Line{i, h, cost});
+        total += cost;
+      }
+      std::stable_sort(line.begin() + at, line.end(),
+                       [](const Line& x, const Line& y) { return x.cost > y.cost; });
+    }
+    i0 = i1;
+  }
+  const int parts = W % kXcds == 0 ? kXcds : 1;
+  std::vector<std::vector<size_t>> lists(W);
+  typedef std::pair<int64_t, int64_t> Slot;  // (load, workgroup)
+  size_t u = 0;
+  int64_t done = 0;
+  for (int x = 0; x < parts; ++x) {
+    const int64_t from = done, until = total * (x + 1) / parts;
+    size_t end = u;
+    // Every workgroup gets a unit, and the last part what is left.
+    const size_t least = u + size_t(W / parts), most = line.size() - size_t((parts - 1 - x) * (W / parts));
+    while (end < most && (end < least || x == parts - 1 || done + line[end].cost / 2 < until))
+      done += line[end++].cost;
+    size_t tail = end;
+    for (int64_t rest = (done - from) / 4; tail > u && rest > 0; --tail) rest -= line[tail - 1].cost;
+    std::stable_sort(line.begin() + tail, line.begin() + end,
+                     [](const Line& p, const Line& q) { return p.cost > q.cost; });
+    std::priority_queue<Slot, std::vector<Slot>, std::greater<Slot>> free_at;
+    for (int64_t b = x; b < W; b += parts) free_at.push(Slot(0, b));
+    for (; u < end; ++u) {
+      const Slot sl = free_at.top();
+      free_at.pop();
+      lists[sl.second].push_back(u);
+      free_at.push(Slot(sl.first + line[u].cost, sl.second));
+    }
+  }
+  const int64_t table = table_ints(W);
+  std::fill_n(plan_host, table, 0);
+  int64_t next = 0;
+  for (int64_t b = 0; b < W; ++b) {
+    plan_host[2 * b] = int32_t(next);
+    plan_host[2 * b + 1] = int32_t(lists[b].size());
+    for (const size_t i : lists[b]) {
+      int32_t* dst = plan_host + table + next * kUnitInts;
+      std::copy_n(rec.data() + line[i].item * kUnitInts, kUnitInts, dst);
+      dst[0] = line[i].head;
+      ++next;
+    }
+  }
+}
 
 int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batch, int32_t hq,
                 int32_t hkv, int32_t head_dim, int32_t causal, kvc_prompt_schedule* sched,
@@ -957,11 +1033,11 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
   sched->total_kv = int32_t(end_kv);
   sched->max_key_tiles = max_tiles;
   sched->reserved = 0;
-  sched->plan_ints = unit_table_ints(W) + n * hkv * kUnitInts;
+  sched->plan_ints = table_ints(W) + n * hkv * kUnitInts;
   KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
               KVC_ERR_WORKSPACE,
               "plan buffer too small: need " + std::to_string(sched->plan_ints) + " int32");
-  write_unit_plan(rec, n, hkv, W, plan_host);
+  if (n > 0) write_plan(rec, n, hkv, W, plan_host);
   return ok();
 }
 
@@ -998,7 +1074,7 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
                   (D == 64 || D == 128 || D == 256) && sched->num_units >= 0 &&
                   sched->tile_tokens == tile_rows(D) / (Hq / Hkv) &&
                   sched->num_workgroups == plan_workgroups(sched->num_units) &&
-                  sched->plan_ints == unit_table_ints(sched->num_workgroups) +
+                  sched->plan_ints == table_ints(sched->num_workgroups) +
                                           int64_t(sched->num_units) * kUnitInts,
               KVC_ERR_INVALID_ARG, "schedule not produced by kvc_prompt_plan");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
@@ -1029,7 +1105,7 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
   a.k_stride = key_token_stride;
   a.v_stride = value_token_stride;
   a.wg_units = reinterpret_cast<const int2*>(plan);
-  a.units = reinterpret_cast<const int4*>(plan + unit_table_ints(sched->num_workgroups));
+  a.units = reinterpret_cast<const int4*>(plan + table_ints(sched->num_workgroups));
   a.num_kv_heads = Hkv;
   a.group = Hq / Hkv;
   a.tile_tokens = sched->tile_tokens;

@@ -20,8 +20,6 @@
 #include <cmath>
 #include <vector>
 
-#include "unit_plan.h"
-
 namespace kvc {
 namespace {
 
@@ -87,6 +85,7 @@ __device__ __forceinline__ void store_weight(const WeightsArgs& a, int32_t block
 //   KV head, first key, q_len, kv_len | q offset, page offset, request, first new key |
 //   first block, blocks, partial (-1: the unit's sums are the keys' weights), 0
 constexpr int kRecInts = 12;
+constexpr int kJoinInts = 8;
 constexpr int kRows = 32;                          // query rows per block
 constexpr int kKeyBlocks = 2;                      // 32-key blocks per wave
 constexpr int kWaveKeys = 32 * kKeyBlocks;
@@ -548,7 +547,7 @@ int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32
   sched->num_parts = int32_t(n_parts);
   sched->num_joins = int32_t(n_joins);
   sched->total_q = batch ? qo_indptr[batch] : 0;
-  sched->plan_ints = n_units * kRecInts + n_joins * kUnitInts;
+  sched->plan_ints = n_units * kRecInts + n_joins * kJoinInts;
   sched->workspace_bytes = n_parts * kUnitKeys * 4;
   KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
               KVC_ERR_WORKSPACE,
@@ -578,9 +577,9 @@ int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32
           load[xcd] += to - from + 4;
         }
         if (k > 1) {
-          const int32_t r8[kUnitInts] = {h, t.key0, k, kv_len, int32_t(part), kv_indptr[t.b], t.b,
+          const int32_t r8[kJoinInts] = {h, t.key0, k, kv_len, int32_t(part), kv_indptr[t.b], t.b,
                                          t.new_from};
-          join = std::copy_n(r8, kUnitInts, join);
+          join = std::copy_n(r8, kJoinInts, join);
           part += k;
         }
       }
@@ -647,7 +646,7 @@ extern "C" int kvc_batch_attention_weights_run(
                   sched->num_units >= 0 && sched->num_parts >= 0 && sched->num_joins >= 0 &&
                   sched->workspace_bytes == int64_t(sched->num_parts) * kUnitKeys * 4 &&
                   sched->plan_ints == int64_t(sched->num_units) * kRecInts +
-                                          int64_t(sched->num_joins) * kUnitInts,
+                                          int64_t(sched->num_joins) * kJoinInts,
               KVC_ERR_INVALID_ARG, "schedule not produced by kvc_weights_plan");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
               "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
