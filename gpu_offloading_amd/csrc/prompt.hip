@@ -28,6 +28,7 @@ typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int kWaveRows = 32;                 // query rows per wave
@@ -126,9 +127,10 @@ struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles; };
 // so that on each SIMD one wave's matrix instructions run beside the other's
 // exponentials:
 //   slot 2j: team 0 M_j, team 1 X_{j-1};   slot 2j+1: team 0 X_j, team 1 M_j.
-// Team 1 also stages: at the start of slot 2j each of its waves issues the
-// direct-to-LDS loads of its quarter of K_{j+1} and V_j (the buffers were last
-// read in slot 2j-1) and waits for them before the barrier that ends slot 2j+1.
+// Team 0 also stages: in slot 2j, between its matrix instructions, each of its waves
+// issues the direct-to-LDS loads of its quarter of K_{j+1} and V_j (the buffers were
+// last read in slot 2j-1) and waits for them before the barrier that ends slot 2j+1.
+// (Issued by the team in its VALU phase they cost 570 cycles of a slot of 1200.)
 // A workgroup runs a list of units: while one runs, the next one's record and Q
 // are loaded, and its first K tile is staged in the slot 2n of this one.
 //
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int team = wave >> 2;
-  const int sw = wave & 3;                     // team 1: the quarter of a tile it stages
+  const int sw = wave & 3;                     // team 0: the quarter of a tile it stages
   const int lane = threadIdx.x & 63;
   const int r = lane & 31;
   const int half = lane >> 5;
@@ -246,50 +248,71 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   // before the barrier that publishes the tiles).  The resource is bounded to the
   // sequence's last row: rows past it are not read.  No compiler-generated code
   // here uses M0 (tests/test_prompt_m0.py checks the built assembly).
-  auto dma = [&](uint8_t* tile, const uint16_t* base, int64_t stride, uint32_t row_bytes,
-                 const uint32_t (&lane_off)[kDma], const Unit& U, int j)
-      __attribute__((always_inline)) {
+  struct Staging { i32x4_t rsrc; uint32_t to; };
+  auto staging = [&](const uint8_t* tile, const uint16_t* base, int64_t stride,
+                     uint32_t row_bytes, const Unit& U, int j) __attribute__((always_inline)) {
     const int key0 = j * kKeys + sw * kWaveKeys;
-    const int rows = max(0, min(kWaveKeys, U.kv_len - key0));
+    // (past the unit's last tile nothing is read)
+    const int rows = max(0, min(kWaveKeys, min(U.kv_len, U.ntiles * kKeys) - key0));
     const uint64_t p = reinterpret_cast<uint64_t>(base + (int64_t(U.k_off) + key0) * stride +
                                                   U.h * D);
     const int bytes = rows > 0 ? int(uint32_t(rows - 1) * row_bytes + kRow) : 0;
-    const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane(int(uint32_t(p))),
-                          __builtin_amdgcn_readfirstlane(int(uint32_t(p >> 32) & 0xFFFF)),
-                          __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3};
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile + sw * kWaveKeys * kRow));
-#pragma unroll
-    for (int i = 0; i < kDma; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(to + 1024 * i), "v"(lane_off[i]), "s"(rsrc) : "memory");
+    return Staging{i32x4_t{__builtin_amdgcn_readfirstlane(int(uint32_t(p))),
+                           __builtin_amdgcn_readfirstlane(int(uint32_t(p >> 32) & 0xFFFF)),
+                           __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3},
+                   uint32_t(__builtin_amdgcn_readfirstlane(
+                       lds_addr(tile + sw * kWaveKeys * kRow)))};
+  };
+  auto stage_piece = [](const Staging& g, uint32_t lane_off, int i) __attribute__((always_inline)) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(g.to + 1024 * i), "v"(lane_off), "s"(g.rsrc) : "memory");
+  };
+  auto staging_k = [&](const Unit& U, int j) __attribute__((always_inline)) {
+    return staging(lds.k[j & 1], a.k, a.k_stride, k_bytes, U, j);
+  };
+  auto staging_v = [&](const Unit& U, int j) __attribute__((always_inline)) {
+    return staging(lds.v[j & 1], a.v, a.v_stride, v_bytes, U, j);
   };
   auto dma_k = [&](const Unit& U, int j) __attribute__((always_inline)) {
-    dma(lds.k[j & 1], a.k, a.k_stride, k_bytes, lane_k, U, j);
-  };
-  auto dma_v = [&](const Unit& U, int j) __attribute__((always_inline)) {
-    dma(lds.v[j & 1], a.v, a.v_stride, v_bytes, lane_v, U, j);
+    const Staging g = staging_k(U, j);
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) stage_piece(g, lane_k[i], i);
   };
   // A boundary tile's V in LDS (this wave's keys, just staged): inf and NaN
   // and rows past the sequence become 0, as 0 times them must not reach the rows
   // that do not see them; finish_unit gives them to those that do.
   auto clean_v = [&](int j, int stamp) __attribute__((always_inline)) {
-    bool bad = false;
+    uint8_t* mine = lds.v[j & 1] + sw * kWaveKeys * kRow + 16 * lane;
+    // The largest exponent of each half word.
+    u16x2_t top = {0, 0};
 #pragma unroll
     for (int i = 0; i < kDma; ++i) {
-      const int key = kLaneKeys * i + lane / kChunks;
-      uint4* at = reinterpret_cast<uint4*>(lds.v[j & 1] + sw * kWaveKeys * kRow + 1024 * i + 16 * lane);
-      uint4 x = *at;
-      if (j * kKeys + sw * kWaveKeys + key >= cu.kv_len) {
-        x = make_uint4(0, 0, 0, 0);
-      } else {
-        x.x = finite2<T>(x.x, &bad);
-        x.y = finite2<T>(x.y, &bad);
-        x.z = finite2<T>(x.z, &bad);
-        x.w = finite2<T>(x.w, &bad);
-      }
-      *at = x;
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(mine + 1024 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        top = __builtin_elementwise_max(
+            top, __builtin_bit_cast(u16x2_t, x[e] & (T::kExp << 16 | T::kExp)));
     }
-    if (bad) lds.bad[stamp & 1] = stamp;
+    const int left = cu.kv_len - (j * kKeys + sw * kWaveKeys);   // keys of the sequence
+    if (__builtin_amdgcn_ballot_w64(top[0] == T::kExp || top[1] == T::kExp) != 0 ||
+        left < kWaveKeys) {
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < kDma; ++i) {
+        uint4* at = reinterpret_cast<uint4*>(mine + 1024 * i);
+        uint4 x = *at;
+        if (kLaneKeys * i + lane / kChunks >= left) {
+          x = make_uint4(0, 0, 0, 0);
+        } else {
+          x.x = finite2<T>(x.x, &bad);
+          x.y = finite2<T>(x.y, &bad);
+          x.z = finite2<T>(x.z, &bad);
+          x.w = finite2<T>(x.w, &bad);
+        }
+        *at = x;
+      }
+      if (bad) lds.bad[stamp & 1] = stamp;
+    }
   };
 
   uint32_t v_rd[kBlocks];
@@ -334,7 +357,8 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   // p over this lane's half of the keys (fp32, before p is rounded).
   float m_run = -INFINITY, l_half = 0.f;
 
-  auto mfma_phase = [&](int j, auto do_o_c, auto do_s_c) __attribute__((always_inline)) {
+  auto mfma_phase = [&](int j, auto do_o_c, auto do_s_c, auto between)
+      __attribute__((always_inline)) {
     // One run of MFMAs, each operand read kAhead before its own: the first K operands
     // come in while the last output MFMAs run.
     constexpr int NO = decltype(do_o_c)::value ? 2 * KB * kBlocks : 0;
@@ -361,6 +385,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
         const int m = i - NO;
         s[m % KB] = T::mfma(op[i], qb[m / KB], m < KB ? zero : s[m % KB]);
       }
+      between(i);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -425,7 +450,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   // The unit's rows leave through the wave's LDS staging: a lane holds 8-byte
   // pieces of one row; read back, kChunks lanes hold a whole row.  Non-temporal
   // stores: the output is not read again here, and the caches keep K and V.
-  auto finish_unit = [&](int k) __attribute__((always_inline)) {
+  auto finish_unit = [&](int k, auto before_stores) __attribute__((always_inline)) {
     const float l = l_half + __shfl_xor(l_half, 32);
     const float inv = l == 0.f ? 0.f : 1.f / l;    // a row that sees no key: 0
 #pragma unroll
@@ -464,6 +489,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     const int c = lane % kChunks;
     uint8_t* obase = reinterpret_cast<uint8_t*>(
         a.out + int64_t(cu.q_off + cu.tok0) * a.out_stride + int64_t(cu.h * a.group) * D);
+    before_stores();
     // (a row's place is below that of the first token that is not there)
     const uint32_t end = uint32_t(min(a.tile_tokens, cu.q_len - cu.tok0) * a.out_stride) * 2;
 #pragma unroll
@@ -501,17 +527,29 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   using no = std::false_type;
   auto run = [&](auto team_c) __attribute__((always_inline)) {
     constexpr int kTeam = decltype(team_c)::value;
-    auto mfma = [&](int j, auto do_o_c, auto do_s_c) __attribute__((always_inline)) {
+    auto mfma = [&](int j, auto do_o_c, auto do_s_c, auto between) __attribute__((always_inline)) {
       __builtin_amdgcn_s_setprio(1);
-      mfma_phase(j, do_o_c, do_s_c);
+      mfma_phase(j, do_o_c, do_s_c, between);
       __builtin_amdgcn_s_setprio(0);
     };
-    auto staged_all = [&](int j, int k) __attribute__((always_inline)) {   // team 1, slot 2j+1
+    auto nothing = [](int) {};
+    // Between the first MFMAs of team 0's M_j: K_{j+1} and V_j on their way.
+    Staging gk{}, gv{};
+    auto stage_tile = [&](int j) __attribute__((always_inline)) {
+      return [&, j](int i) __attribute__((always_inline)) {
+        if (i == 0) gk = staging_k(cu, j + 1);
+        if (i >= 1 && i <= kDma) stage_piece(gk, lane_k[i - 1], i - 1);
+        if (i == kDma + 1) gv = staging_v(cu, j);
+        if (i > kDma + 1 && i <= 2 * kDma + 1) stage_piece(gv, lane_v[i - kDma - 2], i - kDma - 2);
+      };
+    };
+    static_assert(KB * kSteps > 2 * kDma + 1, "the loads fit between the MFMAs");
+    auto staged_all = [&](int j, int k) __attribute__((always_inline)) {   // team 0, slot 2j+1
       wait_dma();
       if (j >= n_full) clean_v(j, k);
     };
     Unit nu = u_count > 1 ? to_unit(fetch_unit(u_first + 1)) : cu;  // the next unit
-    RawUnit nnu{};                                                   // the one after
+    RawUnit nnu = fetch_unit(u_first);                               // the one after
     bool staged = false;
     for (int k = 0; k < u_count; ++k) {
       const bool has_next = k + 1 < u_count;
@@ -519,58 +557,56 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
       if (k + 2 < u_count) nnu = fetch_unit(u_first + k + 2);
       if (n > 0) {
         if (kTeam == 0) {
-          if (!staged) __syncthreads();
-          mfma(0, no{}, yes{});
-          __syncthreads();
-          valu_phase(0);
-          __syncthreads();
-          for (int j = 1; j < n; ++j) {
-            mfma(j, yes{}, yes{});
-            __syncthreads();
-            valu_phase(j);
-            __syncthreads();
-          }
-          // Q is not read again in this unit.
-          if (has_next) load_q(nu, qb);
-          mfma(n, yes{}, no{});
-          __syncthreads();
-          finish_unit(k);
-          __syncthreads();
-        } else {
           if (!staged) {
             dma_k(cu, 0);
             wait_dma();
             __syncthreads();
           }
-          if (1 < n) dma_k(cu, 1);
-          dma_v(cu, 0);
+          mfma(0, no{}, yes{}, stage_tile(0));
           __syncthreads();
-          mfma(0, no{}, yes{});
+          valu_phase(0);
           staged_all(0, k);
           __syncthreads();
           for (int j = 1; j < n; ++j) {
-            if (j + 1 < n) dma_k(cu, j + 1);
-            dma_v(cu, j);
-            valu_phase(j - 1);
+            mfma(j, yes{}, yes{}, stage_tile(j));
             __syncthreads();
-            mfma(j, yes{}, yes{});
+            valu_phase(j);
             staged_all(j, k);
             __syncthreads();
           }
+          // Q is not read again in this unit (without a next one it is the same
+          // again: a branch would make the compiler wait for it and copy it).  The
+          // next unit's first K tile goes into lds.k[0], last read in slot 2n-1 or
+          // earlier.
+          load_q(nu, qb);
+          mfma(n, yes{}, no{}, [&](int i) __attribute__((always_inline)) {
+            if (i == 0) gk = staging_k(nu, 0);
+            if (i >= 1 && i <= kDma) stage_piece(gk, lane_k[i - 1], i - 1);
+          });
+          __syncthreads();
+          finish_unit(k, wait_dma);
+          __syncthreads();
+        } else {
+          if (!staged) __syncthreads();
+          __syncthreads();
+          mfma(0, no{}, yes{}, nothing);
+          __syncthreads();
+          for (int j = 1; j < n; ++j) {
+            valu_phase(j - 1);
+            __syncthreads();
+            mfma(j, yes{}, yes{}, nothing);
+            __syncthreads();
+          }
           valu_phase(n - 1);
-          // The next unit's Q, and its first K tile into lds.k[0], last read in slot
-          // 2n-1 or earlier.
-          if (has_next) load_q(nu, qb);
-          if (has_next && nu.ntiles > 0) dma_k(nu, 0);
+          load_q(nu, qb);
           __syncthreads();
-          mfma(n, yes{}, no{});
-          wait_dma();
+          mfma(n, yes{}, no{}, nothing);
           __syncthreads();
-          finish_unit(k);
+          finish_unit(k, [] {});
         }
       } else {
-        if (has_next) load_q(nu, qb);
-        finish_unit(k);
+        load_q(nu, qb);
+        finish_unit(k, [] {});
       }
       if (has_next) {
         staged = n > 0 && nu.ntiles > 0;
