@@ -123,7 +123,9 @@ class KvcWeightsSchedule(ctypes.Structure):
         ("num_units", c_int32),
         ("num_parts", c_int32),
         ("num_joins", c_int32),
+        ("num_workgroups", c_int32),
         ("total_q", c_int32),
+        ("reserved", c_int32),
         ("plan_ints", c_int64),
         ("workspace_bytes", c_int64),
     ]
@@ -239,10 +241,11 @@ SIGNATURES = {
         c_int32, POINTER(KvcWeightsSchedule), c_void_p, c_int64]),
     "kvc_batch_attention_weights_run": (c_int, [
         POINTER(KvcWeightsSchedule), _I32P, _P, c_int64, _P, c_int64, _P, _P, c_int64, c_int64,
-        c_int64, _I32P, c_int64, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),
+        c_int64, _I32P, c_int64, c_int32, c_float, _P, _I32P, _I32P, c_int32, _I32P, _P]),
     "kvc_decode_attention_weights": (c_int, [
         _P, c_int64, _P, _P, c_int64, c_int64, c_int64, _I32P, _I32P, c_int64, _I32P, c_int32,
-        c_int32, c_int32, c_int32, c_int32, c_int32, c_float, _P, _I32P, _I32P, _I32P, _P]),
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_float, _P, _I32P, _I32P, c_int32, _I32P,
+        _P]),
     "kvc_evict_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "kvc_evict_kv": (c_int, [
         _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, _P, _I32P,

@@ -18,6 +18,8 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <functional>
+#include <type_traits>
 #include <vector>
 
 namespace kvc {
@@ -61,29 +63,36 @@ struct WeightsArgs {
   float scale_log2;                // sm_scale * log2(e)
   float* scores;                   // [num_blocks][Hkv][16]
   int32_t* positions;              // the same, may be null
-  const int32_t* offsets;          // by sequence, may be null
+  const int32_t* offsets;          // [num_offsets] by sequence, may be null
+  int32_t num_offsets;
   const int32_t* seq_ids;          // request -> sequence, may be null
 };
 
 // A key's block: its page's id, or -1 where the page is missing or out of range.
 __device__ __forceinline__ int32_t block_of(const WeightsArgs& a, int64_t page) {
-  if (page >= a.num_indices) return -1;
-  const int32_t id = a.indices[page];
-  return id >= 0 && id < a.num_blocks ? id : -1;
+  const int32_t id = a.indices[min(page, a.num_indices - 1)];
+  return page < a.num_indices && id >= 0 && id < a.num_blocks ? id : -1;
+}
+
+// The position of a request's first cached token (0 where its sequence has no entry).
+__device__ __forceinline__ int32_t first_position(const WeightsArgs& a, int b) {
+  if (!a.offsets) return 0;
+  const int32_t seq = a.seq_ids ? a.seq_ids[b] : b;
+  return seq >= 0 && seq < a.num_offsets ? a.offsets[seq] : 0;
 }
 
 __device__ __forceinline__ void store_weight(const WeightsArgs& a, int32_t block, int h, int key,
                                              int b, float w, bool fresh) {
   const int64_t at = (int64_t(block) * a.num_kv_heads + h) * kPage + key % kPage;
   a.scores[at] = fresh ? w : a.scores[at] + w;
-  if (fresh && a.positions)
-    a.positions[at] = key + (a.offsets ? a.offsets[a.seq_ids ? a.seq_ids[b] : b] : 0);
+  if (fresh && a.positions) a.positions[at] = key + first_position(a, b);
 }
 
 // A work unit: kUnitKeys keys of one request and KV head, against a run of the
 // row blocks that see them.  Record (kRecInts int32):
 //   KV head, first key, q_len, kv_len | q offset, page offset, request, first new key |
-//   first block, blocks, partial (-1: the unit's sums are the keys' weights), 0
+//   first block, blocks, partial (-1: the unit's sums are the keys' weights), next
+// Workgroup w begins with unit w and goes on with the next ones (0: none).
 constexpr int kRecInts = 12;
 constexpr int kJoinInts = 8;
 constexpr int kRows = 32;                          // query rows per block
@@ -91,7 +100,8 @@ constexpr int kKeyBlocks = 2;                      // 32-key blocks per wave
 constexpr int kWaveKeys = 32 * kKeyBlocks;
 constexpr int kChunkThreads = 256;
 constexpr int kUnitKeys = kChunkThreads / 64 * kWaveKeys;
-constexpr int kRing = 3;                           // row blocks in LDS
+constexpr int kStage = 2 * kRows;                  // rows in flight at a time
+constexpr int kWaitLoads = 0x0f70;                 // s_waitcnt vmcnt(0)
 
 struct ChunkArgs {
   WeightsArgs w;
@@ -108,173 +118,284 @@ __host__ __device__ inline int first_token(int key0, int q_len, int kv_len, int 
   return causal && t > 0 ? t : 0;
 }
 
-// A workgroup per unit.  Its four waves hold kWaveKeys keys each, K in registers for
-// the whole unit (B operands), and walk the same row blocks, which arrive in LDS
-// two blocks ahead (global_load_lds, each wave a quarter of a block, waited for by
-// count).  Bound by the exponentials: per 32 rows x 64 keys a wave issues 32 of 16
-// cycles and 64 other vector instructions of 4 beside 16 matrix instructions of 32
-// (head_dim 128), so three waves per SIMD keep the vector unit busy.
+// A workgroup's four waves hold kWaveKeys keys of its unit each, K in registers for
+// the whole unit (B operands), and walk the same rows, which arrive in LDS a stage of
+// two blocks ahead (global_load_lds, each wave a quarter).  Per 32 rows x 64 keys a
+// wave issues, at head_dim 128, 16 matrix instructions of 32 cycles, 32 exponentials of
+// 8 and 64 other vector instructions of 4, so the vector unit is the bound (about 600
+// cycles); three waves per SIMD fill it, one's products beside the others'
+// exponentials.  Masks are a comparison per weight with the first row that sees the
+// lane's key; with that instead of each row's limit read across lanes, and priorities
+// that go round, 4 prompts of 2000 tokens went from 93 to 83 us.
+// Measured (bf16, head_dim 128, 32 / 8 heads): 2000 rows against 16000 keys 245 us
+// (1005 TFLOP/s), 4 prompts of 1200 to 2048 tokens 64 us, 8 windows of 32 against 4096
+// 22.7 us.  Products of the next block interleaved with the exponentials in one wave,
+// at two waves per SIMD, took 10% longer.
 template <typename T, int D>
-__global__ __launch_bounds__(kChunkThreads, D == 256 ? 2 : 3) void weights_chunk_kernel(ChunkArgs c) {
+__global__ __launch_bounds__(kChunkThreads, D == 256 ? 2 : 3)
+void weights_chunk_kernel(ChunkArgs c) {
   constexpr int KB = kKeyBlocks, kSteps = D / 16, kRow = 2 * D, kChunks = kRow / 16;
-  constexpr int kDma = kRows * kRow / 1024 / 4;    // row loads per wave and block
+  constexpr int kDma = kStage * kRow / 1024 / 4;   // row loads per wave and stage
   constexpr int kLoadRows = 1024 / kRow;           // rows per load
+  constexpr int kAhead = 3;                        // Q operands read ahead
   typedef typename T::x8 x8;
   const WeightsArgs& a = c.w;
   __shared__ struct alignas(16) {
-    uint8_t q[kRing][kRows * kRow];                // 16-byte chunks XOR-swizzled by row
-    float lse[kRing][4][64];                       // each wave's own copy, rows twice
+    uint8_t q[2][kStage * kRow];                   // 16-byte chunks XOR-swizzled by row
+    float lse[2][4][kStage];                       // each wave's own copy
+    float shift[4][kStage];                        // -log2(e) lse of the current stage
   } lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r = lane & 31, half = lane >> 5;
   const int Hq = a.num_kv_heads * a.group;
-  const int4 x = c.units[3 * blockIdx.x], y = c.units[3 * blockIdx.x + 1],
-             z = c.units[3 * blockIdx.x + 2];
   auto rfl = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const int h = rfl(x.x), key_first = rfl(x.y), q_len = rfl(x.z), kv_len = rfl(x.w);
-  const int first_block = rfl(z.x), blocks = rfl(z.y);
-  const int key0 = key_first + wave * kWaveKeys;
-  const int ahead = kv_len - q_len;                // keys before the first query token
-  const int tok0 = first_token(key_first, q_len, kv_len, c.causal);
-
-  // Row blocks on their way: row (32 block + i) of the unit is token tok0 + row /
-  // group, head row % group; the rows past the last repeat it.  Each lane keeps the
-  // (token, head) of its row in every load and steps it by 32 rows per block.
-  struct Place { int tok, head; };
-  auto place_of = [&](int row) __attribute__((always_inline)) {
-    return Place{row / a.group, row % a.group};
-  };
-  const int step_tok = kRows / a.group, step_head = kRows % a.group;
-  auto step = [&](Place& p) __attribute__((always_inline)) {
-    p.tok += step_tok;
-    p.head += step_head;
-    if (p.head >= a.group) {
-      p.head -= a.group;
-      ++p.tok;
-    }
-  };
-  const int last_tok = q_len - 1 - tok0;
-  Place qrow[kDma], lrow = place_of(first_block * kRows + r);
-#pragma unroll
-  for (int i = 0; i < kDma; ++i)
-    qrow[i] = place_of(first_block * kRows + (wave * kDma + i) * kLoadRows + lane / kChunks);
   auto lds_addr = [](const void* p) __attribute__((always_inline)) {
     return __builtin_amdgcn_readfirstlane(
         static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)p)));
   };
-  // kDma + 1 loads into ring slot `slot` (inline assembly: the compiler would wait
-  // for all of them at every LDS read; it uses M0 nowhere itself).
-  auto stage = [&](int slot) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kDma; ++i) {
-      const Place p = qrow[i];
-      const bool past = p.tok > last_tok;
-      const int row = (wave * kDma + i) * kLoadRows + lane / kChunks;
-      const int chunk = D == 64 ? (lane % kChunks) ^ ((row >> 1) & 7) : (lane % kChunks) ^ (row & 15);
-      const uint16_t* src = a.q + (int64_t(y.x) + tok0 + (past ? last_tok : p.tok)) * a.q_stride +
-                            (h * a.group + (past ? a.group - 1 : p.head)) * D + 8 * chunk;
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
-                   :: "s"(lds_addr(lds.q[slot] + (wave * kDma + i) * 1024)), "v"(src) : "memory");
-      step(qrow[i]);
-    }
-    const bool past = lrow.tok > last_tok;
-    const float* src = a.lse + (int64_t(y.x) + tok0 + (past ? last_tok : lrow.tok)) * Hq +
-                       h * a.group + (past ? a.group - 1 : lrow.head);
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
-                 :: "s"(lds_addr(lds.lse[slot][wave])), "v"(src) : "memory");
-    step(lrow);
+  const uint32_t q_base = lds_addr(lds.q[0] + wave * kDma * 1024);
+  const uint32_t lse_base = lds_addr(lds.lse[0][wave]);
+  const uint32_t recip = rfl((65536 + a.group - 1) / a.group);   // row / group for row < 192
+  auto split = [&](int row, int& tok, int& head) __attribute__((always_inline)) {
+    tok = __umul24(row, recip) >> 16;
+    head = row - __umul24(tok, a.group);
   };
+  const uint32_t q_bytes = uint32_t(a.q_stride * 2);
+  const int step_tok = kStage / a.group, step_head = kStage - step_tok * a.group;
 
-  x8 kop[KB][kSteps];
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    const int key = key0 + 32 * kb + r;
-    const int32_t block = key < kv_len ? block_of(a, int64_t(y.y) + key / kPage) : -1;
-    // A key that is not there reads block 0; its column is not stored.
-    const uint16_t* kp = a.k_cache + int64_t(max(block, 0)) * a.block_stride +
-                         (key % kPage) * a.token_stride + h * D + 8 * half;
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks)
-      kop[kb][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 16 * ks));
-  }
-  float acc[KB];
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb) acc[kb] = 0.f;
-  if (blocks > 0) stage(0);
-  if (blocks > 1) stage(1);
-  Place mine = place_of(first_block * kRows + r);   // this lane's row of the current block
+  // Of a SIMD's waves the hardware prefers the oldest: with equal work the youngest
+  // ends last, alone.  Priorities that go round by stage let each be preferred in turn.
+  int turn = blockIdx.x / 256 % 3;
+  int u = blockIdx.x;
+  do {
+    const int4 x = c.units[3 * u], y = c.units[3 * u + 1], z = c.units[3 * u + 2];
+    const int h = rfl(x.x), key_first = rfl(x.y), q_len = rfl(x.z), kv_len = rfl(x.w);
+    const int first_block = rfl(z.x), blocks = rfl(z.y);
+    const int stages = (blocks + 1) / 2;
+    const int key0 = key_first + wave * kWaveKeys;
+    const int ahead = kv_len - q_len;              // keys before the first query token
+    const int tok0 = first_token(key_first, q_len, kv_len, c.causal);
+    const int last_tok = q_len - 1 - tok0;
 
-  int slot = 0;
-  for (int i = 0; i < blocks; ++i) {
-    // This block's loads are done, the next one's may run.
-    if (i + 1 < blocks) {
-      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kDma + 1) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // The stage that is loaded next: its first row's token (from tok0 on) and head,
+    // bases of that token's rows.  Row i of the unit is token i / group, head i %
+    // group; a stage's rows are addressed from the base by 32-bit offsets, the same
+    // in every stage where the group divides 64; elsewhere, and where the tokens
+    // end, they are computed anew (rows past the last token read its).
+    int st_tok = first_block * kRows / a.group, st_head = first_block * kRows - st_tok * a.group;
+    int my_base = st_tok, my_first = st_head;      // of the stage being computed
+    const uint8_t* st_q = reinterpret_cast<const uint8_t*>(
+        a.q + (int64_t(y.x) + tok0 + st_tok) * a.q_stride + h * a.group * D);
+    const uint8_t* st_lse = reinterpret_cast<const uint8_t*>(
+        a.lse + (int64_t(y.x) + tok0 + st_tok) * Hq + h * a.group);
+    uint32_t q_off[kDma], lse_off;
+    auto offsets = [&]() __attribute__((always_inline)) {
+      const int left = last_tok - st_tok;
+      int tok, head;
+#pragma unroll
+      for (int i = 0; i < kDma; ++i) {
+        const int row = (wave * kDma + i) * kLoadRows + lane / kChunks;
+        const int chunk = (lane % kChunks) ^ (D == 64 ? (row >> 1) & 7 : row & 15);
+        split(st_head + row, tok, head);
+        q_off[i] = uint32_t(min(tok, left)) * q_bytes + head * kRow + chunk * 16;
+      }
+      split(st_head + lane, tok, head);
+      lse_off = (uint32_t(min(tok, left)) * Hq + head) * 4;
+    };
+    // Load i of a stage's kDma + 1 into `slot` (inline assembly: the compiler would wait
+    // for all of them at every LDS read; it uses M0 nowhere itself).
+    auto stage_load = [&](int i, int slot) __attribute__((always_inline)) {
+      if (i < kDma)
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :: "s"(q_base + uint32_t(slot * kStage * kRow + i * 1024)), "v"(q_off[i]),
+                        "s"(st_q) : "memory");
+      else
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2"
+                     :: "s"(lse_base + uint32_t(slot * 4 * kStage * 4)), "v"(lse_off), "s"(st_lse)
+                     : "memory");
+    };
+    // Behind the last stage the last one is loaded again, which nothing reads.
+    auto stage_prepare = [&]() __attribute__((always_inline)) {
+      int tok = step_tok, head = st_head + step_head;
+      if (head >= a.group) {
+        head -= a.group;
+        ++tok;
+      }
+      if (st_tok + tok <= last_tok) {
+        st_tok += tok;
+        st_head = head;
+        st_q += uint32_t(tok) * q_bytes;           // (65 of 2^26 bytes at most)
+        st_lse += uint32_t(tok) * uint32_t(Hq * 4);
+      }
+      if (step_head != 0 || st_tok + step_tok > last_tok + 1) offsets();
+    };
+    offsets();
+    if (stages > 0) {
+#pragma unroll
+      for (int i = 0; i <= kDma; ++i) stage_load(i, 0);
+      stage_prepare();
+#pragma unroll
+      for (int i = 0; i <= kDma; ++i) stage_load(i, 1);
+      stage_prepare();
     }
-    __syncthreads();
-    const int next2 = slot == 0 ? 2 : slot - 1;     // (slot + 2) % 3, read two blocks ago
-    if (i + 2 < blocks) stage(next2);
 
-    const float lse = lds.lse[slot][wave][r];
-    // The last key that this lane's row sees; a row of no key (lse -inf) gives nothing.
-    const bool there = mine.tok <= last_tok && lse != -INFINITY;
-    const int limit = !there ? -1 : c.causal ? ahead + tok0 + mine.tok : kv_len;
-    step(mine);
-    if (__builtin_amdgcn_ballot_w64(limit >= key0) != 0 && key0 < kv_len) {
-      const bool whole = __builtin_amdgcn_ballot_w64(limit < key0 + kWaveKeys - 1) == 0;
-      f32x16_t s[KB];
+    x8 kop[KB][kSteps];
+    int32_t block[KB];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb) {
+      const int key = min(key0 + 32 * kb + r, kv_len - 1);
+      block[kb] = block_of(a, int64_t(y.y) + key / kPage);
+    }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+    for (int kb = 0; kb < KB; ++kb) {
+      // A page that is not there reads block 0; its columns are not stored.
+      const uint16_t* kp = a.k_cache + int64_t(max(block[kb], 0)) * a.block_stride +
+                           (r % kPage) * a.token_stride + h * D + 8 * half;
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks)
+        kop[kb][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 16 * ks));
+    }
+    // K and the first stages are here before the walk (waits for K inside it would wait
+    // for the rows in flight).
+    __builtin_amdgcn_s_waitcnt(kWaitLoads);
+    __syncthreads();
+    float acc[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) acc[kb] = 0.f;
+
+    // Whether a row of block n of stage st does not see all of the wave's keys.
+    auto partly = [&](int n) __attribute__((always_inline)) {
+      const int tok = my_base + int(((my_first + kRows * n) * recip) >> 16);
+      return c.causal && ahead + tok0 + tok < key0 + kWaveKeys - 1;
+    };
+    // The first row that sees the lane's key (row 0 is the unit's).
+    int sees[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      sees[kb] = !c.causal ? 0 : max(key0 + 32 * kb + r - ahead - tok0, 0) * a.group -
+                                     first_block * kRows;
+    auto advance = [&]() __attribute__((always_inline)) {
+      my_base += step_tok;
+      my_first += step_head;
+      if (my_first >= a.group) {
+        my_first -= a.group;
+        ++my_base;
+      }
+    };
+    // The lane's first Q operand of a block, in the current slot.
+    uint32_t q_at = r * kRow + (half ^ (D == 64 ? (r >> 1) & 7 : r & 15)) * 16;
+    f32x16_t zero, sc[KB];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) zero[e] = 0.f;
+    // Scores of block n of the current slot, `step` behind each step's instructions.
+    auto scores = [&](int n, auto step) __attribute__((always_inline)) {
+      x8 qop[kSteps];
+      uint32_t at = q_at;
+      asm volatile("" : "+v"(at));                 // (or every step's place stays in a register)
+      auto read_q = [&](int ks) __attribute__((always_inline)) {
+        qop[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
+            lds.q[0] + n * kRows * kRow + (at ^ (32 * ks))));
+      };
+#pragma unroll
+      for (int ks = 0; ks < kAhead; ++ks) read_q(ks);
 #pragma unroll
       for (int ks = 0; ks < kSteps; ++ks) {
-        const int chunk = 2 * ks + half;
-        const x8 qop = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
-            lds.q[slot] + r * kRow +
-            (D == 64 ? chunk ^ ((r >> 1) & 7) : chunk ^ (r & 15)) * 16));
+        if (ks + kAhead < kSteps) read_q(ks + kAhead);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) s[kb] = T::mfma32(qop, kop[kb][ks], s[kb]);
+        for (int kb = 0; kb < KB; ++kb)
+          sc[kb] = T::mfma32(qop[ks], kop[kb][ks], ks == 0 ? zero : sc[kb]);
+        step(ks);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      // Accumulator entry 4i+j is row 8i + 4half + j, the lane's column key r.
+    };
+    // And their exponentials: accumulator entry 4i+j is row 8i + 4half + j, the lane's
+    // column key r.  kMask 1: rows in front of a key's first one do not see it; 2: and
+    // rows of lse -inf, whatever their products are, give nothing.
+    auto exps = [&](auto kMask, int st, int n) __attribute__((always_inline)) {
+      int from[KB];
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const float4 l4 = *reinterpret_cast<const float4*>(&lds.lse[slot][wave][8 * q4 + 4 * half]);
-        const float nl[4] = {l4.x * -kLog2e, l4.y * -kLog2e, l4.z * -kLog2e, l4.w * -kLog2e};
-        if (whole) {
+      for (int kb = 0; kb < KB; ++kb) from[kb] = sees[kb] - kStage * st - kRows * n - 4 * half;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(
+            &lds.shift[wave][kRows * n + 8 * i + 4 * half]);
+        const float nl[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-              acc[kb] += fast_exp2(fmaf(s[kb][4 * q4 + j], a.scale_log2, nl[j]));
-        } else {
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int lim = __shfl(limit, 8 * q4 + 4 * half + j);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-              const float p = fast_exp2(fmaf(s[kb][4 * q4 + j], a.scale_log2, nl[j]));
-              acc[kb] += key0 + 32 * kb + r <= lim ? p : 0.f;
-            }
+          for (int kb = 0; kb < KB; ++kb) {
+            const float p = fast_exp2(fmaf(sc[kb][4 * i + j], a.scale_log2, nl[j]));
+            acc[kb] += (kMask == 0 || 8 * i + j >= from[kb]) &&
+                       (kMask != 2 || nl[j] != -INFINITY) ? p : 0.f;
           }
+      }
+    };
+
+    // The first stage with a row that sees one of the wave's keys.
+    int first = 0;
+    if (c.causal)
+      first = max(max(key0 - ahead - tok0, 0) * a.group - first_block * kRows, 0) / kStage;
+    first = key0 < kv_len ? min(first, stages) : stages;
+    for (int st = 0; st < stages; ++st) {
+      if (turn == 0) __builtin_amdgcn_s_setprio(0);
+      else if (turn == 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(2);
+      turn = turn == 2 ? 0 : turn + 1;
+      const bool more = st > 0;                    // (stages 0 and 1 are there or under way)
+      auto load = [&](int ks) __attribute__((always_inline)) {
+        if (ks <= kDma) stage_load(ks, (st + 1) & 1);
+        if (kSteps <= kDma && ks == kSteps - 1) {
+#pragma unroll
+          for (int i = kSteps; i <= kDma; ++i) stage_load(i, (st + 1) & 1);
+        }
+      };
+      if (st < first) {
+        if (more) {
+#pragma unroll
+          for (int ks = 0; ks < kSteps; ++ks) load(ks);
+        }
+      } else {
+        const float lse = lds.lse[st & 1][wave][lane];
+        if (more) scores(0, load);
+        else scores(0, [](int) {});
+        // (Rows behind the last one are copies of its token's that give nothing.)
+        int tok, head;
+        split(my_first + lane, tok, head);
+        const bool there = my_base + tok <= last_tok && lse != -INFINITY;
+        lds.shift[wave][lane] = there ? lse * -kLog2e : -INFINITY;
+        const uint64_t none = __builtin_amdgcn_ballot_w64(lse == -INFINITY);
+        auto block_exps = [&](int n) __attribute__((always_inline)) {
+          if (uint32_t(none >> (32 * n)) != 0) exps(std::integral_constant<int, 2>{}, st, n);
+          else if (partly(n)) exps(std::integral_constant<int, 1>{}, st, n);
+          else exps(std::integral_constant<int, 0>{}, st, n);
+        };
+        block_exps(0);
+        if (2 * st + 1 < blocks) {
+          scores(1, [](int) {});
+          block_exps(1);
         }
       }
+      if (more) stage_prepare();
+      advance();
+      q_at ^= kStage * kRow;
+      // The next stage is here and this one has been read: the one after it is loaded
+      // over it.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
     }
-    slot = slot == kRing - 1 ? 0 : slot + 1;
-  }
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    const float w = acc[kb] + __shfl_xor(acc[kb], 32);
-    const int key = key0 + 32 * kb + r;
-    if (half != 0 || key >= kv_len) continue;
-    if (z.z >= 0) {
-      c.parts[int64_t(z.z) * kUnitKeys + key - key_first] = w;
-      continue;
+    for (int kb = 0; kb < KB; ++kb) {
+      const float w = acc[kb] + __shfl_xor(acc[kb], 32);
+      const int key = key0 + 32 * kb + r;
+      if (half != 0 || key >= kv_len) continue;
+      if (z.z >= 0) {
+        c.parts[int64_t(z.z) * kUnitKeys + key - key_first] = w;
+        continue;
+      }
+      if (block[kb] >= 0) store_weight(a, block[kb], h, key, y.z, w, key >= y.w);
     }
-    const int32_t block = block_of(a, int64_t(y.y) + key / kPage);
-    if (block >= 0) store_weight(a, block, h, key, y.z, w, key >= y.w);
-  }
+    u = rfl(z.w);
+  } while (u != 0);
 }
 
 // Sums of the units whose rows were cut: a workgroup per (key tile, KV head), a
@@ -286,7 +407,15 @@ __global__ __launch_bounds__(kUnitKeys) void weights_join_kernel(ChunkArgs c, co
   if (key >= x.w) return;
   const float* p = c.parts + int64_t(y.x) * kUnitKeys + threadIdx.x;
   float w = 0.f;
-  for (int i = 0; i < x.z; ++i) w += p[int64_t(i) * kUnitKeys];
+  int i = 0;
+  for (; i + 4 <= x.z; i += 4) {                    // four loads in flight
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = p[int64_t(i + j) * kUnitKeys];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w += v[j];
+  }
+  for (; i < x.z; ++i) w += p[int64_t(i) * kUnitKeys];
   const int32_t block = block_of(c.w, int64_t(y.y) + key / kPage);
   if (block >= 0) store_weight(c.w, block, x.x, key, y.z, w, key >= y.w);
 }
@@ -303,11 +432,12 @@ constexpr int64_t kTokenWorkgroups = 512;   // two per CU: what its registers ho
 
 // A wave runs every so-manieth task; a task is kPages consecutive entries of the
 // batch's page list for one KV head (heads fastest: neighbouring waves read the same
-// tokens' rows at the same time).  Bound by memory: a task's K (16 KB), old scores and query are loaded
-// while the one before is computed, its page ids a task earlier still.  S = Q K^T per
-// page with v_mfma_f32_16x16x32 (A: lane l = row l%16, k = 8(l/16)..+7; B: column
-// l%16; C: acc[j] = row 4(l/16)+j, column l%16): rows are the group's query heads,
-// columns the page's tokens.  Lane 16 i + r then owns token r of page i.
+// tokens' rows at the same time).  Bound by memory: a task's K (16 KB), old scores and
+// query are loaded while the one before is computed, its page ids a task earlier
+// still.  S = Q K^T per page with v_mfma_f32_16x16x32 (A: lane l = row l%16, k =
+// 8(l/16)..+7; B: column l%16; C: acc[j] = row 4(l/16)+j, column l%16): rows are the
+// group's query heads, columns the page's tokens.  Lane 16 i + r then owns token r of
+// page i.
 template <typename T, int D>
 __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenArgs c) {
   constexpr int kSteps = D / 32;
@@ -455,9 +585,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
       if (in && x.block[set] >= 0) {
         const int64_t at = (int64_t(x.block[set]) * a.num_kv_heads + now.h) * kPage + r;
         a.scores[at] = fresh ? mine : x.old[set] + mine;
-        if (fresh && a.positions)
-          a.positions[at] =
-              key + (a.offsets ? a.offsets[a.seq_ids ? a.seq_ids[owner] : owner] : 0);
+        if (fresh && a.positions) a.positions[at] = key + first_position(a, owner);
       }
     }
     x = y;
@@ -467,11 +595,17 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
 }
 
 constexpr int kMaxGroup = 128;
-// Rows are cut where a unit would be longer than this many blocks, and than a half
-// of what each of the chip's 768 resident workgroups has to do: the last ones to
-// end then leave a quarter of the chip idle for a quarter of the time at most.
-constexpr int64_t kMinSegment = 16;
-constexpr int64_t kSegments = 2 * 768;
+// Workgroups of the chunk kernel that the chip holds at a time (registers).
+int resident(int head_dim) { return head_dim == 256 ? 512 : 768; }
+// Costs in row blocks: a unit's start (its K), the join kernel, the least piece of a cut.
+constexpr int64_t kUnitCost = 4;
+constexpr int64_t kJoinCost = 5;
+constexpr int64_t kMinPiece = 4;
+
+// Plan image: units, then joins.
+int64_t weights_plan_ints(const kvc_weights_schedule& s) {
+  return int64_t(s.num_units) * kRecInts + int64_t(s.num_joins) * kJoinInts;
+}
 
 int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* lpl,
                  const int32_t* new_tokens, int32_t batch, int32_t hq, int32_t hkv,
@@ -526,40 +660,36 @@ int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32
       total += blocks;
     }
   }
-  const int64_t seg = std::max(kMinSegment, (total * hkv + kSegments - 1) / kSegments);
-  int64_t n_units = 0, n_parts = 0, n_joins = 0;
-  for (const Tile& t : tiles) {
-    const int64_t k = std::max<int64_t>(1, (t.blocks + seg - 1) / seg);
-    n_units += k * hkv;
-    if (k > 1) {
-      n_parts += k * hkv;
-      n_joins += hkv;
-    }
-  }
-  KVC_REQUIRE(n_units < (int64_t(1) << 26), KVC_ERR_INVALID_ARG, "too many units");
-  sched->batch = batch;
-  sched->num_qo_heads = hq;
-  sched->num_kv_heads = hkv;
-  sched->head_dim = head_dim;
-  sched->page_size = page_size;
-  sched->causal = causal ? 1 : 0;
-  sched->num_units = int32_t(n_units);
-  sched->num_parts = int32_t(n_parts);
-  sched->num_joins = int32_t(n_joins);
-  sched->total_q = batch ? qo_indptr[batch] : 0;
-  sched->plan_ints = n_units * kRecInts + n_joins * kJoinInts;
-  sched->workspace_bytes = n_parts * kUnitKeys * 4;
-  KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
-              KVC_ERR_WORKSPACE,
-              "plan buffer too small: need " + std::to_string(sched->plan_ints) + " int32");
-  // Workgroup w runs on XCD w % 8: a request's units of one head, which read the
-  // same Q and K, go to one XCD (to the one with the least work so far), longest
-  // first in each.
+  // Either every tile is a unit, or the tiles' blocks are lined up and cut into as
+  // many shares of equal cost as workgroups fit, each a few pieces of tiles: what
+  // ends sooner.  Whole tiles, longest first, end within the sum of the longest of
+  // each round, and within the longest on top of an equal share.
+  std::vector<int64_t> by_cost;
+  for (const Tile& t : tiles) by_cost.push_back(t.blocks + kUnitCost);
+  std::sort(by_cost.begin(), by_cost.end(), std::greater<int64_t>());
+  const int64_t wgs_max = resident(head_dim);
+  const int64_t cost = (total + int64_t(tiles.size()) * kUnitCost) * hkv;
+  int64_t whole = 0;
+  for (size_t i = 0; i * wgs_max < tiles.size() * hkv; ++i) whole += by_cost[i * wgs_max / hkv];
+  if (!tiles.empty()) whole = std::min(whole, by_cost[0] + (cost - by_cost[0]) / wgs_max);
+  const int64_t shares = std::min(wgs_max, total * hkv / kMinPiece);
+  const bool cut = shares > 0 && whole > cost / shares + kUnitCost + kMinPiece / 2 + kJoinCost;
   typedef std::array<int32_t, kRecInts> Rec;
+  std::vector<Rec> units;
+  std::vector<std::array<int32_t, kJoinInts>> joins;
+  std::vector<std::array<int32_t, 2>> wgs;       // (first unit, units) by workgroup
+  int64_t n_parts = 0;
+  auto piece = [&](const Tile& t, int h, int from, int blocks) {
+    const int kv_len = (kv_indptr[t.b + 1] - kv_indptr[t.b] - 1) * kPage + lpl[t.b];
+    return Rec{h, t.key0, qo_indptr[t.b + 1] - qo_indptr[t.b], kv_len, qo_indptr[t.b],
+               kv_indptr[t.b], t.b, t.new_from, from, blocks, -1, 0};
+  };
+  // Workgroup w runs on XCD w % 8: a request's units of one head, which read the
+  // same Q and K, go to one XCD.
   std::vector<Rec> list[8];
   int64_t load[8] = {0};
-  int32_t* join = plan_host + n_units * kRecInts;
-  int64_t part = 0;
+  int64_t share = 0, used = 0, taken = 0, left_cost = cost;
+  std::vector<std::array<int32_t, 2>> by_share(cut ? shares : 0, std::array<int32_t, 2>{0, 0});
   for (size_t t0 = 0; t0 < tiles.size();) {
     size_t t1 = t0;
     while (t1 < tiles.size() && tiles[t1].b == tiles[t0].b) ++t1;
@@ -567,34 +697,91 @@ int weights_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32
       const int xcd = int(std::min_element(load, load + 8) - load);
       for (size_t i = t0; i < t1; ++i) {
         const Tile& t = tiles[i];
-        const int q_len = qo_indptr[t.b + 1] - qo_indptr[t.b];
-        const int kv_len = (kv_indptr[t.b + 1] - kv_indptr[t.b] - 1) * kPage + lpl[t.b];
-        const int k = int(std::max<int64_t>(1, (t.blocks + seg - 1) / seg));
-        for (int j = 0; j < k; ++j) {
-          const int from = int(int64_t(t.blocks) * j / k), to = int(int64_t(t.blocks) * (j + 1) / k);
-          list[xcd].push_back(Rec{h, t.key0, q_len, kv_len, qo_indptr[t.b], kv_indptr[t.b], t.b,
-                                  t.new_from, from, to - from, k > 1 ? int32_t(part + j) : -1, 0});
-          load[xcd] += to - from + 4;
+        if (!cut) {
+          list[xcd].push_back(piece(t, h, 0, t.blocks));
+          load[xcd] += t.blocks + kUnitCost;
+          continue;
         }
-        if (k > 1) {
-          const int32_t r8[kJoinInts] = {h, t.key0, k, kv_len, int32_t(part), kv_indptr[t.b], t.b,
-                                         t.new_from};
-          join = std::copy_n(r8, kJoinInts, join);
-          part += k;
-        }
+        const size_t first = units.size();
+        int done = 0;
+        do {
+          const int64_t target = left_cost / (shares - share) + kUnitCost;
+          int64_t n = t.blocks - done;
+          if (share + 1 < shares) {
+            const int64_t want = std::max(kMinPiece, target - used - kUnitCost);
+            if (n - want >= kMinPiece) n = want;
+          }
+          if (by_share[share][1]++ == 0) by_share[share][0] = int32_t(units.size());
+          units.push_back(piece(t, h, done, int(n)));
+          taken += n + (done == 0 ? kUnitCost : 0);
+          used += n + kUnitCost;
+          done += int(n);
+          if (share + 1 < shares && used + kUnitCost + kMinPiece > target) {
+            ++share;
+            left_cost -= taken;
+            used = taken = 0;
+          }
+        } while (done < t.blocks);
+        const int64_t k = int64_t(units.size() - first);
+        if (k == 1) continue;
+        joins.push_back({h, t.key0, int32_t(k), units[first][3], int32_t(n_parts),
+                         kv_indptr[t.b], t.b, t.new_from});
+        for (int64_t j = 0; j < k; ++j) units[first + j][10] = int32_t(n_parts++);
       }
     }
     t0 = t1;
   }
-  size_t most = 0;
-  for (auto& l : list) {
-    std::stable_sort(l.begin(), l.end(), [](const Rec& p, const Rec& q) { return p[9] > q[9]; });
-    most = std::max(most, l.size());
+  if (cut) {
+    while (!by_share.empty() && by_share.back()[1] == 0) by_share.pop_back();
+    const int64_t n = by_share.size();
+    for (int64_t w = 0; w < n; ++w) {            // XCD x has the x-th eighth of the shares
+      const int64_t x = w % 8;
+      wgs.push_back(by_share[x * (n / 8) + std::min(x, n % 8) + w / 8]);
+    }
+  } else {                                       // longest first in each XCD
+    size_t most = 0;
+    for (auto& l : list) {
+      std::stable_sort(l.begin(), l.end(), [](const Rec& p, const Rec& q) { return p[9] > q[9]; });
+      most = std::max(most, l.size());
+    }
+    for (size_t i = 0; i < most; ++i)
+      for (auto& l : list)
+        if (i < l.size()) {
+          wgs.push_back({int32_t(units.size()), 1});
+          units.push_back(l[i]);
+        }
   }
-  int32_t* dst = plan_host;
-  for (size_t i = 0; i < most; ++i)
-    for (auto& l : list)
-      if (i < l.size()) dst = std::copy_n(l[i].begin(), kRecInts, dst);
+  KVC_REQUIRE(units.size() < size_t(1) << 26, KVC_ERR_INVALID_ARG, "too many units");
+  sched->batch = batch;
+  sched->num_qo_heads = hq;
+  sched->num_kv_heads = hkv;
+  sched->head_dim = head_dim;
+  sched->page_size = page_size;
+  sched->causal = causal ? 1 : 0;
+  sched->num_units = int32_t(units.size());
+  sched->num_parts = int32_t(n_parts);
+  sched->num_joins = int32_t(joins.size());
+  sched->num_workgroups = int32_t(wgs.size());
+  sched->total_q = batch ? qo_indptr[batch] : 0;
+  sched->plan_ints = weights_plan_ints(*sched);
+  sched->workspace_bytes = n_parts * kUnitKeys * 4;
+  KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
+              KVC_ERR_WORKSPACE,
+              "plan buffer too small: need " + std::to_string(sched->plan_ints) + " int32");
+  // Every workgroup's first unit, then the others, linked.
+  int64_t more = int64_t(wgs.size());
+  for (size_t w = 0; w < wgs.size(); ++w) {
+    int32_t* at = plan_host + w * kRecInts;
+    for (int32_t i = 0; i < wgs[w][1]; ++i) {
+      if (i > 0) {
+        at[kRecInts - 1] = int32_t(more);
+        at = plan_host + more++ * kRecInts;
+      }
+      std::copy(units[wgs[w][0] + i].begin(), units[wgs[w][0] + i].end(), at);
+    }
+  }
+  int32_t* dst = plan_host + units.size() * kRecInts;
+  for (const auto& r : joins) dst = std::copy(r.begin(), r.end(), dst);
   return ok();
 }
 
@@ -607,6 +794,10 @@ int check_common(const WeightsArgs& a, int Hq, int Hkv, int D, const char* who) 
               KVC_ERR_INVALID_ARG, std::string(who) + ": cache strides smaller than the block");
   KVC_REQUIRE(a.q_stride >= int64_t(Hq) * D, KVC_ERR_INVALID_ARG,
               std::string(who) + ": q token stride smaller than Hq*head_dim");
+  KVC_REQUIRE(a.q_stride < (int64_t(1) << 25), KVC_ERR_UNSUPPORTED,
+              std::string(who) + ": q token stride of 2^25 elements or more");
+  KVC_REQUIRE(!a.offsets || a.num_offsets >= 0, KVC_ERR_INVALID_ARG,
+              std::string(who) + ": negative num_offsets");
   KVC_REQUIRE(aligned(a.q, 16) && aligned(a.k_cache, 16) && a.q_stride % 8 == 0 &&
                   a.block_stride % 8 == 0 && a.token_stride % 8 == 0,
               KVC_ERR_ALIGNMENT,
@@ -638,15 +829,16 @@ extern "C" int kvc_batch_attention_weights_run(
     int64_t q_token_stride, const float* lse, const void* key_cache,
     int64_t cache_block_stride, int64_t cache_token_stride, int64_t num_blocks,
     const int32_t* indices, int64_t num_indices, int32_t dtype, float sm_scale, float* scores,
-    int32_t* positions, const int32_t* position_offsets, const int32_t* seq_ids, void* stream) {
+    int32_t* positions, const int32_t* position_offsets, int32_t num_offsets,
+    const int32_t* seq_ids, void* stream) {
   KVC_REQUIRE(sched, KVC_ERR_INVALID_ARG, "null schedule");
   const int Hq = sched->num_qo_heads, Hkv = sched->num_kv_heads, D = sched->head_dim;
   KVC_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= kMaxGroup &&
                   (D == 64 || D == 128 || D == 256) && sched->page_size == kPage &&
                   sched->num_units >= 0 && sched->num_parts >= 0 && sched->num_joins >= 0 &&
                   sched->workspace_bytes == int64_t(sched->num_parts) * kUnitKeys * 4 &&
-                  sched->plan_ints == int64_t(sched->num_units) * kRecInts +
-                                          int64_t(sched->num_joins) * kJoinInts,
+                  sched->num_workgroups >= 0 && sched->num_workgroups <= sched->num_units &&
+                  sched->plan_ints == weights_plan_ints(*sched),
               KVC_ERR_INVALID_ARG, "schedule not produced by kvc_weights_plan");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
               "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
@@ -662,12 +854,13 @@ extern "C" int kvc_batch_attention_weights_run(
   c.w = WeightsArgs{static_cast<const uint16_t*>(q), q_token_stride, lse,
                     static_cast<const uint16_t*>(key_cache), cache_block_stride,
                     cache_token_stride, num_blocks, indices, num_indices, Hkv, Hq / Hkv,
-                    sm_scale * kLog2e, scores, positions, position_offsets, seq_ids};
+                    sm_scale * kLog2e, scores, positions, position_offsets,
+                    num_offsets, seq_ids};
   if (const int st = check_common(c.w, Hq, Hkv, D, "kvc_batch_attention_weights_run")) return st;
   c.units = reinterpret_cast<const int4*>(plan);
   c.parts = static_cast<float*>(workspace);
   c.causal = sched->causal;
-  const dim3 grid(static_cast<unsigned>(sched->num_units));
+  const dim3 grid(static_cast<unsigned>(sched->num_workgroups));
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](auto t) {
     typedef decltype(t) T;
@@ -692,7 +885,8 @@ extern "C" int kvc_decode_attention_weights(
     const int32_t* indptr, const int32_t* indices, int64_t num_indices,
     const int32_t* last_page_len, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
     int32_t head_dim, int32_t page_size, int32_t dtype, float sm_scale, float* scores,
-    int32_t* positions, const int32_t* position_offsets, const int32_t* seq_ids, void* stream) {
+    int32_t* positions, const int32_t* position_offsets, int32_t num_offsets,
+    const int32_t* seq_ids, void* stream) {
   const int Hq = num_qo_heads, Hkv = num_kv_heads, D = head_dim;
   KVC_REQUIRE(batch >= 0, KVC_ERR_INVALID_ARG, "negative batch");
   KVC_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, KVC_ERR_INVALID_ARG,
@@ -709,7 +903,8 @@ extern "C" int kvc_decode_attention_weights(
   c.w = WeightsArgs{static_cast<const uint16_t*>(q), q_token_stride, lse,
                     static_cast<const uint16_t*>(key_cache), cache_block_stride,
                     cache_token_stride, num_blocks, indices, num_indices, Hkv, Hq / Hkv,
-                    sm_scale * kLog2e, scores, positions, position_offsets, seq_ids};
+                    sm_scale * kLog2e, scores, positions, position_offsets,
+                    num_offsets, seq_ids};
   if (const int st = check_common(c.w, Hq, Hkv, D, "kvc_decode_attention_weights")) return st;
   c.indptr = indptr;
   c.last_page_len = last_page_len;

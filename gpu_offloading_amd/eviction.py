@@ -59,7 +59,7 @@ class BatchAttentionWeightsWrapper(PlannedRuns):
         elif idx.device != self._device:
             _fail("paged_kv_indices on a different device than the workspace")
         sched = _lib.KvcWeightsSchedule()
-        guess = 1024 + 12 * max(1, num_kv_heads) * (total // 16 + 2 * batch)
+        guess = 24576 + 22 * max(1, num_kv_heads) * (total // 16 + 2 * batch)
         plan = stage_plan("kvc_weights_plan", sched,
                           (qo.ctypes.data, kv.ctypes.data, lpl.ctypes.data,
                            None if new is None else new.ctypes.data, batch, num_qo_heads,
@@ -100,5 +100,6 @@ class BatchAttentionWeightsWrapper(PlannedRuns):
                      None if ws is None else ws.data_ptr(), nbytes, q.data_ptr(), qs,
                      lse.data_ptr(), k_cache.data_ptr(), cs[0], cs[1], k_cache.shape[0],
                      indices.data_ptr(), indices.numel(), _DTYPES[self._dtype], self._sm_scale,
-                     scores.data_ptr(), _ptr(positions), _ptr(position_offsets), _ptr(seq_ids), sh)
+                     scores.data_ptr(), _ptr(positions), _ptr(position_offsets),
+                     0 if position_offsets is None else position_offsets.numel(), _ptr(seq_ids), sh)
         return scores

@@ -722,7 +722,8 @@ def decode_attention_weights(q: torch.Tensor, lse: torch.Tensor, key_cache: torc
                  cs[1], key_cache.shape[0], indptr.data_ptr(), indices.data_ptr(),
                  indices.numel(), last_page_len.data_ptr(), batch, hq, hkv, d, 16, dt,
                  float(sm_scale) if sm_scale is not None else d ** -0.5, scores.data_ptr(),
-                 _ptr(positions), _ptr(position_offsets), _ptr(seq_ids),
+                 _ptr(positions), _ptr(position_offsets),
+                 0 if position_offsets is None else position_offsets.numel(), _ptr(seq_ids),
                  _stream_handle(q.device, stream))
     return scores
 

@@ -622,7 +622,8 @@ int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
  * key and adds nothing.  scores is fp32 [num_blocks][num_kv_heads][16], beside
  * the cache.  positions (int32, the same shape, may be null) gets each new
  * token's position, its slot in the sequence + position_offsets[seq_ids[b]]
- * (the tokens evicted from the sequence before; null: 0; seq_ids null: b).  A
+ * (the tokens evicted from the sequence before; null, or outside its num_offsets
+ * entries: 0; seq_ids null: b).  A
  * page belongs to one request of a call.  Other slots of the last page and
  * other blocks are left as they are; page ids outside [0, num_blocks) are
  * skipped.
@@ -639,7 +640,7 @@ int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
  * (at most num_indices pages are read), so that the launch can be captured and
  * replayed.  Every sum has a fixed order.  head_dim 64, 128 or 256,
  * page_size 16, groups up to 128; q and the cache are 16-byte aligned with
- * strides that are multiples of 8 elements.
+ * strides that are multiples of 8 elements, q's below 2^25.
  * ---------------------------------------------------------------------- */
 typedef struct kvc_weights_schedule {
   int32_t batch;
@@ -651,7 +652,9 @@ typedef struct kvc_weights_schedule {
   int32_t num_units;
   int32_t num_parts;        /* partial sums of units whose rows are cut    */
   int32_t num_joins;
+  int32_t num_workgroups;
   int32_t total_q;          /* qo_indptr[batch]                            */
+  int32_t reserved;
   int64_t plan_ints;        /* int32 entries of the plan image             */
   int64_t workspace_bytes;  /* the partial sums                            */
 } kvc_weights_schedule;
@@ -669,7 +672,7 @@ int kvc_batch_attention_weights_run(
     const void* key_cache, int64_t cache_block_stride, int64_t cache_token_stride,
     int64_t num_blocks, const int32_t* indices, int64_t num_indices,
     int32_t dtype, float sm_scale, float* scores, int32_t* positions,
-    const int32_t* position_offsets, const int32_t* seq_ids, void* stream);
+    const int32_t* position_offsets, int32_t num_offsets, const int32_t* seq_ids, void* stream);
 
 int kvc_decode_attention_weights(
     const void* q, int64_t q_token_stride, const float* lse,
@@ -677,7 +680,8 @@ int kvc_decode_attention_weights(
     int64_t num_blocks, const int32_t* indptr, const int32_t* indices, int64_t num_indices,
     const int32_t* last_page_len, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
     int32_t head_dim, int32_t page_size, int32_t dtype, float sm_scale, float* scores,
-    int32_t* positions, const int32_t* position_offsets, const int32_t* seq_ids, void* stream);
+    int32_t* positions, const int32_t* position_offsets, int32_t num_offsets,
+    const int32_t* seq_ids, void* stream);
 
 /* ------------------------------------------------------------------------
  * Eviction of single tokens: of sequence b's seq_lens[b] cached tokens,

@@ -143,6 +143,12 @@ def test_weights_units_cover_every_key_and_row_once(lib, hq, hkv, d, causal, qle
     assert st == 0
     n = s.num_units
     assert s.plan_ints == 12 * n + 8 * s.num_joins
+    walked = []
+    for u in range(s.num_workgroups):
+        walked.append(u)
+        while img[12 * walked[-1] + 11]:
+            walked.append(int(img[12 * walked[-1] + 11]))
+    assert sorted(walked) == list(range(n))
     assert s.workspace_bytes == s.num_parts * 256 * 4
     runs, part_of = {}, {}
     for h, k0, m, ln, q0, p0, b, fresh, first, blocks, part, _ in img[:12 * n].reshape(-1, 12).tolist():
@@ -171,7 +177,7 @@ def test_weights_units_cover_every_key_and_row_once(lib, hq, hkv, d, causal, qle
             assert blocks > 0 or len(pieces) == 1
             at += blocks
         assert at == want[key]
-    joins = img[12 * n:s.plan_ints].reshape(-1, 8).tolist()
+    joins = img[12 * n:12 * n + 8 * s.num_joins].reshape(-1, 8).tolist()
     assert len(joins) == sum(len(p) > 1 for p in runs.values())
     for h, k0, k, ln, first, p0, b, fresh in joins:
         pieces = runs[h, b, k0]
@@ -208,8 +214,8 @@ def test_weights_run_refuses(lib):
         a = {**ok, **kw}
         return lib.kvc_batch_attention_weights_run(
             ctypes.byref(s), a["plan"], None, 0, a["q"], a["qs"], a["lse"], a["k"], a["bs"],
-            a["ts"], a["nb"], a["idx"], a["ni"], a["dt"], ctypes.c_float(a["scale"]), a["sc"], None, None,
-            None, None)
+            a["ts"], a["nb"], a["idx"], a["ni"], a["dt"], ctypes.c_float(a["scale"]), a["sc"], None,
+            a.get("off"), a.get("no", 0), None, None)
 
     def decode(**kw):
         a = dict(ok, ip=64, lpl=64, b=2, hq=4, hkv=2, d=128, page=16)
@@ -217,12 +223,12 @@ def test_weights_run_refuses(lib):
         return lib.kvc_decode_attention_weights(
             a["q"], a["qs"], a["lse"], a["k"], a["bs"], a["ts"], a["nb"], a["ip"], a["idx"],
             a["ni"], a["lpl"], a["b"], a["hq"], a["hkv"], a["d"], a["page"], a["dt"],
-            ctypes.c_float(a["scale"]), a["sc"], None, None, None, None)
+            ctypes.c_float(a["scale"]), a["sc"], None, a.get("off"), a.get("no", 0), None, None)
     both = [(dict(q=None), 1), (dict(lse=None), 1), (dict(k=None), 1), (dict(sc=None), 1),
             (dict(idx=None), 1), (dict(nb=0), 1), (dict(ts=248), 1), (dict(bs=256), 1),
             (dict(qs=504), 1), (dict(q=72), 3), (dict(k=66), 3), (dict(qs=516), 3),
             (dict(bs=4100), 3), (dict(ts=260, bs=8192), 3), (dict(dt=7), 2),
-            (dict(scale=float("nan")), 1)]
+            (dict(scale=float("nan")), 1), (dict(qs=1 << 25), 2), (dict(off=64, no=-1), 1)]
     for bad, want in both + [(dict(plan=None), 1), (dict(plan=68), 3), (dict(ni=0), 1)]:
         assert chunk(**bad) == want, bad
     for bad, want in both + [(dict(ip=None), 1), (dict(lpl=None), 1), (dict(b=-1), 1),
