@@ -749,9 +749,9 @@ def evict_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: torch.T
     of positions ``>= seq_lens[b] + position_offsets[b] - recent[b]``, without
     those of the last slots.  ``seq_lens``, ``keep``, ``recent``, ``position_offsets``
     are int32 per sequence, on the device; sequence b's pages are row
-    ``seq_ids[b]`` (default b) of ``block_table``.  ``max_seq_len`` (host int) must
-    bound every length.  ``workspace`` (uint8, ``evict_workspace_bytes``) is
-    allocated if not given."""
+    ``seq_ids[b]`` (distinct; default b) of ``block_table``.  ``max_seq_len`` (host
+    int) must bound every length.  ``workspace`` (uint8, ``evict_workspace_bytes``,
+    of one call at a time) is allocated if not given."""
     dev = _check_cuda(key_cache, value_cache, scores, block_table, seq_lens, keep, recent,
                       positions, position_offsets, seq_ids, workspace)
     shape, cs = _check_cache(key_cache, "key_cache")

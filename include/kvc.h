@@ -693,7 +693,7 @@ int kvc_decode_attention_weights(
  * go: K and V rows, scores and positions.  Afterwards the sequence's cache is
  * its slots [0, keep[b]); what the slots above hold is unspecified but was
  * not written.  A sequence of at most keep[b] tokens is left alone.
- * block_table rows are picked by seq_ids (null: row b); max_seq_len bounds every
+ * block_table rows are picked by seq_ids (distinct; null: row b); max_seq_len bounds every
  * seq_lens[b] (tokens past it, or past the table's row, are not considered);
  * tokens of pages outside [0, num_blocks) rank last and do not move.
  * Rows (head_dim * elem_bytes) are multiples of 16 bytes; the caches 16-byte
