@@ -105,8 +105,10 @@ class KvcPromptSchedule(ctypes.Structure):
         ("total_q", c_int32),
         ("total_kv", c_int32),
         ("max_key_tiles", c_int32),
-        ("reserved", c_int32),
+        ("num_joins", c_int32),
         ("plan_ints", c_int64),
+        ("num_parts", c_int64),
+        ("workspace_bytes", c_int64),
     ]
 
 
@@ -234,8 +236,8 @@ SIGNATURES = {
         c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
         POINTER(KvcPromptSchedule), c_void_p, c_int64]),
     "kvc_prompt_run": (c_int, [
-        POINTER(KvcPromptSchedule), _I32P, _P, c_int64, _P, c_int64, _P, c_int64, c_int32,
-        c_float, _P, c_int64, _P, _P]),
+        POINTER(KvcPromptSchedule), _I32P, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64,
+        c_int32, c_float, _P, c_int64, _P, _P]),
     "kvc_weights_plan": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
         c_int32, POINTER(KvcWeightsSchedule), c_void_p, c_int64]),

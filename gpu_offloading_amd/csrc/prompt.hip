@@ -13,6 +13,7 @@
 #include "kvc_common.h"
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <functional>
 #include <queue>
@@ -23,6 +24,7 @@
 namespace kvc {
 namespace {
 
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
@@ -57,13 +59,15 @@ struct PromptArgs {
   int64_t q_stride, k_stride, v_stride;   // elements between tokens
   const int2* wg_units;                   // [workgroups]: (first unit, units)
   const int4* units;                      // [units][2]: (KV head, first query, q_len, kv_len),
-                                          //             (q offset, k offset, key tiles, 0)
+                                          //             (q offset, k offset, key tiles, part)
   int32_t num_kv_heads, group, tile_tokens, causal;
   uint32_t inv_group;                     // 65536 / group, rounded up
   float scale_log2;                       // sm_scale * log2(e)
   uint16_t* out;
   int64_t out_stride;
   float* lse;                             // [total_q][Hq] natural log, may be null
+  float* parts;                           // [parts][tile rows][D] outputs of units' pieces
+  float* part_lse;                        // [parts][tile rows] their log-sum-exp, base 2
 };
 
 // The element types: bf16 and fp16 through the same kernel.
@@ -115,8 +119,27 @@ __device__ __forceinline__ int v_slot(int key, int chunk) {
   return D == 64 ? chunk ^ (4 * ((key >> 1) & 1)) : chunk ^ (4 * (key & 3));
 }
 
-// A work unit's record.
-struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles; };
+// A work unit's record: a tile of query rows of one KV head, against all key tiles that
+// they see (part 0) or against a run of them (part p: the piece's place among the
+// partials + 1; its keys' offset and length are the run's first key's).
+struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles, part; };
+
+// A lane's share of a piece's row (O^T entries as accumulated, normalised) and the
+// row's log-sum-exp.
+template <int D, int kBlocks>
+__device__ __forceinline__ void store_part(const PromptArgs& a, int part, int rows, int row,
+                                           int half, const f32x16_t (&o)[kBlocks], float l,
+                                           float m) {
+  const int64_t at = int64_t(part - 1) * rows + row;
+  float* p = a.parts + at * D + 4 * half;
+#pragma unroll
+  for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4_t*>(p + 32 * db + 8 * i) =
+          f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+  if (half == 0) a.part_lse[at] = l == 0.f ? -INFINITY : m + fast_log2(l);
+}
 
 // head_dim 64 and 128: eight waves in two teams of four, one workgroup per CU,
 // two waves per SIMD: wave w of team 0 and wave w of team 1 share SIMD w.  Each
@@ -195,7 +218,7 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   auto to_unit = [](const RawUnit& t) __attribute__((always_inline)) {
     auto rfl = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     return Unit{rfl(t.x.x), rfl(t.x.y), rfl(t.x.z), rfl(t.x.w), rfl(t.y.x), rfl(t.y.y),
-                rfl(t.y.z)};
+                rfl(t.y.z), rfl(t.y.w)};
   };
   // Rows of no token read the unit's first one; they are never stored.
   auto load_q = [&](const Unit& U, x8 (&dst)[kSteps]) __attribute__((always_inline)) {
@@ -469,47 +492,52 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
           }
       }
     }
-    uint8_t* stg = lds.ostage[wave];
-    // O^T entry (db, 4i+j) is head dim 32db + 8i + 4half + j: (db, i) is the row's
-    // 16-byte chunk 4db + i and half its 8-byte half.
-    uint8_t* wr = stg + r * kORow + 8 * half;
+    if (cu.part) {
+      before_stores();
+      store_part<D, kBlocks>(a, cu.part, 8 * kWaveRows, row, half, o, l, m_run);
+    } else {
+      uint8_t* stg = lds.ostage[wave];
+      // O^T entry (db, 4i+j) is head dim 32db + 8i + 4half + j: (db, i) is the row's
+      // 16-byte chunk 4db + i and half its 8-byte half.
+      uint8_t* wr = stg + r * kORow + 8 * half;
 #pragma unroll
-    for (int db = 0; db < kBlocks; ++db) {
+      for (int db = 0; db < kBlocks; ++db) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint2*>(wr + 16 * (4 * db + i)) =
-            make_uint2(pack2<T>(o[db][4 * i], o[db][4 * i + 1]),
-                       pack2<T>(o[db][4 * i + 2], o[db][4 * i + 3]));
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int kStoreRows = 64 / kChunks;      // rows per store
-    const int c = lane % kChunks;
-    uint8_t* obase = reinterpret_cast<uint8_t*>(
-        a.out + int64_t(cu.q_off + cu.tok0) * a.out_stride + int64_t(cu.h * a.group) * D);
-    before_stores();
-    // (a row's place is below that of the first token that is not there)
-    const uint32_t end = uint32_t(min(a.tile_tokens, cu.q_len - cu.tok0) * a.out_stride) * 2;
-#pragma unroll
-    for (int t0 = 0; t0 < kWaveRows / kStoreRows; t0 += 4) {
-      uint4 v[4];
-      uint32_t off[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int rr = (t0 + i) * kStoreRows + lane / kChunks;
-        v[i] = *reinterpret_cast<const uint4*>(stg + rr * kORow + 16 * c);
-        off[i] = lds.out_off[wave * kWaveRows + rr];
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint2*>(wr + 16 * (4 * db + i)) =
+              make_uint2(pack2<T>(o[db][4 * i], o[db][4 * i + 1]),
+                         pack2<T>(o[db][4 * i + 2], o[db][4 * i + 3]));
+        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      constexpr int kStoreRows = 64 / kChunks;      // rows per store
+      const int c = lane % kChunks;
+      uint8_t* obase = reinterpret_cast<uint8_t*>(
+          a.out + int64_t(cu.q_off + cu.tok0) * a.out_stride + int64_t(cu.h * a.group) * D);
+      before_stores();
+      // (a row's place is below that of the first token that is not there)
+      const uint32_t end = uint32_t(min(a.tile_tokens, cu.q_len - cu.tok0) * a.out_stride) * 2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (off[i] < end) store_stream(obase + (off[i] + uint32_t(16 * c)), v[i]);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int t0 = 0; t0 < kWaveRows / kStoreRows; t0 += 4) {
+        uint4 v[4];
+        uint32_t off[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = (t0 + i) * kStoreRows + lane / kChunks;
+          v[i] = *reinterpret_cast<const uint4*>(stg + rr * kORow + 16 * c);
+          off[i] = lds.out_off[wave * kWaveRows + rr];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (off[i] < end) store_stream(obase + (off[i] + uint32_t(16 * c)), v[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (row_ok && a.lse && half == 0)
+        a.lse[int64_t(cu.q_off + cu.tok0 + row_tok) * Hq + cu.h * a.group + row_head] =
+            l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
     }
-    if (row_ok && a.lse && half == 0)
-      a.lse[int64_t(cu.q_off + cu.tok0 + row_tok) * Hq + cu.h * a.group + row_head] =
-          l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
@@ -672,7 +700,8 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
   auto get_unit = [&](int u) __attribute__((always_inline)) {
     const int4 x = a.units[2 * u], y = a.units[2 * u + 1];
     auto rfl = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    return Unit{rfl(x.x), rfl(x.y), rfl(x.z), rfl(x.w), rfl(y.x), rfl(y.y), rfl(y.z)};
+    return Unit{rfl(x.x), rfl(x.y), rfl(x.z), rfl(x.w), rfl(y.x), rfl(y.y), rfl(y.z),
+                rfl(y.w)};
   };
   x8 qb[kSteps];
   // Rows of no token read the unit's first one; they are never stored.
@@ -916,7 +945,9 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
           }
       }
     }
-    if (row_ok) {
+    if (cu.part) {
+      store_part<D, kBlocks>(a, cu.part, 4 * kWaveRows, row, half, o, l, m_run);
+    } else if (row_ok) {
       // O^T entry (db, 4i+j) is head dim 32db + 8i + 4half + j of this lane's row.
       uint16_t* op = a.out + int64_t(cu.q_off + tok) * a.out_stride +
                      int64_t(cu.h * a.group + row_head) * D + 4 * half;
@@ -936,25 +967,76 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
   }
 }
 
+// Units that were cut along their keys: out = sum_i w_i O_i / sum_i w_i over the pieces,
+// w_i = 2^(lse_i - max lse).  A thread per four dims of a row.  Record: KV head, first
+// query, q_len, q offset | first partial, pieces, 0, 0.
+template <typename T, int D>
+__global__ __launch_bounds__(256)
+void prompt_join_kernel(PromptArgs a, const int4* joins, int rows) {
+  constexpr int kLanes = D / 4;
+  const int4 x = joins[2 * blockIdx.x], y = joins[2 * blockIdx.x + 1];
+  const int row = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, c = threadIdx.x % kLanes;
+  const int row_tok = int(row * a.inv_group >> 16), row_head = row - row_tok * a.group;
+  const int tok = x.y + row_tok;
+  if (row_tok >= a.tile_tokens || tok >= x.z) return;
+  const float* pl = a.part_lse + int64_t(y.x) * rows + row;
+  const f32x4_t* po =
+      reinterpret_cast<const f32x4_t*>(a.parts + (int64_t(y.x) * rows + row) * D) + c;
+  float m = -INFINITY;
+  for (int i = 0; i < y.y; ++i) m = fmaxf(m, pl[int64_t(i) * rows]);
+  const float base = m == -INFINITY ? 0.f : m;   // no piece saw a key: all weights are 0
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < y.y; ++i) {
+    const float w = fast_exp2(pl[int64_t(i) * rows] - base);
+    const f32x4_t v = po[int64_t(i) * rows * kLanes];
+    sum += w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(w, v[j], o[j]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int head = x.x * a.group + row_head;
+  *reinterpret_cast<uint2*>(a.out + int64_t(x.w + tok) * a.out_stride + int64_t(head) * D + 4 * c) =
+      make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+  if (a.lse && c == 0)
+    a.lse[int64_t(x.w + tok) * a.num_kv_heads * a.group + head] =
+        sum == 0.f ? -INFINITY : (base + fast_log2(sum)) * kLn2;
+}
+
 // Persistent workgroups: one per CU of an MI355X.
 constexpr int64_t kMaxWorkgroups = 256;
 constexpr int kUnitInts = 8;
-constexpr int kUnitCost = 3;      // a unit's start and end, in tiles
+constexpr int kJoinInts = 8;
+// Costs in key tiles: a unit's start and end, what a piece's fp32 output adds to them, the
+// join; and the shortest piece.
+constexpr int kUnitCost = 3, kPartCost = 3, kJoinCost = 5, kMinPiece = 4;
 constexpr int kXcds = 8;
 int64_t plan_workgroups(int64_t units) { return std::min(kMaxWorkgroups, units); }
 int64_t table_ints(int64_t workgroups) { return (2 * workgroups + 3) / 4 * 4; }
 
+// Plan image: the work list, then the joins' records.
+int64_t prompt_plan_ints(const kvc_prompt_schedule& s) {
+  return table_ints(s.num_workgroups) + int64_t(s.num_units) * kUnitInts +
+         int64_t(s.num_joins) * kJoinInts;
+}
+int64_t prompt_workspace_bytes(const kvc_prompt_schedule& s) {
+  return s.num_parts * tile_rows(s.head_dim) * (s.head_dim + 1) * 4;
+}
+
 // The work list: a table of the workgroups' (first unit, units), then the unit
 // records in workgroup order.  `rec`: a record per item (entry 0 the sequence, 6 its
-// tiles), sequence by sequence; a unit is an item of one KV head.
+// tiles, 7 a piece's place among the `parts` of one head, + 1), sequence by sequence; a
+// unit is an item of one KV head.
 //
 // Workgroup w runs on XCD w % 8, whose L2 serves the K and V of its units: the units
 // are lined up sequence by sequence and head by head, and the line is cut into eight
 // parts of equal cost, so that a head's K and V go through one XCD (seven heads at
 // most through two).  In each part units are dealt in line order, a head's longest
 // first, to the least loaded workgroup; the last quarter of a part longest first over
-// all its heads, which evens the ends out.
-void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W,
+// all its heads, which evens the ends out.  Where units are cut (few of them) they are
+// all dealt longest first to all workgroups.
+void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W, int parts_per_head,
                 int32_t* plan_host) {
   struct Line { int64_t item; int head, cost; };
   std::vector<Line> line;
@@ -966,7 +1048,8 @@ void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W,
     for (int h = 0; h < hkv; ++h) {
       const size_t at = line.size();
       for (int64_t i = i0; i < i1; ++i) {
-        const int cost = rec[i * kUnitInts + 6] + kUnitCost;
+        const int cost = rec[i * kUnitInts + 6] + kUnitCost +
+                         (rec[i * kUnitInts + 7] ? kPartCost : 0);
         line.push_back(Line{i, h, cost});
         total += cost;
       }
@@ -975,7 +1058,7 @@ void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W,
     }
     i0 = i1;
   }
-  const int parts = W % kXcds == 0 ? kXcds : 1;
+  const int parts = W % kXcds == 0 && !parts_per_head ? kXcds : 1;
   std::vector<std::vector<size_t>> lists(W);
   typedef std::pair<int64_t, int64_t> Slot;  // (load, workgroup)
   size_t u = 0;
@@ -988,7 +1071,7 @@ void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W,
     while (end < most && (end < least || x == parts - 1 || done + line[end].cost / 2 < until))
       done += line[end++].cost;
     size_t tail = end;
-    for (int64_t rest = (done - from) / 4; tail > u && rest > 0; --tail) rest -= line[tail - 1].cost;
+    for (int64_t rest = parts_per_head ? done : (done - from) / 4; tail > u && rest > 0; --tail) rest -= line[tail - 1].cost;
     std::stable_sort(line.begin() + tail, line.begin() + end,
                      [](const Line& p, const Line& q) { return p.cost > q.cost; });
     std::priority_queue<Slot, std::vector<Slot>, std::greater<Slot>> free_at;
@@ -1010,9 +1093,62 @@ void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W,
       int32_t* dst = plan_host + table + next * kUnitInts;
       std::copy_n(rec.data() + line[i].item * kUnitInts, kUnitInts, dst);
       dst[0] = line[i].head;
+      if (dst[7]) dst[7] += line[i].head * parts_per_head;
       ++next;
     }
   }
+}
+
+// Time in tiles of items that are units of hkv heads each, longest first on W workgroups:
+// within the sum of the longest of each round, and within the longest on top of an
+// equal share.
+int64_t estimate(std::vector<int>& costs, int hkv, int64_t W) {
+  std::sort(costs.begin(), costs.end(), std::greater<int>());
+  int64_t total = 0, rounds = 0;
+  for (const int c : costs) total += c;
+  total *= hkv;
+  for (size_t i = 0; i * W < costs.size() * hkv; ++i) rounds += costs[i * W / hkv];
+  return std::min(rounds, costs[0] + (total - costs[0]) / W);
+}
+
+// How units are cut along their keys: where fewer units than two rounds of workgroups
+// leave many of these idle, the items behind the `whole` longest go in pieces of at
+// most `longest` tiles (0: none does).  Measured: 8000 tokens of 4 query heads and one KV
+// head (125 units) 156 us whole, 82 cut; 4 sequences of 1000 to 1200 at head_dim 256, not
+// causal (284 units, two rounds) 92 and 72.
+struct Cut { int64_t whole; int longest; };
+
+Cut choose_cut(const std::vector<int>& tiles, int hkv) {
+  const int64_t n = int64_t(tiles.size()), W = kMaxWorkgroups;
+  if (n == 0 || n * hkv > 2 * W) return Cut{0, 0};
+  std::vector<int> costs;
+  int64_t total = 0;
+  for (const int t : tiles) costs.push_back(t + kUnitCost), total += t + kUnitCost;
+  int64_t best = estimate(costs, hkv, W);
+  if (best <= total * hkv / W + kUnitCost + kPartCost + kJoinCost) return Cut{0, 0};
+  best = best * 19 / 20;                         // (less is not worth the partials' traffic)
+  std::vector<int> sorted = tiles;
+  std::sort(sorted.begin(), sorted.end(), std::greater<int>());
+  Cut cut{0, 0};
+  for (const int64_t whole : {int64_t(0), n * hkv / W * W / hkv}) {
+    if (whole > 0 && whole >= n) continue;
+    for (const int k : {2, 3, 4, 6, 8, 12, 16}) {
+      const int longest = std::max(kMinPiece, (sorted[whole] + k - 1) / k);
+      costs.clear();
+      for (int64_t i = 0; i < n; ++i) {
+        const int t = sorted[i], pieces = i < whole ? 1 : std::max(1, (t + longest - 1) / longest);
+        for (int j = 0; j < pieces; ++j)
+          costs.push_back((t + pieces - 1) / pieces + kUnitCost + (pieces > 1 ? kPartCost : 0));
+      }
+      const int64_t time = estimate(costs, hkv, W) + kJoinCost;
+      if (time < best) {
+        best = time;
+        cut = Cut{whole, longest};
+      }
+    }
+    if (n * hkv < W) break;
+  }
+  return cut;
 }
 
 int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batch, int32_t hq,
@@ -1055,6 +1191,39 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
       rec.insert(rec.end(), r8, r8 + kUnitInts);
     }
   }
+  // Pieces in place of the items that are cut; joins: (first query, q_len, q offset,
+  // first partial, pieces) of one head.
+  std::vector<int> tiles;
+  for (size_t i = 0; i < rec.size(); i += kUnitInts) tiles.push_back(rec[i + 6]);
+  const Cut cut = choose_cut(tiles, hkv);
+  std::vector<std::array<int32_t, 5>> joins;
+  int parts = 0;
+  if (cut.longest > 0) {
+    // The longest `whole` items stay: those over `bar` tiles, and the first ones of them.
+    std::sort(tiles.begin(), tiles.end(), std::greater<int>());
+    const int bar = cut.whole > 0 ? tiles[cut.whole - 1] : INT32_MAX;
+    int64_t at_bar = cut.whole > 0 ? cut.whole - (std::lower_bound(tiles.begin(), tiles.end(), bar,
+                                                                  std::greater<int>()) -
+                                                 tiles.begin())
+                                   : 0;
+    std::vector<int32_t> cut_rec;
+    max_tiles = 0;
+    for (size_t i = 0; i < rec.size(); i += kUnitInts) {
+      const int32_t* r = rec.data() + i;
+      const int t = r[6];
+      const bool stays = t > bar || (t == bar && at_bar-- > 0);
+      const int pieces = stays ? 1 : std::max(1, (t + cut.longest - 1) / cut.longest);
+      if (pieces > 1) joins.push_back({r[1], r[2], r[4], parts, pieces});
+      for (int j = 0; j < pieces; ++j) {
+        const int from = int(int64_t(t) * j / pieces), to = int(int64_t(t) * (j + 1) / pieces);
+        const int32_t r8[kUnitInts] = {r[0], r[1], r[2], r[3] - from * per_tile, r[4],
+                                       r[5] + from * per_tile, to - from, pieces > 1 ? ++parts : 0};
+        cut_rec.insert(cut_rec.end(), r8, r8 + kUnitInts);
+        max_tiles = std::max(max_tiles, to - from);
+      }
+    }
+    rec = std::move(cut_rec);
+  }
   const int64_t n = int64_t(rec.size()) / kUnitInts;
   const int64_t W = plan_workgroups(n * hkv);
   sched->batch = batch;
@@ -1068,12 +1237,20 @@ int prompt_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, int32_t batc
   sched->total_q = int32_t(end_q);
   sched->total_kv = int32_t(end_kv);
   sched->max_key_tiles = max_tiles;
-  sched->reserved = 0;
-  sched->plan_ints = table_ints(W) + n * hkv * kUnitInts;
+  sched->num_joins = int32_t(joins.size()) * hkv;
+  sched->num_parts = int64_t(parts) * hkv;
+  sched->plan_ints = prompt_plan_ints(*sched);
+  sched->workspace_bytes = prompt_workspace_bytes(*sched);
   KVC_REQUIRE(plan_capacity >= sched->plan_ints && (plan_host || sched->plan_ints == 0),
               KVC_ERR_WORKSPACE,
               "plan buffer too small: need " + std::to_string(sched->plan_ints) + " int32");
-  if (n > 0) write_plan(rec, n, hkv, W, plan_host);
+  if (n > 0) write_plan(rec, n, hkv, W, parts, plan_host);
+  int32_t* dst = plan_host + sched->plan_ints - int64_t(sched->num_joins) * kJoinInts;
+  for (int h = 0; h < hkv; ++h)
+    for (const auto& j : joins) {
+      const int32_t r8[kJoinInts] = {h, j[0], j[1], j[2], j[3] + h * parts, j[4], 0, 0};
+      dst = std::copy_n(r8, kJoinInts, dst);
+    }
   return ok();
 }
 
@@ -1083,6 +1260,15 @@ void launch(const PromptArgs& a, int head_dim, unsigned workgroups, hipStream_t 
   if (head_dim == 64) prompt_kernel<T, 64><<<grid, block, 0, s>>>(a);
   else if (head_dim == 128) prompt_kernel<T, 128><<<grid, block, 0, s>>>(a);
   else prompt_wide_kernel<T, 256><<<grid, block, 0, s>>>(a);
+}
+
+template <typename T>
+void launch_join(const PromptArgs& a, int head_dim, const int4* joins, unsigned n, hipStream_t s) {
+  const int rows = tile_rows(head_dim);
+  const dim3 grid{n, unsigned(rows * head_dim / 1024)};
+  if (head_dim == 64) prompt_join_kernel<T, 64><<<grid, 256, 0, s>>>(a, joins, rows);
+  else if (head_dim == 128) prompt_join_kernel<T, 128><<<grid, 256, 0, s>>>(a, joins, rows);
+  else prompt_join_kernel<T, 256><<<grid, 256, 0, s>>>(a, joins, rows);
 }
 
 }  // namespace
@@ -1100,7 +1286,8 @@ extern "C" int kvc_prompt_plan(const int32_t* qo_indptr_host, const int32_t* kv_
 }
 
 extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* plan,
-                              const void* q, int64_t q_token_stride, const void* key,
+                              void* workspace, int64_t workspace_bytes, const void* q,
+                              int64_t q_token_stride, const void* key,
                               int64_t key_token_stride, const void* value,
                               int64_t value_token_stride, int32_t dtype, float sm_scale,
                               void* out, int64_t out_token_stride, float* lse, void* stream) {
@@ -1110,8 +1297,10 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
                   (D == 64 || D == 128 || D == 256) && sched->num_units >= 0 &&
                   sched->tile_tokens == tile_rows(D) / (Hq / Hkv) &&
                   sched->num_workgroups == plan_workgroups(sched->num_units) &&
-                  sched->plan_ints == table_ints(sched->num_workgroups) +
-                                          int64_t(sched->num_units) * kUnitInts,
+                  sched->num_joins >= 0 && sched->num_parts >= 0 &&
+                  sched->num_parts <= sched->num_units &&
+                  sched->plan_ints == prompt_plan_ints(*sched) &&
+                  sched->workspace_bytes == prompt_workspace_bytes(*sched),
               KVC_ERR_INVALID_ARG, "schedule not produced by kvc_prompt_plan");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
               "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
@@ -1133,6 +1322,10 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
                   value_token_stride % 8 == 0 && out_token_stride % 8 == 0,
               KVC_ERR_ALIGNMENT,
               "q/key/value/out/plan must be 16-byte aligned and token strides multiples of 8");
+  KVC_REQUIRE(sched->num_parts == 0 || (workspace && workspace_bytes >= sched->workspace_bytes),
+              KVC_ERR_WORKSPACE,
+              "workspace too small: need " + std::to_string(sched->workspace_bytes) + " bytes");
+  KVC_REQUIRE(aligned(workspace, 16), KVC_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
   PromptArgs a;
   a.q = static_cast<const uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(key);
@@ -1151,9 +1344,18 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
   a.out = static_cast<uint16_t*>(out);
   a.out_stride = out_token_stride;
   a.lse = lse;
+  a.parts = static_cast<float*>(workspace);
+  a.part_lse = a.parts + sched->num_parts * tile_rows(D) * D;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == KVC_DTYPE_BF16) launch<Bf16>(a, D, unsigned(sched->num_workgroups), s);
   else launch<Fp16>(a, D, unsigned(sched->num_workgroups), s);
   KVC_LAUNCH_CHECK();
+  if (sched->num_joins > 0) {
+    const int4* joins = reinterpret_cast<const int4*>(plan + sched->plan_ints -
+                                                      int64_t(sched->num_joins) * kJoinInts);
+    if (dtype == KVC_DTYPE_BF16) launch_join<Bf16>(a, D, joins, unsigned(sched->num_joins), s);
+    else launch_join<Fp16>(a, D, joins, unsigned(sched->num_joins), s);
+    KVC_LAUNCH_CHECK();
+  }
   return ok();
 }

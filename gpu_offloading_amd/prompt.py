@@ -127,7 +127,7 @@ class BatchPromptAttentionWrapper(PlannedRuns):
         sched = _lib.KvcPromptSchedule()
         group = max(1, num_qo_heads // max(1, num_kv_heads))
         tokens = int(max(0, int(qo[-1]) - int(qo[0])))
-        guess = 1024 + 8 * max(1, num_kv_heads) * (tokens * group // 256 + batch)
+        guess = 16384 + 8 * max(1, num_kv_heads) * (tokens * group // 256 + batch)
         plan = stage_plan("kvc_prompt_plan", sched,
                           (qo.ctypes.data, kv.ctypes.data, batch, num_qo_heads, num_kv_heads,
                            head_dim, 1 if causal else 0), guess, self._device)
@@ -166,8 +166,12 @@ class BatchPromptAttentionWrapper(PlannedRuns):
         elif (lse.dtype != torch.float32 or not lse.is_contiguous()
               or lse.numel() < total * hq or lse.device != self._device):
             _fail("lse must be contiguous float32 [tokens, num_qo_heads] on the wrapper's device")
-        _lib.call_on(dev, "kvc_prompt_run", s, self._plan_ptr, q.data_ptr(), qs, k.data_ptr(), ks,
-                     v.data_ptr(), vs, _DTYPES[dt], self._sm_scale, out.data_ptr(), os,
+        nbytes, ws = s.workspace_bytes, None
+        if nbytes:
+            ws = _empty(nbytes, torch.uint8, self._device, stream)
+        _lib.call_on(dev, "kvc_prompt_run", s, self._plan_ptr,
+                     None if ws is None else ws.data_ptr(), nbytes, q.data_ptr(), qs,
+                     k.data_ptr(), ks, v.data_ptr(), vs, _DTYPES[dt], self._sm_scale, out.data_ptr(), os,
                      None if lse is None else lse.data_ptr(), self._run_stream(stream))
         return (out, lse) if return_lse else out
 

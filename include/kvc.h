@@ -573,7 +573,10 @@ int kvc_decode_step_setup(const int32_t* host_image, int32_t* dev_image,
  * the value product.
  *
  * kvc_prompt_plan is host-only: one work unit per (tile of tile_tokens query
- * tokens, KV head), longest first, dealt to num_workgroups workgroups.  If
+ * tokens, KV head), dealt to num_workgroups workgroups.  Where few units would
+ * leave many workgroups idle, units are cut along their keys into pieces whose
+ * outputs (fp32, in workspace_bytes of device memory, 16-byte aligned, not kept
+ * between calls) a second kernel joins.  If
  * plan_capacity is too small it fills schedule->plan_ints and returns
  * KVC_ERR_WORKSPACE.  The caller copies the image (16-byte aligned) to the
  * device for kvc_prompt_run.  head_dim 64, 128 or 256, groups up to 128.
@@ -596,8 +599,10 @@ typedef struct kvc_prompt_schedule {
   int32_t total_q;          /* qo_indptr[batch]                            */
   int32_t total_kv;         /* kv_indptr[batch]                            */
   int32_t max_key_tiles;    /* most key tiles one unit visits              */
-  int32_t reserved;
+  int32_t num_joins;        /* (query tile, KV head) whose keys are cut    */
   int64_t plan_ints;        /* int32 entries of the plan image             */
+  int64_t num_parts;        /* units that are pieces of one                */
+  int64_t workspace_bytes;  /* the pieces' outputs                         */
 } kvc_prompt_schedule;
 
 int kvc_prompt_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host,
@@ -606,6 +611,7 @@ int kvc_prompt_plan(const int32_t* qo_indptr_host, const int32_t* kv_indptr_host
                     int32_t* plan_host, int64_t plan_capacity);
 
 int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
+                   void* workspace, int64_t workspace_bytes,
                    const void* q, int64_t q_token_stride,
                    const void* key, int64_t key_token_stride,
                    const void* value, int64_t value_token_stride,

@@ -208,3 +208,58 @@ def test_many_sequences_and_a_longer_one(gpu):
                                          i, True, 0.125)
         ref.assert_within(out[at + i:at + i + 1], o, otol, f"row {i}")
         ref.assert_within(lse[at + i:at + i + 1], l, ltol, f"row {i} lse")
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("qlens,kvlens,causal", [
+    ([2100], [2100], True), ([700, 1], [1900, 1], False), ([1700], [1300], True),
+    ([2900], [2400], True)])
+def test_keys_of_few_units_in_pieces(gpu, d, dtype, qlens, kvlens, causal):
+    """Few query tiles over many keys: pieces of them joined, in the same order every
+    time; queries that see no key, or none of a piece, among them."""
+    q, k, v, out, lse, w = _run(gpu, qlens, kvlens, 1, 3, d, dtype, causal, seed=d)
+    assert w.schedule.num_parts > 0 or (d == 64 and kvlens == [1300])
+    again, l2 = w.run(q, k, v, return_lse=True)
+    assert torch.equal(again, out[:sum(qlens)]) and torch.equal(l2, lse[:sum(qlens)])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_pieces_of_keys_that_are_not_finite(gpu, d, bad):
+    """In a late key's K or V they reach the queries that see it and no other."""
+    n, at = 2200, 1500
+    q = _randn(gpu, n, 2, d, seed=1, dtype=BF)
+    k, v = (_randn(gpu, n, 1, d, seed=i, dtype=BF) for i in (2, 3))
+    w = _wrapper(gpu)
+    w.plan(torch.tensor([0, n], dtype=torch.int32), num_qo_heads=2, num_kv_heads=1, head_dim=d)
+    assert w.schedule.num_parts > 0
+    want, wl = w.run(q, k, v, return_lse=True)
+    v[at, 0, 5] = bad
+    got, gl = w.run(q, k, v, return_lse=True)
+    assert torch.equal(got[:at], want[:at]) and torch.equal(gl, wl)
+    assert not torch.isfinite(got[at:, :, 5]).any()
+    rest = [i for i in range(d) if i != 5]
+    assert torch.equal(got[:, :, rest], want[:, :, rest])
+    k[at, 0, 5] = math.nan
+    got, gl = w.run(q, k, v, return_lse=True)
+    assert torch.equal(got[:at], want[:at]) and torch.equal(gl[:at], wl[:at])
+    assert torch.isnan(got[at:]).all() and torch.isnan(gl[at:]).all()
+
+
+def test_pieces_captured_and_replayed(gpu):
+    q, k, v, out, lse, w = _run(gpu, [1500], [1500], 1, 4, 128, BF, True, seed=5)
+    assert w.schedule.num_parts > 0
+    outs = [torch.empty_like(out) for _ in range(2)]
+    graphs = []
+    for o in outs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            w.run(q, k, v, out=o)
+    for seed in (1, 2, 3):
+        q.copy_(_randn(gpu, *q.shape, seed=seed, dtype=BF))
+        for g in graphs:
+            g.replay()
+        want = w.run(q, k, v)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o[:1500], want) for o in outs)

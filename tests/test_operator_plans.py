@@ -41,8 +41,8 @@ def _units(s, img):
         at += n
     assert at == s.num_units
     base = (2 * w + 3) // 4 * 4
-    assert s.plan_ints == base + 8 * s.num_units
-    return img[base:s.plan_ints].reshape(-1, 8)
+    assert s.plan_ints == base + 8 * s.num_units + 8 * s.num_joins
+    return img[base:base + 8 * s.num_units].reshape(-1, 8)
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (6, 2, 64), (7, 1, 256), (128, 1, 128)])
@@ -64,6 +64,45 @@ def test_prompt_units_cover_every_query_once(lib, hq, hkv, d, causal):
     want = {(h, int(qo[b]) + t) for h in range(hkv) for b in range(6)
             for t in range(0, qlens[b], s.tile_tokens)}
     assert seen == want and s.num_units == len(want)
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d,causal", [
+    ([4000], 4, 1, 128, 1), ([2300], 8, 1, 64, 1), ([5000], 2, 2, 256, 1),
+    ([2900, 200], 6, 2, 64, 0), ([1070, 1180, 1192, 991], 8, 4, 256, 0), ([2900, 1], 7, 1, 128, 0)])
+def test_prompt_pieces_cover_every_key_once(lib, lens, hq, hkv, d, causal):
+    """Few units: they are cut along their keys, and a join lists the pieces in order."""
+    qo, kv = _cum(lens), _cum([n + 100 for n in lens])
+    st, s, img = _prompt(lib, qo, kv, hq, hkv, d, causal)
+    assert st == 0 and s.num_joins > 0 and s.num_parts > 0
+    per, rows = 128 if d == 64 else 64, 128 if d == 256 else 256
+    assert s.tile_tokens == rows // (hq // hkv)
+    assert s.workspace_bytes == s.num_parts * rows * (d + 1) * 4
+    runs, part_of = {}, {}
+    for h, t0, m, n, q0, k0, tiles, part in _units(s, img).tolist():
+        b = [i for i in range(len(lens)) if qo[i] == q0 and lens[i] == m][0]
+        first = (k0 - int(kv[b])) // per
+        assert k0 - kv[b] == first * per and n == lens[b] + 100 - first * per and tiles > 0
+        runs.setdefault((h, b, t0), []).append((first, tiles, part))
+        if part:
+            assert part not in part_of
+            part_of[part] = (h, b, t0, first)
+    assert sorted(part_of) == list(range(1, s.num_parts + 1))
+    assert set(runs) == {(h, b, t) for h in range(hkv) for b in range(len(lens))
+                         for t in range(0, lens[b], s.tile_tokens)}
+    for (h, b, t0), pieces in runs.items():
+        last = min(t0 + s.tile_tokens, lens[b]) - 1
+        keys = min(lens[b] + 100, last + 101) if causal else lens[b] + 100
+        at = 0
+        for first, tiles, part in sorted(pieces):
+            assert first == at and (part > 0) == (len(pieces) > 1)
+            at += tiles
+        assert at == -(-keys // per)
+    joins = img[s.plan_ints - 8 * s.num_joins:s.plan_ints].reshape(-1, 8).tolist()
+    assert len(joins) == sum(len(p) > 1 for p in runs.values())
+    for h, t0, m, q0, part, n, *_ in joins:
+        b = [i for i in range(len(lens)) if qo[i] == q0][0]
+        assert m == lens[b] and n == len(runs[h, b, t0])
+        assert [p for _, _, p in sorted(runs[h, b, t0])] == list(range(part + 1, part + n + 1))
 
 
 def test_prompt_plan_asks_for_its_capacity(lib):
@@ -98,9 +137,9 @@ def test_prompt_run_refuses(lib):
 
     def run(**kw):
         a = {**ok, **kw}
-        return lib.kvc_prompt_run(ctypes.byref(s), a["plan"], a["q"], a["qs"], a["k"], a["ks"],
-                                  a["v"], a["vs"], a["dt"], ctypes.c_float(a["scale"]), a["out"],
-                                  a["os"], None, None)
+        return lib.kvc_prompt_run(ctypes.byref(s), a["plan"], a.get("ws"), a.get("wb", 0), a["q"],
+                                  a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["dt"],
+                                  ctypes.c_float(a["scale"]), a["out"], a["os"], None, None)
     for bad, want in ((dict(plan=None), 1), (dict(q=None), 1), (dict(v=None), 1),
                       (dict(out=None), 1), (dict(qs=1016), 1), (dict(ks=248), 1),
                       (dict(os=8), 1), (dict(vs=1 << 22), 1),
@@ -112,7 +151,13 @@ def test_prompt_run_refuses(lib):
         assert run(**bad) == want, bad
     s.num_units += 1
     assert run() == 1
-    assert lib.kvc_prompt_run(None, 64, 64, 1024, 64, 256, 64, 256, 1, ctypes.c_float(1.0), 64,
+    _, s, _ = _prompt(lib, _cum([4000]), _cum([4000]), 4, 1, 128)
+    assert s.num_parts > 0 and s.workspace_bytes == s.num_parts * 256 * 129 * 4
+    assert run(qs=512, os=512, ks=128, vs=128) == 4                        # no workspace
+    need = s.workspace_bytes
+    assert run(qs=512, os=512, ks=128, vs=128, ws=64, wb=need - 1) == 4
+    assert run(qs=512, os=512, ks=128, vs=128, ws=72, wb=need) == 3
+    assert lib.kvc_prompt_run(None, 64, None, 0, 64, 1024, 64, 256, 64, 256, 1, ctypes.c_float(1.0), 64,
                               1024, None, None) == 1
 
 
