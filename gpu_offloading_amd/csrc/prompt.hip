@@ -155,7 +155,7 @@ __device__ __forceinline__ void store_part(const PromptArgs& a, int part, int ro
 // last read in slot 2j-1) and waits for them before the barrier that ends slot 2j+1.
 // (Issued by the team in its VALU phase they cost 570 cycles of a slot of 1200.)
 // A workgroup runs a list of units: while one runs, the next one's record and Q
-// are loaded, and its first K tile is staged in the slot 2n of this one.
+// are loaded (slot 1), and its first K tile is staged in the slot 2n of this one.
 //
 // S^T tiles come from v_mfma_f32_32x32x16 (A: lane l = row l%32, k =
 // 8(l/32)..+7; B: column l%32, same k; C: acc[4i+j] = row 8i+4(l/32)+j, column
@@ -179,15 +179,17 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   typedef typename T::x8 x8;
   // One LDS object with the tiles first: operand reads then use immediate
   // offsets.  ostage: each wave's finished rows on their way out, padded so that
-  // one instruction's pieces spread over the banks.  out_off: the rows' places in the
-  // output, in bytes from the tile's first (kept in registers, they would spill, and a
-  // reload waits for every load and store in flight).  bad: the last unit (by its
+  // one instruction's pieces spread over the banks, and before that its next rows of Q on
+  // their way in (chunks swizzled as K's).  out_off, q_off: the rows' places in the
+  // output and in Q, in bytes from the tile's first (kept in registers, they would
+  // spill, and a reload waits for every load and store in flight).  bad: the last unit (by its
   // parity) whose boundary tiles held an inf or NaN in V.
   struct Lds {
     uint8_t k[2][kTile];
     uint8_t v[2][kTile];
     uint8_t ostage[8][kWaveRows * kORow];
     uint32_t out_off[8 * kWaveRows];
+    uint32_t q_off[8 * kWaveRows];
     int bad[2];
   };
   __shared__ alignas(16) Lds lds;
@@ -203,9 +205,11 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   const int row_head = row - row_tok * a.group;
   const int Hq = a.num_kv_heads * a.group;
   if (threadIdx.x < 2) lds.bad[threadIdx.x] = -1;
-  if (half == 0)
-    lds.out_off[row] = row_tok < a.tile_tokens
-                           ? uint32_t(row_tok * a.out_stride + row_head * D) * 2 : UINT32_MAX;
+  if (half == 0) {
+    const bool in_tile = row_tok < a.tile_tokens;
+    lds.out_off[row] = in_tile ? uint32_t(row_tok * a.out_stride + row_head * D) * 2 : UINT32_MAX;
+    lds.q_off[row] = in_tile ? uint32_t(row_tok * a.q_stride + row_head * D) * 2 : UINT32_MAX;
+  }
 
   const int2 span = a.wg_units[blockIdx.x];
   const int u_first = __builtin_amdgcn_readfirstlane(span.x);
@@ -244,8 +248,11 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     n_full = max(0, min(U.ntiles, (lim_lo + 1) / kKeys));
   };
   set_unit(cu);
+  // (Q is waited for here: where the loads may still be under way by one of its paths, the
+  // first score products of every unit wait for all that is, stores included.)
   x8 qb[kSteps];
   load_q(cu, qb);
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
 
   // Direct-to-LDS staging: load i of a wave fetches keys kLaneKeys i .. of its quarter,
   // lane L key kLaneKeys i + L / kChunks, the chunk whose swizzled slot is
@@ -470,6 +477,34 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     l_half += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
 
+  // Q of the next unit, straight into the wave's LDS staging (it is free from one unit's
+  // end to the next one's) and read from there where the current one is done with.
+  // Loads into the registers, 32 rows' lines each, held up both teams' last slots of a
+  // unit, and the waits for them its stores (64 x 512 tokens 211 us with them, 203
+  // so).  Rows of no token read the unit's first one.
+  constexpr int kQRows = 64 / kChunks;           // rows per load
+  struct QRows { const uint8_t* from; uint32_t end, to; };
+  auto q_rows = [&](const Unit& U) __attribute__((always_inline)) {
+    return QRows{reinterpret_cast<const uint8_t*>(a.q + int64_t(U.q_off + U.tok0) * a.q_stride +
+                                                  int64_t(U.h * a.group) * D),
+                 uint32_t(min(a.tile_tokens, U.q_len - U.tok0) * a.q_stride) * 2,
+                 uint32_t(__builtin_amdgcn_readfirstlane(lds_addr(lds.ostage[wave])))};
+  };
+  auto q_piece = [&](const QRows& w, int i) __attribute__((always_inline)) {
+    const int rr = i * kQRows + lane / kChunks;
+    const uint32_t off = lds.q_off[wave * kWaveRows + rr];
+    const uint32_t at = (off < w.end ? off : 0) + k_slot<D>(rr, lane % kChunks) * 16;
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(w.to + 1024 * i), "v"(at), "s"(w.from) : "memory");
+  };
+  auto read_q = [&]() __attribute__((always_inline)) {
+    wait_dma();
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks)
+      qb[ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(
+          lds.ostage[wave] + r * kRow + k_slot<D>(r, 2 * ks + half) * 16));
+  };
+
   // The unit's rows leave through the wave's LDS staging: a lane holds 8-byte
   // pieces of one row; read back, kChunks lanes hold a whole row.  Non-temporal
   // stores: the output is not read again here, and the caches keep K and V.
@@ -572,12 +607,17 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
       };
     };
     static_assert(KB * kSteps > 2 * kDma + 1, "the loads fit between the MFMAs");
-    auto staged_all = [&](int j, int k) __attribute__((always_inline)) {   // team 0, slot 2j+1
-      wait_dma();
+    // Team 0, slot 2j+1 (the loads of Q that slot 1 issues may still run).
+    auto staged_all = [&](int j, int k, auto with_q) __attribute__((always_inline)) {
+      if (with_q) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kWaveRows / kQRows) : "memory");
+      else wait_dma();
       if (j >= n_full) clean_v(j, k);
     };
     Unit nu = u_count > 1 ? to_unit(fetch_unit(u_first + 1)) : cu;  // the next unit
-    RawUnit nnu = fetch_unit(u_first);                               // the one after
+    // The one after, and taken from its registers before the unit's stores (a wait for
+    // its load behind them would wait for them).
+    RawUnit nnu = fetch_unit(u_first);
+    Unit after = cu;
     bool staged = false;
     for (int k = 0; k < u_count; ++k) {
       const bool has_next = k + 1 < u_count;
@@ -592,21 +632,26 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
           }
           mfma(0, no{}, yes{}, stage_tile(0));
           __syncthreads();
+          {
+            const QRows w = q_rows(nu);
+#pragma unroll
+            for (int i = 0; i < kWaveRows / kQRows; ++i) q_piece(w, i);
+          }
           valu_phase(0);
-          staged_all(0, k);
+          staged_all(0, k, yes{});
           __syncthreads();
           for (int j = 1; j < n; ++j) {
             mfma(j, yes{}, yes{}, stage_tile(j));
             __syncthreads();
             valu_phase(j);
-            staged_all(j, k);
+            staged_all(j, k, no{});
             __syncthreads();
           }
           // Q is not read again in this unit (without a next one it is the same
-          // again: a branch would make the compiler wait for it and copy it).  The
-          // next unit's first K tile goes into lds.k[0], last read in slot 2n-1 or
-          // earlier.
-          load_q(nu, qb);
+          // again).  The next unit's first K tile goes into lds.k[0], last read in
+          // slot 2n-1 or earlier.
+          read_q();
+          after = to_unit(nnu);
           mfma(n, yes{}, no{}, [&](int i) __attribute__((always_inline)) {
             if (i == 0) gk = staging_k(nu, 0);
             if (i >= 1 && i <= kDma) stage_piece(gk, lane_k[i - 1], i - 1);
@@ -617,7 +662,10 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
         } else {
           if (!staged) __syncthreads();
           __syncthreads();
-          mfma(0, no{}, yes{}, nothing);
+          const QRows w = q_rows(nu);
+          mfma(0, no{}, yes{}, [&](int i) __attribute__((always_inline)) {
+            if (i >= 1 && i <= kWaveRows / kQRows) q_piece(w, i - 1);
+          });
           __syncthreads();
           for (int j = 1; j < n; ++j) {
             valu_phase(j - 1);
@@ -626,7 +674,8 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
             __syncthreads();
           }
           valu_phase(n - 1);
-          load_q(nu, qb);
+          read_q();
+          after = to_unit(nnu);
           __syncthreads();
           mfma(n, yes{}, no{}, nothing);
           __syncthreads();
@@ -634,12 +683,14 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
         }
       } else {
         load_q(nu, qb);
+        __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+        after = to_unit(nnu);
         finish_unit(k, [] {});
       }
       if (has_next) {
         staged = n > 0 && nu.ntiles > 0;
         set_unit(nu);
-        if (k + 2 < u_count) nu = to_unit(nnu);
+        if (k + 2 < u_count) nu = after;
       }
     }
   };
@@ -1314,9 +1365,9 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
                   value_token_stride >= kw,
               KVC_ERR_INVALID_ARG, "token stride smaller than the token's heads");
   // (a tile's tokens are addressed by 32-bit byte offsets)
-  KVC_REQUIRE(key_token_stride < (int64_t(1) << 22) && value_token_stride < (int64_t(1) << 22) &&
-                  out_token_stride < (int64_t(1) << 22),
-              KVC_ERR_INVALID_ARG, "key, value or out tokens 8 MiB or more apart");
+  KVC_REQUIRE(q_token_stride < (int64_t(1) << 22) && key_token_stride < (int64_t(1) << 22) &&
+                  value_token_stride < (int64_t(1) << 22) && out_token_stride < (int64_t(1) << 22),
+              KVC_ERR_INVALID_ARG, "q, key, value or out tokens 8 MiB or more apart");
   KVC_REQUIRE(aligned(q, 16) && aligned(key, 16) && aligned(value, 16) && aligned(out, 16) &&
                   aligned(plan, 16) && q_token_stride % 8 == 0 && key_token_stride % 8 == 0 &&
                   value_token_stride % 8 == 0 && out_token_stride % 8 == 0,

@@ -143,7 +143,7 @@ def test_prompt_run_refuses(lib):
     for bad, want in ((dict(plan=None), 1), (dict(q=None), 1), (dict(v=None), 1),
                       (dict(out=None), 1), (dict(qs=1016), 1), (dict(ks=248), 1),
                       (dict(os=8), 1), (dict(vs=1 << 22), 1),
-                      (dict(ks=1 << 22), 1), (dict(os=1 << 22), 1), (dict(q=72), 3), (dict(k=66), 3),
+                      (dict(ks=1 << 22), 1), (dict(os=1 << 22), 1), (dict(qs=1 << 22), 1), (dict(q=72), 3), (dict(k=66), 3),
                       (dict(out=68), 3), (dict(plan=68), 3), (dict(qs=1028), 3),
                       (dict(vs=260), 3), (dict(dt=2), 2), (dict(scale=0.0), 1),
                       (dict(scale=-1.0), 1), (dict(scale=float("nan")), 1),
