@@ -429,6 +429,10 @@ struct TokenArgs {
 
 constexpr int kTokenThreads = 256;
 constexpr int64_t kTokenWorkgroups = 512;   // two per CU: what its registers hold
+// Pages per task: 64 registers of K, twice; at head_dim 256 32, as its query takes 32 more
+// (two pages spilled, and a reload waits for all of K: 64 requests of 512 to 4096
+// tokens 141 us, 129 with one).
+constexpr int token_pages(int head_dim) { return head_dim == 256 ? 1 : 512 / head_dim; }
 
 // A wave runs every so-manieth task; a task is kPages consecutive entries of the
 // batch's page list for one KV head (heads fastest: neighbouring waves read the same
@@ -441,7 +445,7 @@ constexpr int64_t kTokenWorkgroups = 512;   // two per CU: what its registers ho
 template <typename T, int D>
 __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenArgs c) {
   constexpr int kSteps = D / 32;
-  constexpr int kPages = 512 / D;             // 64 registers of K
+  constexpr int kPages = token_pages(D);
   constexpr int kSets = (kPages + 3) / 4;     // of four pages, a quarter wave each
   typedef typename T::x8 x8;
   const WeightsArgs& a = c.w;
@@ -909,7 +913,7 @@ extern "C" int kvc_decode_attention_weights(
   c.indptr = indptr;
   c.last_page_len = last_page_len;
   c.batch = batch;
-  const int64_t tasks = (num_indices + 512 / D - 1) / (512 / D) * Hkv;
+  const int64_t tasks = (num_indices + token_pages(D) - 1) / token_pages(D) * Hkv;
   const int64_t wgs = (tasks + kTokenThreads / 64 - 1) / (kTokenThreads / 64);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(wgs, kTokenWorkgroups)));
   hipStream_t s = static_cast<hipStream_t>(stream);
