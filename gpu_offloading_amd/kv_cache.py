@@ -713,7 +713,8 @@ class PagedKVCache:
         ``decode_seq_ids`` order) and the prefill wrapper over the
         continuations (``prefill``: their q rows, chunk after chunk).  New
         prompts attend over their own contiguous K/V outside the paged cache,
-        as in the engine (``plan_prompt`` and ``prompt``).  Pages must already cover every new token."""
+        as in the engine (``plan_prompt`` and ``prompt``).  Pages must already
+        cover every new token."""
         self._require_gpu()
         dec = [int(s) for s in decode_seq_ids]
         pre = [int(s) for s in prefill_seq_ids]
@@ -1019,14 +1020,18 @@ class PagedKVCache:
             torch.from_numpy(qo), torch.from_numpy(indptr), indices, torch.from_numpy(lpl),
             self.num_heads, self.num_kv_heads, self.head_dim, self.page_size, causal=True,
             q_data_type=self.dtype, new_tokens=torch.from_numpy(new.astype(np.int32)))
+        self._weights_wrapper._staged += (self._weights_ids,)   # (kept for runs on other streams)
 
     def chunk_weights(self, layer: int, q: torch.Tensor, lse: torch.Tensor) -> None:
         """Accumulate the attention weights of the planned chunks in ``layer``:
         ``q [sum(query_lens), Hq, D]`` with ``lse`` as ``prompt`` or ``prefill``
         returned it for these rows."""
         self._require_tracking()
-        self._weights_wrapper.run(q, lse, self.k_cache[layer], self.scores[layer],
-                                  self.positions[layer], self._evicted_dev, self._weights_ids)
+        w = self._weights_wrapper
+        if w.schedule is None:
+            raise RuntimeError("chunk_weights needs plan_chunk_weights first")
+        w.run(q, lse, self.k_cache[layer], self.scores[layer], self.positions[layer],
+              self._evicted_dev, self._weights_ids)
 
     def evict(self, seq_ids: Sequence[int], keep: Sequence[int] | int,
               recent: Sequence[int] | int = 0) -> None:
