@@ -729,8 +729,8 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
   constexpr int kLaneKeys = 1024 / kRow;       // keys per load
   typedef typename T::x8 x8;
   struct Lds {
+    uint8_t v[2][kTile];                       // (first: within reach of an immediate offset)
     uint8_t k[2][kTile];
-    uint8_t v[2][kTile];
     int bad[2];
   };
   __shared__ alignas(16) Lds lds;
