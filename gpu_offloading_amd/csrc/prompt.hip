@@ -16,7 +16,6 @@
 #include <array>
 #include <cmath>
 #include <functional>
-#include <queue>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -1089,64 +1088,72 @@ int64_t prompt_workspace_bytes(const kvc_prompt_schedule& s) {
 // all dealt longest first to all workgroups.
 void write_plan(const std::vector<int32_t>& rec, int64_t n, int hkv, int64_t W, int parts_per_head,
                 int32_t* plan_host) {
-  struct Line { int64_t item; int head, cost; };
-  std::vector<Line> line;
+  struct Line { int32_t item, head, cost; };
+  const auto longer = [](const Line& x, const Line& y) { return x.cost > y.cost; };
+  std::vector<Line> line, seq;
   line.reserve(size_t(n) * hkv);
   int64_t total = 0;
-  for (int64_t i0 = 0; i0 < n;) {
-    int64_t i1 = i0;
-    while (i1 < n && rec[i1 * kUnitInts] == rec[i0 * kUnitInts]) ++i1;
-    for (int h = 0; h < hkv; ++h) {
-      const size_t at = line.size();
-      for (int64_t i = i0; i < i1; ++i) {
-        const int cost = rec[i * kUnitInts + 6] + kUnitCost +
-                         (rec[i * kUnitInts + 7] ? kPartCost : 0);
-        line.push_back(Line{i, h, cost});
-        total += cost;
-      }
-      std::stable_sort(line.begin() + at, line.end(),
-                       [](const Line& x, const Line& y) { return x.cost > y.cost; });
+  for (int64_t i = 0; i < n;) {
+    const int32_t b = rec[i * kUnitInts];
+    seq.clear();
+    for (; i < n && rec[i * kUnitInts] == b; ++i) {
+      const int32_t* r = rec.data() + i * kUnitInts;
+      seq.push_back(Line{int32_t(i), 0, r[6] + kUnitCost + (r[7] ? kPartCost : 0)});
+      total += int64_t(seq.back().cost) * hkv;
     }
-    i0 = i1;
+    std::stable_sort(seq.begin(), seq.end(), longer);
+    for (int h = 0; h < hkv; ++h)
+      for (const Line& l : seq) line.push_back(Line{l.item, h, l.cost});
   }
   const int parts = W % kXcds == 0 && !parts_per_head ? kXcds : 1;
-  std::vector<std::vector<size_t>> lists(W);
-  typedef std::pair<int64_t, int64_t> Slot;  // (load, workgroup)
+  // The least loaded workgroup: a heap of load * 256 + workgroup.
+  static_assert(kMaxWorkgroups <= 256, "a workgroup's number has 8 bits");
+  std::vector<int64_t> heap;
+  std::vector<uint8_t> owner(line.size());
+  std::vector<int32_t> count(W, 0);
   size_t u = 0;
   int64_t done = 0;
   for (int x = 0; x < parts; ++x) {
     const int64_t from = done, until = total * (x + 1) / parts;
     size_t end = u;
     // Every workgroup gets a unit, and the last part what is left.
-    const size_t least = u + size_t(W / parts), most = line.size() - size_t((parts - 1 - x) * (W / parts));
+    const size_t each = size_t(W / parts), least = u + each;
+    const size_t most = line.size() - size_t(parts - 1 - x) * each;
     while (end < most && (end < least || x == parts - 1 || done + line[end].cost / 2 < until))
       done += line[end++].cost;
     size_t tail = end;
-    for (int64_t rest = parts_per_head ? done : (done - from) / 4; tail > u && rest > 0; --tail) rest -= line[tail - 1].cost;
-    std::stable_sort(line.begin() + tail, line.begin() + end,
-                     [](const Line& p, const Line& q) { return p.cost > q.cost; });
-    std::priority_queue<Slot, std::vector<Slot>, std::greater<Slot>> free_at;
-    for (int64_t b = x; b < W; b += parts) free_at.push(Slot(0, b));
+    int64_t rest = parts_per_head ? done : (done - from) / 4;
+    while (tail > u && rest > 0) rest -= line[--tail].cost;
+    std::stable_sort(line.begin() + tail, line.begin() + end, longer);
+    heap.clear();
+    for (int64_t b = x; b < W; b += parts) heap.push_back(b);
     for (; u < end; ++u) {
-      const Slot sl = free_at.top();
-      free_at.pop();
-      lists[sl.second].push_back(u);
-      free_at.push(Slot(sl.first + line[u].cost, sl.second));
+      const int wg = int(heap[0] & 255);
+      owner[u] = uint8_t(wg);
+      ++count[wg];
+      const int64_t key = heap[0] + int64_t(line[u].cost) * 256;
+      size_t at = 0;
+      for (size_t child; (child = 2 * at + 1) < heap.size(); at = child) {
+        if (child + 1 < heap.size() && heap[child + 1] < heap[child]) ++child;
+        if (heap[child] >= key) break;
+        heap[at] = heap[child];
+      }
+      heap[at] = key;
     }
   }
   const int64_t table = table_ints(W);
   std::fill_n(plan_host, table, 0);
-  int64_t next = 0;
-  for (int64_t b = 0; b < W; ++b) {
+  for (int64_t b = 0, next = 0; b < W; ++b) {
     plan_host[2 * b] = int32_t(next);
-    plan_host[2 * b + 1] = int32_t(lists[b].size());
-    for (const size_t i : lists[b]) {
-      int32_t* dst = plan_host + table + next * kUnitInts;
-      std::copy_n(rec.data() + line[i].item * kUnitInts, kUnitInts, dst);
-      dst[0] = line[i].head;
-      if (dst[7]) dst[7] += line[i].head * parts_per_head;
-      ++next;
-    }
+    plan_host[2 * b + 1] = count[b];
+    next += count[b];
+    count[b] = plan_host[2 * b];                 // and on: the place of its next unit
+  }
+  for (size_t i = 0; i < line.size(); ++i) {
+    int32_t* dst = plan_host + table + int64_t(count[owner[i]]++) * kUnitInts;
+    std::copy_n(rec.data() + int64_t(line[i].item) * kUnitInts, kUnitInts, dst);
+    dst[0] = line[i].head;
+    if (dst[7]) dst[7] += line[i].head * parts_per_head;
   }
 }
 
