@@ -291,7 +291,7 @@ def test_weights_run_refuses(lib):
 def test_evict_refuses(lib):
     need = lib.kvc_evict_workspace_bytes(2, 3, 100)
     assert need >= 2 * 3 * 50 * 8 and lib.kvc_evict_workspace_bytes(0, 3, 100) == 0
-    ok = dict(k=64, v=64, nb=4, h=3, d=64, page=16, e=2, bs=3072 + 1024, ts=256, sc=64, bt=64,
+    ok = dict(k=64, v=64, nb=4, h=3, d=64, page=16, e=2, bs=4096, ts=256, sc=64, bt=64,
               rs=7, w=7, rows=2, lens=64, keep=64, rec=64, b=2, top=100, ws=64, wb=need)
 
     def run(**kw):
