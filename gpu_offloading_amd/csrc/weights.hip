@@ -132,7 +132,7 @@ __host__ __device__ inline int first_token(int key0, int q_len, int kv_len, int 
 // 22.7 us.  Products of the next block interleaved with the exponentials in one wave,
 // at two waves per SIMD, took 10% longer.
 template <typename T, int D>
-__global__ __launch_bounds__(kChunkThreads, D == 256 ? 2 : 3)
+__global__ __launch_bounds__(kChunkThreads, D == 64 ? 4 : D == 128 ? 3 : 2)
 void weights_chunk_kernel(ChunkArgs c) {
   constexpr int KB = kKeyBlocks, kSteps = D / 16, kRow = 2 * D, kChunks = kRow / 16;
   constexpr int kDma = kStage * kRow / 1024 / 4;   // row loads per wave and stage
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
 
 constexpr int kMaxGroup = 128;
 // Workgroups of the chunk kernel that the chip holds at a time (registers).
-int resident(int head_dim) { return head_dim == 256 ? 512 : 768; }
+int resident(int head_dim) { return head_dim == 64 ? 1024 : head_dim == 128 ? 768 : 512; }
 // Costs in row blocks: a unit's start (its K), the join kernel, the least piece of a cut.
 constexpr int64_t kUnitCost = 4;
 constexpr int64_t kJoinCost = 5;
