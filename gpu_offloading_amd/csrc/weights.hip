@@ -128,8 +128,8 @@ __host__ __device__ inline int first_token(int key0, int q_len, int kv_len, int 
 // lane's key; with that instead of each row's limit read across lanes, and priorities
 // that go round, 4 prompts of 2000 tokens went from 93 to 83 us.
 // Measured (bf16, head_dim 128, 32 / 8 heads): 2000 rows against 16000 keys 245 us
-// (1005 TFLOP/s), 4 prompts of 1200 to 2048 tokens 64 us, 8 windows of 32 against 4096
-// 22.7 us.  Products of the next block interleaved with the exponentials in one wave,
+// (1005 TFLOP/s), 4 prompts of 1200 to 2048 tokens 62 us, 8 windows of 32 against 4096
+// 22.4 us.  Products of the next block interleaved with the exponentials in one wave,
 // at two waves per SIMD, took 10% longer.
 template <typename T, int D>
 __global__ __launch_bounds__(kChunkThreads, D == 64 ? 4 : D == 128 ? 3 : 2)
@@ -234,9 +234,6 @@ void weights_chunk_kernel(ChunkArgs c) {
 #pragma unroll
       for (int i = 0; i <= kDma; ++i) stage_load(i, 0);
       stage_prepare();
-#pragma unroll
-      for (int i = 0; i <= kDma; ++i) stage_load(i, 1);
-      stage_prepare();
     }
 
     x8 kop[KB][kSteps];
@@ -255,7 +252,7 @@ void weights_chunk_kernel(ChunkArgs c) {
       for (int ks = 0; ks < kSteps; ++ks)
         kop[kb][ks] = __builtin_bit_cast(x8, *reinterpret_cast<const uint4*>(kp + 16 * ks));
     }
-    // K and the first stages are here before the walk (waits for K inside it would wait
+    // K and the first stage are here before the walk (waits for K inside it would wait
     // for the rows in flight).
     __builtin_amdgcn_s_waitcnt(kWaitLoads);
     __syncthreads();
@@ -341,7 +338,6 @@ void weights_chunk_kernel(ChunkArgs c) {
       else if (turn == 1) __builtin_amdgcn_s_setprio(1);
       else __builtin_amdgcn_s_setprio(2);
       turn = turn == 2 ? 0 : turn + 1;
-      const bool more = st > 0;                    // (stages 0 and 1 are there or under way)
       auto load = [&](int ks) __attribute__((always_inline)) {
         if (ks <= kDma) stage_load(ks, (st + 1) & 1);
         if (kSteps <= kDma && ks == kSteps - 1) {
@@ -350,14 +346,11 @@ void weights_chunk_kernel(ChunkArgs c) {
         }
       };
       if (st < first) {
-        if (more) {
 #pragma unroll
-          for (int ks = 0; ks < kSteps; ++ks) load(ks);
-        }
+        for (int ks = 0; ks < kSteps; ++ks) load(ks);
       } else {
         const float lse = lds.lse[st & 1][wave][lane];
-        if (more) scores(0, load);
-        else scores(0, [](int) {});
+        scores(0, load);
         // (Rows behind the last one are copies of its token's that give nothing.)
         int tok, head;
         split(my_first + lane, tok, head);
@@ -375,7 +368,7 @@ void weights_chunk_kernel(ChunkArgs c) {
           block_exps(1);
         }
       }
-      if (more) stage_prepare();
+      stage_prepare();
       advance();
       q_at ^= kStage * kRow;
       // The next stage is here and this one has been read: the one after it is loaded
