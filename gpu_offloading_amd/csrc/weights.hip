@@ -14,6 +14,7 @@
 //
 // Single-token form (weights_token_kernel): reads K once and is bound by that.
 #include "kvc_common.h"
+#include "weights_rows.h"
 
 #include <algorithm>
 #include <array>
@@ -95,12 +96,10 @@ __device__ __forceinline__ void store_weight(const WeightsArgs& a, int32_t block
 // Workgroup w begins with unit w and goes on with the next ones (0: none).
 constexpr int kRecInts = 12;
 constexpr int kJoinInts = 8;
-constexpr int kRows = 32;                          // query rows per block
 constexpr int kKeyBlocks = 2;                      // 32-key blocks per wave
 constexpr int kWaveKeys = 32 * kKeyBlocks;
 constexpr int kChunkThreads = 256;
 constexpr int kUnitKeys = kChunkThreads / 64 * kWaveKeys;
-constexpr int kStage = 2 * kRows;                  // rows in flight at a time
 constexpr int kWaitLoads = 0x0f70;                 // s_waitcnt vmcnt(0)
 
 struct ChunkArgs {
@@ -161,7 +160,6 @@ void weights_chunk_kernel(ChunkArgs c) {
     head = row - __umul24(tok, a.group);
   };
   const uint32_t q_bytes = uint32_t(a.q_stride * 2);
-  const int step_tok = kStage / a.group, step_head = kStage - step_tok * a.group;
 
   // Of a SIMD's waves the hardware prefers the oldest: with equal work the youngest
   // ends last, alone.  Priorities that go round by stage let each be preferred in turn.
@@ -177,29 +175,28 @@ void weights_chunk_kernel(ChunkArgs c) {
     const int tok0 = first_token(key_first, q_len, kv_len, c.causal);
     const int last_tok = q_len - 1 - tok0;
 
-    // The stage that is loaded next: its first row's token (from tok0 on) and head,
-    // bases of that token's rows.  Row i of the unit is token i / group, head i %
-    // group; a stage's rows are addressed from the base by 32-bit offsets, the same
-    // in every stage where the group divides 64; elsewhere, and where the tokens
-    // end, they are computed anew (rows past the last token read its).
-    int st_tok = first_block * kRows / a.group, st_head = first_block * kRows - st_tok * a.group;
-    int my_base = st_tok, my_first = st_head;      // of the stage being computed
+    // The stage that is loaded next, tokens from tok0 on, and the bases of its first
+    // row's token.  The rows' 32-bit offsets from them are the same in every stage
+    // where the group divides 64 and no token ends.
+    RowWalk at(a.group, last_tok, first_block * kRows);
+    const int step_tok = at.step_tok, step_head = at.step_head;
+    int my_base = at.tok, my_first = at.head;      // of the stage being computed
     const uint8_t* st_q = reinterpret_cast<const uint8_t*>(
-        a.q + (int64_t(y.x) + tok0 + st_tok) * a.q_stride + h * a.group * D);
+        a.q + (int64_t(y.x) + tok0 + at.tok) * a.q_stride + h * a.group * D);
     const uint8_t* st_lse = reinterpret_cast<const uint8_t*>(
-        a.lse + (int64_t(y.x) + tok0 + st_tok) * Hq + h * a.group);
+        a.lse + (int64_t(y.x) + tok0 + at.tok) * Hq + h * a.group);
     uint32_t q_off[kDma], lse_off;
     auto offsets = [&]() __attribute__((always_inline)) {
-      const int left = last_tok - st_tok;
+      const int left = at.left();
       int tok, head;
 #pragma unroll
       for (int i = 0; i < kDma; ++i) {
         const int row = (wave * kDma + i) * kLoadRows + lane / kChunks;
         const int chunk = (lane % kChunks) ^ (D == 64 ? (row >> 1) & 7 : row & 15);
-        split(st_head + row, tok, head);
+        split(at.head + row, tok, head);
         q_off[i] = uint32_t(min(tok, left)) * q_bytes + head * kRow + chunk * 16;
       }
-      split(st_head + lane, tok, head);
+      split(at.head + lane, tok, head);
       lse_off = (uint32_t(min(tok, left)) * Hq + head) * 4;
     };
     // Load i of a stage's kDma + 1 into `slot` (inline assembly: the compiler would wait
@@ -216,18 +213,10 @@ void weights_chunk_kernel(ChunkArgs c) {
     };
     // Behind the last stage the last one is loaded again, which nothing reads.
     auto stage_prepare = [&]() __attribute__((always_inline)) {
-      int tok = step_tok, head = st_head + step_head;
-      if (head >= a.group) {
-        head -= a.group;
-        ++tok;
-      }
-      if (st_tok + tok <= last_tok) {
-        st_tok += tok;
-        st_head = head;
-        st_q += uint32_t(tok) * q_bytes;           // (65 of 2^26 bytes at most)
-        st_lse += uint32_t(tok) * uint32_t(Hq * 4);
-      }
-      if (step_head != 0 || st_tok + step_tok > last_tok + 1) offsets();
+      const uint32_t tok = uint32_t(at.next());
+      st_q += tok * q_bytes;                       // (64 of less than 2^26 bytes at most)
+      st_lse += tok * uint32_t(Hq * 4);
+      if (at.offsets_change()) offsets();
     };
     offsets();
     if (stages > 0) {
