@@ -133,6 +133,16 @@ __device__ __forceinline__ float fast_log2(float x) {
 // exp2(m_old - m_new) never evaluates (-inf) - (-inf).
 constexpr float kNegBig = -1.0e30f;
 
+// Inline assembly owes the hardware the wait states that hipcc sees to elsewhere.  A
+// direct-to-LDS load reads its LDS address from M0 one wait state or more after M0 was
+// written: here s_nop 0, as its word, so that the two instructions stay neighbours
+// in a listing, where the tests that M0 has no other use look for that.
+#define KVC_SET_M0(from) "s_mov_b32 m0, " from "\n\t.long 0xbf800000\n\t"
+// And a memory instruction reads an SGPR five wait states or more after a VALU
+// instruction (v_readfirstlane_b32) wrote it: in front of the first load that uses
+// fresh ones, with KVC_SET_M0 behind it.
+#define KVC_SGPR_WAIT "s_nop 2\n\t"
+
 inline int cdiv(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
 }  // namespace kvc

@@ -300,8 +300,12 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
                        lds_addr(tile + sw * kWaveKeys * kRow)))};
   };
   auto stage_piece = [](const Staging& g, uint32_t lane_off, int i) __attribute__((always_inline)) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(g.to + 1024 * i), "v"(lane_off), "s"(g.rsrc) : "memory");
+    if (i == 0)
+      asm volatile(KVC_SGPR_WAIT KVC_SET_M0("%0") "buffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(g.to), "v"(lane_off), "s"(g.rsrc) : "memory");
+    else
+      asm volatile(KVC_SET_M0("%0") "buffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(g.to + 1024 * i), "v"(lane_off), "s"(g.rsrc) : "memory");
   };
   auto staging_k = [&](const Unit& U, int j) __attribute__((always_inline)) {
     return staging(lds.k[j & 1], a.k, a.k_stride, k_bytes, U, j);
@@ -500,8 +504,12 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
     const int rr = i * kQRows + lane / kChunks;
     const uint32_t off = lds.q_off[wave * kWaveRows + rr];
     const uint32_t at = (off < w.end ? off : 0) + k_slot<D>(rr, lane % kChunks) * 16;
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :: "s"(w.to + 1024 * i), "v"(at), "s"(w.from) : "memory");
+    if (i == 0)
+      asm volatile(KVC_SGPR_WAIT KVC_SET_M0("%0") "global_load_lds_dwordx4 %1, %2"
+                   :: "s"(w.to), "v"(at), "s"(w.from) : "memory");
+    else
+      asm volatile(KVC_SET_M0("%0") "global_load_lds_dwordx4 %1, %2"
+                   :: "s"(w.to + 1024 * i), "v"(at), "s"(w.from) : "memory");
   };
   auto read_q = [&]() __attribute__((always_inline)) {
     wait_dma();
@@ -801,9 +809,14 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
                           __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3};
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(tile + wave * 16 * kRow));
 #pragma unroll
-    for (int i = 0; i < kDma; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(to + 1024 * i), "v"(lane_off[i]), "s"(rsrc) : "memory");
+    for (int i = 0; i < kDma; ++i) {
+      if (i == 0)
+        asm volatile(KVC_SGPR_WAIT KVC_SET_M0("%0") "buffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :: "s"(to), "v"(lane_off[i]), "s"(rsrc) : "memory");
+      else
+        asm volatile(KVC_SET_M0("%0") "buffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :: "s"(to + 1024 * i), "v"(lane_off[i]), "s"(rsrc) : "memory");
+    }
   };
   auto dma_k = [&](const Unit& U, int j) __attribute__((always_inline)) {
     dma(lds.k[j & 1], a.k, a.k_stride, k_bytes, lane_k, U, j);

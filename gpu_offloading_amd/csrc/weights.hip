@@ -203,11 +203,11 @@ void weights_chunk_kernel(ChunkArgs c) {
     // for all of them at every LDS read; it uses M0 nowhere itself).
     auto stage_load = [&](int i, int slot) __attribute__((always_inline)) {
       if (i < kDma)
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+        asm volatile(KVC_SET_M0("%0") "global_load_lds_dwordx4 %1, %2"
                      :: "s"(q_base + uint32_t(slot * kStage * kRow + i * 1024)), "v"(q_off[i]),
                         "s"(st_q) : "memory");
       else
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2"
+        asm volatile(KVC_SET_M0("%0") "global_load_lds_dword %1, %2"
                      :: "s"(lse_base + uint32_t(slot * 4 * kStage * 4)), "v"(lse_off), "s"(st_lse)
                      : "memory");
     };
