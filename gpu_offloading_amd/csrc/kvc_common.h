@@ -138,6 +138,7 @@ constexpr float kNegBig = -1.0e30f;
 // written: here s_nop 0, as its word, so that the two instructions stay neighbours
 // in a listing, where the tests that M0 has no other use look for that.
 #define KVC_SET_M0(from) "s_mov_b32 m0, " from "\n\t.long 0xbf800000\n\t"
+#define KVC_STEP_M0(by) "s_add_u32 m0, m0, " by "\n\t.long 0xbf800000\n\t"
 // And a memory instruction reads an SGPR five wait states or more after a VALU
 // instruction (v_readfirstlane_b32) wrote it: in front of the first load that uses
 // fresh ones, with KVC_SET_M0 behind it.

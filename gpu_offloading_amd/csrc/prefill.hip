@@ -307,10 +307,10 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_kernel(PrefillArgs a
   // stepped by 1 KB between them.
   auto dma_k = [&](KTile& buf, const Pages& p) __attribute__((always_inline)) {
     const uint64_t blk = sgpr64(reinterpret_cast<uint64_t>(kbase + p.off));
-    asm volatile("s_mov_b32 m0, %0\n\t"
-                 "global_load_lds_dwordx4 %1, %5\n\ts_add_u32 m0, m0, 0x400\n\t"
-                 "global_load_lds_dwordx4 %2, %5\n\ts_add_u32 m0, m0, 0x400\n\t"
-                 "global_load_lds_dwordx4 %3, %5\n\ts_add_u32 m0, m0, 0x400\n\t"
+    asm volatile(KVC_SGPR_WAIT KVC_SET_M0("%0")
+                 "global_load_lds_dwordx4 %1, %5\n\t" KVC_STEP_M0("0x400")
+                 "global_load_lds_dwordx4 %2, %5\n\t" KVC_STEP_M0("0x400")
+                 "global_load_lds_dwordx4 %3, %5\n\t" KVC_STEP_M0("0x400")
                  "global_load_lds_dwordx4 %4, %5"
                  :: "s"(lds_addr(buf.b + pw_idx * kPage * kKRow)), "v"(lane_k[0]), "v"(lane_k[1]),
                     "v"(lane_k[2]), "v"(lane_k[3]), "s"(blk) : "memory", "scc");
@@ -333,10 +333,10 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_mfma_kernel(PrefillArgs a
     const i32x4_t rsrc = {__builtin_amdgcn_readfirstlane(int(uint32_t(blk))),
                           __builtin_amdgcn_readfirstlane(int(uint32_t(blk >> 32) & 0xFFFF)),
                           __builtin_amdgcn_readfirstlane(bytes), kBufferRsrcWord3};
-    asm volatile("s_mov_b32 m0, %0\n\t"
-                 "buffer_load_dwordx4 %1, %5, 0 offen lds\n\ts_add_u32 m0, m0, 0x400\n\t"
-                 "buffer_load_dwordx4 %2, %5, 0 offen lds\n\ts_add_u32 m0, m0, 0x400\n\t"
-                 "buffer_load_dwordx4 %3, %5, 0 offen lds\n\ts_add_u32 m0, m0, 0x400\n\t"
+    asm volatile(KVC_SGPR_WAIT KVC_SET_M0("%0")
+                 "buffer_load_dwordx4 %1, %5, 0 offen lds\n\t" KVC_STEP_M0("0x400")
+                 "buffer_load_dwordx4 %2, %5, 0 offen lds\n\t" KVC_STEP_M0("0x400")
+                 "buffer_load_dwordx4 %3, %5, 0 offen lds\n\t" KVC_STEP_M0("0x400")
                  "buffer_load_dwordx4 %4, %5, 0 offen lds"
                  :: "s"(lds_addr(buf.b + pw_idx * kPage * kKRow)), "v"(lane_v[0]), "v"(lane_v[1]),
                     "v"(lane_v[2]), "v"(lane_v[3]), "s"(rsrc) : "memory", "scc");

@@ -103,7 +103,7 @@ def test_the_check_itself():
 
 
 @pytest.mark.skipif(not os.access(HIPCC, os.X_OK), reason="hipcc not available")
-@pytest.mark.parametrize("source", ["prompt", "weights"])
+@pytest.mark.parametrize("source", ["prompt", "weights", "prefill"])
 def test_direct_lds_loads_wait_for_their_scalars(tmp_path, source):
     out = tmp_path / (source + ".s")
     subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang",
