@@ -48,6 +48,7 @@ constexpr int kBufferRsrcWord3 = 0x00020000;
 // s_waitcnt vmcnt(0) with the other counters unconstrained (gfx9 encoding).
 constexpr int kWaitVmcnt0 = 0x0F70;
 constexpr float kRescaleLog2 = 8.f;           // lazy-rescale threshold (base 2)
+constexpr float kLargeLog2 = 16777216.f;      // 2^24: a maximum's rounding passes 1/2
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -66,7 +67,7 @@ struct PromptArgs {
   int64_t out_stride;
   float* lse;                             // [total_q][Hq] natural log, may be null
   float* parts;                           // [parts][tile rows][D] outputs of units' pieces
-  float* part_lse;                        // [parts][tile rows] their log-sum-exp, base 2
+  float* part_max;                        // [parts][tile rows] the maximum m under their sums
 };
 
 // The element types: bf16 and fp16 through the same kernel.
@@ -123,8 +124,33 @@ __device__ __forceinline__ int v_slot(int key, int chunk) {
 // partials + 1; its keys' offset and length are the run's first key's).
 struct Unit { int h, tok0, q_len, kv_len, q_off, k_off, ntiles, part; };
 
-// A lane's share of a piece's row (O^T entries as accumulated, normalised) and the
-// row's log-sum-exp.
+// The maximum to subtract from a tile's scaled scores, rounded as m = RN(max s * scale)
+// is.  fmaf(s, scale, -m) has the exact product in it: the largest score's exponent is
+// not 0 but m's rounding, half a step, up to 1/2 below kLargeLog2.  It cancels against
+// the sum, but from there on it would soon overflow the exponential, or flush it
+// to 0.  There (no model's scores) scores are scaled and rounded first, so that equal ones
+// have equal exponents, the largest 0; divided by the scale again they take the common
+// path with a maximum of 0.
+template <int KB>
+__device__ __forceinline__ float settle_scores(f32x16_t (&s)[KB], float m, float scale_log2) {
+#pragma clang fp contract(off)
+  const bool large = fabsf(m) >= kLargeLog2;
+  if (__builtin_amdgcn_ballot_w64(large) == 0) return m;
+  const float inv = __builtin_amdgcn_rcpf(scale_log2);   // (at least 2^-104 here)
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float scaled = s[b][e] * scale_log2;
+      s[b][e] = large ? (scaled - m) * inv : s[b][e];
+    }
+  return large ? 0.f : m;
+}
+
+// A lane's share of a piece's row (O^T entries as accumulated, normalised), the row's
+// maximum m and the sum l under it.  (Their log-sum-exp m + log2 l in one number would
+// lose l beside a large m.)  l's 32 bits take the place of the lowest four of dims
+// 0 to 7, whose other 20 are far more than the output keeps.
 template <int D, int kBlocks>
 __device__ __forceinline__ void store_part(const PromptArgs& a, int part, int rows, int row,
                                            int half, const f32x16_t (&o)[kBlocks], float l,
@@ -134,10 +160,24 @@ __device__ __forceinline__ void store_part(const PromptArgs& a, int part, int ro
 #pragma unroll
   for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = db == 0; i < 4; ++i)
       *reinterpret_cast<f32x4_t*>(p + 32 * db + 8 * i) =
           f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-  if (half == 0) a.part_lse[at] = l == 0.f ? -INFINITY : m + fast_log2(l);
+  const uint32_t bits = __float_as_uint(l) >> (16 * half);
+  u32x4_t first;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    first[j] = (__float_as_uint(o[0][j]) & ~15u) | (bits >> (4 * j) & 15u);
+  *reinterpret_cast<u32x4_t*>(p) = first;
+  if (half == 0) a.part_max[at] = m;
+}
+
+// l from a piece's dims 0 to 7.
+__device__ __forceinline__ float part_sum(u32x4_t lo, u32x4_t hi) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bits |= (lo[j] & 15u) << (4 * j) | (hi[j] & 15u) << (16 + 4 * j);
+  return __uint_as_float(bits);
 }
 
 // head_dim 64 and 128: eight waves in two teams of four, one workgroup per CU,
@@ -468,7 +508,8 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db) o[db] *= alpha;
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
+    const float m_use =                            // no key seen yet: all p are 0
+        settle_scores(s, m_run == -INFINITY ? 0.f : m_run, a.scale_log2);
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 8 * KB; ++i) {
@@ -962,7 +1003,8 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[db][e] = scale_acc(o[db][e], alpha);
         }
-        const float m_use = m_run == -INFINITY ? 0.f : m_run;   // no key seen yet: all p are 0
+        const float m_use =                        // no key seen yet: all p are 0
+            settle_scores(s, m_run == -INFINITY ? 0.f : m_run, a.scale_log2);
 #pragma unroll
         for (int i = 8; i < kS; ++i) {
           score(i);
@@ -1039,7 +1081,7 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
 }
 
 // Units that were cut along their keys: out = sum_i w_i O_i / sum_i w_i over the pieces,
-// w_i = 2^(lse_i - max lse).  A thread per four dims of a row.  Record: KV head, first
+// w_i = l_i 2^(m_i - max m).  A thread per four dims of a row.  Record: KV head, first
 // query, q_len, q offset | first partial, pieces, 0, 0.
 template <typename T, int D>
 __global__ __launch_bounds__(256)
@@ -1050,21 +1092,23 @@ void prompt_join_kernel(PromptArgs a, const int4* joins, int rows) {
   const int row_tok = int(row * a.inv_group >> 16), row_head = row - row_tok * a.group;
   const int tok = x.y + row_tok;
   if (row_tok >= a.tile_tokens || tok >= x.z) return;
-  const float* pl = a.part_lse + int64_t(y.x) * rows + row;
-  const f32x4_t* po =
-      reinterpret_cast<const f32x4_t*>(a.parts + (int64_t(y.x) * rows + row) * D) + c;
+  const float* pm = a.part_max + int64_t(y.x) * rows + row;
+  const u32x4_t* po =
+      reinterpret_cast<const u32x4_t*>(a.parts + (int64_t(y.x) * rows + row) * D);
+  const uint32_t keep = c < 2 ? ~15u : ~0u;      // (the first dims' lowest bits are l's)
   float m = -INFINITY;
-  for (int i = 0; i < y.y; ++i) m = fmaxf(m, pl[int64_t(i) * rows]);
+  for (int i = 0; i < y.y; ++i) m = fmaxf(m, pm[int64_t(i) * rows]);
   const float base = m == -INFINITY ? 0.f : m;   // no piece saw a key: all weights are 0
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   float sum = 0.f;
 #pragma unroll 4
   for (int i = 0; i < y.y; ++i) {
-    const float w = fast_exp2(pl[int64_t(i) * rows] - base);
-    const f32x4_t v = po[int64_t(i) * rows * kLanes];
+    const u32x4_t* p = po + int64_t(i) * rows * kLanes;
+    const float w = part_sum(p[0], p[1]) * fast_exp2(pm[int64_t(i) * rows] - base);
+    const u32x4_t v = p[c];
     sum += w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = fmaf(w, v[j], o[j]);
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(w, __uint_as_float(v[j] & keep), o[j]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int head = x.x * a.group + row_head;
@@ -1424,7 +1468,7 @@ extern "C" int kvc_prompt_run(const kvc_prompt_schedule* sched, const int32_t* p
   a.out_stride = out_token_stride;
   a.lse = lse;
   a.parts = static_cast<float*>(workspace);
-  a.part_lse = a.parts + sched->num_parts * tile_rows(D) * D;
+  a.part_max = a.parts + sched->num_parts * tile_rows(D) * D;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == KVC_DTYPE_BF16) launch<Bf16>(a, D, unsigned(sched->num_workgroups), s);
   else launch<Fp16>(a, D, unsigned(sched->num_workgroups), s);

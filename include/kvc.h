@@ -570,7 +570,8 @@ int kvc_decode_step_setup(const int32_t* host_image, int32_t* dev_image,
  * no effect on it, inf and NaN included.  Optional lse[row][hq] is the
  * natural-log log-sum-exp of the scaled logits, from fp32 sums of the
  * unrounded exponentials; the exponentials are rounded to the element type for
- * the value product.
+ * the value product.  Scores may have any size for which sm_scale * log2(e) times
+ * them is finite in fp32: scaled and rounded to fp32, equal ones share.
  *
  * kvc_prompt_plan is host-only: one work unit per (tile of tile_tokens query
  * tokens, KV head), dealt to num_workgroups workgroups.  Where few units would
