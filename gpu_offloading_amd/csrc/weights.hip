@@ -545,7 +545,8 @@ __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenAr
           load_q(b, now.h, 0, x.q, x.lse);
         }
         const int first = req.first, last = req.end - 1;
-        const int tokens = p < last ? kPage : req.lpl;
+        // (a page in front of the first request's has none)
+        const int tokens = p < first ? 0 : p < last ? kPage : req.lpl;
         float w = 0.f;
         for (int g0 = 0; g0 < a.group; g0 += 16) {
           if (g0 > 0) load_q(b, now.h, g0, x.q, x.lse);

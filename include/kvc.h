@@ -644,7 +644,8 @@ int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
  * kernel.
  * Decode form: one query token per request, its last cached token, which is
  * new; indptr, indices and last_page_len are device arrays as the decode's
- * (at most num_indices pages are read), so that the launch can be captured and
+ * (at most num_indices pages are read; indptr[0] may be above 0, as in a part of a
+ * batch: the pages in front are left alone), so that the launch can be captured and
  * replayed.  Every sum has a fixed order.  head_dim 64, 128 or 256,
  * page_size 16, groups up to 128; q and the cache are 16-byte aligned with
  * strides that are multiples of 8 elements, q's below 2^25.
