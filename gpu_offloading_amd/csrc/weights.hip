@@ -830,7 +830,8 @@ extern "C" int kvc_batch_attention_weights_run(
               KVC_ERR_INVALID_ARG, "schedule not produced by kvc_weights_plan");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
               "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
-  KVC_REQUIRE(std::isfinite(sm_scale), KVC_ERR_INVALID_ARG, "sm_scale must be finite");
+  KVC_REQUIRE(sm_scale > 0.f && std::isfinite(sm_scale), KVC_ERR_INVALID_ARG,
+              "sm_scale must be positive and finite");
   if (sched->num_units == 0) return ok();
   KVC_REQUIRE(plan && (sched->total_q == 0 || (q && lse)), KVC_ERR_INVALID_ARG, "null pointer");
   KVC_REQUIRE(aligned(plan, 16), KVC_ERR_ALIGNMENT, "plan must be 16-byte aligned");
@@ -884,7 +885,8 @@ extern "C" int kvc_decode_attention_weights(
                                    "16 and groups up to 128");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,
               "dtype must be KVC_DTYPE_FP16 or KVC_DTYPE_BF16");
-  KVC_REQUIRE(std::isfinite(sm_scale), KVC_ERR_INVALID_ARG, "sm_scale must be finite");
+  KVC_REQUIRE(sm_scale > 0.f && std::isfinite(sm_scale), KVC_ERR_INVALID_ARG,
+              "sm_scale must be positive and finite");
   if (batch == 0 || num_indices == 0) return ok();
   KVC_REQUIRE(q && lse && indptr && last_page_len, KVC_ERR_INVALID_ARG, "null pointer");
   TokenArgs c;
