@@ -148,7 +148,7 @@ class PagedKVCache:
         self._step_handle: Optional[int] = None
         self._step_stream_obj = None
         self._step_users: dict = {}
-        self._mixed_step_buf: Optional[torch.Tensor] = None
+        self._step_temps: tuple = ()
         self.seq_lens = torch.zeros(max_seqs, dtype=torch.int32, device=self.device)
         self._seq_lens_cpu = torch.zeros(max_seqs, dtype=torch.int32)
         self._pool = PagePool(self.total_pages, max_seqs, self.max_pages_per_seq,
@@ -183,6 +183,9 @@ class PagedKVCache:
         self._evicted = np.zeros(max_seqs, dtype=np.int32)
         self._evicted_dev: Optional[torch.Tensor] = None
         self._evicted_dirty = False
+        # stream and event of the last upload; the streams that read it since
+        self._evicted_at: Optional[tuple] = None
+        self._evicted_users: dict = {}
         self._decode_ids: Optional[torch.Tensor] = None   # the decode plan's sequences
         self._weights_ids: Optional[torch.Tensor] = None  # the chunk weights plan's
 
@@ -441,7 +444,6 @@ class PagedKVCache:
         if b == 0:
             return
         self._sync_seqs(seq_ids)
-        self._upload_evicted()
         lens = self._seq_lens_cpu.numpy()[ids].astype(np.int32)
         nblk = (lens + self.page_size - 1) // self.page_size
         indptr = np.zeros(b + 1, dtype=np.int32)
@@ -449,6 +451,8 @@ class PagedKVCache:
         lpl = lens % self.page_size
         lpl = np.where((lpl == 0) & (lens != 0), self.page_size, lpl).astype(np.int32)
         self._check_page_counts(nblk)
+        self._claim_step_buffer()
+        self._upload_evicted()
         indptr_d = self._to_device(indptr)
         ids_d = self._to_device(ids.astype(np.int32))
         self._decode_ids = ids_d
@@ -458,6 +462,7 @@ class PagedKVCache:
             torch.from_numpy(indptr), self._plan_indices_gpu[:total], torch.from_numpy(lpl),
             num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
             page_size=self.page_size, pos_encoding_mode="NONE", q_data_type=self.dtype)
+        self._step_temps = (ids_d, self._decode_wrapper._plan_dev)
 
     def plan_prefill(self, seq_ids: Sequence[int], chunk_lens: Sequence[int]) -> None:
         """moe_engine.py:3649-3727: plan paged-KV prefill for continuation
@@ -539,7 +544,6 @@ class PagedKVCache:
             return slots
         ids = self._check_seq_ids(seq_ids)
         self._sync_seqs(seq_ids)
-        self._upload_evicted()
         lens_all = self._seq_lens_cpu.numpy()
         ms, ps = self.max_seqs, self.page_size
         lens = lens_all[ids].astype(np.int32) + 1
@@ -592,7 +596,8 @@ class PagedKVCache:
             cap = (sched.plan_ints + 3) // 4 * 4
 
         sh = self._claim_step_buffer()
-        self._mixed_step_buf = None
+        self._upload_evicted()
+        self._step_temps = ()
         if self._step_dev is None or self._step_dev.numel() < n:
             # grows rarely (more requests or block-table writes than before);
             # a graph captured before must then be captured again
@@ -661,10 +666,10 @@ class PagedKVCache:
                                                                   device=self.device)
             cur.wait_stream(self._step_stream_obj)
             self._step_users[sh] = cur
-            if self._mixed_step_buf is not None:
-                # a mixed step's buffer is freed at the next plan: keep the
-                # allocator from reusing it before this stream ran
-                self._mixed_step_buf.record_stream(cur)
+            # what a mixed step or plan_decode staged is freed at the next plan:
+            # keep the allocator from reusing it before this stream ran
+            for t in self._step_temps:
+                t.record_stream(cur)
         return sh
 
     def decode_graph_key(self) -> tuple:
@@ -737,7 +742,6 @@ class PagedKVCache:
         if R == 0:
             return torch.full((graph_n,), -1, dtype=torch.int64, device=self.device)
         self._sync_seqs(ids.tolist())
-        self._upload_evicted()
         lens_all = self._seq_lens_cpu.numpy()
         ms, ps = self.max_seqs, self.page_size
         before = lens_all[ids].astype(np.int64)
@@ -822,8 +826,9 @@ class PagedKVCache:
 
         # The step's one upload; the plans' unused capacity is not sent.
         self._claim_step_buffer()
+        self._upload_evicted()
         dm = torch.empty(hs.numel(), dtype=torch.int32, device=self.device)
-        self._mixed_step_buf = dm
+        self._step_temps = (dm,)
         ops.stage_from_host(hs, dm, o_dplan + (int(dsched.plan_ints) if D else 0),
                             o_pplan, o_pplan + (int(psched.plan_ints) if C else 0))
         self._host_image_sent()
@@ -943,7 +948,8 @@ class PagedKVCache:
                        for _ in range(self.num_layers)]
         self.positions = [torch.zeros(shape, dtype=torch.int32, device=self.device)
                           for _ in range(self.num_layers)]
-        self._evicted_dev = torch.zeros(self.max_seqs, dtype=torch.int32, device=self.device)
+        self._evicted_dev = torch.empty(self.max_seqs, dtype=torch.int32, device=self.device)
+        self._evicted_dirty = True
 
     def _require_tracking(self) -> None:
         self._require_gpu()
@@ -956,12 +962,35 @@ class PagedKVCache:
             self._evicted_dirty = True
 
     def _upload_evicted(self) -> None:
-        """The device's evicted counts, which the weights kernels read, as the
-        host has them (a plan or a step's setup calls this on its stream)."""
-        if self._evicted_dirty and self._evicted_dev is not None:
+        """Have the device's evicted counts, which the weights kernels read, as the
+        host has them, for what the current stream runs next (a plan or a step's
+        setup calls this): after the calls that still read the old ones, and after
+        an upload on another stream."""
+        if self._evicted_dev is None:
+            return
+        sh = _lib.current_stream_handle(self.device)
+        if self._evicted_at is not None and self._evicted_at[0] != sh:
+            torch.cuda.current_stream(self.device).wait_event(self._evicted_at[1])
+        if self._evicted_dirty:
+            self._wait_for_weights()
             self._evicted_dev.copy_(torch.from_numpy(self._evicted).pin_memory(),
                                     non_blocking=True)
+            event = torch.cuda.Event()
+            event.record(torch.cuda.current_stream(self.device))
+            self._evicted_at = (sh, event)
             self._evicted_dirty = False
+
+    def _wait_for_weights(self) -> None:
+        """Order the current stream after the weights calls of other streams."""
+        sh = _lib.current_stream_handle(self.device)
+        for h, st in self._evicted_users.items():
+            if h != sh:
+                torch.cuda.current_stream(self.device).wait_stream(st)
+        self._evicted_users = {}
+
+    def _note_weights_call(self, sh: int) -> None:
+        if sh not in self._evicted_users and not torch.cuda.is_current_stream_capturing():
+            self._evicted_users[sh] = torch.cuda.current_stream(self.device)
 
     def next_position(self, seq_id: int) -> int:
         """Position of the sequence's next token: its cached tokens and those
@@ -979,7 +1008,7 @@ class PagedKVCache:
         b = w.schedule.batch
         if q.dim() != 3 or q.shape[0] < b or lse.dim() != 2 or lse.shape[0] < b:
             raise RuntimeError(f"q and lse need a row for each of the step's {b} requests")
-        self._step_stream_for_call()
+        self._note_weights_call(self._step_stream_for_call())
         ops.decode_attention_weights(q[:b], lse[:b], self.k_cache[layer], w._indptr, w._indices,
                                      w._lpl, self.scores[layer], self.positions[layer],
                                      self._evicted_dev, seq_ids=self._decode_ids,
@@ -1030,6 +1059,7 @@ class PagedKVCache:
         w = self._weights_wrapper
         if w.schedule is None:
             raise RuntimeError("chunk_weights needs plan_chunk_weights first")
+        self._note_weights_call(_lib.current_stream_handle(self.device))
         w.run(q, lse, self.k_cache[layer], self.scores[layer], self.positions[layer],
               self._evicted_dev, self._weights_ids)
 
@@ -1039,8 +1069,9 @@ class PagedKVCache:
         head: the ``recent`` last ones stay, and of the others those of the
         largest ``scores`` (which the caller may have smoothed before).  Sets the
         lengths, frees the pages that are no longer needed and drops the current
-        plans.  Sequences of at most ``keep`` tokens are left alone; the lists
-        are one entry per sequence."""
+        plans.  Runs after the eager attention and weights calls of the current
+        step, whatever their streams.  Sequences of at most ``keep`` tokens are left
+        alone; the lists are one entry per sequence."""
         self._require_tracking()
         ids = self._check_seq_ids(seq_ids)
         b = len(ids)
@@ -1054,6 +1085,8 @@ class PagedKVCache:
             return
         ids, keeps, recents, lens = ids[cut], keeps[cut], recents[cut], lens[cut]
         self._sync_seqs(ids.tolist())
+        self._claim_step_buffer()
+        self._wait_for_weights()
         meta = self._to_device(np.stack([ids, lens, keeps, recents,
                                          self._evicted[ids]]).astype(np.int32))
         top = int(lens.max())
