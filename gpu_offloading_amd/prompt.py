@@ -44,8 +44,10 @@ def _scale(sm_scale: Optional[float], head_dim: int) -> float:
 def stage_plan(name: str, sched, args: tuple, capacity: int, device: torch.device) -> torch.Tensor:
     """The host plan function ``name(*args, sched, image, capacity)``, run again
     with the capacity it asks for where ``capacity`` int32 are too few, and its
-    image's device copy."""
+    image's device copy.  (The guess comes from index pointers that the function
+    is the first to check: 16 MiB at most.)"""
     lib = _lib.load()
+    capacity = min(capacity, 1 << 22)
     while True:
         image = torch.empty(max(capacity, 8), dtype=torch.int32, pin_memory=True)
         st = getattr(lib, name)(*args, sched, image.data_ptr(), image.numel())
