@@ -793,4 +793,6 @@ def evict_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scores: torch.T
 
 def evict_workspace_bytes(batch: int, num_kv_heads: int, max_seq_len: int) -> int:
     """Device memory that ``evict_kv`` needs for its move lists."""
+    if not 0 <= max_seq_len < 1 << 31:
+        _fail(f"max_seq_len must be in 0..2^31-1, got {max_seq_len}")
     return int(_lib.load().kvc_evict_workspace_bytes(batch, num_kv_heads, max_seq_len))
