@@ -3,7 +3,11 @@
 //
 //   s_ij = scale q_i . k_j   (j <= i + kv_len - q_len where causal)
 //   out_i = sum_j e^(s_ij - m_i) v_j / l_i,   l_i = sum_j e^(s_ij - m_i),   lse_i = m_i + ln l_i
-// in one pass over the keys with a running maximum m and sum l (online softmax).
+// in one pass over the keys with a running maximum m and sum l (online softmax), both
+// fp32.  The exponentials are rounded to the element type for the second product, as
+// the matrix instructions take them in that type: half a step each, independent from
+// key to key, which moves an output by about as much as its own rounding does.  l and
+// lse are sums of the unrounded ones.
 //
 // Work unit = (sequence, tile of query rows) x one KV head.  A query row is a
 // (token, query head) pair: the `group` query heads of a KV head are packed into
@@ -203,12 +207,13 @@ __device__ __forceinline__ float part_sum(u32x4_t lo, u32x4_t hi) {
 // of O^T += V^T P^T, keys in the order {4h..4h+3, 8+4h..8+4h+3} for lane half h,
 // and O^T's columns are query rows too.
 //
-// Measured: head_dim 128, bf16, 32 / 8 heads, 4 x 4096 tokens not causal 890 us (1235
-// TFLOP/s), one causal prompt of 16384 1.80 to 1.86 ms (68% of the matrix rate at the
-// 1.7 GHz that the power cap leaves), 64 x 512 203 us (bound by Q and the output at
-// each unit's ends); head_dim 64, fp16, 64 / 8 heads, 8 x 4096 not causal 2.29 ms (960
-// TFLOP/s, bound by the vector unit: exponential, maximum, sum and conversion of a
-// score cost 22 cycles beside 16 of products).
+// Measured: head_dim 128, bf16, 32 / 8 heads, 4 x 4096 tokens not causal 890 to 932 us
+// (1235 to 1179 TFLOP/s, by box), one causal prompt of 16384 1.85 to 1.89 ms (67% of the
+// matrix rate at the 1.7 GHz that the power cap leaves), 64 x 512 203 to 207 us (bound by
+// Q and the output at each unit's ends); head_dim 64, fp16, 64 / 8 heads, 8 x 4096 not
+// causal 2.29 to 2.37 ms (960 to 927 TFLOP/s; in a slot the vector unit is the bound:
+// exponential, maximum, sum and conversion of a score cost 22 cycles beside 16 of
+// products; ragged prompts spend nearly half their time around units' ends).
 template <typename T, int D>
 __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
   constexpr int kRow = 2 * D;                  // bytes per K or V row
@@ -569,7 +574,8 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) o[db] *= inv;
     if (cu.ntiles > 0 && lds.bad[k & 1] == k) {
-      // p > 0 times an inf or NaN that the row sees.
+      // p times an inf or NaN that the row sees, with p > 0 (one that vanished gives
+      // an inf here, where an interior tile's product gives NaN).
       for (int t = n_full * kKeys; t < min(cu.ntiles * kKeys, cu.kv_len); ++t) {
         const uint16_t* vr = a.v + (int64_t(cu.k_off) + t) * a.v_stride + cu.h * D + 4 * half;
 #pragma unroll
@@ -760,7 +766,8 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 // (about as many cycles), then the 32 of O^T += V_j^T P_j^T.  One barrier per tile:
 // behind it K_{j+1} and V_j are in LDS for all, and the loads of K_{j+2} and
 // V_{j+1} start into the buffers read last before it.  Measured: bf16, 16 / 8 heads, 4 x
-// 4096 tokens not causal 1141 us (964 TFLOP/s); bound by what one wave can issue.
+// 4096 tokens not causal 1141 to 1159 us (964 to 949 TFLOP/s); bound by what one wave
+// can issue.
 //
 // x * alpha of an accumulator register.  In plain code the rare rescaling of O would
 // pull all of it into the ordinary registers and back in every tile (256 moves).  At
@@ -1045,7 +1052,7 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) o[db] *= inv;
     if (n > 0 && lds.bad[k & 1] == k) {
-      // p > 0 times an inf or NaN that the row sees.
+      // As in prompt_kernel.
       for (int t = n_full * kKeys; t < min(n * kKeys, cu.kv_len); ++t) {
         const uint16_t* vr = a.v + (int64_t(cu.k_off) + t) * a.v_stride + cu.h * D + 4 * half;
 #pragma unroll
@@ -1237,8 +1244,8 @@ int64_t estimate(std::vector<int>& costs, int hkv, int64_t W) {
 // How units are cut along their keys: where fewer units than two rounds of workgroups
 // leave many of these idle, the items behind the `whole` longest go in pieces of at
 // most `longest` tiles (0: none does).  Measured: 8000 tokens of 4 query heads and one KV
-// head (125 units) 156 us whole, 82 cut; 4 sequences of 1000 to 1200 at head_dim 256, not
-// causal (284 units, two rounds) 92 and 72.
+// head (125 units) 156 us whole, 84 cut; 4 sequences of 1000 to 1200 at head_dim 256, not
+// causal (284 units, two rounds) 92 and 73.
 struct Cut { int64_t whole; int longest; };
 
 Cut choose_cut(const std::vector<int>& tiles, int hkv) {

@@ -8,8 +8,8 @@
 // exponential each.  S = Q K^T tiles from v_mfma_f32_32x32x16 (A: lane l = row
 // l%32, k = 8(l/32)..+7; B: column l%32, same k; C: acc[4i+j] = row
 // 8i+4(l/32)+j, column l%32) with query rows as A and keys as B: a key is a
-// column, so all its terms end up in two lanes and a row's masks and sums never
-// cross lanes.  A wave keeps its keys' K in registers for the whole unit and
+// column, so all its terms end up in two lanes (fp32 sums in row order, joined at the
+// end) and a row's masks and sums never cross lanes.  A wave keeps its keys' K in registers for the whole unit and
 // streams Q past them.
 //
 // Single-token form (weights_token_kernel): reads K once and is bound by that.
@@ -121,14 +121,15 @@ __host__ __device__ inline int first_token(int key0, int q_len, int kv_len, int 
 // the whole unit (B operands), and walk the same rows, which arrive in LDS a stage of
 // two blocks ahead (global_load_lds, each wave a quarter).  Per 32 rows x 64 keys a
 // wave issues, at head_dim 128, 16 matrix instructions of 32 cycles, 32 exponentials of
-// 8 and 64 other vector instructions of 4, so the vector unit is the bound (about 600
-// cycles); three waves per SIMD fill it, one's products beside the others'
-// exponentials.  Masks are a comparison per weight with the first row that sees the
+// 8 and 64 other vector instructions of 4, so in the walk the vector unit is the bound
+// (about 600 cycles; a block takes 800); three waves per SIMD share it, one's products
+// beside the others' exponentials.  Units of few rows are bound by their start: K is
+// waited for before the first product.  Masks are a comparison per weight with the first row that sees the
 // lane's key; with that instead of each row's limit read across lanes, and priorities
 // that go round, 4 prompts of 2000 tokens went from 93 to 83 us.
-// Measured (bf16, head_dim 128, 32 / 8 heads): 2000 rows against 16000 keys 245 us
-// (1005 TFLOP/s), 4 prompts of 1200 to 2048 tokens 62 us, 8 windows of 32 against 4096
-// 22.4 us.  Products of the next block interleaved with the exponentials in one wave,
+// Measured (bf16, head_dim 128, 32 / 8 heads): 2000 rows against 16000 keys 245 to 250
+// us (1005 to 985 TFLOP/s), 4 prompts of 1200 to 2048 tokens 64 us (the walk is half of
+// it), 8 windows of 32 against 4096 22 us.  Products of the next block interleaved with the exponentials in one wave,
 // at two waves per SIMD, took 10% longer.
 template <typename T, int D>
 __global__ __launch_bounds__(kChunkThreads, D == 64 ? 4 : D == 128 ? 3 : 2)
@@ -413,7 +414,7 @@ constexpr int kTokenThreads = 256;
 constexpr int64_t kTokenWorkgroups = 512;   // two per CU: what its registers hold
 // Pages per task: 64 registers of K, twice; at head_dim 256 32, as its query takes 32 more
 // (two pages spilled, and a reload waits for all of K: 64 requests of 512 to 4096
-// tokens 141 us, 129 with one).
+// tokens 141 us, 129 to 132 with one).
 constexpr int token_pages(int head_dim) { return head_dim == 256 ? 1 : 512 / head_dim; }
 
 // A wave runs every so-manieth task; a task is kPages consecutive entries of the
@@ -424,7 +425,7 @@ constexpr int token_pages(int head_dim) { return head_dim == 256 ? 1 : 512 / hea
 // 8(l/16)..+7; B: column l%16; C: acc[j] = row 4(l/16)+j, column l%16): rows are the
 // group's query heads, columns the page's tokens.  Lane 16 i + r then owns token r of
 // page i.  64 requests of 512 to 4096 tokens, 32 / 8 heads of 128: 288 MB in 58 us, 5.0
-// TB/s.
+// TB/s (the decode kernels' non-temporal loads of whole pages reach 6.2 to 7.0).
 template <typename T, int D>
 __global__ __launch_bounds__(kTokenThreads, 2) void weights_token_kernel(TokenArgs c) {
   constexpr int kSteps = D / 32;

@@ -936,8 +936,10 @@ class PagedKVCache:
         16]`` beside the cache (8 bytes per token and KV head).  Call it while no
         sequence holds tokens.  From then on every step's ``decode_weights`` /
         ``chunk_weights`` must follow its attention in every layer, as a token
-        gets its position and first score there; ``evict`` needs both.  Swapped
-        sequences keep theirs on the device; ``kv_snapshot`` does not cover them."""
+        gets its position and first score there; ``evict`` needs both.  (Of a cache
+        that ``decode`` or ``prefill`` does not take, fp16 or of another group, the
+        caller's own attention has to return the log-sum-exp.)  Swapped sequences
+        keep theirs on the device; ``kv_snapshot`` does not cover them."""
         self._require_gpu()
         if self.scores is not None:
             return

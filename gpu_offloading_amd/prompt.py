@@ -17,12 +17,11 @@ import numpy as np
 import torch
 
 from . import _lib
+from .ops import _WDTYPES as _DTYPES
 from .prefill import _fail, _host_int32
 
 __all__ = ["BatchPromptAttentionWrapper"]
 
-# KVC_DTYPE_* of include/kvc.h
-_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _DTYPE_NAMES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
                 "float16": torch.float16, "fp16": torch.float16, "half": torch.float16}
 

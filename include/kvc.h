@@ -567,7 +567,8 @@ int kvc_decode_step_setup(const int32_t* host_image, int32_t* dev_image,
  * j <= i + kv_len - q_len (causal) or always (causal = 0):
  *   out[i][hq] = softmax_j(sm_scale q[i][hq] . key[j][hq/group]) . value[j][hq/group]
  * A query that sees no key gets 0 (lse -inf).  What a query does not see has
- * no effect on it, inf and NaN included.  Optional lse[row][hq] is the
+ * no effect on it, inf and NaN included.  An inf in a value that it sees gives inf,
+ * or, where the value's weight vanishes in the element type, inf or NaN.  Optional lse[row][hq] is the
  * natural-log log-sum-exp of the scaled logits, from fp32 sums of the
  * unrounded exponentials; the exponentials are rounded to the element type for
  * the value product.  Scores may have any size for which sm_scale * log2(e) times
@@ -625,8 +626,9 @@ int kvc_prompt_run(const kvc_prompt_schedule* schedule, const int32_t* plan,
  *             exp(sm_scale q[i][hq] . K[t][h] - lse[i][hq])
  *   scores[block][h][slot] = w (a new token) or += w (an older one)
  * where lse is the natural-log log-sum-exp that the attention over the same
- * keys returned (decode, prefill or prompt run).  A row whose lse is -inf saw no
- * key and adds nothing.  scores is fp32 [num_blocks][num_kv_heads][16], beside
+ * keys returned (decode, prefill or prompt run).  A weight is as exact as an fp32 lse
+ * lets it be, |lse| 2^-23 of it: beyond some 2^20 it means little.  A row whose lse is
+ * -inf saw no key and adds nothing.  scores is fp32 [num_blocks][num_kv_heads][16], beside
  * the cache.  positions (int32, the same shape, may be null) gets each new
  * token's position, its slot in the sequence + position_offsets[seq_ids[b]]
  * (the tokens evicted from the sequence before; null, or outside its num_offsets
