@@ -151,6 +151,25 @@ __device__ __forceinline__ float settle_scores(f32x16_t (&s)[KB], float m, float
   return large ? 0.f : m;
 }
 
+// Whether the weight of key t (of the unit's) for the lane's row vanishes in the element
+// type under the maximum m: lanes l and l^32 each add up half of the dims.
+template <typename T, int D>
+__device__ __forceinline__ bool weight_vanishes(const PromptArgs& a, const Unit& U, int tok,
+                                                int head, int half, int t, float m) {
+#pragma clang fp contract(off)
+  asm volatile("" : "+v"(tok), "+v"(head), "+v"(half));   // (addresses here, not ahead of all)
+  const uint16_t* q = a.q + int64_t(U.q_off + tok) * a.q_stride +
+                      int64_t(U.h * a.group + head) * D + half * (D / 2);
+  const uint16_t* k = a.k + (int64_t(U.k_off) + t) * a.k_stride + U.h * D + half * (D / 2);
+  float dot = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < D / 2; ++i)
+    dot += float(__builtin_bit_cast(typename T::e, q[i])) *
+           float(__builtin_bit_cast(typename T::e, k[i]));
+  dot += __shfl_xor(dot, 32);
+  return float(static_cast<typename T::e>(fast_exp2(dot * a.scale_log2 - m))) == 0.f;
+}
+
 // A lane's share of a piece's row (O^T entries as accumulated, normalised), the row's
 // maximum m and the sum l under it.  (Their log-sum-exp m + log2 l in one number would
 // lose l beside a large m.)  l's 32 bits take the place of the lowest four of dims
@@ -574,17 +593,18 @@ __global__ __launch_bounds__(512, 1) void prompt_kernel(PromptArgs a) {
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) o[db] *= inv;
     if (cu.ntiles > 0 && lds.bad[k & 1] == k) {
-      // p times an inf or NaN that the row sees, with p > 0 (one that vanished gives
-      // an inf here, where an interior tile's product gives NaN).
+      // p times an inf or NaN that the row sees: NaN where p vanishes, as a product gives.
       for (int t = n_full * kKeys; t < min(cu.ntiles * kKeys, cu.kv_len); ++t) {
         const uint16_t* vr = a.v + (int64_t(cu.k_off) + t) * a.v_stride + cu.h * D + 4 * half;
+        const bool gone = weight_vanishes<T, D>(a, cu, cu.tok0 + (row_ok ? row_tok : 0),
+                                                row_ok ? row_head : 0, half, t, m_run);
 #pragma unroll
         for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const uint16_t w = vr[32 * db + 8 * (e >> 2) + (e & 3)];
             if (t <= limit && (w & T::kExp) == T::kExp)
-              o[db][e] += float(__builtin_bit_cast(typename T::e, w));
+              o[db][e] += gone ? NAN : float(__builtin_bit_cast(typename T::e, w));
           }
       }
     }
@@ -1055,13 +1075,15 @@ __global__ __launch_bounds__(256, 1) void prompt_wide_kernel(PromptArgs a) {
       // As in prompt_kernel.
       for (int t = n_full * kKeys; t < min(n * kKeys, cu.kv_len); ++t) {
         const uint16_t* vr = a.v + (int64_t(cu.k_off) + t) * a.v_stride + cu.h * D + 4 * half;
+        const bool gone = weight_vanishes<T, D>(a, cu, cu.tok0 + (row_ok ? row_tok : 0),
+                                                row_ok ? row_head : 0, half, t, m_run);
 #pragma unroll
         for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const uint16_t w = vr[32 * db + 8 * (e >> 2) + (e & 3)];
             if (t <= limit && (w & T::kExp) == T::kExp)
-              o[db][e] += float(__builtin_bit_cast(typename T::e, w));
+              o[db][e] += gone ? NAN : float(__builtin_bit_cast(typename T::e, w));
           }
       }
     }

@@ -568,7 +568,7 @@ int kvc_decode_step_setup(const int32_t* host_image, int32_t* dev_image,
  *   out[i][hq] = softmax_j(sm_scale q[i][hq] . key[j][hq/group]) . value[j][hq/group]
  * A query that sees no key gets 0 (lse -inf).  What a query does not see has
  * no effect on it, inf and NaN included.  An inf in a value that it sees gives inf,
- * or, where the value's weight vanishes in the element type, inf or NaN.  Optional lse[row][hq] is the
+ * or, where the value's weight vanishes in the element type, NaN.  Optional lse[row][hq] is the
  * natural-log log-sum-exp of the scaled logits, from fp32 sums of the
  * unrounded exponentials; the exponentials are rounded to the element type for
  * the value product.  Scores may have any size for which sm_scale * log2(e) times
