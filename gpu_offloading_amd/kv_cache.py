@@ -950,7 +950,7 @@ class PagedKVCache:
                        for _ in range(self.num_layers)]
         self.positions = [torch.zeros(shape, dtype=torch.int32, device=self.device)
                           for _ in range(self.num_layers)]
-        self._evicted_dev = torch.empty(self.max_seqs, dtype=torch.int32, device=self.device)
+        self._evicted_dev = torch.zeros(self.max_seqs, dtype=torch.int32, device=self.device)
         self._evicted_dirty = True
 
     def _require_tracking(self) -> None:

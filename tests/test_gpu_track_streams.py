@@ -173,3 +173,13 @@ def test_the_upload_reaches_other_streams(gpu):
         n = int(c._seq_lens_cpu[s])
         page = int(c.block_table[s, (n - 1) // 16])
         assert (c.positions[0][page, :, (n - 1) % 16] == want[s]).all()
+
+
+def test_counts_are_zero_before_the_first_plan(gpu):
+    """A plan made before track_attention: its weights calls read no stale memory."""
+    junk = [torch.full((4,), 12345, dtype=torch.int32, device=gpu) for _ in range(64)]
+    del junk
+    c = PagedKVCache(1, HKV, D, max_seqs=4, max_seq_len=400, num_qo_heads=HQ, kv_page_budget=60,
+                     device=gpu)
+    c.track_attention()
+    assert not c._evicted_dev.any()
