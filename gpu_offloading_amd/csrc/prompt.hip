@@ -227,7 +227,7 @@ __device__ __forceinline__ float part_sum(u32x4_t lo, u32x4_t hi) {
 // and O^T's columns are query rows too.
 //
 // Measured: head_dim 128, bf16, 32 / 8 heads, 4 x 4096 tokens not causal 890 to 932 us
-// (1235 to 1179 TFLOP/s, by box), one causal prompt of 16384 1.84 to 1.89 ms (67% of the
+// (1235 to 1179 TFLOP/s from card to card), one causal prompt of 16384 1.84 to 1.89 ms (67% of the
 // matrix rate at the 1.7 GHz that the power cap leaves), 64 x 512 203 to 207 us (bound by
 // Q and the output at each unit's ends); head_dim 64, fp16, 64 / 8 heads, 8 x 4096 not
 // causal 2.29 to 2.37 ms (960 to 927 TFLOP/s; in a slot the vector unit is the bound:
