@@ -253,6 +253,18 @@ SIGNATURES = {
         _P, _P, c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, _P, _I32P,
         _I32P, c_int64, c_int32, c_int32, _I32P, _I32P, _I32P, _I32P, _I32P, c_int32, c_int32,
         _P, c_int64, _P]),
+    "kvc_reshape_and_cache_quantized": (c_int, [
+        _P, _P, _P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
+        c_int64, c_int64, c_int64, c_int64, _I32P, _P]),
+    "kvc_gather_quantized_kv": (c_int, [
+        _P, _P, _P, _I32P, c_int64, c_int32, _I32P, _I32P, c_int32, c_int32, c_int32, c_int32,
+        c_int32, c_int64, c_int32, c_int32, c_int64, c_int64, _P, _P, c_int64, c_int64, _I32P,
+        _P]),
+    "kvc_quantized_decode_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "kvc_quantized_decode": (c_int, [
+        _P, c_int64, _P, _P, _P, c_int64, c_int64, c_int64, _I32P, _I32P, c_int64, _I32P, c_int32,
+        c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, _P, c_int64, _P, c_int64,
+        _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -722,6 +722,65 @@ int kvc_evict_kv(
     const int32_t* keep, const int32_t* recent, const int32_t* position_offsets,
     int32_t batch, int32_t max_seq_len, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Quantised cache: 8-bit codes and one fp32 scale per token's row of a KV head.
+ *   key_cache, value_cache  codes [num_blocks][num_kv_heads][16][head_dim]
+ *   scales                  fp32  [num_blocks][num_kv_heads][2][16]  (K's, V's)
+ * with block strides of their own (codes; floats), everything within a block packed.  A code
+ * stands for code * scale:
+ *   KVC_CODE_E4M3  scale 2^e, the least with amax / 2^e <= 448; code = x / scale
+ *                  rounded to e4m3 (OCP)
+ *   KVC_CODE_INT8  scale amax / 127; code = x * (127 / amax) rounded to a whole number
+ * (nearest, ties to even; amax the row's largest |x|, at least 2^-100).  A row with
+ * an infinity or a NaN gets the scale NaN: its values read as NaN.
+ * head_dim 64, 128 or 256, block_size 16, dtype (of the rows outside the cache) KVC_DTYPE_*.
+ * Caches and scales are 16-byte aligned, block strides multiples of 16 bytes.
+ *
+ * Write: kvc_reshape_and_cache_flash's contract (a negative slot is padding, one
+ * past the end is skipped and counted).  The slots of one call are distinct: of two tokens in
+ * one slot the codes of one may end up with the scale of the other.
+ * Read: kvc_gather_kv's contract, values = code * scale in fp32, rounded once to dtype;
+ * rows at or past max_seq_len of a sequence are not written.
+ * Decode: kvc_batch_decode_run's result over the values that the cache stands for
+ * (one query token per request; groups up to 16), without a plan: indptr
+ * [batch + 1], indices and last_page_len [batch] are read on the device, so
+ * that a captured launch serves other lengths and pages.  indptr[0] may be above 0.
+ * Pages whose id is outside [0, num_blocks), or past num_indices, hold no tokens;
+ * a request without tokens gets 0 and lse -inf.  The weights enter the product with V as bf16 (dtype
+ * bf16) or pairs of bf16 (fp16), sums are fp32.  workspace:
+ * kvc_quantized_decode_workspace_bytes of device memory, zeroed before its first use and of one
+ * call at a time; each call leaves it ready for the next.
+ * ---------------------------------------------------------------------- */
+enum { KVC_CODE_E4M3 = 0, KVC_CODE_INT8 = 1 };
+
+int kvc_reshape_and_cache_quantized(
+    const void* key, const void* value, void* key_cache, void* value_cache, float* scales,
+    const int64_t* slot_mapping, int64_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int64_t num_blocks, int32_t dtype, int32_t code,
+    int64_t key_token_stride, int64_t value_token_stride, int64_t cache_block_stride,
+    int64_t scales_block_stride, int32_t* oob_count, void* stream);
+
+int kvc_gather_quantized_kv(
+    const void* key_cache, const void* value_cache, const float* scales,
+    const int32_t* block_table, int64_t block_table_row_stride, int32_t block_table_width,
+    const int32_t* cu_seq_lens, const int32_t* seq_starts, int32_t batch, int32_t max_seq_len,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t num_blocks,
+    int32_t dtype, int32_t code, int64_t cache_block_stride, int64_t scales_block_stride,
+    void* out_key, void* out_value, int64_t out_token_stride, int64_t out_rows,
+    int32_t* oob_count, void* stream);
+
+int64_t kvc_quantized_decode_workspace_bytes(int32_t batch, int32_t num_qo_heads,
+                                             int32_t num_kv_heads, int32_t head_dim);
+
+int kvc_quantized_decode(
+    const void* q, int64_t q_batch_stride, const void* key_cache, const void* value_cache,
+    const float* scales, int64_t cache_block_stride, int64_t scales_block_stride,
+    int64_t num_blocks, const int32_t* indptr, const int32_t* indices, int64_t num_indices,
+    const int32_t* last_page_len, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t page_size, int32_t dtype, int32_t code, float sm_scale,
+    void* workspace, int64_t workspace_bytes, void* out, int64_t out_batch_stride, float* lse,
+    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

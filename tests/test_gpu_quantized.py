@@ -1,0 +1,515 @@
+"""GPU tests of the quantised cache's ops: the write bit for bit against its definition, the
+read-back against the same codes rounded once, decode attention against 64 bits within
+derived bounds; lengths from none to long ones, pages in any order, slots that hold
+garbage, strides, streams, graphs, offsets past 4 GiB."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import quant_ref as ref
+from gpu_offloading_amd import quantized as qz
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def bits(t):
+    return t.detach().cpu().contiguous().view(torch.uint8).numpy()
+
+
+def rows(shape, seed, dtype, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    size = torch.exp(spread * torch.randn(*shape[:-1], 1, generator=g))
+    return (torch.randn(*shape, generator=g) * size).to(dtype)
+
+
+def poisoned(blocks, h, d, codec, device):
+    """A cache in which every code and scale is something that must not be used."""
+    c = qz.quantized_cache(blocks, h, d, codec, device)
+    c.storage.fill_(0x7f)
+    c.scales.fill_(float("nan"))
+    return c
+
+
+# ------------------------------------------------------------------- write
+def check_written(cache, key, value, slots, codec):
+    """The slots hold the rows' codes and scales, all others what ``poisoned`` left."""
+    for x, c, i in ((key, cache.key_cache, 0), (value, cache.value_cache, 1)):
+        codes, scale = ref.encode(x[:len(slots)], codec)
+        got, gots = bits(c), cache.scales[:, :, i].cpu().numpy()
+        want, wants = np.full(got.shape, 0x7f, np.uint8), np.full(gots.shape, np.nan, np.float32)
+        skip = np.zeros(gots.shape, bool)
+        for t, s in enumerate(slots):
+            if 0 <= s < c.shape[0] * 16:
+                want[s // 16, :, s % 16] = codes[t]
+                wants[s // 16, :, s % 16] = scale[t]
+                skip[s // 16, :, s % 16] = np.isnan(scale[t])
+        assert np.array_equal(gots, wants, equal_nan=True)
+        assert np.array_equal(got[~skip], want[~skip])
+
+
+@pytest.mark.parametrize("codec", ref.CODECS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,d", [(1, 64), (3, 128), (8, 128), (2, 256)])
+@pytest.mark.parametrize("n", [1, 15, 33, 130])
+def test_write(gpu, codec, dtype, h, d, n):
+    cache = poisoned(12, h, d, codec, gpu)
+    k, v = rows((n, h, d), n, dtype, 2.0), rows((n, h, d), n + 1, dtype, 2.0)
+    slots = np.random.default_rng(n).permutation(12 * 16)[:n]
+    slots[::7] = -1
+    qz.reshape_and_cache_quantized(k.to(gpu), v.to(gpu), cache.key_cache, cache.value_cache,
+                                   cache.scales, torch.from_numpy(slots).to(gpu))
+    check_written(cache, k, v, slots, codec)
+
+
+@pytest.mark.parametrize("codec", ref.CODECS)
+def test_write_special_rows(gpu, codec):
+    """Rows of zeros, of the smallest and the largest values, of ties, with infinities and NaN."""
+    h, d = 2, 128
+    big, tiny = torch.finfo(torch.bfloat16).max, 2.0 ** -133
+    k = torch.zeros(9, h, d)
+    k[1] = tiny
+    k[2] = -big
+    k[2, :, ::3] = big / 3
+    k[3] = torch.arange(d) - 64.0
+    k[4] = 2.0 ** -101
+    k[4, :, 5] = -2.0 ** -100
+    k[5, 0, 7] = math.inf
+    k[6, 1, 100] = -math.nan
+    k[7] = 448 * 2.0 ** -6
+    k[7, 1] = 450                          # above 1.75 * 2^8: the next scale
+    k[8] = torch.linspace(-1, 1, d)
+    k = k.to(torch.bfloat16)
+    v = k.flip(0).contiguous()
+    cache = poisoned(2, h, d, codec, gpu)
+    slots = torch.arange(9, device=gpu) + 5
+    qz.reshape_and_cache_quantized(k.to(gpu), v.to(gpu), *cache[:3], slots)
+    check_written(cache, k, v, slots.tolist(), codec)
+    # what is not finite reads back as NaN, in its own token and head only
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=gpu)
+    cu = torch.tensor([0, 9], dtype=torch.int32, device=gpu)
+    gk, gv = qz.gather_quantized_kv(*cache[:3], table, cu, 9,
+                                    seq_starts=torch.tensor([5], dtype=torch.int32, device=gpu))
+    bad = torch.zeros(9, h, dtype=torch.bool)
+    bad[5, 0] = bad[6, 1] = True
+    assert torch.equal(gk.isnan().all(-1).cpu(), bad) and torch.equal(gk.isnan().any(-1).cpu(), bad)
+    assert torch.equal(gv.isnan().any(-1).cpu(), bad.flip(0))
+
+
+def test_write_strided_and_unaligned_sources(gpu):
+    """Slices of a fused tensor, rows that are not 16-byte aligned, more rows than slots."""
+    h, d, n = 4, 64, 37
+    for codec in ref.CODECS:
+        for pad in (0, 1, 4):
+            fused = rows((n, 6 * h * d + pad), 3, torch.float16, 0.5).to(gpu)
+            at = 2 * h * d + pad
+            k = fused[:, at:at + h * d].unflatten(1, (h, d))
+            v = fused[:, at + h * d:at + 2 * h * d].unflatten(1, (h, d))
+            cache = poisoned(3, h, d, codec, gpu)
+            slots = np.arange(n - 2)[::-1].copy()
+            qz.reshape_and_cache_quantized(k, v, *cache[:3], torch.from_numpy(slots).to(gpu))
+            check_written(cache, k, v, slots, codec)
+
+
+def test_write_skips_and_counts_slots_past_the_end(gpu):
+    cache = poisoned(3, 2, 128, ref.E4M3, gpu)
+    k = rows((5, 2, 128), 1, torch.bfloat16)
+    slots = np.array([48, 0, -1, 10 ** 12, 47])
+    oob = torch.zeros(1, dtype=torch.int32, device=gpu)
+    qz.reshape_and_cache_quantized(k.to(gpu), k.to(gpu), *cache[:3],
+                                   torch.from_numpy(slots).to(gpu), oob_count=oob)
+    assert int(oob) == 2
+    check_written(cache, k, k, slots, ref.E4M3)
+    qz.reshape_and_cache_quantized(k.to(gpu), k.to(gpu), *cache[:3],
+                                   torch.empty(0, dtype=torch.int64, device=gpu))
+
+
+# -------------------------------------------------------------------- read
+def random_cache(lens, h, d, codec, device, seed, extra=3):
+    """A poisoned cache holding sequences of random codes in permuted pages: (cache, table rows
+    padded with -1, code values and scales of each sequence [2][n, H, D] / [2][n, H], on the host)."""
+    rng = np.random.default_rng(seed)
+    need = [(n + 15) // 16 for n in lens]
+    blocks = sum(need) + extra
+    c = poisoned(blocks, h, d, codec, device)
+    codes = [bits(t).copy() for t in (c.key_cache, c.value_cache)]
+    scales = np.full((blocks, h, 2, 16), np.nan, np.float32)
+    scales[::2] = np.inf                       # (of slots that hold no token)
+    order = rng.permutation(blocks)
+    table = np.full((len(lens), max(need + [1]) + 1), -1, np.int32)
+    held, at = [], 0
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = order[at:at + need[b]]
+        at += need[b]
+        t = np.arange(n)
+        blk, off = table[b, t // 16], t % 16
+        seq = []
+        for i in range(2):
+            x = rng.integers(0, 256, (n, h, d)).astype(np.uint8)
+            if codec is ref.E4M3:
+                x[(x & 127) == 127] = 0
+                x = np.where(rng.random(x.shape) < 0.5, x & 0xbf, x)     # fewer large codes
+            s = np.exp(rng.normal(-4.0, 1.0, (n, h))).astype(np.float32)
+            codes[i][blk, :, off] = x
+            scales[blk, :, i, off] = s
+            seq.append((ref.values(x, codec), s))
+        held.append(seq)
+    for t, x in zip((c.key_cache, c.value_cache), codes):
+        t.copy_(torch.from_numpy(x).view(t.dtype).to(device))
+    c.scales.copy_(torch.from_numpy(scales))
+    return c, table, held
+
+
+def ints(x, device):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("codec", ref.CODECS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,d", [(1, 128), (8, 128), (3, 64), (2, 256)])
+def test_read(gpu, codec, dtype, h, d):
+    lens, starts = [40, 1, 0, 16, 333, 31], [7, 0, 0, 16, 160, 15]
+    part = [33, 1, 0, 0, 100, 16]
+    cache, table, held = random_cache(lens, h, d, codec, gpu, 1)
+    cu = np.concatenate([[2], 2 + np.cumsum(part)])
+    outs = [torch.full((cu[-1] + 3, h, d), 7.0, dtype=dtype, device=gpu) for _ in "kv"]
+    got = qz.gather_quantized_kv(*cache[:3], ints(table, gpu), ints(cu, gpu), 100, *outs,
+                                 ints(starts, gpu))
+    for i, t in enumerate(got):
+        assert t is outs[i]
+        want = torch.full(t.shape, 7.0, dtype=dtype)
+        for b, (n, s) in enumerate(zip(part, starts)):
+            x, scale = (y[s:s + n] for y in held[b][i])
+            want[cu[b]:cu[b + 1]] = (torch.from_numpy(x).float() *
+                                     torch.from_numpy(scale)[..., None]).to(dtype)
+        assert np.array_equal(bits(t), bits(want))
+
+
+def test_read_whole_sequences_and_odd_outputs(gpu):
+    """Outputs made by the call, and outputs whose rows are not 16-byte aligned."""
+    h, d = 4, 64
+    cache, table, held = random_cache([100, 17], h, d, ref.INT8, gpu, 2)
+    cu = ints([0, 100, 117], gpu)
+    gk, gv = qz.gather_quantized_kv(*cache[:3], ints(table, gpu), cu, 100, dtype=torch.float16)
+    assert gk.dtype is gv.dtype is torch.float16 and gk.shape == (117, h, d)
+    for i, t in enumerate((gk, gv)):
+        want = torch.cat([torch.from_numpy(x).float() * torch.from_numpy(s)[..., None]
+                          for x, s in (held[0][i], held[1][i])]).to(torch.float16)
+        assert torch.equal(t.cpu(), want)
+        room = torch.zeros(117 * (h * d + 3) + 1, dtype=torch.float16, device=gpu)
+    wide = [room.clone()[1:].unflatten(0, (117, h * d + 3))[:, :h * d].unflatten(1, (h, d))
+            for _ in "kv"]
+    qz.gather_quantized_kv(*cache[:3], ints(table, gpu), cu, 100, *wide)
+    assert torch.equal(wide[0], gk) and torch.equal(wide[1], gv)
+
+
+def test_read_bad_places(gpu):
+    """Missing pages read as zeros and are counted; rows past the outputs or past max_seq_len
+    are left alone."""
+    h, d = 2, 128
+    cache, table, held = random_cache([64, 64], h, d, ref.E4M3, gpu, 3)
+    table[0, 1], table[1, 2] = -1, 10 ** 6
+    oob = torch.zeros(1, dtype=torch.int32, device=gpu)
+    outs = [torch.full((120, h, d), 7.0, dtype=torch.bfloat16, device=gpu) for _ in "kv"]
+    qz.gather_quantized_kv(*cache[:3], ints(table, gpu), ints([0, 64, 128], gpu), 60, *outs,
+                           oob_count=oob)
+    for i, t in enumerate(outs):
+        want = torch.full(t.shape, 7.0, dtype=torch.bfloat16)
+        for b in range(2):
+            x, s = held[b][i]
+            y = (torch.from_numpy(x).float() * torch.from_numpy(s)[..., None]).to(torch.bfloat16)
+            y[16 * (b + 1):16 * (b + 2)] = 0
+            m = min(60, 120 - 64 * b)
+            want[64 * b:64 * b + m] = y[:m]
+        assert torch.equal(t.cpu(), want)
+    assert int(oob) == 32 + 4                  # two pages; rows 120 .. 123 of the second sequence
+    # a range that begins before its sequence
+    oob.zero_()
+    qz.gather_quantized_kv(*cache[:3], ints(table[1:], gpu), ints([0, 20], gpu), 20, *outs,
+                           ints([-5], gpu), oob_count=oob)
+    assert int(oob) == 5 and not outs[0][:5].any()
+    x, s = held[1][0]
+    assert torch.equal(outs[0][5:20].cpu(), (torch.from_numpy(x).float() *
+                                             torch.from_numpy(s)[..., None]).to(torch.bfloat16)[:15])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_e4m3_values_are_fixed_points(gpu, dtype, d):
+    """What is read back and written again gives the same codes and scales."""
+    h, n = 3, 50
+    a, b = (poisoned(4, h, d, ref.E4M3, gpu) for _ in "ab")
+    k, v = rows((n, h, d), 1, dtype).to(gpu), rows((n, h, d), 2, dtype).to(gpu)
+    slots = torch.randperm(64, generator=torch.Generator().manual_seed(1))[:n].to(gpu)
+    table, cu = ints([[0, 1, 2, 3]], gpu), ints([0, 64], gpu)
+    qz.reshape_and_cache_quantized(k, v, *a[:3], slots)
+    gk, gv = qz.gather_quantized_kv(*a[:3], table, cu, 64, dtype=dtype)
+    qz.reshape_and_cache_quantized(gk[slots], gv[slots], *b[:3], slots)
+    rk, rv = qz.gather_quantized_kv(*b[:3], table, cu, 64, dtype=dtype)
+    assert torch.equal(gk[slots], rk[slots]) and torch.equal(gv[slots], rv[slots])
+
+
+# ------------------------------------------------------------------ decode
+def pages(table, lens, first=0):
+    need = [(n + 15) // 16 for n in lens]
+    ip = np.concatenate([[0], np.cumsum(need)]) + first
+    idx = np.concatenate([np.full(first, 10 ** 6, np.int32)] +
+                         [table[b, :m] for b, m in enumerate(need)] + [np.zeros(0, np.int32)])
+    return ip, idx, [(n - 1) % 16 + 1 if n else 0 for n in lens]
+
+
+def check_decode(out, lse, q, held, lens, scale, dtype):
+    hkv = held[0][0][0].shape[1]
+    group = q.shape[1] // hkv
+    for b, n in enumerate(lens):
+        for h in range(hkv):
+            g = slice(h * group, (h + 1) * group)
+            (k, ks), (v, vs) = ((torch.from_numpy(x[:n, h]), torch.from_numpy(s[:n, h]))
+                                for x, s in held[b])
+            o, l, ot, lt = ref.attention(q[b, g].cpu(), k, ks, v, vs, scale, dtype)
+            err, lerr = (out[b, g].cpu().double() - o).abs(), (lse[b, g].cpu().double() - l).abs()
+            assert (err <= ot).all(), (b, h, n, (err / ot).max())
+            if n:
+                assert (lerr <= lt).all(), (b, h, n, (lerr / lt).max())
+            else:
+                assert (lse[b, g] == -math.inf).all() and not out[b, g].any()
+
+
+@pytest.mark.parametrize("codec", ref.CODECS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hkv,group", [(1, 1), (2, 3), (8, 4), (1, 16), (3, 8)])
+def test_decode(gpu, codec, dtype, d, hkv, group):
+    lens = [1, 16, 17, 0, 33, 300, 15, 64, 0, 700]
+    cache, table, held = random_cache(lens, hkv, d, codec, gpu, d + group)
+    ip, idx, lpl = pages(table, lens)
+    q = rows((len(lens), hkv * group, d), 5, dtype, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True)
+    check_decode(*got, q, held, lens, d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("lens", [[1], [0], [0, 0, 5, 0], [129], [4096], [20000], [16] * 70,
+                                  [513] * 9 + [0] * 80 + [31], [2000, 1, 3000, 17]])
+@pytest.mark.parametrize("codec", ref.CODECS)
+def test_decode_lengths(gpu, lens, codec):
+    """One request to many, cut into few segments and many; a scale of its own."""
+    hkv, group, d = 2, 4, 128
+    cache, table, held = random_cache(lens, hkv, d, codec, gpu, sum(lens))
+    ip, idx, lpl = pages(table, lens)
+    q = rows((len(lens), hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True, sm_scale=0.03)
+    check_decode(*got, q, held, lens, 0.03, torch.bfloat16)
+
+
+def test_decode_outputs_strides_and_page_offsets(gpu):
+    """q and out as slices, given outputs with more rows, an indptr that begins above 0, a
+    workspace used again and again."""
+    lens, hkv, group, d = [50, 3, 900, 0], 4, 2, 128
+    hq = hkv * group
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, 9)
+    ip, idx, lpl = pages(table, lens, first=5)
+    fused = rows((4, hq + 2 * hkv, d), 2, torch.bfloat16, 0.3).to(gpu)
+    q = fused[:, :hq]
+    room = torch.full((6, hq + 1, d), 7.0, dtype=torch.bfloat16, device=gpu)
+    lse = torch.full((6, hq), 7.0, device=gpu)
+    ws = qz.decode_workspace(4, hq, hkv, d, gpu)
+    first = None
+    for _ in range(3):
+        out, l = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                               ints(lpl, gpu), out=room[:, :hq], lse=lse,
+                                               return_lse=True, workspace=ws)
+        assert l is lse and out.data_ptr() == room.data_ptr()
+        check_decode(out, lse, q, held, lens, d ** -0.5, torch.bfloat16)
+        if first is not None:
+            assert torch.equal(room, first)        # bit for bit, call after call
+        first = room.clone()
+    assert (room[:, hq] == 7).all() and (room[4:] == 7).all() and (lse[4:] == 7).all()
+    only = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                         ints(lpl, gpu))
+    assert torch.equal(only, room[:4, :hq])
+
+
+def test_decode_pages_that_are_missing(gpu):
+    """Page ids outside the cache, and pages past the index list, hold no tokens; a last
+    page length outside 0..16 counts as the nearest."""
+    lens, hkv, group, d = [100, 64, 40], 2, 4, 128
+    cache, table, held = random_cache(lens, hkv, d, ref.INT8, gpu, 4)
+    ip, idx, lpl = pages(table, lens)
+    idx = idx.copy()
+    idx[1], idx[4], idx[7:11] = -7, 10 ** 9, [-1, -2, 10 ** 7, -1]
+    q = rows((3, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx[:-1], gpu),
+                                        ints([lpl[0], 99, lpl[2]], gpu), return_lse=True)
+    left = [np.r_[0:16, 32:64, 80:100], np.arange(0), np.arange(32)]
+    kept = [[(x[t], s[t]) for x, s in seq] for t, seq in zip(left, held)]
+    check_decode(*got, q, kept, [len(t) for t in left], d ** -0.5, torch.bfloat16)
+
+
+def test_decode_of_rows_that_are_not_finite(gpu):
+    """A NaN row of K makes its head's outputs NaN, one of V its values; other heads and
+    requests, and tokens past the end, are as before."""
+    lens, hkv, group, d = [40, 40, 40], 2, 4, 128
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, 6)
+    ip, idx, lpl = pages(table, lens)
+    q = rows((3, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    args = ints(ip, gpu), ints(idx, gpu), ints(lpl, gpu)
+    base, blse = qz.quantized_decode_attention(q, *cache[:3], *args, return_lse=True)
+    cache.scales[table[1, 1], 0, 0, 3] = math.nan          # K of request 1, head 0
+    cache.scales[table[2, 2], 1, 1, 7] = math.nan          # V of request 2, head 1
+    out, lse = qz.quantized_decode_attention(q, *cache[:3], *args, return_lse=True)
+    bad = torch.zeros(3, hkv * group, dtype=torch.bool)
+    bad[1, :group] = bad[2, group:] = True
+    assert out[bad].isnan().all() and torch.equal(out[~bad], base[~bad])
+    bad[2] = False
+    assert lse[bad].isnan().all() and torch.equal(lse[~bad], blse[~bad])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decode_of_large_and_small_scales(gpu, dtype):
+    """V rows of very different sizes, scores far apart, logits beyond 2^20."""
+    lens, hkv, group, d = [200, 77], 1, 4, 128
+    cache, table, held = random_cache(lens, hkv, d, ref.INT8, gpu, 8)
+    for b, n in enumerate(lens):
+        t = np.arange(n)
+        for i in range(2):
+            e = 2.0 ** ((t * 7) % 25 - (20 if i else 4)).astype(np.float32)
+            held[b][i][1][:] *= e[:, None]
+            blk = torch.from_numpy(table[b, t // 16]).long().to(gpu)
+            off = torch.from_numpy(t % 16).to(gpu)
+            cache.scales[blk, :, i, off] = torch.from_numpy(held[b][i][1]).to(gpu)
+    if dtype is torch.float16:          # outputs within its range
+        cache.scales[:, :, 1] *= 2.0 ** -6
+        for b in range(2):
+            held[b][1][1][:] *= 2.0 ** -6
+    ip, idx, lpl = pages(table, lens)
+    q = rows((2, group, d), 5, dtype, 1.0).to(gpu)
+    for scale in (1e-4, 1.0, 64.0):
+        got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                            ints(lpl, gpu), return_lse=True, sm_scale=scale)
+        assert got[0].isfinite().all()
+        check_decode(*got, q, held, lens, scale, dtype)
+
+
+# ------------------------------------------------- streams, graphs, offsets
+def test_step_captured_and_replayed(gpu):
+    """Write, read back and decode in one graph, replayed with new tokens, lengths and pages,
+    eager work between the replays; every replay equals the eager calls bit for bit."""
+    hkv, group, d, batch = 2, 4, 128, 5
+    cache = poisoned(90, hkv, d, ref.E4M3, gpu)
+    rng = np.random.default_rng(0)
+    table = rng.permutation(90)[:batch * 16].reshape(batch, 16).astype(np.int32)
+    k, v = (torch.empty(batch, hkv, d, dtype=torch.bfloat16, device=gpu) for _ in "kv")
+    q = torch.empty(batch, hkv * group, d, dtype=torch.bfloat16, device=gpu)
+    slots = torch.empty(batch, dtype=torch.int64, device=gpu)
+    ip, idx = ints(np.zeros(batch + 1), gpu), ints(np.zeros(batch * 16), gpu)
+    lpl, start = ints(np.zeros(batch), gpu), ints(np.zeros(batch), gpu)
+    tab, cu = ints(table, gpu), ints(np.arange(batch + 1), gpu)
+    ok, ov, out = torch.empty_like(k), torch.empty_like(v), torch.empty_like(q)
+    lse = torch.empty(batch, hkv * group, device=gpu)
+    ws = qz.decode_workspace(batch, hkv * group, hkv, d, gpu)
+
+    def fill(step):
+        lens = [(step * 37 + 60 * b) % 250 + 1 for b in range(batch)]
+        for i, t in enumerate((k, v, q)):
+            t.copy_(rows(tuple(t.shape), step * 3 + i, torch.bfloat16, 0.3))
+        pos = np.array(lens) - 1
+        slots.copy_(torch.from_numpy(table[np.arange(batch), pos // 16].astype(np.int64) * 16 + pos % 16))
+        p, x, l = pages(table, lens)
+        ip.copy_(torch.from_numpy(p))
+        idx[:len(x)].copy_(torch.from_numpy(x))
+        lpl.copy_(ints(l, gpu))
+        start.copy_(torch.from_numpy(pos))
+
+    def step():
+        qz.reshape_and_cache_quantized(k, v, *cache[:3], slots)
+        qz.gather_quantized_kv(*cache[:3], tab, cu, 1, ok, ov, start)
+        qz.quantized_decode_attention(q, *cache[:3], ip, idx, lpl, out=out, lse=lse, workspace=ws)
+
+    # every slot that a step may attend to holds a token
+    full = torch.arange(90 * 16, device=gpu)
+    qz.reshape_and_cache_quantized(rows((1440, hkv, d), 1, torch.bfloat16).to(gpu),
+                                   rows((1440, hkv, d), 2, torch.bfloat16).to(gpu), *cache[:3], full)
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n in range(6):
+        fill(n)
+        for t in (ok, ov, out, lse):
+            t.fill_(7.0)
+        graph.replay()
+        got = [t.clone() for t in (ok, ov, out, lse)]
+        before = cache.storage.clone()
+        for t in (ok, ov, out, lse):
+            t.fill_(7.0)
+        step()
+        assert all(torch.equal(a, b) for a, b in zip(got, (ok, ov, out, lse)))
+        assert torch.equal(before, cache.storage)
+
+
+def test_ops_on_a_given_stream(gpu):
+    """Each op on a stream that is not the current one, its outputs from that stream."""
+    lens, hkv, group, d = [700, 90], 2, 4, 128
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, 3)
+    ip, idx, lpl = (ints(x, gpu) for x in pages(table, lens))
+    q = rows((2, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    want = qz.quantized_decode_attention(q, *cache[:3], ip, idx, lpl, return_lse=True)
+    tab, cu = ints(table, gpu), ints([0, 700, 790], gpu)
+    wk, wv = qz.gather_quantized_kv(*cache[:3], tab, cu, 700)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = qz.quantized_decode_attention(q, *cache[:3], ip, idx, lpl, return_lse=True,
+                                            stream=side)
+        outs = [torch.empty_like(wk) for _ in "kv"]
+        side.wait_stream(torch.cuda.current_stream())
+        gk, gv = qz.gather_quantized_kv(*cache[:3], tab, cu, 700, *outs, stream=side)
+        side.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(gk, wk) and torch.equal(gv, wv)
+    k = rows((1, hkv, d), 1, torch.bfloat16).to(gpu)
+    slot = torch.tensor([int(table[0, 0]) * 16 + 3], device=gpu)
+    side.wait_stream(torch.cuda.current_stream())
+    qz.reshape_and_cache_quantized(k, k, *cache[:3], slot, stream=side)
+    side.synchronize()
+    codes, scale = ref.encode(k, ref.E4M3)
+    assert np.array_equal(bits(cache.key_cache)[table[0, 0], :, 3], codes[0])
+
+
+def test_offsets_past_4_gib(gpu):
+    """Blocks whose codes and scales lie beyond 4 GiB, in one storage of blocks."""
+    h, d, blocks = 8, 128, 140_000
+    c = qz.quantized_cache(blocks, h, d, ref.E4M3, gpu)
+    assert c.storage.numel() > 1 << 32
+    lens = [300, 40]
+    rng = np.random.default_rng(1)
+    table = np.concatenate([[blocks - 1, 0], rng.choice(np.arange(130_000, blocks - 1), 20,
+                                                        replace=False)]).astype(np.int32)
+    table = np.stack([table[:19], np.r_[table[19:22], [-1] * 16]]).astype(np.int32)
+    n = sum(lens)
+    slots = np.concatenate([table[b, np.arange(m) // 16].astype(np.int64) * 16 + np.arange(m) % 16
+                            for b, m in enumerate(lens)])
+    k, v = rows((n, h, d), 1, torch.bfloat16), rows((n, h, d), 2, torch.bfloat16)
+    qz.reshape_and_cache_quantized(k.to(gpu), v.to(gpu), *c[:3], torch.from_numpy(slots).to(gpu))
+    held = []
+    enc = [ref.encode(x, ref.E4M3) for x in (k, v)]
+    for a, m in ((0, 300), (300, 40)):
+        held.append([(ref.values(x[a:a + m], ref.E4M3), s[a:a + m]) for x, s in enc])
+    gk, gv = qz.gather_quantized_kv(*c[:3], ints(table, gpu), ints([0, 300, 340], gpu), 300)
+    for t, (x, s) in zip((gk, gv), enc):
+        assert torch.equal(t.cpu(), (torch.from_numpy(ref.values(x, ref.E4M3)).float() *
+                                     torch.from_numpy(s)[..., None]).to(torch.bfloat16))
+    q = rows((2, 32, d), 3, torch.bfloat16, 0.3).to(gpu)
+    ip, idx, lpl = (ints(x, gpu) for x in pages(table, lens))
+    got = qz.quantized_decode_attention(q, *c[:3], ip, idx, lpl, return_lse=True)
+    check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
