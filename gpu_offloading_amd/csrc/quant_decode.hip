@@ -19,11 +19,12 @@
 // A row's running maximum is only raised (and O rescaled) where a score exceeds it by 2^8:
 // the maximum needs no cross-lane step per tile.
 //
-// Split: the batch's pages, laid end to end, are cut into equal segments, one per
-// workgroup and KV head; each finds its first request in indptr by itself.  The launch
-// depends on the batch size alone, so a captured one serves other lengths and pages.  The
-// part of a request in one segment is a piece; one that is a whole request is written out,
-// the others leave (m, l, O) in the workspace, joined by quant_merge_kernel.
+// Split: the batch's pages, laid end to end, are cut into equal segments, one per workgroup
+// and KV head; each finds its first request in indptr by itself.  The launch depends on the
+// batch size alone, so a captured one serves other lengths and pages.  The part of a
+// request in one segment is a piece, whose tiles the workgroup's waves take in turn and join in
+// LDS.  A piece that is a whole request is written out; the others leave (m, l, O) in the
+// workspace, which quant_merge_kernel joins, in the order of the pieces.
 #include "quant.h"
 
 #include <algorithm>
@@ -35,6 +36,10 @@ namespace {
 
 constexpr int kWaves = 4;             // waves of a workgroup
 constexpr int kMinPages = 16;         // of a segment
+
+// Waves per SIMD, which bounds their registers.
+constexpr int per_simd(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
+
 constexpr float kRaise = 8.f;         // log2: how far a score may exceed the running maximum
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -60,7 +65,7 @@ struct QuantDecodeArgs {
   int32_t batch, hq, hkv, group;
   int32_t segments;          // per KV head
   float scale_log2;
-  float* parts;              // [hkv][segments][2][group][D + 2]: m, l, O
+  float* parts;              // [hkv][segments][2][group][D + 4]: m, l, -, -, O
   uint16_t* out;
   int64_t out_stride;        // elements between requests
   float* lse;                // may be null
@@ -69,6 +74,13 @@ struct QuantDecodeArgs {
 // Pages per segment; the kernels agree on it.
 __device__ __forceinline__ int segment_pages(const QuantDecodeArgs& a, int total) {
   return max(kMinPages, int((int64_t(total) + a.segments - 1) / a.segments));
+}
+
+// Index arrays are read through the scalar cache, ahead of use: a vector load of a page id
+// would have to be waited for together with all the K and V loads in front of it.
+typedef const int32_t __attribute__((address_space(4))) * ScalarInts;
+__device__ __forceinline__ ScalarInts scalar_ints(const int32_t* p) {
+  return (ScalarInts)reinterpret_cast<uintptr_t>(p);
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -94,23 +106,42 @@ __device__ __forceinline__ float across(float v, F f) {
   return f(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
-// First request whose pages reach past `page` (pages counted from indptr[0]); the last one
-// if none does.  64 entries of indptr are compared at a time.
-__device__ __forceinline__ int find_request(const int32_t* indptr, int batch, int base, int page) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = batch;
-  while (n > 1) {
-    const int step = (n + 63) / 64;
-    const int i = min((lane + 1) * step, n);
-    // requests before the one looked for end at or below `page`
-    const bool below = lane * step < n && indptr[lo + i] - base <= page;
-    const int c = __popcll(__ballot(below));
-    lo = uniform(min(lo + c * step, lo + n - 1));
-    n = min(step, batch - lo);
-    if (step == 1) break;
+// First request whose pages reach past a page (pages counted from indptr[0]; the last one if
+// none does), and where it begins and ends.  64 entries of indptr are compared at a time; the
+// first 64 are loaded before the page is known, beside what it depends on.
+struct Search {
+  int entry, step;
+
+  __device__ __forceinline__ void start(const int32_t* indptr, int batch) {
+    const int lane = threadIdx.x & 63;
+    step = (batch + 63) / 64;
+    entry = indptr[min((lane + 1) * step, batch)];
   }
-  return lo;
-}
+  __device__ __forceinline__ int find(const int32_t* indptr, int batch, int base, int page,
+                                      int& first, int& last) const {
+    const int lane = threadIdx.x & 63;
+    // blocks of `step` requests before the one looked for end at or below `page`
+    int c = __popcll(__ballot(lane * step < batch && entry - base <= page));
+    if (step == 1) {
+      c = uniform(min(c, batch - 1));
+      last = __builtin_amdgcn_readlane(entry, c) - base;
+      first = c ? __builtin_amdgcn_readlane(entry, max(c - 1, 0)) - base : 0;
+      return c;
+    }
+    int lo = uniform(min(c * step, batch - 1)), n = min(step, batch - lo);
+    while (n > 1) {
+      const int s = (n + 63) / 64;
+      const int e = indptr[lo + min((lane + 1) * s, n)];
+      c = __popcll(__ballot(lane * s < n && e - base <= page));
+      const int skip = min(c * s, n - 1);
+      lo = uniform(lo + skip);
+      n = s == 1 ? 1 : min(s, n - skip);
+    }
+    first = scalar_ints(indptr)[lo] - base;
+    last = scalar_ints(indptr)[lo + 1] - base;
+    return lo;
+  }
+};
 
 template <int D>
 struct VWord;
@@ -129,179 +160,262 @@ __device__ __forceinline__ uint32_t word(typename VWord<D>::type v, int i) {
     return v[i];
 }
 
+// Barrier between the waves' uses of LDS.  (__syncthreads would also wait for the global loads.)
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Dims 4 c .. 4 c + 3 of a finished query row.
+template <int D, bool kHalf>
+__device__ __forceinline__ void write_out(const QuantDecodeArgs& a, int b, int hq, int c, float top,
+                                          float sum, f32x4_t acc) {
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(a.out + b * a.out_stride + int64_t(hq) * D + c * 4) =
+      make_uint2(pack2<kHalf>(acc[0] * f, acc[1] * f), pack2<kHalf>(acc[2] * f, acc[3] * f));
+  if (a.lse && c == 0)
+    a.lse[int64_t(b) * a.hq + hq] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+}
+
 template <int D, int kCode, bool kHalf>
-__global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void quant_decode_kernel(
+__global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     QuantDecodeArgs a) {
   using V = typename VWord<D>::type;
   constexpr int kKLoads = D / 64;   // 16-byte pieces of a K row per lane
   constexpr int kDims = D / 16;     // dims of a V row per lane
+  constexpr int kRound = 2 * kWaves;   // pages that the waves take at a time
   extern __shared__ float lds[];    // [kWaves][group][D + 4]: m, l, -, -, O
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int row = lane & 15, g = lane >> 4;
-  const uint32_t k_lane = row * D + g * 16, v_lane = g * 4 * D + row * kDims, s_lane = g * 16;
   const int head = blockIdx.x % a.hkv, segment = blockIdx.x / a.hkv;
-  const int base = a.indptr[0], total = a.indptr[a.batch] - base;
+  // K rows of 128 bytes and more are loaded as whole 128-byte lines, eight rows at a time: lane (t,
+  // g) loads the piece 2 g + t / 8 of rows t % 8 and t % 8 + 8, and trades one of the two with lane
+  // (t ^ 8, g).  (The same bytes in halves of lines: 6.5 TB/s of loads alone instead of 6.9.)
+  const uint32_t k_lane = D == 64 ? row * D + g * 16 : (row & 7) * D + (g * 2 + (row >> 3)) * 16;
+  const uint32_t v_lane = g * 4 * D + row * kDims, s_lane = g * 16;
+  const ScalarInts indptr = scalar_ints(a.indptr), indices = scalar_ints(a.indices);
+  const ScalarInts lengths = scalar_ints(a.last_page_len);
+  Search search;
+  search.start(a.indptr, a.batch);
+  const int base = indptr[0], total = indptr[a.batch] - base;
   const int pages = segment_pages(a, total);
   const int group = a.group;
-  float* const out_lse = a.lse;
+  const int64_t begin64 = int64_t(segment) * pages;
+  const int end = a.num_indices == 0 ? 0 : int(min(begin64 + pages, int64_t(total)));
+  const int begin = int(min(begin64, int64_t(max(end, 0))));
 
-  // Requests without tokens: zeros, and -inf.
-  for (int b = segment; b < a.batch; b += a.segments) {
-    if (a.indptr[b + 1] > a.indptr[b]) continue;
-    for (int i = threadIdx.x; i < group * D; i += kWaves * 64)
-      a.out[b * a.out_stride + int64_t(head) * group * D + i] = 0;
-    if (out_lse && threadIdx.x < group)
-      out_lse[int64_t(b) * a.hq + head * group + threadIdx.x] = -INFINITY;
-  }
-  int64_t at64 = int64_t(segment) * pages;
-  if (at64 >= total) return;
-  int at = int(at64);
-  const int end = int(min(at64 + pages, int64_t(total)));
-  int b = find_request(a.indptr, a.batch, base, at);
+  // The query rows of the head's group, as the B operand.  (Rows past the group are copies
+  // of its last: nothing reads what comes of them.)
+  uint4 q[kKLoads][2];
+  // Two pages per tile, in two sets of registers: a tile's successor is on its way while it is
+  // worked on.
+  float m, l;
+  f32x4_t o[kDims];
+  u32x4_t k[2][2][kKLoads];
+  V v[2][2][4];
+  f32x4_t ks[2][2], vs[2][2];
+  int count[2][2];           // tokens that a page holds
+  int raw[2];                // the next tile's ids, as indices has them
+  auto fetch = [&](int page) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      raw[i] = indices[max(min(int64_t(base) + page + i, a.num_indices - 1), int64_t(0))];
+  };
+  // Pages `page` and `page` + 1 of a piece that ends at `stop`, its request at `last`.
+  auto load = [&](auto to_buffer, int page, int stop, int last, int tail) {
+    constexpr int B = decltype(to_buffer)::value;
+    int64_t id[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t slot = int64_t(base) + page + i;
+      const bool held = page + i < stop && slot >= 0 && slot < a.num_indices && raw[i] >= 0 &&
+                        raw[i] < a.num_blocks;
+      id[i] = held ? raw[i] : 0;
+      count[B][i] = !held ? 0 : page + i == last - 1 ? tail : kQuantPage;
+    }
+    // (a uniform base and the lane's fixed 32-bit offset: no address arithmetic in VGPRs)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* from = a.k_cache + id[i] * a.block_stride + int64_t(head) * (kQuantPage * D);
+#pragma unroll
+      for (int j = 0; j < kKLoads; ++j)
+        k[B][i][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
+            from + (k_lane + uint32_t(j / 2 * 128 + j % 2 * 8 * D))));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(
+          a.scales + id[i] * a.scales_stride + head * (2 * kQuantPage));
+      ks[B][i] = *reinterpret_cast<const f32x4_t*>(from + s_lane);
+      vs[B][i] = *reinterpret_cast<const f32x4_t*>(from + (s_lane + uint32_t(kQuantPage * 4)));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* from = a.v_cache + id[i] * a.block_stride + int64_t(head) * (kQuantPage * D);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[B][i][j] = __builtin_nontemporal_load(
+            reinterpret_cast<const V*>(from + (v_lane + uint32_t(j * D))));
+    }
+  };
+  auto tile = [&](auto at_buffer) {
+    constexpr int B = decltype(at_buffer)::value;
+    if constexpr (D > 64) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kKLoads; j += 2)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t x0 = k[B][i][j][w], x1 = k[B][i][j + 1][w];
+            k[B][i][j][w] = __builtin_amdgcn_update_dpp(x0, x1, kDppRowRor8, 0xF, 0xC, false);
+            k[B][i][j + 1][w] = __builtin_amdgcn_update_dpp(x1, x0, kDppRowRor8, 0xF, 0x3, false);
+          }
+    }
+    f32x4_t x[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < kKLoads; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w0 = k[B][i][j][2 * h], w1 = k[B][i][j][2 * h + 1];
+          x[i] = mfma<kHalf>(make_uint4(decode2<kCode, kHalf, 0>(w0), decode2<kCode, kHalf, 1>(w0),
+                                        decode2<kCode, kHalf, 0>(w1), decode2<kCode, kHalf, 1>(w1)),
+                             q[j][h], x[i]);
+        }
+    float most = kLowest;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // The scaled score is rounded before the maximum is taken from it: their difference is
+      // never above the running maximum's by a rounding.
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[i][j] = x[i][j] * ks[B][i][j] * a.scale_log2;
+        if (count[B][i] < kQuantPage && g * 4 + j >= count[B][i]) x[i][j] = -INFINITY;
+        most = fmaxf(most, x[i][j]);
+      }
+    }
+    if (__any(most > m + kRaise)) {
+      const float top = fmaxf(m, across(most, [](float s, float t) { return fmaxf(s, t); }));
+      const float f = fast_exp2(m - top);
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < kDims; ++e) o[e] *= f;
+      m = top;
+    }
+    // Weights: exact to fp32 in l; for the products they carry the V rows' scales and are
+    // bf16 (half a step 2^-8 of each weight, as an output's own rounding), for fp16 outputs
+    // a pair of bf16 (2^-16): fp16 itself has no room for any scale.
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = fast_exp2(x[i][j] - m);
+        l += e;
+        w[i * 4 + j] = e * vs[B][i][j];
+      }
+    if (count[B][0] < kQuantPage || count[B][1] < kQuantPage) {
+      // What masked slots hold (codes that are NaN, scales that are anything) does not enter.
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (g * 4 + j >= count[B][i]) {
+            w[i * 4 + j] = 0.f;
+            v[B][i][j] = V{};
+          }
+    }
+    uint4 hi, lo;
+    hi.x = pack2<false>(w[0], w[1]);
+    hi.y = pack2<false>(w[2], w[3]);
+    hi.z = pack2<false>(w[4], w[5]);
+    hi.w = pack2<false>(w[6], w[7]);
+    if constexpr (kHalf) {
+      lo.x = pack2<false>(w[0] - bf16lo(hi.x), w[1] - bf16hi(hi.x));
+      lo.y = pack2<false>(w[2] - bf16lo(hi.y), w[3] - bf16hi(hi.y));
+      lo.z = pack2<false>(w[4] - bf16lo(hi.z), w[5] - bf16hi(hi.z));
+      lo.w = pack2<false>(w[6] - bf16lo(hi.w), w[7] - bf16hi(hi.w));
+    }
+#pragma unroll
+    for (int e4 = 0; e4 < kDims / 4; ++e4) {
+      // bytes e of four tokens -> one word per dim
+      uint32_t t[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t r0 = word<D>(v[B][i][0], e4), r1 = word<D>(v[B][i][1], e4);
+        const uint32_t r2 = word<D>(v[B][i][2], e4), r3 = word<D>(v[B][i][3], e4);
+        const uint32_t a01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);   // r0.0 r1.0 r0.1 r1.1
+        const uint32_t a23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
+        const uint32_t b01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);   // r0.2 r1.2 r0.3 r1.3
+        const uint32_t b23 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+        t[i][0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        t[i][1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        t[i][2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+        t[i][3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint4 vt = make_uint4(
+            decode2<kCode, false, 0>(t[0][e]), decode2<kCode, false, 1>(t[0][e]),
+            decode2<kCode, false, 0>(t[1][e]), decode2<kCode, false, 1>(t[1][e]));
+        o[e4 * 4 + e] = mfma<false>(vt, hi, o[e4 * 4 + e]);
+        if constexpr (kHalf) o[e4 * 4 + e] = mfma<false>(vt, lo, o[e4 * 4 + e]);
+      }
+    }
+  };
 
-  while (at < end) {
-    int first = a.indptr[b] - base, last = a.indptr[b + 1] - base;
+  int first, last;
+  int b = begin < end ? search.find(a.indptr, a.batch, base, begin, first, last) : 0;
+  for (int at = begin; at < end;) {
     while (b < a.batch - 1 && last <= at) {
       first = last;
-      last = a.indptr[++b + 1] - base;
+      last = indptr[++b + 1] - base;
     }
     if (last <= at) break;   // (an indptr that goes down)
     const int stop = min(last, end);
-    const int tail = min(max(a.last_page_len[b], 0), kQuantPage);
+    const int tail = min(max(lengths[b], 0), kQuantPage);
+    m = kLowest;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < kDims; ++e) o[e] = f32x4_t{};
 
-    // The query rows of the head's group, as the B operand.
-    uint4 q[kKLoads][2];
-    const uint16_t* qp = a.q + b * a.q_stride + (int64_t(head) * group + min(row, group - 1)) * D;
+    int p = at + 2 * wave;
+    if (p < stop) {
+      const auto first_buffer = std::integral_constant<int, 0>{};
+      const auto other_buffer = std::integral_constant<int, 1>{};
+      fetch(p);
+      const uint16_t* from =
+          a.q + b * a.q_stride + (int64_t(head) * group + min(row, group - 1)) * D;
 #pragma unroll
-    for (int j = 0; j < kKLoads; ++j)
+      for (int j = 0; j < kKLoads; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        q[j][h] = *reinterpret_cast<const uint4*>(qp + j * 64 + g * 16 + h * 8);
-        if (row >= group) q[j][h] = make_uint4(0, 0, 0, 0);
-      }
-
-    float m = kLowest, l = 0.f;
-    f32x4_t o[kDims] = {};
-    for (int p = at + 2 * wave; p < stop; p += 2 * kWaves) {
-      u32x4_t k[2][kKLoads];
-      V v[2][4];
-      f32x4_t ks[2], vs[2];
-      int count[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t slot = int64_t(base) + p + i;
-        int id = p + i < stop && slot >= 0 && slot < a.num_indices ? a.indices[slot] : -1;
-        const bool held = id >= 0 && id < a.num_blocks;
-        count[i] = uniform(!held ? 0 : p + i == last - 1 ? tail : kQuantPage);
-        id = uniform(held ? id : 0);
-        // (a uniform base and the lane's fixed 32-bit offset: no address arithmetic in VGPRs)
-        const int64_t tile = int64_t(id) * a.block_stride + int64_t(head) * (kQuantPage * D);
-        const uint8_t* kp = a.k_cache + tile;
-#pragma unroll
-        for (int j = 0; j < kKLoads; ++j)
-          k[i][j] = __builtin_nontemporal_load(
-              reinterpret_cast<const u32x4_t*>(kp + (k_lane + uint32_t(j * 64))));
-        const uint8_t* vp = a.v_cache + tile;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[i][j] = __builtin_nontemporal_load(
-              reinterpret_cast<const V*>(vp + (v_lane + uint32_t(j * D))));
-        const uint8_t* sp = reinterpret_cast<const uint8_t*>(
-            a.scales + int64_t(id) * a.scales_stride + head * (2 * kQuantPage));
-        ks[i] = *reinterpret_cast<const f32x4_t*>(sp + s_lane);
-        vs[i] = *reinterpret_cast<const f32x4_t*>(sp + (s_lane + uint32_t(kQuantPage * 4)));
-      }
-
-      f32x4_t x[2] = {};
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < kKLoads; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t w0 = k[i][j][2 * h], w1 = k[i][j][2 * h + 1];
-            x[i] = mfma<kHalf>(make_uint4(decode2<kCode, kHalf, 0>(w0), decode2<kCode, kHalf, 1>(w0),
-                                          decode2<kCode, kHalf, 0>(w1), decode2<kCode, kHalf, 1>(w1)),
-                               q[j][h], x[i]);
-          }
-      float most = kLowest;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // One rounding per factor: the difference from the maximum is then exact where it counts.
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[i][j] = x[i][j] * ks[i][j] * a.scale_log2;
-          if (count[i] < kQuantPage && g * 4 + j >= count[i]) x[i][j] = -INFINITY;
-          most = fmaxf(most, x[i][j]);
+        for (int h = 0; h < 2; ++h)
+          q[j][h] = *reinterpret_cast<const uint4*>(
+              from + (D == 64 ? g * 16 : j / 2 * 128 + g * 32 + j % 2 * 16) + h * 8);
+      load(first_buffer, p, stop, last, tail);
+      fetch(p + kRound);
+      // (The last tile is a copy of the loop's body: a branch around the loads would
+      // make the compiler wait for all of them.)
+      for (;;) {
+        p += kRound;
+        if (p >= stop) {
+          tile(first_buffer);
+          break;
         }
-      }
-      if (__any(most > m + kRaise)) {
-        const float top = fmaxf(m, across(most, [](float s, float t) { return fmaxf(s, t); }));
-        const float f = fast_exp2(m - top);
-        l *= f;
-#pragma unroll
-        for (int e = 0; e < kDims; ++e) o[e] *= f;
-        m = top;
-      }
-      // Weights: exact to fp32 in l; for the products they carry the V rows' scales and are
-      // bf16 (2^-9 of each weight, below an output's own bf16 step), for fp16 outputs a
-      // pair of bf16 (2^-17): fp16 itself has no room for any scale.
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e = fast_exp2(x[i][j] - m);
-          l += e;
-          w[i * 4 + j] = e * vs[i][j];
+        load(other_buffer, p, stop, last, tail);
+        fetch(p + kRound);
+        tile(first_buffer);
+        p += kRound;
+        if (p >= stop) {
+          tile(other_buffer);
+          break;
         }
-      if (count[0] < kQuantPage || count[1] < kQuantPage) {
-        // What masked slots hold (codes that are NaN, scales that are anything) does not enter.
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (g * 4 + j >= count[i]) {
-              w[i * 4 + j] = 0.f;
-              v[i][j] = V{};
-            }
-      }
-      uint4 hi, lo;
-      hi.x = pack2<false>(w[0], w[1]);
-      hi.y = pack2<false>(w[2], w[3]);
-      hi.z = pack2<false>(w[4], w[5]);
-      hi.w = pack2<false>(w[6], w[7]);
-      if constexpr (kHalf) {
-        lo.x = pack2<false>(w[0] - bf16lo(hi.x), w[1] - bf16hi(hi.x));
-        lo.y = pack2<false>(w[2] - bf16lo(hi.y), w[3] - bf16hi(hi.y));
-        lo.z = pack2<false>(w[4] - bf16lo(hi.z), w[5] - bf16hi(hi.z));
-        lo.w = pack2<false>(w[6] - bf16lo(hi.w), w[7] - bf16hi(hi.w));
-      }
-#pragma unroll
-      for (int e4 = 0; e4 < kDims / 4; ++e4) {
-        // bytes e of four tokens -> one word per dim
-        uint32_t t[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t r0 = word<D>(v[i][0], e4), r1 = word<D>(v[i][1], e4);
-          const uint32_t r2 = word<D>(v[i][2], e4), r3 = word<D>(v[i][3], e4);
-          const uint32_t a01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);   // r0.0 r1.0 r0.1 r1.1
-          const uint32_t a23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
-          const uint32_t b01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);   // r0.2 r1.2 r0.3 r1.3
-          const uint32_t b23 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-          t[i][0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
-          t[i][1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
-          t[i][2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
-          t[i][3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint4 vt = make_uint4(
-              decode2<kCode, false, 0>(t[0][e]), decode2<kCode, false, 1>(t[0][e]),
-              decode2<kCode, false, 0>(t[1][e]), decode2<kCode, false, 1>(t[1][e]));
-          o[e4 * 4 + e] = mfma<false>(vt, hi, o[e4 * 4 + e]);
-          if constexpr (kHalf) o[e4 * 4 + e] = mfma<false>(vt, lo, o[e4 * 4 + e]);
-        }
+        load(first_buffer, p, stop, last, tail);
+        fetch(p + kRound);
+        tile(other_buffer);
       }
     }
 
@@ -320,10 +434,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void quant_decode_ke
           *reinterpret_cast<f32x4_t*>(to + 4 + (g * 4 + i) * kDims + e) =
               f32x4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
     }
-    __syncthreads();
-    const bool whole = first >= at && last <= end;
-    float* part = a.parts + ((int64_t(head) * a.segments + segment) * 2 + (first > at64 ? 1 : 0)) *
-                                (int64_t(group) * (D + 2));
+    lds_barrier();
+    const bool whole = first >= begin && last <= end;
+    float* part = a.parts + ((int64_t(head) * a.segments + segment) * 2 + (first > begin ? 1 : 0)) *
+                                (int64_t(group) * (D + 4));
     for (int i = threadIdx.x; i < group * (D / 4); i += kWaves * 64) {
       const int r = i / (D / 4), c = i % (D / 4);
       float top = kLowest, sum = 0.f;
@@ -338,65 +452,113 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void quant_decode_ke
         acc += *reinterpret_cast<const f32x4_t*>(from + 4 + c * 4) * f;
       }
       if (whole) {
-        const float f = sum == 0.f ? 0.f : 1.f / sum;
-        uint2 packed;
-        packed.x = pack2<kHalf>(acc[0] * f, acc[1] * f);
-        packed.y = pack2<kHalf>(acc[2] * f, acc[3] * f);
-        *reinterpret_cast<uint2*>(a.out + b * a.out_stride + (int64_t(head) * group + r) * D + c * 4) =
-            packed;
-        if (out_lse && c == 0)
-          out_lse[int64_t(b) * a.hq + head * group + r] =
-              sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+        write_out<D, kHalf>(a, b, head * group + r, c, top, sum, acc);
       } else {
-        float* to = part + r * (D + 2);
-        if (c == 0) {
-          to[0] = top;
-          to[1] = sum;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[2 + c * 4 + e] = acc[e];
+        float* to = part + r * (D + 4);
+        if (c == 0) *reinterpret_cast<float2*>(to) = make_float2(top, sum);
+        *reinterpret_cast<f32x4_t*>(to + 4 + c * 4) = acc;
       }
     }
-    __syncthreads();
+    lds_barrier();
     at = stop;
+  }
+
+  // Requests without pages: zeros, and -inf.
+  for (int i = segment; i < a.batch; i += a.segments) {
+    if (indptr[i + 1] > indptr[i] && a.num_indices > 0) continue;
+    for (int j = threadIdx.x; j < group * D; j += kWaves * 64)
+      a.out[i * a.out_stride + int64_t(head) * group * D + j] = 0;
+    if (a.lse && int(threadIdx.x) < group)
+      a.lse[int64_t(i) * a.hq + head * group + threadIdx.x] = -INFINITY;
   }
 }
 
-// Joins the pieces of one request and query head.
+// Joins a request's pieces.  Workgroups (i, KV head), each `rows` query rows: request i, or in
+// batches of more requests than there are borders between segments the request that border i + 1 cuts
+// first.  A thread takes four dims of a row and every share-th piece; the sums of the threads of
+// a column meet in LDS.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(D) void quant_merge_kernel(QuantDecodeArgs a) {
-  const int b = blockIdx.y, hq = blockIdx.x;
-  const int base = a.indptr[0], total = a.indptr[a.batch] - base;
-  const int first = a.indptr[b] - base, last = a.indptr[b + 1] - base;
+__global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int rows) {
+  constexpr int kDeep = 4;
+  __shared__ float lds[256 * 8];
+  const int head = blockIdx.x % a.hkv, i = blockIdx.x / a.hkv;
+  const ScalarInts indptr = scalar_ints(a.indptr);
+  const int base = indptr[0], total = indptr[a.batch] - base;
   const int pages = segment_pages(a, total);
-  if (first < 0 || last <= first || last > total) return;
-  const int s0 = first / pages, s1 = (last - 1) / pages;
-  if (s0 == s1) return;
-  const int head = hq / a.group, r = hq % a.group;
-  const int64_t step = int64_t(a.group) * (D + 2);
-  const float* p0 = a.parts + (int64_t(head) * a.segments + s0) * 2 * step + r * (D + 2) +
-                    (first > s0 * pages ? step : 0);
-  const float* ps = a.parts + (int64_t(head) * a.segments) * 2 * step + r * (D + 2);
-  float top = p0[0];
-  for (int s = s0 + 1; s <= s1; ++s) top = fmaxf(top, ps[s * 2 * step]);
-  float f = fast_exp2(p0[0] - top), sum = p0[1] * f, acc = p0[2 + threadIdx.x] * f;
-  for (int s = s0 + 1; s <= s1; ++s) {
-    const float* p = ps + s * 2 * step;
-    f = fast_exp2(p[0] - top);
-    sum += p[1] * f;
-    acc += p[2 + threadIdx.x] * f;
+  int b, first, last;
+  if (a.batch < a.segments) {
+    b = i;
+    first = indptr[b] - base;
+    last = indptr[b + 1] - base;
+  } else {
+    Search search;
+    search.start(a.indptr, a.batch);
+    const int64_t cut = int64_t(i + 1) * pages;
+    if (cut >= total) return;
+    b = search.find(a.indptr, a.batch, base, int(cut), first, last);
+    if (first >= cut || first < cut - pages) return;
   }
-  const float y = sum == 0.f ? 0.f : acc / sum;
-  a.out[b * a.out_stride + int64_t(hq) * D + threadIdx.x] = uint16_t(pack2<kHalf>(y, y));
-  if (a.lse && threadIdx.x == 0)
-    a.lse[int64_t(b) * a.hq + hq] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+  if (first < 0 || last <= first || last > total) return;
+  const int s0 = first / pages, n = (last - 1) / pages - s0 + 1;
+  if (n == 1) return;
+  const int64_t step = int64_t(a.group) * (D + 4);
+  const int64_t skip = first > int64_t(s0) * pages ? step : 0;   // of the first piece's slot
+  const int r0 = blockIdx.y * rows, columns = min(rows, a.group - r0) * (D / 4);
+  const int share = max(1, 256 / columns);
+  for (int i0 = 0; i0 < columns; i0 += 256) {
+    const int mine = threadIdx.x / columns, column = i0 + threadIdx.x - mine * columns;
+    const bool active = mine < share && column < columns;
+    const int r = r0 + column / (D / 4), c = column % (D / 4);
+    const float* parts = a.parts + (int64_t(head) * a.segments + s0) * 2 * step + r * (D + 4);
+    float top = kLowest, sum = 0.f;
+    f32x4_t acc = {};
+    for (int s = mine; active && s < n; s += share * kDeep) {
+      float2 ml[kDeep];
+      f32x4_t x[kDeep];
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        const int j = min(s + u * share, n - 1);
+        const float* from = parts + j * 2 * step + (j == 0 ? skip : 0);
+        ml[u] = *reinterpret_cast<const float2*>(from);
+        x[u] = *reinterpret_cast<const f32x4_t*>(from + 4 + c * 4);
+      }
+      float most = top;
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) most = fmaxf(most, ml[u].x);
+      float f = fast_exp2(top - most);
+      sum *= f;
+      acc *= f;
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u)
+        if (s + u * share < n) {
+          f = fast_exp2(ml[u].x - most);
+          sum += ml[u].y * f;
+          acc += x[u] * f;
+        }
+      top = most;
+    }
+    if (share > 1) {   // (then the columns are done at once)
+      float* to = lds + threadIdx.x * 8;
+      to[0] = top;
+      to[1] = sum;
+      *reinterpret_cast<f32x4_t*>(to + 4) = acc;
+      __syncthreads();
+      if (mine != 0) return;
+      for (int w = 1; w < min(share, n); ++w) {
+        const float* from = lds + (w * columns + column) * 8;
+        const float most = fmaxf(top, from[0]);
+        const float f = fast_exp2(top - most), h = fast_exp2(from[0] - most);
+        sum = sum * f + from[1] * h;
+        acc = acc * f + *reinterpret_cast<const f32x4_t*>(from + 4) * h;
+        top = most;
+      }
+    }
+    if (active) write_out<D, kHalf>(a, b, head * a.group + r, c, top, sum, acc);
+  }
 }
 
 // Segments per KV head: the workgroups that the GPU holds at once, over the heads.
-int segments_of(int hkv, int head_dim) {
-  const int held = 256 * (head_dim == 256 ? 2 : 4);
-  return std::max(1, held / hkv);
-}
+int segments_of(int hkv, int head_dim) { return std::max(1, 256 * per_simd(head_dim) / hkv); }
 
 }  // namespace
 }  // namespace kvc
@@ -406,7 +568,7 @@ using namespace kvc;
 extern "C" int64_t kvc_quantized_decode_workspace_bytes(int32_t batch, int32_t num_qo_heads,
                                                         int32_t num_kv_heads, int32_t head_dim) {
   if (batch < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
-  return int64_t(segments_of(num_kv_heads, head_dim)) * 2 * num_qo_heads * (head_dim + 2) * 4;
+  return int64_t(segments_of(num_kv_heads, head_dim)) * 2 * num_qo_heads * (head_dim + 4) * 4;
 }
 
 extern "C" int kvc_quantized_decode(
@@ -478,6 +640,8 @@ extern "C" int kvc_quantized_decode(
   hipStream_t s = static_cast<hipStream_t>(stream);
   const unsigned grid = unsigned(a.segments) * unsigned(num_kv_heads);
   const unsigned lds = unsigned(kWaves * group * (head_dim + 4) * 4);
+  // So few pages are never cut.
+  const bool cut = num_indices > kMinPages && a.segments > 1;
 
   auto launch = [&](auto d, auto c, auto half) {
     constexpr int D = decltype(d)::value, C = decltype(c)::value;
@@ -487,7 +651,12 @@ extern "C" int kvc_quantized_decode(
       (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
     kernel<<<grid, kWaves * 64, lds, s>>>(a);
-    quant_merge_kernel<D, H><<<dim3(unsigned(num_qo_heads), unsigned(batch)), D, 0, s>>>(a);
+    if (cut) {
+      const int joins = std::min(batch, a.segments - 1) * num_kv_heads;
+      // Few joins: a query row per workgroup.
+      const int rows = joins * group <= 512 ? 1 : group;
+      quant_merge_kernel<D, H><<<dim3(unsigned(joins), unsigned(group / rows)), 256, 0, s>>>(a, rows);
+    }
   };
   auto by_type = [&](auto d, auto c) {
     if (dtype == KVC_DTYPE_FP16)
