@@ -35,10 +35,14 @@ namespace kvc {
 namespace {
 
 constexpr int kWaves = 4;             // waves of a workgroup
+constexpr int kScan = 4096;            // requests that are looked through for longer ones
 constexpr int kMinPages = 16;         // of a segment
 
-// Waves per SIMD, which bounds their registers.
-constexpr int per_simd(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
+// Waves per SIMD, which bounds their registers, ...
+constexpr int per_simd(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2; }
+// ... and workgroups per CU that a batch is cut for: two already keep 17 to 33 KB of loads each in
+// flight, and more only compete (16 x 32767 tokens at head_dim 128: 166 us with 2, 169 with 3).
+constexpr int cut_for(int head_dim) { return head_dim == 64 ? 4 : 2; }
 
 constexpr float kRaise = 8.f;         // log2: how far a score may exceed the running maximum
 constexpr float kLowest = -3.4028234663852886e38f;
@@ -64,6 +68,7 @@ struct QuantDecodeArgs {
   const int32_t* last_page_len;
   int32_t batch, hq, hkv, group;
   int32_t segments;          // per KV head
+  int32_t groups;            // workgroups per KV head, at least as many
   float scale_log2;
   float* parts;              // [hkv][segments][2][group][D + 4]: m, l, -, -, O
   uint16_t* out;
@@ -160,6 +165,28 @@ __device__ __forceinline__ uint32_t word(typename VWord<D>::type v, int i) {
     return v[i];
 }
 
+// Whether no request has more pages than one workgroup streams in about the time that cutting
+// and joining it costs: then each is a workgroup's (per KV head) and none is cut.  64 pages where the
+// requests alone fill the GPU (64 requests of 600 to 1000 tokens, 8 KV heads: 26.2 -> 23.2 us),
+// else 48 (8 of 300: 10.2 -> 8.0; but one of 1000: 8.7 cut, 10.1 whole).  Every wave looks through indptr by
+// itself, beside loads that it waits for anyway; batches too large for that are cut.
+__host__ __device__ inline int whole_pages(int batch, int hkv) {
+  return int64_t(batch) * hkv >= 256 ? 64 : 48;
+}
+__device__ __forceinline__ bool all_short(const int32_t* indptr, int batch, int hkv) {
+  if (batch > kScan) return false;
+  const int most = whole_pages(batch, hkv);
+  bool large = false;
+  for (int i = threadIdx.x & 63; i < batch; i += 256) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = min(i + u * 64, batch - 1);
+      large |= indptr[j + 1] - indptr[j] > most;
+    }
+  }
+  return !__any(large);
+}
+
 // Barrier between the waves' uses of LDS.  (__syncthreads would also wait for the global loads.)
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -201,21 +228,25 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   const int base = indptr[0], total = indptr[a.batch] - base;
   const int pages = segment_pages(a, total);
   const int group = a.group;
+  const bool whole_requests = all_short(a.indptr, a.batch, a.hkv);
+  if (!whole_requests && segment >= a.segments) return;
   const int64_t begin64 = int64_t(segment) * pages;
-  const int end = a.num_indices == 0 ? 0 : int(min(begin64 + pages, int64_t(total)));
-  const int begin = int(min(begin64, int64_t(max(end, 0))));
+  int end = a.num_indices == 0 ? 0 : int(min(begin64 + pages, int64_t(total)));
+  int begin = int(min(begin64, int64_t(max(end, 0))));
 
   // The query rows of the head's group, as the B operand.  (Rows past the group are copies
   // of its last: nothing reads what comes of them.)
   uint4 q[kKLoads][2];
-  // Two pages per tile, in two sets of registers: a tile's successor is on its way while it is
-  // worked on.
+  // Two pages per tile.  A tile's successor is loaded part by part as the registers fall free: K
+  // after the scores, V after the products.  (Two sets of registers, all of the successor
+  // ahead of the work, were no faster over long requests and leave room for fewer waves.)
   float m, l;
   f32x4_t o[kDims];
-  u32x4_t k[2][2][kKLoads];
-  V v[2][2][4];
-  f32x4_t ks[2][2], vs[2][2];
-  int count[2][2];           // tokens that a page holds
+  u32x4_t k[2][kKLoads];
+  V v[2][4];
+  f32x4_t ks[2], vs[2];
+  int count[2];              // tokens that a page holds
+  int64_t id[2];
   int raw[2];                // the next tile's ids, as indices has them
   auto fetch = [&](int page) {
 #pragma unroll
@@ -223,44 +254,47 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       raw[i] = indices[max(min(int64_t(base) + page + i, a.num_indices - 1), int64_t(0))];
   };
   // Pages `page` and `page` + 1 of a piece that ends at `stop`, its request at `last`.
-  auto load = [&](auto to_buffer, int page, int stop, int last, int tail) {
-    constexpr int B = decltype(to_buffer)::value;
-    int64_t id[2];
+  auto place = [&](int (&n)[2], int page, int stop, int last, int tail) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t slot = int64_t(base) + page + i;
       const bool held = page + i < stop && slot >= 0 && slot < a.num_indices && raw[i] >= 0 &&
                         raw[i] < a.num_blocks;
       id[i] = held ? raw[i] : 0;
-      count[B][i] = !held ? 0 : page + i == last - 1 ? tail : kQuantPage;
+      n[i] = !held ? 0 : page + i == last - 1 ? tail : kQuantPage;
     }
-    // (a uniform base and the lane's fixed 32-bit offset: no address arithmetic in VGPRs)
+  };
+  // (a uniform base and the lane's fixed 32-bit offset: no address arithmetic in VGPRs)
+  auto load_k = [&] {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* from = a.k_cache + id[i] * a.block_stride + int64_t(head) * (kQuantPage * D);
 #pragma unroll
       for (int j = 0; j < kKLoads; ++j)
-        k[B][i][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
+        k[i][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
             from + (k_lane + uint32_t(j / 2 * 128 + j % 2 * 8 * D))));
     }
+  };
+  auto load_s = [&](f32x4_t (&to)[2], int kv) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* from = reinterpret_cast<const uint8_t*>(
-          a.scales + id[i] * a.scales_stride + head * (2 * kQuantPage));
-      ks[B][i] = *reinterpret_cast<const f32x4_t*>(from + s_lane);
-      vs[B][i] = *reinterpret_cast<const f32x4_t*>(from + (s_lane + uint32_t(kQuantPage * 4)));
+          a.scales + id[i] * a.scales_stride + (head * 2 + kv) * kQuantPage);
+      to[i] = *reinterpret_cast<const f32x4_t*>(from + s_lane);
     }
+  };
+  auto load_v = [&] {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* from = a.v_cache + id[i] * a.block_stride + int64_t(head) * (kQuantPage * D);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        v[B][i][j] = __builtin_nontemporal_load(
+        v[i][j] = __builtin_nontemporal_load(
             reinterpret_cast<const V*>(from + (v_lane + uint32_t(j * D))));
     }
   };
-  auto tile = [&](auto at_buffer) {
-    constexpr int B = decltype(at_buffer)::value;
+  auto tile = [&](auto more) {
+    constexpr bool kMore = decltype(more)::value;
     if constexpr (D > 64) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -268,9 +302,9 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
         for (int j = 0; j < kKLoads; j += 2)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t x0 = k[B][i][j][w], x1 = k[B][i][j + 1][w];
-            k[B][i][j][w] = __builtin_amdgcn_update_dpp(x0, x1, kDppRowRor8, 0xF, 0xC, false);
-            k[B][i][j + 1][w] = __builtin_amdgcn_update_dpp(x1, x0, kDppRowRor8, 0xF, 0x3, false);
+            const uint32_t x0 = k[i][j][w], x1 = k[i][j + 1][w];
+            k[i][j][w] = __builtin_amdgcn_update_dpp(x0, x1, kDppRowRor8, 0xF, 0xC, false);
+            k[i][j + 1][w] = __builtin_amdgcn_update_dpp(x1, x0, kDppRowRor8, 0xF, 0x3, false);
           }
     }
     f32x4_t x[2] = {};
@@ -280,23 +314,37 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       for (int j = 0; j < kKLoads; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = k[B][i][j][2 * h], w1 = k[B][i][j][2 * h + 1];
+          const uint32_t w0 = k[i][j][2 * h], w1 = k[i][j][2 * h + 1];
           x[i] = mfma<kHalf>(make_uint4(decode2<kCode, kHalf, 0>(w0), decode2<kCode, kHalf, 1>(w0),
                                         decode2<kCode, kHalf, 0>(w1), decode2<kCode, kHalf, 1>(w1)),
                              q[j][h], x[i]);
         }
+    if constexpr (kMore) load_k();
+    // The scaled score is rounded before the maximum is taken from it: their difference is
+    // never above the running maximum's by a rounding.
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] = x[i][j] * ks[i][j] * a.scale_log2;
+    if constexpr (kMore) load_s(ks, 0);
+    const bool partial = count[0] < kQuantPage || count[1] < kQuantPage;
+    if (partial) {
+      // What masked slots hold (codes that are NaN, scales that are anything) does not enter.
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (g * 4 + j >= count[i]) {
+            x[i][j] = -INFINITY;
+            vs[i][j] = 0.f;
+            v[i][j] = V{};
+          }
+    }
     float most = kLowest;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      // The scaled score is rounded before the maximum is taken from it: their difference is
-      // never above the running maximum's by a rounding.
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[i][j] = x[i][j] * ks[B][i][j] * a.scale_log2;
-        if (count[B][i] < kQuantPage && g * 4 + j >= count[B][i]) x[i][j] = -INFINITY;
-        most = fmaxf(most, x[i][j]);
-      }
-    }
+      for (int j = 0; j < 4; ++j) most = fmaxf(most, x[i][j]);
     if (__any(most > m + kRaise)) {
       const float top = fmaxf(m, across(most, [](float s, float t) { return fmaxf(s, t); }));
       const float f = fast_exp2(m - top);
@@ -315,19 +363,9 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       for (int j = 0; j < 4; ++j) {
         const float e = fast_exp2(x[i][j] - m);
         l += e;
-        w[i * 4 + j] = e * vs[B][i][j];
+        w[i * 4 + j] = e * vs[i][j];
       }
-    if (count[B][0] < kQuantPage || count[B][1] < kQuantPage) {
-      // What masked slots hold (codes that are NaN, scales that are anything) does not enter.
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (g * 4 + j >= count[B][i]) {
-            w[i * 4 + j] = 0.f;
-            v[B][i][j] = V{};
-          }
-    }
+    if constexpr (kMore) load_s(vs, 1);
     uint4 hi, lo;
     hi.x = pack2<false>(w[0], w[1]);
     hi.y = pack2<false>(w[2], w[3]);
@@ -345,8 +383,8 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       uint32_t t[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t r0 = word<D>(v[B][i][0], e4), r1 = word<D>(v[B][i][1], e4);
-        const uint32_t r2 = word<D>(v[B][i][2], e4), r3 = word<D>(v[B][i][3], e4);
+        const uint32_t r0 = word<D>(v[i][0], e4), r1 = word<D>(v[i][1], e4);
+        const uint32_t r2 = word<D>(v[i][2], e4), r3 = word<D>(v[i][3], e4);
         const uint32_t a01 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);   // r0.0 r1.0 r0.1 r1.1
         const uint32_t a23 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
         const uint32_t b01 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);   // r0.2 r1.2 r0.3 r1.3
@@ -365,16 +403,31 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
         if constexpr (kHalf) o[e4 * 4 + e] = mfma<false>(vt, lo, o[e4 * 4 + e]);
       }
     }
+    if constexpr (kMore) load_v();
   };
 
-  int first, last;
-  int b = begin < end ? search.find(a.indptr, a.batch, base, begin, first, last) : 0;
-  for (int at = begin; at < end;) {
-    while (b < a.batch - 1 && last <= at) {
-      first = last;
-      last = indptr[++b + 1] - base;
+  int first = 0, last = 0, b = segment;
+  if (!whole_requests && begin < end)
+    b = search.find(a.indptr, a.batch, base, begin, first, last);
+  for (int at = begin;;) {
+    if (whole_requests) {
+      if (b >= a.batch || a.num_indices == 0) break;
+      first = indptr[b] - base;
+      last = indptr[b + 1] - base;
+      if (last <= first) {
+        b += a.groups;
+        continue;
+      }
+      at = begin = first;
+      end = last;
+    } else {
+      if (at >= end) break;
+      while (b < a.batch - 1 && last <= at) {
+        first = last;
+        last = indptr[++b + 1] - base;
+      }
+      if (last <= at) break;   // (an indptr that goes down)
     }
-    if (last <= at) break;   // (an indptr that goes down)
     const int stop = min(last, end);
     const int tail = min(max(lengths[b], 0), kQuantPage);
     m = kLowest;
@@ -384,8 +437,6 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
 
     int p = at + 2 * wave;
     if (p < stop) {
-      const auto first_buffer = std::integral_constant<int, 0>{};
-      const auto other_buffer = std::integral_constant<int, 1>{};
       fetch(p);
       const uint16_t* from =
           a.q + b * a.q_stride + (int64_t(head) * group + min(row, group - 1)) * D;
@@ -395,28 +446,23 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
         for (int h = 0; h < 2; ++h)
           q[j][h] = *reinterpret_cast<const uint4*>(
               from + (D == 64 ? g * 16 : j / 2 * 128 + g * 32 + j % 2 * 16) + h * 8);
-      load(first_buffer, p, stop, last, tail);
+      place(count, p, stop, last, tail);
       fetch(p + kRound);
-      // (The last tile is a copy of the loop's body: a branch around the loads would
-      // make the compiler wait for all of them.)
-      for (;;) {
-        p += kRound;
-        if (p >= stop) {
-          tile(first_buffer);
-          break;
-        }
-        load(other_buffer, p, stop, last, tail);
-        fetch(p + kRound);
-        tile(first_buffer);
-        p += kRound;
-        if (p >= stop) {
-          tile(other_buffer);
-          break;
-        }
-        load(first_buffer, p, stop, last, tail);
-        fetch(p + kRound);
-        tile(other_buffer);
+      load_k();
+      load_s(ks, 0);
+      load_s(vs, 1);
+      load_v();
+      // (The last tile is a copy of the loop's body: a branch around the loads would make the
+      // compiler wait for all of them.)
+      for (; p + kRound < stop; p += kRound) {
+        int n[2];
+        place(n, p + kRound, stop, last, tail);
+        fetch(p + 2 * kRound);
+        tile(std::true_type{});
+        count[0] = n[0];
+        count[1] = n[1];
       }
+      tile(std::false_type{});
     }
 
     // The waves' parts of the piece, joined in LDS.
@@ -461,10 +507,11 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     }
     lds_barrier();
     at = stop;
+    if (whole_requests) b += a.groups;
   }
 
   // Requests without pages: zeros, and -inf.
-  for (int i = segment; i < a.batch; i += a.segments) {
+  for (int i = segment; i < a.batch; i += whole_requests ? a.groups : a.segments) {
     if (indptr[i + 1] > indptr[i] && a.num_indices > 0) continue;
     for (int j = threadIdx.x; j < group * D; j += kWaves * 64)
       a.out[i * a.out_stride + int64_t(head) * group * D + j] = 0;
@@ -498,7 +545,7 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
     b = search.find(a.indptr, a.batch, base, int(cut), first, last);
     if (first >= cut || first < cut - pages) return;
   }
-  if (first < 0 || last <= first || last > total) return;
+  if (first < 0 || last <= first || last > total || all_short(a.indptr, a.batch, a.hkv)) return;
   const int s0 = first / pages, n = (last - 1) / pages - s0 + 1;
   if (n == 1) return;
   const int64_t step = int64_t(a.group) * (D + 4);
@@ -557,8 +604,8 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
   }
 }
 
-// Segments per KV head: the workgroups that the GPU holds at once, over the heads.
-int segments_of(int hkv, int head_dim) { return std::max(1, 256 * per_simd(head_dim) / hkv); }
+// Segments per KV head.
+int segments_of(int hkv, int head_dim) { return std::max(1, 256 * cut_for(head_dim) / hkv); }
 
 }  // namespace
 }  // namespace kvc
@@ -638,10 +685,11 @@ extern "C" int kvc_quantized_decode(
   a.out_stride = out_batch_stride;
   a.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned grid = unsigned(a.segments) * unsigned(num_kv_heads);
+  a.groups = std::max(a.segments, std::min(batch, 256 * per_simd(head_dim) / num_kv_heads));
+  const unsigned grid = unsigned(a.groups) * unsigned(num_kv_heads);
   const unsigned lds = unsigned(kWaves * group * (head_dim + 4) * 4);
-  // So few pages are never cut.
-  const bool cut = num_indices > kMinPages && a.segments > 1;
+  // (So few pages are not cut.)
+  const bool cut = num_indices > whole_pages(batch, num_kv_heads) && a.segments > 1;
 
   auto launch = [&](auto d, auto c, auto half) {
     constexpr int D = decltype(d)::value, C = decltype(c)::value;
