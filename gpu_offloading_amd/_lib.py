@@ -375,3 +375,16 @@ def current_stream_handle(device) -> int:
 
 
 _raw_stream = None
+
+
+def current_stream_of(index: int) -> int:
+    """``current_stream_handle`` of GPU ``index``."""
+    global _raw_stream_of
+    if _raw_stream_of is None:
+        import torch
+        _raw_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream_of(index)
+
+
+_raw_stream_of = None

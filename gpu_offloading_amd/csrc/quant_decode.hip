@@ -40,9 +40,10 @@ constexpr int kMinPages = 16;         // of a segment
 
 // Waves per SIMD, which bounds their registers, ...
 constexpr int per_simd(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2; }
-// ... and workgroups per CU that a batch is cut for: two already keep 17 to 33 KB of loads each in
-// flight, and more only compete (16 x 32767 tokens at head_dim 128: 166 us with 2, 169 with 3).
-constexpr int cut_for(int head_dim) { return head_dim == 64 ? 4 : 2; }
+// ... and workgroups per CU that a batch is cut for: these keep 34 KB of loads in flight, and
+// more only compete (16 x 32767 tokens at head_dim 128: 166 us with 2, 169 with 3; 16 of 20000 to
+// 32000 at head_dim 64: 79 with 2, 81 with 4) and leave more to join.
+constexpr int cut_for(int head_dim) { return head_dim == 256 ? 1 : 2; }
 
 constexpr float kRaise = 8.f;         // log2: how far a score may exceed the running maximum
 constexpr float kLowest = -3.4028234663852886e38f;

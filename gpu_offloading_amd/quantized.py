@@ -21,8 +21,9 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .ops import (_WDTYPES as _DTYPES, _check_cuda, _check_ints, _fail, _oob_ptr, _ptr,
-                  _stream_handle)
+from .ops import _WDTYPES as _DTYPES
+from .ops import _check_cuda, _check_ints, _fail, _oob_ptr, _ptr
+from .prompt import _empty
 
 __all__ = ["QuantizedCache", "quantized_cache", "reshape_and_cache_quantized",
            "gather_quantized_kv", "quantized_decode_attention", "decode_workspace"]
@@ -64,27 +65,27 @@ def quantized_cache(num_blocks: int, num_kv_heads: int, head_dim: int,
 def _check_quantized(key_cache: torch.Tensor, value_cache: torch.Tensor, scales: torch.Tensor):
     """Shapes, types and strides of a cache's tensors; returns (blocks, heads, dim, code,
     block stride of the codes, block stride of the scales)."""
-    shape, st = key_cache.shape, key_cache.stride()
-    code = CODES.get(key_cache.dtype)
-    if code is None or value_cache.dtype is not key_cache.dtype:
+    shape, st, ss, dt = key_cache.shape, key_cache.stride(), scales.stride(), key_cache.dtype
+    code = CODES.get(dt)
+    if code is None or value_cache.dtype is not dt:
         _fail("key_cache and value_cache must both be float8_e4m3fn or int8, got "
-              f"{key_cache.dtype} and {value_cache.dtype}")
+              f"{dt} and {value_cache.dtype}")
     if len(shape) != 4 or shape[2] != PAGE:
         _fail(f"key_cache must be [num_blocks, num_kv_heads, 16, head_dim], got {tuple(shape)}")
     nb, h, _, d = shape
     if value_cache.shape != shape or value_cache.stride() != st:
         _fail("key_cache and value_cache must have the same shape and strides")
-    if st[3] != 1 or st[2] != d or (h > 1 and st[1] != PAGE * d):
-        _fail(f"key_cache: a block must be contiguous (strides {st})")
-    ss = scales.stride()
     if scales.dtype is not torch.float32 or scales.shape != (nb, h, 2, PAGE):
         _fail(f"scales must be float32 [{nb}, {h}, 2, 16], got {scales.dtype} "
               f"{tuple(scales.shape)}")
-    if ss[3] != 1 or ss[2] != PAGE or (h > 1 and ss[1] != 2 * PAGE):
+    if st[1:] != (PAGE * d, d, 1) and (st[3] != 1 or st[2] != d or h > 1):
+        _fail(f"key_cache: a block must be contiguous (strides {st})")
+    if ss[1:] != (2 * PAGE, PAGE, 1) and (ss[3] != 1 or ss[2] != PAGE or h > 1):
         _fail(f"scales: a block must be contiguous (strides {ss})")
+    if nb > 1:
+        return nb, h, d, code, st[0], ss[0]
     # (of a single block any stride is valid)
-    return (nb, h, d, code, st[0] if nb > 1 else max(st[0], h * PAGE * d),
-            ss[0] if nb > 1 else max(ss[0], h * 2 * PAGE))
+    return nb, h, d, code, max(st[0], h * PAGE * d), max(ss[0], h * 2 * PAGE)
 
 
 def _check_tokens(name: str, t: torch.Tensor, heads: int, dim: int) -> int:
@@ -95,9 +96,22 @@ def _check_tokens(name: str, t: torch.Tensor, heads: int, dim: int) -> int:
         _fail(f"{name} must be [tokens, {heads}, {dim}], got {tuple(sh)}")
     if t.dtype not in _DTYPES:
         _fail(f"{name} must be bfloat16 or float16, got {t.dtype}")
-    if st[2] != 1 or (heads > 1 and st[1] != dim):
+    if st[2] != 1 or (st[1] != dim and heads > 1):
         _fail(f"{name}: heads of a token must be contiguous (strides {st})")
     return st[0] if sh[0] > 1 else heads * dim
+
+
+def _stream(index: int, stream: Optional[torch.cuda.Stream]) -> int:
+    return stream.cuda_stream if stream is not None else _lib.current_stream_of(index)
+
+
+def _check_device(*ts: Optional[torch.Tensor]) -> int:
+    """The GPU that all of them are on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != index or index < 0):
+            _check_cuda(*ts)                    # (says which)
+    return index
 
 
 def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -112,7 +126,7 @@ def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cach
     slot_mapping whose length is the token count, a negative slot is padding.  The
     slots of a call must be distinct.  A row that holds an infinity or a NaN reads back
     as NaN."""
-    dev = _check_cuda(key, value, key_cache, value_cache, scales, slot_mapping, oob_count)
+    index = _check_device(key_cache, value_cache, scales, key, value, slot_mapping, oob_count)
     nb, h, d, code, cs, ss = _check_quantized(key_cache, value_cache, scales)
     if slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 \
             or not slot_mapping.is_contiguous():
@@ -124,11 +138,11 @@ def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cach
     if key.shape[0] < n or value.shape[0] < n:
         _fail(f"key and value have {key.shape[0]} and {value.shape[0]} rows but slot_mapping "
               f"has {n}")
-    _lib.call_on(key.get_device(), "kvc_reshape_and_cache_quantized", key.data_ptr(),
+    _lib.call_on(index, "kvc_reshape_and_cache_quantized", key.data_ptr(),
                  value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
                  scales.data_ptr(), slot_mapping.data_ptr(), n, h, d, PAGE, nb,
                  _DTYPES[key.dtype], code, ks, vs, cs, ss, _oob_ptr(oob_count),
-                 _stream_handle(dev, stream))
+                 _stream(index, stream))
 
 
 def gather_quantized_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scales: torch.Tensor,
@@ -148,12 +162,11 @@ def gather_quantized_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scal
     once (e4m3 values in bf16 are exact).  Returns ``(out_key, out_value)``, each
     ``[total_tokens, num_kv_heads, head_dim]``; give both to avoid reading the total back
     from the device."""
-    dev = _check_cuda(key_cache, value_cache, scales, block_table, cu_seq_lens, seq_starts,
-                      out_key, out_value, oob_count)
+    index = _check_device(key_cache, value_cache, scales, block_table, cu_seq_lens, seq_starts,
+                          out_key, out_value, oob_count)
     nb, h, d, code, cs, ss = _check_quantized(key_cache, value_cache, scales)
     if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         _fail("block_table must be a 2-D int32 tensor with contiguous rows")
-    index = key_cache.get_device()
     batch = cu_seq_lens.numel() - 1
     _check_ints("cu_seq_lens", cu_seq_lens, 1, index)
     if batch > block_table.shape[0]:
@@ -166,14 +179,11 @@ def gather_quantized_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scal
         given = out_key if out_key is not None else out_value
         dt = dtype if given is None else given.dtype
         total = int(cu_seq_lens[-1].item()) if batch > 0 else 0
-        made = _lib_empty((total, h, d), dt, dev, stream)
+        dev = key_cache.device
         if out_key is None:
-            out_key = made
-            if out_value is None:
-                out_value = torch.empty_like(made) if stream is None else \
-                    _lib_empty((total, h, d), dt, dev, stream)
-        else:
-            out_value = made
+            out_key = _empty((total, h, d), dt, dev, stream)
+        if out_value is None:
+            out_value = _empty((total, h, d), dt, dev, stream)
     os = _check_tokens("out_key", out_key, h, d)
     ov = _check_tokens("out_value", out_value, h, d)
     if out_key.dtype is not out_value.dtype:
@@ -188,17 +198,8 @@ def gather_quantized_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scal
                  block_table.shape[1], cu_seq_lens.data_ptr(), _ptr(seq_starts), batch,
                  int(max_seq_len), h, d, PAGE, nb, _DTYPES[out_key.dtype], code, cs, ss,
                  out_key.data_ptr(), out_value.data_ptr(), max(os, ov), rows,
-                 _oob_ptr(oob_count), _stream_handle(dev, stream))
+                 _oob_ptr(oob_count), _stream(index, stream))
     return out_key, out_value
-
-
-def _lib_empty(shape, dtype: torch.dtype, device: torch.device,
-               stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
-    """An output from the memory of the stream that writes it."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def decode_workspace(batch: int, num_qo_heads: int, num_kv_heads: int, head_dim: int,
@@ -229,13 +230,12 @@ def quantized_decode_attention(q: torch.Tensor, key_cache: torch.Tensor,
     float32 ``[B, num_qo_heads]``, the natural-log log-sum-exp of the scaled logits (-inf, and
     ``out`` 0, for a request without tokens).  ``workspace``: from ``decode_workspace``;
     made for the call if not given."""
-    dev = _check_cuda(q, key_cache, value_cache, scales, indptr, indices, last_page_len, out, lse,
-                      workspace)
+    index = _check_device(key_cache, value_cache, scales, q, indptr, indices, last_page_len, out,
+                          lse, workspace)
     nb, hkv, d, code, cs, ss = _check_quantized(key_cache, value_cache, scales)
     if q.dim() != 3:
         _fail(f"q must be [requests, num_qo_heads, head_dim], got {tuple(q.shape)}")
-    batch, hq = q.shape[0], q.shape[1]
-    index = q.get_device()
+    batch, hq = q.shape[:2]
     qs = _check_tokens("q", q, hq, d)
     if hq == 0 or hq % hkv:
         _fail(f"num_qo_heads ({hq}) must be a multiple of num_kv_heads ({hkv})")
@@ -243,7 +243,8 @@ def quantized_decode_attention(q: torch.Tensor, key_cache: torch.Tensor,
     _check_ints("indices", indices, 0, index)
     _check_ints("last_page_len", last_page_len, batch, index)
     if out is None:
-        out = _lib_empty((batch, hq, d), q.dtype, dev, stream)
+        out = q.new_empty((batch, hq, d)) if stream is None else \
+            _empty((batch, hq, d), q.dtype, q.device, stream)
         os = hq * d
     else:
         os = _check_tokens("out", out, hq, d)
@@ -252,15 +253,16 @@ def quantized_decode_attention(q: torch.Tensor, key_cache: torch.Tensor,
                   f"{tuple(out.shape)}")
     if lse is None:
         if return_lse:
-            lse = _lib_empty((batch, hq), torch.float32, dev, stream)
+            lse = q.new_empty((batch, hq), dtype=torch.float32) if stream is None else \
+                _empty((batch, hq), torch.float32, q.device, stream)
     elif lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.numel() < batch * hq:
         _fail("lse must be contiguous float32 [requests, num_qo_heads]")
     if workspace is None:
         if stream is None:
-            workspace = decode_workspace(batch, hq, hkv, d, dev)
+            workspace = decode_workspace(batch, hq, hkv, d, q.device)
         else:
             with torch.cuda.stream(stream):     # the memory of the stream that uses it
-                workspace = decode_workspace(batch, hq, hkv, d, dev)
+                workspace = decode_workspace(batch, hq, hkv, d, q.device)
     elif not workspace.is_contiguous():
         _fail("workspace must be contiguous (decode_workspace makes it)")
     _lib.call_on(index, "kvc_quantized_decode", q.data_ptr(), qs, key_cache.data_ptr(),
@@ -269,5 +271,5 @@ def quantized_decode_attention(q: torch.Tensor, key_cache: torch.Tensor,
                  PAGE, _DTYPES[q.dtype], code,
                  float(sm_scale) if sm_scale is not None else d ** -0.5, workspace.data_ptr(),
                  workspace.numel() * workspace.element_size(), out.data_ptr(), os, _ptr(lse),
-                 _stream_handle(dev, stream))
+                 _stream(index, stream))
     return (out, lse) if return_lse else out
