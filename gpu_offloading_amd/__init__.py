@@ -10,6 +10,7 @@ Modules:
   decode     BatchDecodeWithPagedKVCacheWrapper (plan / run)
   prompt     BatchPromptAttentionWrapper: new prompts over their own K/V
   eviction   BatchAttentionWeightsWrapper: attention weight per cached token
+  quantized  the cache in 8 bits: write, read back, decode attention
   kv_cache   PagedKVCache: caches, block table, page pool, step setup, swap
   allocator  PageAllocator protocol, PagePool, pages_needed
   workloads  seeded synthetic workloads of the benchmark configurations
@@ -23,7 +24,7 @@ __version__ = "0.1.0"
 def __getattr__(name):
     # Lazy imports keep `import gpu_offloading_amd` cheap (no torch) for the
     # allocator-only users, e.g. CPU scheduler tests.
-    if name in ("ops", "decode", "prompt", "eviction", "kv_cache", "workloads", "build",
+    if name in ("ops", "decode", "prompt", "eviction", "quantized", "kv_cache", "workloads", "build",
                 "_lib"):
         import importlib
         return importlib.import_module(f".{name}", __name__)

@@ -25,7 +25,7 @@ from typing import Iterable, Optional, Sequence
 import numpy as np
 import torch
 
-from . import _lib, hostmem, ops
+from . import _lib, hostmem, ops, quantized
 from .allocator import PagePool, pages_needed
 from .decode import BatchDecodeWithPagedKVCacheWrapper
 from .eviction import BatchAttentionWeightsWrapper
@@ -86,6 +86,14 @@ class PagedKVCache:
     ``max_seqs * ceil(max_seq_len / page_size)`` with identity block-table rows.
     ``free_page_order`` optionally replaces the initial FIFO free list
     ``range(total_pages)`` (e.g. a seeded permutation for a fragmented pool).
+
+    ``kv_dtype`` ``torch.float8_e4m3fn`` or ``torch.int8`` holds the cache in 8 bits
+    (``quantized``): ``k_cache`` / ``v_cache`` are then codes ``[pages, Hkv, 16, D]`` beside
+    ``kv_scales``, half the bytes on the card and over the host link.  ``append``
+    quantises, ``gather`` and ``prefill`` read back in ``dtype`` (bf16 or fp16), ``decode`` attends to
+    the codes, for any group of up to 16 query heads and head_dim 64, 128 or 256.  New
+    prompts attend to their own K/V as they are.  Attention tracking and eviction of single
+    tokens need an unquantised cache.
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_seqs: int,
@@ -95,9 +103,17 @@ class PagedKVCache:
                  free_page_order: Optional[Iterable[int]] = None,
                  workspace_bytes: int = 128 * 1024 * 1024,
                  staging_bytes: int = 256 * 1024 * 1024,
-                 num_segments: Optional[int] = None):
+                 num_segments: Optional[int] = None, kv_dtype: Optional[torch.dtype] = None):
         if page_size != 16:
             raise ValueError("page_size must be 16 (the engine's page size)")
+        if kv_dtype is not None:
+            group, rest = divmod(num_qo_heads or num_kv_heads, max(num_kv_heads, 1))
+            if kv_dtype not in quantized.CODES or dtype not in (torch.bfloat16, torch.float16) \
+                    or head_dim not in (64, 128, 256) or rest or not 1 <= group <= 16:
+                raise ValueError("a quantised cache needs kv_dtype float8_e4m3fn or int8, dtype "
+                                 "bfloat16 or float16, head_dim 64, 128 or 256 and at most 16 "
+                                 "query heads per KV head")
+        self.kv_dtype = kv_dtype
         self.device = torch.device(device)
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
@@ -117,14 +133,34 @@ class PagedKVCache:
         # distinct memory pages as with separate K and V tensors (cfg2 step
         # 3.23 -> 3.12 ms).  k_cache[l] / v_cache[l] are the engine's
         # [pages, page_size, Hkv, D] caches, as views.
-        self.kv_cache = [torch.zeros((self.total_pages, 2, page_size, num_kv_heads, head_dim),
-                                     dtype=dtype, device=self.device) for _ in range(num_layers)]
-        self.k_cache = [t[:, 0] for t in self.kv_cache]
-        self.v_cache = [t[:, 1] for t in self.kv_cache]
+        # (Quantised: one tensor of blocks [K codes | V codes | scales] per layer.)
+        self.kv_scales: Optional[list[torch.Tensor]] = None
+        if kv_dtype is not None:
+            layers = [quantized.quantized_cache(self.total_pages, num_kv_heads, head_dim, kv_dtype,
+                                                self.device) for _ in range(num_layers)]
+            self.kv_cache = [x.storage for x in layers]
+            self.k_cache = [x.key_cache for x in layers]
+            self.v_cache = [x.value_cache for x in layers]
+            self.kv_scales = [x.scales for x in layers]
+            # The swap moves a block as two halves of equal size, whatever is in them.
+            half = self.kv_cache[0].shape[1] // 2
+            self._halves = [tuple(t[:, i * half:(i + 1) * half].view(-1, 1, 1, half)
+                                  for i in range(2)) for t in self.kv_cache]
+        else:
+            self.kv_cache = [torch.zeros((self.total_pages, 2, page_size, num_kv_heads, head_dim),
+                                         dtype=dtype, device=self.device)
+                             for _ in range(num_layers)]
+            self.k_cache = [t[:, 0] for t in self.kv_cache]
+            self.v_cache = [t[:, 1] for t in self.kv_cache]
+            self._halves = list(zip(self.k_cache, self.v_cache))
         # Each layer's cache arguments of a decode launch (pointers, block and
         # token strides, blocks): fixed for the cache's life.
         self._layer_kv = [(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.shape[0])
                           for k, v in zip(self.k_cache, self.v_cache)]
+        # A quantised cache's decode: (requests, indptr, indices, last_page_len) on the device, and
+        # its chunks' (table rows, cu_seq_lens, tokens, longest).
+        self._quant_step: Optional[tuple] = None
+        self._quant_chunks: Optional[tuple] = None
 
         if self._dynamic_pages:
             self._bt = torch.full((max_seqs, self.max_pages_per_seq), -1,
@@ -209,6 +245,10 @@ class PagedKVCache:
                                                 dtype=torch.int32, device=self.device)
         self._prompt_wrapper = BatchPromptAttentionWrapper(self._workspace_buf)
         self._weights_wrapper = BatchAttentionWeightsWrapper(self._workspace_buf)
+        if self.kv_dtype is not None:
+            self._chunk_wrapper = BatchPromptAttentionWrapper(self._workspace_buf)
+            self._quant_workspace = quantized.decode_workspace(
+                self.max_seqs, self.num_heads, self.num_kv_heads, self.head_dim, self.device)
 
     def _to_device(self, arr) -> torch.Tensor:
         """Async H2D of a small host array through a fresh pinned buffer."""
@@ -260,6 +300,11 @@ class PagedKVCache:
         d = self._to_device(both)
         self._bt.view(-1).scatter_(0, d[:len(pos)], d[len(pos):].to(torch.int32))
         self._bt_pending.clear()
+
+    @property
+    def page_bytes(self) -> int:
+        """Bytes of a page in one layer: K, V and, if quantised, their scales."""
+        return 2 * ops.block_bytes(self._halves[0][0])
 
     def _require_gpu(self) -> None:
         if self._decode_wrapper is None:
@@ -347,9 +392,9 @@ class PagedKVCache:
         self._step_slots = None
         self.seq_lens.zero_()
         self._seq_lens_cpu.zero_()
-        for kc, vc in zip(self.k_cache, self.v_cache):
-            kc.zero_()
-            vc.zero_()
+        self._quant_step = self._quant_chunks = None
+        for t in self.kv_cache:
+            t.zero_()
         if self._dynamic_pages:
             self._pool.reset()
             self._bt_pending.clear()
@@ -363,16 +408,28 @@ class PagedKVCache:
 
     # ----------------------------------------------------- snapshot / fill
     def fill_kv_random(self, std: float = 0.01, generator: Optional[torch.Generator] = None) -> None:
+        if self.kv_dtype is not None:
+            step = 1 << 14      # slots at a time
+            slots = torch.arange(self.total_pages * self.page_size, device=self.device)
+            for layer in range(self.num_layers):
+                for part in slots.split(step):
+                    k, v = (torch.empty((len(part), self.num_kv_heads, self.head_dim),
+                                        dtype=self.dtype, device=self.device)
+                            .normal_(0, std, generator=generator) for _ in range(2))
+                    self.append(layer, k, v, part)
+            return
         for kc, vc in zip(self.k_cache, self.v_cache):
             kc.normal_(0, std, generator=generator)
             vc.normal_(0, std, generator=generator)
 
     def kv_snapshot(self):
+        if self.kv_dtype is not None:
+            return [t.clone() for t in self.kv_cache], []
         return ([kc.clone() for kc in self.k_cache], [vc.clone() for vc in self.v_cache])
 
     def kv_restore(self, snapshot) -> None:
         a, b = snapshot
-        for kc, s in zip(self.k_cache, a):
+        for kc, s in zip(self.k_cache if self.kv_dtype is None else self.kv_cache, a):
             kc.copy_(s)
         for vc, s in zip(self.v_cache, b):
             vc.copy_(s)
@@ -438,7 +495,7 @@ class PagedKVCache:
         """moe_engine.py:1896-1955: indptr / last_page_len on the host,
         page indices flattened on the device, then ``wrapper.plan``."""
         self._require_gpu()
-        self._step_slots = None
+        self._step_slots = self._quant_step = None
         ids = self._check_seq_ids(seq_ids)
         b = len(ids)
         if b == 0:
@@ -458,6 +515,11 @@ class PagedKVCache:
         self._decode_ids = ids_d
         ops.copy_page_indices(self.block_table, indptr_d, self._plan_indices_gpu, seq_ids=ids_d)
         total = int(indptr[b])
+        if self.kv_dtype is not None:
+            lpl_d = self._to_device(lpl)
+            self._quant_step = (b, indptr_d, self._plan_indices_gpu[:total], lpl_d)
+            self._step_temps = (indptr_d, lpl_d)
+            return
         self._decode_wrapper.plan(
             torch.from_numpy(indptr), self._plan_indices_gpu[:total], torch.from_numpy(lpl),
             num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
@@ -480,6 +542,9 @@ class PagedKVCache:
         clen = np.asarray(chunk_lens, dtype=np.int64)
         if (clen < 0).any() or (clen > lens).any():
             raise ValueError("a chunk must be part of its sequence's cached tokens")
+        if self.kv_dtype is not None:
+            self._plan_quant_chunks(ids, clen, lens)
+            return
         nblk = (lens + self.page_size - 1) // self.page_size
         kv_indptr = np.zeros(b + 1, dtype=np.int32)
         np.cumsum(nblk, out=kv_indptr[1:])
@@ -498,6 +563,23 @@ class PagedKVCache:
             head_dim_qk=self.head_dim, page_size=self.page_size, causal=True,
             q_data_type=self.dtype)
 
+    def _plan_quant_chunks(self, ids: np.ndarray, clen: np.ndarray, lens: np.ndarray) -> None:
+        """Plan chunks of a quantised cache: their sequences' K/V, read back into contiguous
+        rows, are the keys of the prompt attention."""
+        self._check_page_counts((lens + self.page_size - 1) // self.page_size)
+        cu, qo = (np.concatenate([[0], np.cumsum(x)]) for x in (lens, clen))
+        if cu[-1] > np.iinfo(np.int32).max:
+            raise RuntimeError(f"the chunks' sequences hold {int(cu[-1])} tokens, more than one "
+                               "plan takes; split the batch")
+        cu, qo = cu.astype(np.int32), qo.astype(np.int32)
+        rows = self.block_table.index_select(0, self._to_device(ids))
+        self._chunk_wrapper.plan(torch.from_numpy(qo), torch.from_numpy(cu),
+                                 num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
+                                 head_dim=self.head_dim, causal=True, q_data_type=self.dtype)
+        cu_d = self._to_device(cu)
+        self._chunk_wrapper._set_staged(*self._chunk_wrapper._staged, rows, cu_d)
+        self._quant_chunks = (rows, cu_d, int(cu[-1]), int(lens.max()) if len(lens) else 0)
+
     def prepare_prefill_chunk(self, seq_ids: Sequence[int], chunk_lens: Sequence[int]) -> torch.Tensor:
         """Setup of a continuation-prefill step (moe_engine.py:1678-1751):
         slot mapping of the chunk's tokens from the current lengths, then
@@ -515,6 +597,17 @@ class PagedKVCache:
         """Causal attention of the planned chunks' queries ``[sum(chunk), Hq, D]``
         over the paged cache of ``layer`` (moe_engine.py:3939-3941)."""
         self._require_gpu()
+        if self.kv_dtype is not None:
+            if self._quant_chunks is None:
+                raise RuntimeError("prefill needs plan_prefill first")
+            rows, cu, total, longest = self._quant_chunks
+            w = self._chunk_wrapper
+            w._run_stream(None)        # (behind the plan's uploads, which the read needs, too)
+            k, v = (torch.empty((total, self.num_kv_heads, self.head_dim), dtype=self.dtype,
+                                device=self.device) for _ in range(2))
+            quantized.gather_quantized_kv(self.k_cache[layer], self.v_cache[layer],
+                                          self.kv_scales[layer], rows, cu, longest, k, v)
+            return w.run(q, k, v, out=out, return_lse=return_lse)
         self._step_stream_for_call()
         return self._prefill_wrapper.run(q, (self.k_cache[layer], self.v_cache[layer]),
                                          out=out, return_lse=return_lse)
@@ -537,7 +630,7 @@ class PagedKVCache:
         self._require_gpu()
         b = len(seq_ids)
         graph_n = b if graph_n is None else graph_n
-        self._step_slots = None
+        self._step_slots = self._quant_step = None
         if b == 0 or graph_n < b:
             # Nothing to plan, or an error for slot_mapping to report.
             slots = self.slot_mapping(seq_ids, [1] * b, graph_n)
@@ -566,7 +659,8 @@ class PagedKVCache:
         pend = self._peek_bt_pending()
         u = 0 if pend is None else len(pend[0])
         w = self._decode_wrapper
-        cap = w._plan_capacity(b)
+        quant = self.kv_dtype is not None      # (whose decode needs no schedule)
+        cap = 0 if quant else w._plan_capacity(b)
         while True:
             o_ids = cap
             o_pos = o_ids + b
@@ -588,6 +682,8 @@ class PagedKVCache:
             if u:
                 h[o_bpos:o_bpos + 2 * u].view(np.int64)[:] = pend[0]
                 h[o_bval:o_bval + u] = pend[1]
+            if quant:
+                break
             sched = w._schedule_into(h[o_ip:o_ip + b + 1], h[o_lpl:o_lpl + b], b,
                                      self.num_heads, self.num_kv_heads, self.head_dim, ps,
                                      h[0:cap])
@@ -615,7 +711,8 @@ class PagedKVCache:
                                 dm[o_ids:o_ids + b])
         _, plan_v, indptr_v, lpl_v, slots, step_slots, self._decode_ids = self._step_views
         lay = self._step_layout
-        lay.plan_ints = int(sched.plan_ints)   # the plan's unused capacity is not sent
+        # the plan's unused capacity is not sent
+        lay.plan_ints = 0 if quant else int(sched.plan_ints)
         lay.tail_begin, lay.tail_end = cap, n
         lay.ids, lay.positions, lay.indptr, lay.lens_after = o_ids, o_pos, o_ip, o_la
         lay.bt_pos, lay.bt_val = o_bpos, o_bval
@@ -627,8 +724,11 @@ class PagedKVCache:
             self._bt_pending.clear()
         # The whole page-index buffer goes to the decode (its pages are bounded
         # by the plan), so the launch does not change with the page count.
-        w._install(sched, plan_v, indptr_v, lpl_v, self._plan_indices_gpu, self.num_heads,
-                   self.num_kv_heads, self.head_dim, ps)
+        if quant:
+            self._quant_step = (b, indptr_v, self._plan_indices_gpu, lpl_v)
+        else:
+            w._install(sched, plan_v, indptr_v, lpl_v, self._plan_indices_gpu, self.num_heads,
+                       self.num_kv_heads, self.head_dim, ps)
         lens_all[ids] += 1
         self._step_slots = step_slots
         return slots
@@ -682,6 +782,12 @@ class PagedKVCache:
         buffers); when it changes, capture again and drop the old graph: its
         launches address a step buffer that may have been freed.  An empty
         key means the current plan is not a decode step's."""
+        if self.kv_dtype is not None:
+            if self._step_slots is None or self._quant_step is None:
+                return ()
+            b, indptr, indices, lpl = self._quant_step
+            return (b, indptr.data_ptr(), indices.data_ptr(), indices.numel(), lpl.data_ptr(),
+                    self._step_slots.data_ptr())
         w = self._decode_wrapper
         s = w.schedule
         if (s is None or self._step_dev is None or self._step_slots is None
@@ -784,8 +890,9 @@ class PagedKVCache:
         o_val = o_pos + 2 * u
         o_dplan = (o_val + u + 3) // 4 * 4
         group = self.num_heads // self.num_kv_heads
-        pcap = pw._plan_capacity(np.asarray(clen), group, self.num_kv_heads) if C else 0
-        dcap = dw._plan_capacity(D) if D else 0
+        quant = self.kv_dtype is not None
+        pcap = pw._plan_capacity(np.asarray(clen), group, self.num_kv_heads) if C and not quant else 0
+        dcap = dw._plan_capacity(D) if D and not quant else 0
         while True:
             o_pplan = o_dplan + dcap
             hs = self._host_image(o_pplan + pcap)
@@ -808,7 +915,7 @@ class PagedKVCache:
                 h[o_pos:o_pos + 2 * u].view(np.int64)[:] = pend[0]
                 h[o_val:o_val + u] = pend[1]
             dsched = None
-            if D:
+            if D and not quant:
                 dsched = dw._schedule_into(h[o_dip:o_dlpl], h[o_dlpl:o_cqo], D, self.num_heads,
                                            self.num_kv_heads, self.head_dim, ps,
                                            hs[o_dplan:o_pplan])
@@ -817,7 +924,7 @@ class PagedKVCache:
                     continue
             break
         psched = None
-        if C:
+        if C and not quant:
             psched = pw._schedule_into(h[o_cqo:o_cip], h[o_cip:o_clpl], h[o_clpl:o_clpl + C], C,
                                        self.num_heads, self.num_kv_heads, self.head_dim, ps,
                                        True, hs[o_pplan:])
@@ -829,8 +936,8 @@ class PagedKVCache:
         self._upload_evicted()
         dm = torch.empty(hs.numel(), dtype=torch.int32, device=self.device)
         self._step_temps = (dm,)
-        ops.stage_from_host(hs, dm, o_dplan + (int(dsched.plan_ints) if D else 0),
-                            o_pplan, o_pplan + (int(psched.plan_ints) if C else 0))
+        ops.stage_from_host(hs, dm, o_dplan + (int(dsched.plan_ints) if dsched else 0),
+                            o_pplan, o_pplan + (int(psched.plan_ints) if psched else 0))
         self._host_image_sent()
         if u:
             self._bt.view(-1).scatter_(0, dm[o_pos:o_val].view(torch.int64), dm[o_val:o_val + u])
@@ -846,15 +953,22 @@ class PagedKVCache:
             dw._sched = None
         if not C:
             pw._sched = None
+        self._quant_step = self._quant_chunks = None
         if D:
             total = int(dip[-1])
             self._decode_ids = ids_d[:D]
             ops.copy_page_indices(self._bt, dm[o_dip:o_dlpl], self._plan_indices_gpu,
                                   seq_ids=ids_d[:D])
+            if quant:
+                self._quant_step = (D, dm[o_dip:o_dlpl], self._plan_indices_gpu[:total],
+                                    dm[o_dlpl:o_cqo])
+        if D and not quant:
             dw._install(dsched, dm[o_dplan:o_dplan + dcap], dm[o_dip:o_dlpl],
                         dm[o_dlpl:o_cqo], self._plan_indices_gpu[:total], self.num_heads,
                         self.num_kv_heads, self.head_dim, ps)
-        if C:
+        if C and quant:
+            self._plan_quant_chunks(ids[D + P:], np.asarray(clen, np.int64), c_after)
+        elif C:
             total = int(cip[-1])
             ops.copy_page_indices(self._bt, dm[o_cip:o_clpl], self._prefill_indices_gpu,
                                   seq_ids=ids_d[D + P:])
@@ -867,6 +981,11 @@ class PagedKVCache:
     # ------------------------------------------------------- per-layer ops
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor,
                slot_mapping: torch.Tensor) -> None:
+        if self.kv_dtype is not None:
+            quantized.reshape_and_cache_quantized(key, value, self.k_cache[layer],
+                                                  self.v_cache[layer], self.kv_scales[layer],
+                                                  slot_mapping)
+            return
         ops.reshape_and_cache_flash(key, value, self.k_cache[layer], self.v_cache[layer],
                                     slot_mapping, "auto")
 
@@ -889,6 +1008,10 @@ class PagedKVCache:
         if slots is None:
             self._require_gpu()
             raise RuntimeError("append_and_decode needs a prepare_decode_step first")
+        if self.kv_dtype is not None:
+            self._step_stream_for_call()
+            self.append(layer, key, value, slots)
+            return self.decode(layer, q, out, return_lse)
         w = self._decode_wrapper
         sh = self._step_stream_for_call()
         kv = self._layer_kv[layer]
@@ -902,6 +1025,18 @@ class PagedKVCache:
         """Decode attention of the planned requests over ``layer`` (the
         engine's FlashInfer run, moe_engine.py:3907-3909)."""
         self._require_gpu()
+        if self.kv_dtype is not None:
+            if self._quant_step is None:
+                raise RuntimeError("decode needs a planned decode step")
+            b, indptr, indices, lpl = self._quant_step
+            if q.dim() != 3 or q.shape[0] < b or q.dtype is not self.dtype \
+                    or q.shape[1] != self.num_heads:
+                raise RuntimeError(f"q must be {self.dtype} [{b}, {self.num_heads}, "
+                                   f"{self.head_dim}], got {q.dtype} {tuple(q.shape)}")
+            self._step_stream_for_call()
+            return quantized.quantized_decode_attention(
+                q[:b], self.k_cache[layer], self.v_cache[layer], self.kv_scales[layer], indptr,
+                indices, lpl, out=out, return_lse=return_lse, workspace=self._quant_workspace)
         return self._decode_wrapper._launch(q, None, out, None, return_lse,
                                             self._step_stream_for_call(), None, None,
                                             self._layer_kv[layer])
@@ -941,6 +1076,8 @@ class PagedKVCache:
         caller's own attention has to return the log-sum-exp.)  Swapped sequences
         keep theirs on the device; ``kv_snapshot`` does not cover them."""
         self._require_gpu()
+        if self.kv_dtype is not None:
+            raise RuntimeError("a quantised cache does not track attention")
         if self.scores is not None:
             return
         if int(self._seq_lens_cpu.max()) > 0:
@@ -1138,6 +1275,10 @@ class PagedKVCache:
         if out_value is None:
             out_value = torch.empty(total, self.num_kv_heads, self.head_dim, dtype=self.dtype,
                                     device=self.device)
+        if self.kv_dtype is not None:
+            return quantized.gather_quantized_kv(
+                self.k_cache[layer], self.v_cache[layer], self.kv_scales[layer], rows, cu_t,
+                int(lens.max()) if len(lens) else 0, out_key, out_value)
         return ops.gather_kv(self.k_cache[layer], self.v_cache[layer], rows, cu_t,
                              int(lens.max()) if len(lens) else 0, out_key, out_value)
 
@@ -1258,12 +1399,12 @@ class PagedKVCache:
             e = torch.cuda.Event()
             e.record(dma)
             side.wait_event(e)
-        per = 2 * ops.block_bytes(self.k_cache[0])
+        per = self.page_bytes
         if per <= st.numel():
             with torch.cuda.stream(side):
                 ids0 = torch.zeros(1, dtype=torch.int32, device=self.device)
             for layer in range(self.num_layers):
-                ops.gather_blocks(self.k_cache[layer], self.v_cache[layer], ids0, st[:per],
+                ops.gather_blocks(*self._halves[layer], ids0, st[:per],
                                   stream=side)
         side.synchronize()
         dma.synchronize()
@@ -1292,7 +1433,7 @@ class PagedKVCache:
         completed.  Returns (start, end) events; the side stream has already
         waited for the current stream."""
         side, dma = self._side_stream(), self._dma_stream()
-        bb = ops.block_bytes(self.k_cache[0])
+        bb = ops.block_bytes(self._halves[0][0])
         per = 2 * bb
         halves, chunk = self._staging_halves(per)
         start = torch.cuda.Event(enable_timing=True)
@@ -1319,7 +1460,7 @@ class PagedKVCache:
                 if self._staging_free[b] is not None:
                     side.wait_event(self._staging_free[b])
                 for layer, j0, j1, o in segs:
-                    ops.gather_blocks(self.k_cache[layer], self.v_cache[layer], ids_t[j0:j1],
+                    ops.gather_blocks(*self._halves[layer], ids_t[j0:j1],
                                       buf[o * per: (o + j1 - j0) * per], stream=side)
                 gathered = torch.cuda.Event()
                 gathered.record(side)
@@ -1337,7 +1478,7 @@ class PagedKVCache:
                 side.wait_event(loaded)
                 for layer, j0, j1, o in segs:
                     ops.scatter_blocks(buf[o * per: (o + j1 - j0) * per], ids_t[j0:j1],
-                                       self.k_cache[layer], self.v_cache[layer], stream=side)
+                                       *self._halves[layer], stream=side)
                 done.record(side)
             self._staging_free[b] = done
             end = done
@@ -1394,7 +1535,7 @@ class PagedKVCache:
         for sid in seq_ids:
             evicted.append(int(self._evicted[sid]))
             self._set_evicted(sid, 0)
-        bb = ops.block_bytes(self.k_cache[0])
+        bb = ops.block_bytes(self._halves[0][0])
         nbytes = self.num_layers * n * 2 * bb
         if host is None:
             host = hostmem.pinned_empty(nbytes, self.device)

@@ -71,8 +71,7 @@ class SwapPreemption:
         """Whether the victim's KV fits the host budget."""
         if self.host_budget_bytes is None:
             return True
-        need = self.cache.num_layers * self.cache.seq_pages(slot) * 2 * \
-            self.cache.k_cache[0][0].numel() * self.cache.k_cache[0].element_size()
+        need = self.cache.num_layers * self.cache.seq_pages(slot) * self.cache.page_bytes
         return self.host_bytes_in_use + need <= self.host_budget_bytes
 
     def preempt(self, slot: int, key, host=None) -> SwapHandle:

@@ -204,12 +204,12 @@ def gather_quantized_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scal
 
 def decode_workspace(batch: int, num_qo_heads: int, num_kv_heads: int, head_dim: int,
                      device: str | torch.device = "cuda") -> torch.Tensor:
-    """A workspace of ``quantized_decode_attention`` for batches of up to ``batch``
-    requests: zeroed once here, left ready by each call, of one call at a time (calls
-    on several streams, and graphs that may run side by side, need one each)."""
+    """Device memory for ``quantized_decode_attention``, for batches of up to ``batch``
+    requests: of one call at a time (calls on several streams, and graphs that may run
+    side by side, need one each); nothing is kept in it between calls."""
     need = _lib.load().kvc_quantized_decode_workspace_bytes(batch, num_qo_heads, num_kv_heads,
                                                             head_dim)
-    return torch.zeros(max(int(need), 16), dtype=torch.uint8, device=device)
+    return torch.empty(max(int(need), 16), dtype=torch.uint8, device=device)
 
 
 def quantized_decode_attention(q: torch.Tensor, key_cache: torch.Tensor,

@@ -748,8 +748,8 @@ int kvc_evict_kv(
  * Pages whose id is outside [0, num_blocks), or past num_indices, hold no tokens;
  * a request without tokens gets 0 and lse -inf.  The weights enter the product with V as bf16 (dtype
  * bf16) or pairs of bf16 (fp16), sums are fp32.  workspace:
- * kvc_quantized_decode_workspace_bytes of device memory, zeroed before its first use and of one
- * call at a time; each call leaves it ready for the next.
+ * kvc_quantized_decode_workspace_bytes of device memory, 16-byte aligned, of one call at a
+ * time, not kept between calls.
  * ---------------------------------------------------------------------- */
 enum { KVC_CODE_E4M3 = 0, KVC_CODE_INT8 = 1 };
 
