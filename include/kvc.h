@@ -746,8 +746,8 @@ int kvc_evict_kv(
  * [batch + 1], indices and last_page_len [batch] are read on the device, so
  * that a captured launch serves other lengths and pages.  indptr[0] may be above 0.
  * Pages whose id is outside [0, num_blocks), or past num_indices, hold no tokens;
- * a request without tokens gets 0 and lse -inf.  The weights enter the product with V as bf16 (dtype
- * bf16) or pairs of bf16 (fp16), sums are fp32.  workspace:
+ * a request without tokens gets 0 and lse -inf.  The weights enter the product with V as pairs of
+ * bf16 (within 2^-15), sums are fp32.  workspace:
  * kvc_quantized_decode_workspace_bytes of device memory, 16-byte aligned, of one call at a
  * time, not kept between calls.
  * ---------------------------------------------------------------------- */

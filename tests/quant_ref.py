@@ -78,9 +78,10 @@ def attention(q, k, ks, v, vs, scale: float, dtype: torch.dtype):
     mag = ((q.abs() @ k.abs().T) * ks.abs()).max(1, keepdim=True).values * scale
     spread = (top - x.min(1, keepdim=True).values + x.abs().max(1, keepdim=True).values)
     rel = (d + 8) * 2 * U32 * mag + 4 * U32 * spread * 1.45 + 2.0 ** -21
-    # Each weight with its V row's scale is rounded to bf16, or to a pair of bf16 for fp16
-    # outputs; sums over n tokens and the joins are fp32; the result is rounded once.
-    w = 2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -15
+    # Each weight with its V row's scale becomes a pair of bf16 (what the first rounding leaves,
+    # 2^-8 of it at most, is rounded again); sums over n tokens and the joins are fp32; the result is
+    # rounded once.
+    w = 2.0 ** -15
     sums = 2 * (n + 64) * U32
     u = half_step(dtype)
     otol = (p @ val.abs()) * (w + 2 * rel + 2 * sums) * 1.01 + u * 1.01 * out.abs()
