@@ -169,8 +169,8 @@ __device__ __forceinline__ uint32_t word(typename VWord<D>::type v, int i) {
 // Whether no request has more pages than one workgroup streams in about the time that cutting
 // and joining it costs: then each is a workgroup's (per KV head) and none is cut.  64 pages where the
 // requests alone fill the GPU (64 requests of 600 to 1000 tokens, 8 KV heads: 26.2 -> 23.2 us),
-// else 48 (8 of 300: 10.2 -> 8.0; but one of 1000: 8.7 cut, 10.1 whole).  Every wave looks through indptr by
-// itself, beside loads that it waits for anyway; batches too large for that are cut.
+// else 48 (8 of 300: 10.2 -> 8.0; but one of 1000: 8.7 cut, 10.1 whole).  Every wave looks through
+// indptr by itself, beside loads that it waits for anyway; batches too large for that are cut.
 __host__ __device__ inline int whole_pages(int batch, int hkv) {
   return int64_t(batch) * hkv >= 256 ? 64 : 48;
 }
@@ -422,9 +422,11 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       end = last;
     } else {
       if (at >= end) break;
-      while (b < a.batch - 1 && last <= at) {
+      if (last <= at && b < a.batch - 1) {
         first = last;
         last = indptr[++b + 1] - base;
+        // (behind requests without pages)
+        if (last <= at) b = search.find(a.indptr, a.batch, base, at, first, last);
       }
       if (last <= at) break;   // (an indptr that goes down)
     }

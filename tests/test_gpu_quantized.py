@@ -306,6 +306,55 @@ def test_decode_lengths(gpu, lens, codec):
     check_decode(*got, q, held, lens, 0.03, torch.bfloat16)
 
 
+@pytest.mark.parametrize("long", [[], [3000, 1500]])
+@pytest.mark.parametrize("batch", [65, 300, 5000])
+def test_decode_of_large_batches(gpu, batch, long):
+    """Whole requests and cut ones, runs of empty requests between them, more than 4096 of them."""
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, 40, batch) * (rng.random(batch) < 0.7)
+    lens[batch // 2:batch // 2 + 50] = 0
+    lens[[7, batch - 2][:len(long)]] = long
+    lens = lens.tolist()
+    hkv, group, d = 1, 2, 64
+    cache, table, held = random_cache(lens, hkv, d, ref.INT8, gpu, batch)
+    ip, idx, lpl = pages(table, lens)
+    q = rows((batch, group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True)
+    check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
+
+
+def test_decode_of_queries_that_are_not_finite(gpu):
+    """A NaN or an infinity in a query head's row stays in that head."""
+    lens, hkv, group, d = [40, 2000], 2, 4, 128
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, 6)
+    ip, idx, lpl = pages(table, lens)
+    q = rows((2, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    args = ints(ip, gpu), ints(idx, gpu), ints(lpl, gpu)
+    base, blse = qz.quantized_decode_attention(q, *cache[:3], *args, return_lse=True)
+    bad = torch.zeros(2, hkv * group, dtype=torch.bool)
+    for b, h, x in ((0, 1, math.nan), (1, 3, math.inf), (1, 6, -math.inf)):
+        q[b, h, 9] = x
+        bad[b, h] = True
+    out, lse = qz.quantized_decode_attention(q, *cache[:3], *args, return_lse=True)
+    assert out[bad].isnan().all()
+    assert torch.equal(out[~bad], base[~bad]) and torch.equal(lse[~bad], blse[~bad])
+
+
+def test_decode_of_shared_pages(gpu):
+    """Requests that share pages, and one that holds a page twice."""
+    hkv, group, d = 2, 4, 128
+    cache, table, held = random_cache([160], hkv, d, ref.E4M3, gpu, 6)
+    t = table[0]
+    idx = np.concatenate([t[:10], t[:4], [t[3], t[3], t[0]]])
+    q = rows((3, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints([0, 10, 14, 17], gpu), ints(idx, gpu),
+                                        ints([16, 5, 16], gpu), return_lse=True)
+    at = [np.arange(160), np.arange(53), np.r_[48:64, 48:64, 0:16]]
+    kept = [[(x[i], s[i]) for x, s in held[0]] for i in at]
+    check_decode(*got, q, kept, [160, 53, 48], d ** -0.5, torch.bfloat16)
+
+
 def test_decode_outputs_strides_and_page_offsets(gpu):
     """q and out as slices, given outputs with more rows, an indptr that begins above 0, a
     workspace used again and again."""
