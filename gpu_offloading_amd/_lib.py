@@ -309,6 +309,38 @@ def load(path: str | None = None) -> ctypes.CDLL:
         return lib
 
 
+def binding():
+    """The module of csrc/bind.cpp, bound to the loaded library: the quantised ops'
+    short way to their C entries."""
+    global _bind
+    if _bind is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch
+
+        from .build import BIND_PATH
+        lib = load()
+        if not os.path.exists(BIND_PATH):
+            raise RuntimeError(f"{BIND_PATH} is not built. Build it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
+        loader = importlib.machinery.ExtensionFileLoader("kvc_bind", BIND_PATH)
+        mod = importlib.util.module_from_spec(
+            importlib.util.spec_from_file_location("kvc_bind", BIND_PATH, loader=loader))
+        loader.exec_module(mod)
+        mod.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value
+                   for name in ("kvc_reshape_and_cache_quantized", "kvc_gather_quantized_kv",
+                                "kvc_quantized_decode")),
+                 getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+                 getattr(torch._C, "_cuda_getCurrentRawStream", None) or
+                 (lambda i: torch.cuda.current_stream(i).cuda_stream))
+        _bind = mod
+    return _bind
+
+
+_bind = None
+
+
 def _check_fresh() -> None:
     """Refuse a library built from other sources than the ones beside it: its
     entry points may take other arguments than this table declares."""

@@ -1,7 +1,9 @@
-"""Build libkvc.so (all HIP sources of csrc/) for gfx950 with hipcc.
+"""Build libkvc.so (all HIP sources of csrc/) for gfx950 with hipcc, and the Python
+binding of some of its entries (csrc/bind.cpp) with g++ against torch's headers.
 
-One shared library, compiled in-tree so that it travels with the repository:
+Compiled in-tree so that they travel with the repository:
     gpu_offloading_amd/lib/libkvc.so
+    gpu_offloading_amd/lib/kvc_bind.so
 Flags: -O3, C++17, gfx950 only, packed-FP32 instruction selection disabled
 (``-Xclang -target-feature -Xclang -packed-fp32-ops``; hipcc's host pass
 warns that it does not know the feature, which is harmless).
@@ -42,24 +44,41 @@ def hipcc() -> str:
 
 STAMP_PATH = LIB_PATH + ".srchash"
 
+BIND_SRC = os.path.join(CSRC, "bind.cpp")
+BIND_PATH = os.path.join(LIB_DIR, "kvc_bind.so")
+BIND_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall"]
+
+
+def _bind_command(out: str) -> list[str]:
+    """g++ line of the binding: Python's and torch's headers, torch's libraries (loaded
+    already wherever the binding is)."""
+    import importlib.util
+    import sysconfig
+
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    includes = [sysconfig.get_paths()["include"], INCLUDE, os.path.join(torch_dir, "include"),
+                os.path.join(torch_dir, "include", "torch", "csrc", "api", "include")]
+    return ["g++", *BIND_FLAGS, *(f"-I{p}" for p in includes), BIND_SRC, "-o", out,
+            "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
 
 def sources() -> list[str]:
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
 
 
 def source_hash() -> str:
-    """SHA-256 of everything libkvc.so is built from (sources, headers,
-    flags): a library whose stamp differs was built from other sources."""
+    """SHA-256 of everything libkvc.so and its binding are built from (sources,
+    headers, flags): a library whose stamp differs was built from other sources."""
     import hashlib
 
     h = hashlib.sha256()
     files = sources() + sorted(glob.glob(os.path.join(CSRC, "*.h"))) + \
-        [os.path.join(INCLUDE, "kvc.h")]
+        [os.path.join(INCLUDE, "kvc.h"), BIND_SRC]
     for path in files:
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:
             h.update(f.read())
-    h.update(" ".join(HIP_FLAGS).encode())
+    h.update(" ".join(HIP_FLAGS + BIND_FLAGS).encode())
     return h.hexdigest()
 
 
@@ -71,8 +90,8 @@ def _run(cmd: list[str]) -> tuple[int, list[str]]:
 
 
 def build_library(verbose: bool = False, jobs: int | None = None) -> str:
-    """Compile every csrc/*.hip into libkvc.so (always recompiles): one hipcc
-    process per source file, in parallel, then one link."""
+    """Compile every csrc/*.hip into libkvc.so, and the binding (always
+    recompiles): one process per source file, in parallel, then one link."""
     from concurrent.futures import ThreadPoolExecutor
 
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -82,6 +101,9 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
     objs = [os.path.join(obj_dir, os.path.basename(s)[:-4] + ".o") for s in srcs]
     cmds = [[hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o]
             for s, o in zip(srcs, objs)]
+    bind_tmp = BIND_PATH + ".tmp"
+    srcs.append(BIND_SRC)
+    cmds.append(_bind_command(bind_tmp))
     jobs = jobs or min(len(cmds), max(1, min(os.cpu_count() or 1, 16)))
     if verbose:
         for c in cmds:
@@ -90,7 +112,7 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
         results = list(ex.map(_run, cmds))
     failed = [(s, m) for s, (rc, m) in zip(srcs, results) if rc != 0]
     if failed:
-        raise RuntimeError("hipcc failed:\n" + "\n".join(
+        raise RuntimeError("compilation failed:\n" + "\n".join(
             f"{s}:\n" + "\n".join(m) for s, m in failed))
     msgs = [ln for _, m in results for ln in m]
     tmp = LIB_PATH + ".tmp"
@@ -104,6 +126,7 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
     if verbose and msgs:
         print("\n".join(msgs), file=sys.stderr)
     os.replace(tmp, LIB_PATH)
+    os.replace(bind_tmp, BIND_PATH)
     with open(STAMP_PATH, "w") as f:
         f.write(source_hash() + "\n")
     return LIB_PATH

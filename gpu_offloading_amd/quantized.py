@@ -11,7 +11,7 @@ bytes.  A code stands for ``code * scale``:
 
 The ops keep the manner of ``ops`` (``RuntimeError`` for bad arguments, the current torch
 stream unless one is given, no fallback) and launch the kernels of
-csrc/quant_cache.hip and csrc/quant_decode.hip.  ``PagedKVCache(kv_dtype=...)`` is
+csrc/quant_cache.hip and csrc/quant_decode.hip, ordinary calls by way of csrc/bind.cpp.  ``PagedKVCache(kv_dtype=...)`` is
 the cache manager over them.
 """
 from __future__ import annotations
@@ -114,6 +114,11 @@ def _check_device(*ts: Optional[torch.Tensor]) -> int:
     return index
 
 
+def _status(name: str, st: int) -> None:
+    if st:
+        _lib.check(name, st)
+
+
 def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
                                 value_cache: torch.Tensor, scales: torch.Tensor,
                                 slot_mapping: torch.Tensor, *,
@@ -126,6 +131,10 @@ def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cach
     slot_mapping whose length is the token count, a negative slot is padding.  The
     slots of a call must be distinct.  A row that holds an infinity or a NaN reads back
     as NaN."""
+    st = (_lib._bind or _lib.binding()).write(key, value, key_cache, value_cache, scales,
+                                              slot_mapping, oob_count, stream)
+    if st is not None:
+        return _status("kvc_reshape_and_cache_quantized", st)
     index = _check_device(key_cache, value_cache, scales, key, value, slot_mapping, oob_count)
     nb, h, d, code, cs, ss = _check_quantized(key_cache, value_cache, scales)
     if slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 \
@@ -162,6 +171,12 @@ def gather_quantized_kv(key_cache: torch.Tensor, value_cache: torch.Tensor, scal
     once (e4m3 values in bf16 are exact).  Returns ``(out_key, out_value)``, each
     ``[total_tokens, num_kv_heads, head_dim]``; give both to avoid reading the total back
     from the device."""
+    st = (_lib._bind or _lib.binding()).read(key_cache, value_cache, scales, block_table,
+                                             cu_seq_lens, max_seq_len, out_key, out_value,
+                                             seq_starts, oob_count, stream)
+    if st is not None:
+        _status("kvc_gather_quantized_kv", st)
+        return out_key, out_value
     index = _check_device(key_cache, value_cache, scales, block_table, cu_seq_lens, seq_starts,
                           out_key, out_value, oob_count)
     nb, h, d, code, cs, ss = _check_quantized(key_cache, value_cache, scales)
@@ -230,6 +245,13 @@ def quantized_decode_attention(q: torch.Tensor, key_cache: torch.Tensor,
     float32 ``[B, num_qo_heads]``, the natural-log log-sum-exp of the scaled logits (-inf, and
     ``out`` 0, for a request without tokens).  ``workspace``: from ``decode_workspace``;
     made for the call if not given."""
+    got = (_lib._bind or _lib.binding()).decode(q, key_cache, value_cache, scales, indptr, indices,
+                                                last_page_len, sm_scale, out, lse, return_lse,
+                                                workspace, stream)
+    if got is not None:
+        if got.__class__ is int:
+            _status("kvc_quantized_decode", got)
+        return got
     index = _check_device(key_cache, value_cache, scales, q, indptr, indices, last_page_len, out,
                           lse, workspace)
     nb, hkv, d, code, cs, ss = _check_quantized(key_cache, value_cache, scales)

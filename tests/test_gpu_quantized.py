@@ -562,3 +562,94 @@ def test_offsets_past_4_gib(gpu):
     ip, idx, lpl = (ints(x, gpu) for x in pages(table, lens))
     got = qz.quantized_decode_attention(q, *c[:3], ip, idx, lpl, return_lse=True)
     check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
+
+
+# ------------------------------------------------- the two ways to the C entries
+def test_binding_and_python_agree(gpu, monkeypatch):
+    """An ordinary call by way of the binding and the same call without it: the same bits;
+    what the binding does not take is refused or done in Python."""
+    lens, hkv, group, d = [700, 90, 0, 5], 2, 4, 128
+    hq = hkv * group
+    cache, table, _ = random_cache(lens, hkv, d, ref.E4M3, gpu, 3)
+    ip, idx, lpl = (ints(x, gpu) for x in pages(table, lens))
+    q = rows((4, hq, d), 5, torch.bfloat16, 0.3).to(gpu)
+    k = rows((9, hkv, d), 6, torch.bfloat16).to(gpu)
+    slots = torch.arange(9, device=gpu) * 7
+    ws = qz.decode_workspace(4, hq, hkv, d, gpu)
+    tab, cu = ints(table, gpu), ints([0, 700, 790, 790, 795], gpu)
+    took = []
+
+    class Counted:
+        def __init__(self, inner):
+            self.inner = inner
+
+        def __getattr__(self, name):
+            def f(*args):
+                got = getattr(self.inner, name)(*args)
+                took.append((name, got is not None))
+                return got
+            return f
+
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    def all_ops():
+        c = [t.clone() for t in cache[:3]]
+        qz.reshape_and_cache_quantized(k, k, *c, slots)
+        outs = [torch.zeros(795, hkv, d, dtype=torch.bfloat16, device=gpu) for _ in "kv"]
+        qz.gather_quantized_kv(*c, tab, cu, 700, *outs)
+        got = qz.quantized_decode_attention(q, *c, ip, idx, lpl, return_lse=True, workspace=ws,
+                                            sm_scale=0.1)
+        return [c[0].view(torch.uint8), c[1].view(torch.uint8), c[2].nan_to_num(3.0), *outs, *got]
+
+    from gpu_offloading_amd import _lib
+    inner = _lib.binding()
+    monkeypatch.setattr(_lib, "_bind", Counted(inner))
+    short = all_ops()
+    assert took == [("write", True), ("read", True), ("decode", True)]
+    monkeypatch.setattr(_lib, "_bind", Nothing())
+    assert all(torch.equal(a, b) for a, b in zip(short, all_ops()))
+    # Unusual and wrong arguments, one at a time: None from the binding, and then either a result or
+    # RuntimeError from Python.
+    monkeypatch.setattr(_lib, "_bind", Counted(inner))
+    c = cache[:3]
+    out = torch.empty_like(q)
+    good = dict(q=q, key_cache=c[0], value_cache=c[1], scales=c[2], indptr=ip, indices=idx,
+                last_page_len=lpl)
+    for name, bad in (("q", q.float()), ("q", q[:, :3]), ("q", q.transpose(0, 1)), ("q", q.cpu()),
+                      ("key_cache", c[0].view(torch.uint8)), ("value_cache", c[1].view(torch.int8)),
+                      ("value_cache", c[1][:2]), ("scales", c[2].half()), ("scales", c[2][:, :1]),
+                      ("indptr", ip[:3]), ("indptr", ip.long()), ("indices", idx.float()),
+                      ("last_page_len", lpl[:3]), ("last_page_len", lpl.cpu())):
+        took.clear()
+        with pytest.raises(RuntimeError):
+            qz.quantized_decode_attention(**{**good, name: bad}, workspace=ws)
+        assert took == [("decode", False)], name
+    for name, bad in (("out", out.half()), ("out", out[:2]), ("lse", torch.empty(2, device=gpu)),
+                      ("workspace", ws[::2])):
+        took.clear()
+        with pytest.raises(RuntimeError):
+            qz.quantized_decode_attention(**{**good, "workspace": ws, name: bad})
+        assert took == [("decode", False)], name
+    with pytest.raises(RuntimeError, match="WORKSPACE"):
+        qz.quantized_decode_attention(**good, workspace=ws[:64])
+    with pytest.raises(RuntimeError, match="sm_scale"):
+        qz.quantized_decode_attention(**good, workspace=ws, sm_scale=-1.0)
+    for args in ((k.float(), k), (k, k.half()), (k[:8], k), (k[:, :1], k), (k, k.cpu())):
+        with pytest.raises(RuntimeError):
+            qz.reshape_and_cache_quantized(*args, *c, slots)
+    for bad in (slots.int(), slots.cpu(), slots[::2], slots[None]):
+        with pytest.raises(RuntimeError):
+            qz.reshape_and_cache_quantized(k, k, *c, bad)
+    outs = [torch.zeros(795, hkv, d, dtype=torch.bfloat16, device=gpu) for _ in "kv"]
+    for args in ((tab.long(), cu, 700), (tab[:2], cu, 700), (tab, cu.long(), 700), (tab, cu, -1),
+                 (tab, cu, 1 << 31), (tab.t(), cu, 700)):
+        with pytest.raises(RuntimeError):
+            qz.gather_quantized_kv(*c, *args, *outs)
+    for pair in ((outs[0], outs[1].half()), (outs[0][:, :1], outs[1]), (outs[0].float(),) * 2,
+                 (outs[0], outs[1].cpu())):
+        with pytest.raises(RuntimeError):
+            qz.gather_quantized_kv(*c, tab, cu, 700, *pair)
+    with pytest.raises(RuntimeError):
+        qz.gather_quantized_kv(*c, tab, cu, 700, *outs, ints([0, 0], gpu))

@@ -159,3 +159,23 @@ def test_nothing_to_do_is_no_error():
     assert decode(batch=0, q=None) == 0
     ws = _lib.load().kvc_quantized_decode_workspace_bytes
     assert ws(1, 32, 8, 128) > 0 and ws(-1, 32, 8, 128) == 0 and ws(1, 0, 8, 128) == 0
+
+
+# ------------------------------------------------------------------ binding
+def test_binding_leaves_what_is_not_ordinary_to_python():
+    """The short way takes nothing that is not on a GPU, whatever it is handed, and raises nothing."""
+    m = _lib.binding()
+    c = qz.quantized_cache(4, 2, 64, ref.INT8, "cpu")
+    k = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    ip = torch.zeros(4, dtype=torch.int32)
+    calls = {m.write: [k, k, *c[:3], torch.arange(3), None, None],
+             m.read: [*c[:3], ip.view(1, 4), ip[:2], 3, k, k, None, None, None],
+             m.decode: [k, *c[:3], ip, ip, ip, None, None, None, True, ip, None]}
+    for f, args in calls.items():
+        assert f(*args) is None
+        assert f(*args[:-1]) is None and f() is None
+        for i in range(len(args)):
+            for odd in (None, 7, "x", 1.5, torch.empty(0)):
+                assert f(*args[:i], odd, *args[i + 1:]) is None
+    with pytest.raises(TypeError):
+        m.bind()
