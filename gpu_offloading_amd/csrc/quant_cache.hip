@@ -9,10 +9,13 @@
 // model's type and 8 of codes, so that both sides are whole lines.  Rows are dealt tile by
 // tile (16 tokens of a head, K and V in turn): 16 neighbouring tokens' codes are one
 // contiguous piece of the cache, and their scales one line that a workgroup completes.
-// All but the scales moves with the non-temporal hint (32768 tokens written 40.4 -> 38.8 us by it
-// on the loads, 41.4 -> 40.4 on the stores; read back 42.4 -> 38.9 on the stores).
-// Measured: 32768 tokens of 8 x 128 written in 38.9 us (5.2 TB/s), read back in 40.5 (5.0); a
-// large device copy reaches 5.1 TB/s.
+// Rows of the model's type move with the non-temporal hint (32768 tokens written 40.4 -> 38.8 us,
+// read back 42.4 -> 38.9), codes without: what is written is read next, by the chunk's read-back or the
+// step's attention (16384 tokens written and read back 40.0 -> 35.6 us by stores that stay in the
+// caches, though the write alone takes 42.0 for 38.9 us at 32768), and histories that fit the 256 MB
+// cache in front of the memory are read from there (8 x 4096 tokens 38.6 -> 30.8 us; 41.5 for 40.5
+// where they do not).  A large device copy reaches 5.1 TB/s; these 4.9 and 4.9, from memory, and
+// 4.7 and 6.6 from the cache.
 #include "quant.h"
 
 #include <algorithm>
@@ -115,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteArgs a) {
                          unpack_hi<kHalf>(w[3]), s.inverse);
     uint8_t* to = (kv[u] ? a.cache[1] : a.cache[0]) + block * a.block_stride +
                   (head[u] * kQuantPage + place) * D + lane * 8;
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x2_t, c), reinterpret_cast<u32x2_t*>(to));
+    *reinterpret_cast<uint2*>(to) = c;
     if (lane == 0)
       a.scales[block * a.scales_stride + (head[u] * 2 + kv[u]) * kQuantPage + place] = s.scale;
   }
@@ -165,8 +168,7 @@ __global__ __launch_bounds__(kThreads) void quant_read_kernel(ReadArgs a) {
     const int kv = pair & 1, head = pair >> 1;
     const uint8_t* p = (kv ? a.cache[1] : a.cache[0]) + id * a.block_stride +
                        (head * kQuantPage + place) * D + lane * 8;
-    c[u] = __builtin_bit_cast(uint2,
-                              __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p)));
+    c[u] = *reinterpret_cast<const uint2*>(p);
     scale[u] = a.scales[id * a.scales_stride + (head * 2 + kv) * kQuantPage + place];
   }
 #pragma unroll
