@@ -537,6 +537,7 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
   const ScalarInts indptr = scalar_ints(a.indptr);
   const int base = indptr[0], total = indptr[a.batch] - base;
   const int pages = segment_pages(a, total);
+  if (all_short(a.indptr, a.batch, a.hkv)) return;
   int b, first, last;
   if (a.batch < a.segments) {
     b = i;
@@ -550,7 +551,7 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
     b = search.find(a.indptr, a.batch, base, int(cut), first, last);
     if (first >= cut || first < cut - pages) return;
   }
-  if (first < 0 || last <= first || last > total || all_short(a.indptr, a.batch, a.hkv)) return;
+  if (first < 0 || last <= first || last > total) return;
   const int s0 = first / pages, n = (last - 1) / pages - s0 + 1;
   if (n == 1) return;
   const int64_t step = int64_t(a.group) * (D + 4);
