@@ -177,18 +177,25 @@ __device__ __forceinline__ uint32_t word(typename VWord<D>::type v, int i) {
 __host__ __device__ inline int whole_pages(int batch, int hkv) {
   return int64_t(batch) * hkv >= 256 ? 64 : 48;
 }
-__device__ __forceinline__ bool all_short(const int32_t* indptr, int batch, int hkv) {
-  if (batch > kScan) return false;
+// Where the requests are more than the workgroups and shorter still, a wave takes one by itself: no
+// round with idle waves, no join (256 requests of 10 to 180 tokens, 8 KV heads: 20.6 -> 17.5 us, of 16
+// to 300 25.3 -> 23.7; but 64 of these, a workgroup each 11.3, a wave each 14.3, and 128 of up to 600
+// tokens 21.6 and 23.7).
+enum class Share { cut, workgroup, wave };
+constexpr int kWavePages = 20, kWaveRequests = 768;
+__device__ __forceinline__ Share share_of(const int32_t* indptr, int batch, int hkv) {
+  if (batch > kScan) return Share::cut;
   const int most = whole_pages(batch, hkv);
-  bool large = false;
+  int longest = 0;
   for (int i = threadIdx.x & 63; i < batch; i += 256) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int j = min(i + u * 64, batch - 1);
-      large |= indptr[j + 1] - indptr[j] > most;
+      longest = max(longest, indptr[j + 1] - indptr[j]);
     }
   }
-  return !__any(large);
+  if (__any(longest > most)) return Share::cut;
+  return int64_t(batch) * hkv >= kWaveRequests && !__any(longest > kWavePages) ? Share::wave : Share::workgroup;
 }
 
 // Barrier between the waves' uses of LDS.  (__syncthreads would also wait for the global loads.)
@@ -215,7 +222,6 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   using V = typename VWord<D>::type;
   constexpr int kKLoads = D / 64;   // 16-byte pieces of a K row per lane
   constexpr int kDims = D / 16;     // dims of a V row per lane
-  constexpr int kRound = 2 * kWaves;   // pages that the waves take at a time
   extern __shared__ float lds[];    // [kWaves][group][D + 4]: m, l, -, -, O
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int row = lane & 15, g = lane >> 4;
@@ -232,8 +238,10 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   const int base = indptr[0], total = indptr[a.batch] - base;
   const int pages = segment_pages(a, total);
   const int group = a.group;
-  const bool whole_requests = all_short(a.indptr, a.batch, a.hkv);
+  const Share share = share_of(a.indptr, a.batch, a.hkv);
+  const bool whole_requests = share != Share::cut, alone = share == Share::wave;
   if (!whole_requests && segment >= a.segments) return;
+  const int round = alone ? 2 : 2 * kWaves;   // pages that are taken at a time
   const int64_t begin64 = int64_t(segment) * pages;
   int end = a.num_indices == 0 ? 0 : int(min(begin64 + pages, int64_t(total)));
   int begin = int(min(begin64, int64_t(max(end, 0))));
@@ -409,7 +417,8 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     if constexpr (kMore) load_v();
   };
 
-  int first = 0, last = 0, b = segment;
+  int first = 0, last = 0, b = alone ? segment * kWaves + wave : segment;
+  const int stride = alone ? a.groups * kWaves : a.groups;
   if (!whole_requests && begin < end)
     b = search.find(a.indptr, a.batch, base, begin, first, last);
   for (int at = begin;;) {
@@ -418,7 +427,7 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       first = indptr[b] - base;
       last = indptr[b + 1] - base;
       if (last <= first) {
-        b += a.groups;
+        b += stride;
         continue;
       }
       at = begin = first;
@@ -440,7 +449,7 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
 #pragma unroll
     for (int e = 0; e < kDims; ++e) o[e] = f32x4_t{};
 
-    int p = at + 2 * wave;
+    int p = alone ? at : at + 2 * wave;
     if (p < stop) {
       fetch(p);
       const uint16_t* from =
@@ -452,17 +461,17 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
           q[j][h] = *reinterpret_cast<const uint4*>(
               from + (D == 64 ? g * 16 : j / 2 * 128 + g * 32 + j % 2 * 16) + h * 8);
       place(count, p, stop, last, tail);
-      fetch(p + kRound);
+      fetch(p + round);
       load_k();
       load_s(ks, 0);
       load_s(vs, 1);
       load_v();
       // (The last tile is a copy of the loop's body: a branch around the loads would make the
       // compiler wait for all of them.)
-      for (; p + kRound < stop; p += kRound) {
+      for (; p + round < stop; p += round) {
         int n[2];
-        place(n, p + kRound, stop, last, tail);
-        fetch(p + 2 * kRound);
+        place(n, p + round, stop, last, tail);
+        fetch(p + 2 * round);
         tile(std::true_type{});
         count[0] = n[0];
         count[1] = n[1];
@@ -470,8 +479,20 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       tile(std::false_type{});
     }
 
-    // The waves' parts of the piece, joined in LDS.
     l = across(l, [](float s, float t) { return s + t; });
+    if (alone) {
+      if (row < group) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < kDims; e += 4)
+            write_out<D, kHalf>(a, b, head * group + row, (g * 4 + i) * (kDims / 4) + e / 4, m, l,
+                                f32x4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]});
+      }
+      b += stride;
+      continue;
+    }
+    // The waves' parts of the piece, joined in LDS.
     if (row < group) {
       float* to = lds + (wave * group + row) * (D + 4);
       if (g == 0) {
@@ -512,7 +533,7 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     }
     lds_barrier();
     at = stop;
-    if (whole_requests) b += a.groups;
+    if (whole_requests) b += stride;
   }
 
   // Requests without pages: zeros, and -inf.
@@ -537,7 +558,7 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
   const ScalarInts indptr = scalar_ints(a.indptr);
   const int base = indptr[0], total = indptr[a.batch] - base;
   const int pages = segment_pages(a, total);
-  if (all_short(a.indptr, a.batch, a.hkv)) return;
+  if (share_of(a.indptr, a.batch, a.hkv) != Share::cut) return;
   int b, first, last;
   if (a.batch < a.segments) {
     b = i;

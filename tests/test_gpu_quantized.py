@@ -292,6 +292,22 @@ def test_decode(gpu, codec, dtype, d, hkv, group):
     check_decode(*got, q, held, lens, d ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("dtype,hkv,group,d", [(torch.bfloat16, 8, 4, 128), (torch.float16, 4, 3, 64),
+                                               (torch.bfloat16, 4, 2, 256)])
+@pytest.mark.parametrize("longest", [320, 321, 800, 1100])
+def test_decode_of_many_short_requests(gpu, dtype, hkv, group, d, longest):
+    """Requests that a wave or a workgroup takes whole, and just too long for that."""
+    rng = np.random.default_rng(longest)
+    lens = rng.integers(0, 100, 200).tolist()
+    lens[150] = longest
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, longest)
+    ip, idx, lpl = pages(table, lens)
+    q = rows((200, hkv * group, d), 5, dtype, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True)
+    check_decode(*got, q, held, lens, d ** -0.5, dtype)
+
+
 @pytest.mark.parametrize("lens", [[1], [0], [0, 0, 5, 0], [129], [4096], [20000], [16] * 70,
                                   [513] * 9 + [0] * 80 + [31], [2000, 1, 3000, 17]])
 @pytest.mark.parametrize("codec", ref.CODECS)
