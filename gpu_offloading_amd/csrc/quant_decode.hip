@@ -82,7 +82,7 @@ struct QuantDecodeArgs {
 // with 8, 12.2 with 16).
 __device__ __forceinline__ int segment_pages(const QuantDecodeArgs& a, int total) {
   const int least = min(max(total / 40, 2 * kWaves), 4 * kWaves);
-  return max(least, int((int64_t(total) + a.segments - 1) / a.segments));
+  return max(least, int((uint32_t(total) + uint32_t(a.segments) - 1) / uint32_t(a.segments)));
 }
 
 // Index arrays are read through the scalar cache, ahead of use: a vector load of a page id
@@ -556,17 +556,15 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
   __shared__ float lds[256 * 8];
   const int head = blockIdx.x % a.hkv, i = blockIdx.x / a.hkv;
   const ScalarInts indptr = scalar_ints(a.indptr);
+  const bool by_request = a.batch < a.segments;
+  int b = by_request ? i : 0;
   const int base = indptr[0], total = indptr[a.batch] - base;
-  const int pages = segment_pages(a, total);
+  int first = indptr[b] - base, last = indptr[b + 1] - base;
+  Search search;
+  search.start(a.indptr, a.batch);
   if (share_of(a.indptr, a.batch, a.hkv) != Share::cut) return;
-  int b, first, last;
-  if (a.batch < a.segments) {
-    b = i;
-    first = indptr[b] - base;
-    last = indptr[b + 1] - base;
-  } else {
-    Search search;
-    search.start(a.indptr, a.batch);
+  const int pages = segment_pages(a, total);
+  if (!by_request) {
     const int64_t cut = int64_t(i + 1) * pages;
     if (cut >= total) return;
     b = search.find(a.indptr, a.batch, base, int(cut), first, last);
