@@ -76,6 +76,11 @@ struct QuantDecodeArgs {
   float* lse;                // may be null
 };
 
+// Pages of the batch: what indptr spans, as far as there are indices (pages past them hold no tokens).
+__device__ __forceinline__ int pages_in_all(const QuantDecodeArgs& a, int base, int end) {
+  return max(int(min(int64_t(end) - base, a.num_indices - max(base, 0))), 0);
+}
+
 // Pages per segment; the kernels agree on it.  Not below a round of the waves, and in batches of
 // many pages not below two: more pieces cost more to join than the shorter segments save (one
 // request of 2000 tokens, 8 KV heads: 8.4 us with 8 pages, 9.3 with 16; of 20000, one KV head: 13.5
@@ -183,19 +188,21 @@ __host__ __device__ inline int whole_pages(int batch, int hkv) {
 // tokens 21.6 and 23.7).
 enum class Share { cut, workgroup, wave };
 constexpr int kWavePages = 20, kWaveRequests = 768;
-__device__ __forceinline__ Share share_of(const int32_t* indptr, int batch, int hkv) {
-  if (batch > kScan) return Share::cut;
-  const int most = whole_pages(batch, hkv);
+__device__ __forceinline__ Share share_of(const QuantDecodeArgs& a) {
+  if (a.batch > kScan) return Share::cut;
+  const int most = whole_pages(a.batch, a.hkv);
+  const int listed = int(min(a.num_indices, int64_t(INT32_MAX)));
   int longest = 0;
-  for (int i = threadIdx.x & 63; i < batch; i += 256) {
+  for (int i = threadIdx.x & 63; i < a.batch; i += 256) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int j = min(i + u * 64, batch - 1);
-      longest = max(longest, indptr[j + 1] - indptr[j]);
+      const int j = min(i + u * 64, a.batch - 1);
+      longest = max(longest, min(a.indptr[j + 1], listed) - a.indptr[j]);
     }
   }
   if (__any(longest > most)) return Share::cut;
-  return int64_t(batch) * hkv >= kWaveRequests && !__any(longest > kWavePages) ? Share::wave : Share::workgroup;
+  return int64_t(a.batch) * a.hkv >= kWaveRequests && !__any(longest > kWavePages) ? Share::wave
+                                                                                   : Share::workgroup;
 }
 
 // Barrier between the waves' uses of LDS.  (__syncthreads would also wait for the global loads.)
@@ -235,16 +242,16 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   const ScalarInts lengths = scalar_ints(a.last_page_len);
   Search search;
   search.start(a.indptr, a.batch);
-  const int base = indptr[0], total = indptr[a.batch] - base;
+  const int base = indptr[0], total = pages_in_all(a, base, indptr[a.batch]);
   const int pages = segment_pages(a, total);
   const int group = a.group;
-  const Share share = share_of(a.indptr, a.batch, a.hkv);
+  const Share share = share_of(a);
   const bool whole_requests = share != Share::cut, alone = share == Share::wave;
   if (!whole_requests && segment >= a.segments) return;
   const int round = alone ? 2 : 2 * kWaves;   // pages that are taken at a time
   const int64_t begin64 = int64_t(segment) * pages;
-  int end = a.num_indices == 0 ? 0 : int(min(begin64 + pages, int64_t(total)));
-  int begin = int(min(begin64, int64_t(max(end, 0))));
+  int end = int(min(begin64 + pages, int64_t(total)));
+  int begin = int(min(begin64, int64_t(end)));
 
   // The query rows of the head's group, as the B operand.  (Rows past the group are copies
   // of its last: nothing reads what comes of them.)
@@ -269,9 +276,7 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   auto place = [&](int (&n)[2], int page, int stop, int last, int tail) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t slot = int64_t(base) + page + i;
-      const bool held = page + i < stop && slot >= 0 && slot < a.num_indices && raw[i] >= 0 &&
-                        raw[i] < a.num_blocks;
+      const bool held = page + i < stop && raw[i] >= 0 && raw[i] < a.num_blocks;
       id[i] = held ? raw[i] : 0;
       n[i] = !held ? 0 : page + i == last - 1 ? tail : kQuantPage;
     }
@@ -423,15 +428,15 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     b = search.find(a.indptr, a.batch, base, begin, first, last);
   for (int at = begin;;) {
     if (whole_requests) {
-      if (b >= a.batch || a.num_indices == 0) break;
-      first = indptr[b] - base;
+      if (b >= a.batch) break;
+      first = max(indptr[b] - base, 0);
       last = indptr[b + 1] - base;
-      if (last <= first) {
+      at = begin = first;
+      end = min(last, total);
+      if (end <= first) {
         b += stride;
         continue;
       }
-      at = begin = first;
-      end = last;
     } else {
       if (at >= end) break;
       if (last <= at && b < a.batch - 1) {
@@ -507,7 +512,7 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
               f32x4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
     }
     lds_barrier();
-    const bool whole = first >= begin && last <= end;
+    const bool whole = first >= begin && min(last, total) <= end;
     float* part = a.parts + ((int64_t(head) * a.segments + segment) * 2 + (first > begin ? 1 : 0)) *
                                 (int64_t(group) * (D + 4));
     for (int i = threadIdx.x; i < group * (D / 4); i += kWaves * 64) {
@@ -536,9 +541,9 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     if (whole_requests) b += stride;
   }
 
-  // Requests without pages: zeros, and -inf.
+  // Requests without pages, or without any that are listed: zeros, and -inf.
   for (int i = segment; i < a.batch; i += whole_requests ? a.groups : a.segments) {
-    if (indptr[i + 1] > indptr[i] && a.num_indices > 0) continue;
+    if (min(indptr[i + 1] - base, total) > max(indptr[i] - base, 0)) continue;
     for (int j = threadIdx.x; j < group * D; j += kWaves * 64)
       a.out[i * a.out_stride + int64_t(head) * group * D + j] = 0;
     if (a.lse && int(threadIdx.x) < group)
@@ -558,11 +563,11 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
   const ScalarInts indptr = scalar_ints(a.indptr);
   const bool by_request = a.batch < a.segments;
   int b = by_request ? i : 0;
-  const int base = indptr[0], total = indptr[a.batch] - base;
+  const int base = indptr[0], total = pages_in_all(a, base, indptr[a.batch]);
   int first = indptr[b] - base, last = indptr[b + 1] - base;
   Search search;
   search.start(a.indptr, a.batch);
-  if (share_of(a.indptr, a.batch, a.hkv) != Share::cut) return;
+  if (share_of(a) != Share::cut) return;
   const int pages = segment_pages(a, total);
   if (!by_request) {
     const int64_t cut = int64_t(i + 1) * pages;
@@ -570,7 +575,8 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
     b = search.find(a.indptr, a.batch, base, int(cut), first, last);
     if (first >= cut || first < cut - pages) return;
   }
-  if (first < 0 || last <= first || last > total) return;
+  last = min(last, total);
+  if (first < 0 || last <= first) return;
   const int s0 = first / pages, n = (last - 1) / pages - s0 + 1;
   if (n == 1) return;
   const int64_t step = int64_t(a.group) * (D + 4);
@@ -713,8 +719,9 @@ extern "C" int kvc_quantized_decode(
   a.groups = std::max(a.segments, std::min(batch, 256 * per_simd(head_dim) / num_kv_heads));
   const unsigned grid = unsigned(a.groups) * unsigned(num_kv_heads);
   const unsigned lds = unsigned(kWaves * group * (head_dim + 4) * 4);
-  // (So few pages are not cut.)
-  const bool cut = num_indices > whole_pages(batch, num_kv_heads) && a.segments > 1;
+  // (So few pages are not cut, unless their requests are too many to look through.)
+  const bool cut = a.segments > 1 &&
+                   (num_indices > whole_pages(batch, num_kv_heads) || batch > kScan);
 
   auto launch = [&](auto d, auto c, auto half) {
     constexpr int D = decltype(d)::value, C = decltype(c)::value;

@@ -415,6 +415,36 @@ def test_decode_pages_that_are_missing(gpu):
     check_decode(*got, q, kept, [len(t) for t in left], d ** -0.5, torch.bfloat16)
 
 
+@pytest.mark.parametrize("batch,span,have", [(1, 100, 20), (2, 70, 30), (3, 70, 0), (4097, 70, 30),
+                                             (4097, 70, 0), (2, 300, 100)])
+def test_decode_of_requests_past_the_index_list(gpu, batch, span, have):
+    """indptr reaches past the ``have`` indices: what they do not name holds no tokens."""
+    hkv, group, d = 2, 4, 128
+    cache, table, held = random_cache([have * 16 + 16], hkv, d, ref.E4M3, gpu, 4)
+    q = rows((batch, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    ip = np.minimum(np.arange(batch + 1) * span, 4 * span)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(table[0, :have], gpu),
+                                        ints([16] * batch, gpu), return_lse=True)
+    lens = [16 * max(min(span, have - b * span), 0) for b in range(batch)]
+    kept = [[(x[span * 16 * b:][:n], s[span * 16 * b:][:n]) for x, s in held[0]]
+            for b, n in enumerate(lens)]
+    check_decode(*got, q, kept, lens, d ** -0.5, torch.bfloat16)
+
+
+@pytest.mark.parametrize("lens", [[600, 100], [900], [17, 17, 17]])
+def test_decode_of_a_large_batch_with_few_pages(gpu, lens):
+    """More than 4096 requests, almost all of them without tokens."""
+    hkv, group, d, batch = 2, 4, 128, 4500
+    every = np.zeros(batch, np.int64)
+    every[[9, 4200, 4400][:len(lens)]] = lens
+    cache, table, held = random_cache(every.tolist(), hkv, d, ref.INT8, gpu, 4)
+    ip, idx, lpl = pages(table, every.tolist())
+    q = rows((batch, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True)
+    check_decode(*got, q, held, every.tolist(), d ** -0.5, torch.bfloat16)
+
+
 def test_decode_of_rows_that_are_not_finite(gpu):
     """A NaN row of K makes its head's outputs NaN, one of V its values; other heads and
     requests, and tokens past the end, are as before."""
