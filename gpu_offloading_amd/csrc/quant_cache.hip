@@ -268,8 +268,9 @@ extern "C" int kvc_reshape_and_cache_quantized(
   KVC_REQUIRE(aligned(key, 2) && aligned(value, 2), KVC_ERR_ALIGNMENT,
               "key and value must be aligned to their type");
   const int64_t rows = (num_tokens + kQuantPage - 1) / kQuantPage * kQuantPage * 2 * num_kv_heads;
-  KVC_REQUIRE(num_tokens < (int64_t(1) << 31) && rows < (int64_t(1) << 31), KVC_ERR_INVALID_ARG,
-              "too many tokens in one call; split the batch");
+  // (A launch has less than 2^32 threads; a workgroup moves 2048 values.)
+  KVC_REQUIRE(num_tokens < (int64_t(1) << 31) && rows * head_dim <= (int64_t(1) << 35) - 2048,
+              KVC_ERR_INVALID_ARG, "too many tokens in one call; split the batch");
 
   WriteArgs a;
   a.src[0] = static_cast<const uint16_t*>(key);
@@ -355,6 +356,8 @@ extern "C" int kvc_gather_quantized_kv(
   // One page more than max_seq_len fills where a range may begin inside one.
   const unsigned pages = unsigned(cdiv(max_seq_len, kQuantPage)) + (seq_starts ? 1u : 0u);
   const int64_t rows = int64_t(num_kv_heads) * 2 * kQuantPage;
+  KVC_REQUIRE(pages < (1u << 24) && rows * head_dim <= 65535 * 2048, KVC_ERR_INVALID_ARG,
+              "max_seq_len or num_kv_heads too large for one call");
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_types(head_dim, code, dtype, [&](auto d, auto c, auto half) {
     constexpr int D = decltype(d)::value, C = decltype(c)::value;

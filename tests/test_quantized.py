@@ -153,6 +153,15 @@ def test_c_entries_refuse(call, want, kw):
     assert _lib.load().kvc_last_error()
 
 
+@pytest.mark.parametrize("call,kw", [
+    (write, dict(n=1 << 26)), (write, dict(n=1 << 25, d=256, ks=512, vs=512, cs=8192)),
+    (write, dict(n=1 << 27, d=64)), (read, dict(top=(1 << 31) - 1)), (read, dict(top=1 << 28)),
+    (read, dict(h=40000, cs=1 << 30, ss=1 << 30, os=1 << 30))])
+def test_c_entries_refuse_more_threads_than_a_launch_has(call, kw):
+    assert call(**kw) == INVALID
+    assert b"one call" in _lib.load().kvc_last_error()
+
+
 def test_nothing_to_do_is_no_error():
     assert write(n=0, key=None) == 0
     assert read(batch=0, cu=None) == 0 and read(top=0) == 0
