@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteArgs a) {
           uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, most),
                                               __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu)));
     most = row_max<kLanes>(most);   // (all lanes, whatever their slots)
-    const RowScale s = row_scale<kCode>(__float_as_uint(unpack_lo<kHalf>(most)));
+    const RowScale s = row_scale<kCode, kHalf>(__float_as_uint(unpack_lo<kHalf>(most)));
     if (slot[u] < 0) continue;
     if (slot[u] >= a.num_slots) {
       if (a.oob_count && lane == 0 && head[u] == 0 && kv[u] == 0) atomicAdd(a.oob_count, 1);
@@ -113,9 +113,9 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteArgs a) {
     const int place = int(slot[u]) & 15;
     uint2 c;
     c.x = encode4<kCode>(unpack_lo<kHalf>(w[0]), unpack_hi<kHalf>(w[0]), unpack_lo<kHalf>(w[1]),
-                         unpack_hi<kHalf>(w[1]), s.inverse);
+                         unpack_hi<kHalf>(w[1]), s);
     c.y = encode4<kCode>(unpack_lo<kHalf>(w[2]), unpack_hi<kHalf>(w[2]), unpack_lo<kHalf>(w[3]),
-                         unpack_hi<kHalf>(w[3]), s.inverse);
+                         unpack_hi<kHalf>(w[3]), s);
     uint8_t* to = (kv[u] ? a.cache[1] : a.cache[0]) + block * a.block_stride +
                   (head[u] * kQuantPage + place) * D + lane * 8;
     *reinterpret_cast<uint2*>(to) = c;

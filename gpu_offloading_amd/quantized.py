@@ -6,7 +6,8 @@ row of a head, ``[blocks, kv_heads, 2, 16]`` (K's scales, then V's): half a bf16
 bytes.  A code stands for ``code * scale``:
 
   e4m3  scale ``2^e``, the least with ``amax / 2^e <= 448``; relative error up to
-        2^-4 of each value (2^-10 of the scale near zero)
+        2^-4 of each value (2^-10 of the scale near zero); the largest values of the rows'
+        type stay finite
   int8  scale ``amax / 127``; error up to ``amax / 254``
 
 The ops keep the manner of ``ops`` (``RuntimeError`` for bad arguments, the current torch

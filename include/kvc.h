@@ -729,7 +729,8 @@ int kvc_evict_kv(
  * with block strides of their own (codes; floats), everything within a block packed.  A code
  * stands for code * scale:
  *   KVC_CODE_E4M3  scale 2^e, the least with amax / 2^e <= 448; code = x / scale
- *                  rounded to e4m3 (OCP)
+ *                  rounded to e4m3 (OCP), to 240 at most where 256 * scale would be beyond the
+ *                  rows' type
  *   KVC_CODE_INT8  scale amax / 127; code = x * (127 / amax) rounded to a whole number
  * (nearest, ties to even; amax the row's largest |x|, at least 2^-100).  A row with
  * an infinity or a NaN gets the scale NaN: its values read as NaN.
@@ -747,7 +748,8 @@ int kvc_evict_kv(
  * that a captured launch serves other lengths and pages.  indptr[0] may be above 0.
  * Pages whose id is outside [0, num_blocks), or past num_indices, hold no tokens;
  * a request without tokens gets 0 and lse -inf.  The weights enter the product with V as pairs of
- * bf16 (within 2^-15), sums are fp32.  workspace:
+ * bf16 (within 2^-15); sums are fp32, unnormalised: values whose size times the number
+ * of tokens reaches 2^119 may give an infinity.  workspace:
  * kvc_quantized_decode_workspace_bytes of device memory, 16-byte aligned, of one call at a
  * time, not kept between calls.
  * ---------------------------------------------------------------------- */

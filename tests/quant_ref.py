@@ -30,6 +30,7 @@ def values(codes: np.ndarray, codec) -> np.ndarray:
 def encode(x: torch.Tensor, codec):
     """(uint8 codes, fp32 scales) of rows ``[..., D]``; the codes of rows that are not finite
     mean nothing."""
+    most = torch.finfo(x.dtype).max
     x = x.detach().cpu().float().numpy()
     amax = np.abs(x).max(-1)
     bad = ~np.isfinite(x).all(-1)
@@ -51,6 +52,8 @@ def encode(x: torch.Tensor, codec):
         down = np.maximum(up - 1, 0)
         low, high = a - table[down], table[up] - a
         pick = np.where((low < high) | ((low == high) & (down % 2 == 0)), down, up)
+        # a code whose value the rows' type cannot hold is the one below
+        pick = np.where(table[pick] * scale[..., None].astype(np.float64) > most, pick - 1, pick)
         codes = (pick + np.where(np.signbit(y), 128, 0)).astype(np.uint8)
     return codes, np.where(bad, np.float32(np.nan), scale).astype(np.float32)
 

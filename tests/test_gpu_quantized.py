@@ -99,6 +99,37 @@ def test_write_special_rows(gpu, codec):
     assert torch.equal(gv.isnan().any(-1).cpu(), bad.flip(0))
 
 
+@pytest.mark.parametrize("codec", ref.CODECS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_largest_values_stay_finite(gpu, codec, dtype):
+    """Rows with values up to the type's largest, read back and attended to."""
+    h, d, n = 2, 128, 20
+    big = torch.finfo(dtype).max
+    x = rows((n, h, d), 3, torch.float32, 0.0).clamp(-2, 2) / 2
+    x[::2, :, 5], x[1::3, 1, 9] = 1, -1
+    x = (x.double() * big).to(dtype)
+    assert x.isfinite().all() and x.abs().max() == big
+    cache = poisoned(2, h, d, codec, gpu)
+    slots = torch.arange(n, device=gpu)
+    qz.reshape_and_cache_quantized(x.to(gpu), x.to(gpu), *cache[:3], slots)
+    check_written(cache, x, x, slots.tolist(), codec)
+    gk, gv = qz.gather_quantized_kv(*cache[:3], ints([[0, 1]], gpu), ints([0, n], gpu), n,
+                                    dtype=dtype)
+    # Half a step of e4m3 (2^-4; 2^-10 of the scale, at most amax / 224, near zero; 255.9375 as 240 is
+    # within it) or of int8 (three fp32 roundings move a code by 127 * 3 * 2^-24 at most), and half a
+    # step of the rows' type.
+    amax = x.double().abs().amax(-1, keepdim=True)
+    step = x.double().abs() / 16 + amax * 2.0 ** -16 if codec is ref.E4M3 else amax / 254 * 1.0002
+    for got in (gk, gv):
+        err = (got.cpu().double() - x.double()).abs()
+        assert (err <= step + torch.finfo(dtype).eps / 2 * amax).all()
+    if dtype is torch.float16:         # (sums over bf16's largest values are beyond fp32)
+        q = rows((1, h, d), 4, dtype, 0.0).to(gpu) * 1e-4
+        out = qz.quantized_decode_attention(q, *cache[:3], ints([0, 2], gpu), ints([0, 1], gpu),
+                                            ints([n - 16], gpu))
+        assert out.isfinite().all()
+
+
 def test_write_strided_and_unaligned_sources(gpu):
     """Slices of a fused tensor, rows that are not 16-byte aligned, more rows than slots."""
     h, d, n = 4, 64, 37
