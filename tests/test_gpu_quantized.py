@@ -583,6 +583,39 @@ def test_step_captured_and_replayed(gpu):
         assert torch.equal(before, cache.storage)
 
 
+def test_two_graphs_at_a_time(gpu):
+    """Decodes captured before any other call of their kind (16 query heads of 256 per KV head: the most
+    LDS), each with its workspace, replayed beside each other on two streams."""
+    lens, hkv, group, d = [1500, 40, 0, 2600], 2, 16, 256
+    cache, table, _ = random_cache(lens, hkv, d, ref.INT8, gpu, 9)
+    ip, idx, lpl = (ints(x, gpu) for x in pages(table, lens))
+    made = []
+    for i in range(2):
+        q = rows((4, hkv * group, d), 7 + i, torch.float16, 0.3).to(gpu)
+        ws, stream, graph = qz.decode_workspace(4, hkv * group, hkv, d, gpu), torch.cuda.Stream(), \
+            torch.cuda.CUDAGraph()
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            got = qz.quantized_decode_attention(q, *cache[:3], ip, idx, lpl, return_lse=True,
+                                                workspace=ws)
+        made.append((q, ws, stream, graph, got))
+    wants = [qz.quantized_decode_attention(q, *cache[:3], ip, idx, lpl, return_lse=True)
+             for q, *_ in made]
+    for _ in range(3):
+        for *_, got in made:
+            for t in got:
+                t.fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for _, _, stream, graph, _ in made:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for (*_, got), want in zip(made, wants):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_ops_on_a_given_stream(gpu):
     """Each op on a stream that is not the current one, its outputs from that stream."""
     lens, hkv, group, d = [700, 90], 2, 4, 128
