@@ -86,11 +86,12 @@ __device__ __forceinline__ float dot2_bf16(uint32_t a, uint32_t b, float c) {
 }
 
 // ------------------------------------------------------------------- DPP ----
-// DPP control words (CDNA ISA): quad_perm, row rotate right.
+// DPP control words (CDNA ISA): quad_perm, row rotate right, half row mirrored.
 constexpr int kDppQuadSwap1 = 0xB1;  // quad_perm:[1,0,3,2]
 constexpr int kDppQuadSwap2 = 0x4E;  // quad_perm:[2,3,0,1]
 constexpr int kDppRowRor4 = 0x124;   // row_ror:4
 constexpr int kDppRowRor8 = 0x128;   // row_ror:8
+constexpr int kDppRowHalfMirror = 0x141;  // row_half_mirror: the other quad of 8 lanes
 
 template <int Ctrl>
 __device__ __forceinline__ float dpp(float v) {

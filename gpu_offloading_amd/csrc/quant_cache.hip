@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   };
   up(dpp_of(std::integral_constant<int, kDppQuadSwap1>{}));
   up(dpp_of(std::integral_constant<int, kDppQuadSwap2>{}));
-  up(dpp_of(std::integral_constant<int, 0x141>{}));   // row_half_mirror: the other quad of 8 lanes
+  up(dpp_of(std::integral_constant<int, kDppRowHalfMirror>{}));
   if constexpr (kLanes >= 16) up(dpp_of(std::integral_constant<int, kDppRowRor8>{}));
   if constexpr (kLanes >= 32) {
     const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);

@@ -53,6 +53,14 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
+// Division of numbers below 2^31 by one of 1 to 512, rounded down (one more for some above 2^23, which
+// the segments can take).  An ordinary division here, in front of all loads, costs 0.2 us.
+struct Divisor {
+  uint64_t inverse;
+  uint32_t by;
+  explicit Divisor(uint32_t n = 1) : inverse(((uint64_t(1) << 32) + n - 1) / n), by(n) {}
+};
+
 struct QuantDecodeArgs {
   const uint16_t* q;
   int64_t q_stride;          // elements between requests
@@ -69,6 +77,8 @@ struct QuantDecodeArgs {
   int32_t batch, hq, hkv, group;
   int32_t segments;          // per KV head
   int32_t groups;            // workgroups per KV head, at least as many
+  Divisor in_all, in_cus;    // by the segments, by the CUs per KV head
+  int32_t even_from;         // pages per segment from which all segments are used
   float scale_log2;
   float* parts;              // [hkv][segments][2][group][D + 4]: m, l, -, -, O
   uint16_t* out;
@@ -81,13 +91,18 @@ __device__ __forceinline__ int pages_in_all(const QuantDecodeArgs& a, int base, 
   return max(int(min(int64_t(end) - base, a.num_indices - max(base, 0))), 0);
 }
 
-// Pages per segment; the kernels agree on it.  Not below a round of the waves, and in batches of
-// many pages not below two: more pieces cost more to join than the shorter segments save (one
-// request of 2000 tokens, 8 KV heads: 8.4 us with 8 pages, 9.3 with 16; of 20000, one KV head: 13.5
-// with 8, 12.2 with 16).
+// Pages per segment; the kernels agree on it.  Segments of few pages are one per CU, and not below
+// one round of the waves, or two where a request might then be in more than 64 pieces: more
+// pieces cost more to join than shorter segments save, and a number between one and two per CU
+// leaves some CUs twice the others' work (one request of 8192 tokens, 8 KV heads: 9.0 us in 256
+// segments, 9.7 in 512, 10.7 in 344; 16 of 1000 to 5000, 2 KV heads: 14.5, 15.6 and 16.1).
 __device__ __forceinline__ int segment_pages(const QuantDecodeArgs& a, int total) {
-  const int least = min(max(total / 40, 2 * kWaves), 4 * kWaves);
-  return max(least, int((uint32_t(total) + uint32_t(a.segments) - 1) / uint32_t(a.segments)));
+  auto ceil_div = [&](Divisor d) {
+    return int(uint64_t(uint32_t(total) + d.by - 1) * d.inverse >> 32);
+  };
+  const int even = ceil_div(a.in_all);
+  if (even >= a.even_from) return even;
+  return max(ceil_div(a.in_cus), total <= 64 * 2 * kWaves ? 2 * kWaves : 4 * kWaves);
 }
 
 // Index arrays are read through the scalar cache, ahead of use: a vector load of a page id
@@ -551,14 +566,14 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   }
 }
 
-// Joins a request's pieces.  Workgroups (i, KV head), each `rows` query rows: request i, or in
-// batches of more requests than there are borders between segments the request that border i + 1 cuts
-// first.  A thread takes four dims of a row and every share-th piece; the sums of the threads of
-// a column meet in LDS.
-template <int D, bool kHalf>
-__global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int rows) {
-  constexpr int kDeep = 4;
-  __shared__ float lds[256 * 8];
+// Joins a request's pieces.  Workgroups (i, KV head, columns): request i, or in batches of more
+// requests than there are borders between segments the request that border i + 1 cuts first; a
+// column is four dims of a query row.  kShare neighbouring lanes take a column's pieces in turn and
+// join theirs by DPP, without LDS: four registers that meet at each step, and no barrier.  What a
+// launch of this takes (4 us) is its start and three loads that wait for each other.
+template <int D, bool kHalf, int kShare>
+__global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a) {
+  constexpr int kDeep = kShare >= 8 ? 1 : 2;   // pieces that a lane loads at a time
   const int head = blockIdx.x % a.hkv, i = blockIdx.x / a.hkv;
   const ScalarInts indptr = scalar_ints(a.indptr);
   const bool by_request = a.batch < a.segments;
@@ -577,62 +592,57 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a, int
   }
   last = min(last, total);
   if (first < 0 || last <= first) return;
-  const int s0 = first / pages, n = (last - 1) / pages - s0 + 1;
+  const int s0 = uint32_t(first) / uint32_t(pages);
+  const int n = int(uint32_t(last - 1) / uint32_t(pages)) - s0 + 1;
   if (n == 1) return;
   const int64_t step = int64_t(a.group) * (D + 4);
   const int64_t skip = first > int64_t(s0) * pages ? step : 0;   // of the first piece's slot
-  const int r0 = blockIdx.y * rows, columns = min(rows, a.group - r0) * (D / 4);
-  const int share = max(1, 256 / columns);
-  for (int i0 = 0; i0 < columns; i0 += 256) {
-    const int mine = threadIdx.x / columns, column = i0 + threadIdx.x - mine * columns;
-    const bool active = mine < share && column < columns;
-    const int r = r0 + column / (D / 4), c = column % (D / 4);
-    const float* parts = a.parts + (int64_t(head) * a.segments + s0) * 2 * step + r * (D + 4);
-    float top = kLowest, sum = 0.f;
-    f32x4_t acc = {};
-    for (int s = mine; active && s < n; s += share * kDeep) {
-      float2 ml[kDeep];
-      f32x4_t x[kDeep];
+  const int column = blockIdx.y * (256 / kShare) + threadIdx.x / kShare;
+  const int r = min(column / (D / 4), a.group - 1), c = column % (D / 4);
+  const float* parts = a.parts + (int64_t(head) * a.segments + s0) * 2 * step + r * (D + 4);
+  float top = kLowest, sum = 0.f;
+  f32x4_t acc = {};
+  for (int s = threadIdx.x % kShare; s < n; s += kShare * kDeep) {
+    float2 ml[kDeep];
+    f32x4_t x[kDeep];
 #pragma unroll
-      for (int u = 0; u < kDeep; ++u) {
-        const int j = min(s + u * share, n - 1);
-        const float* from = parts + j * 2 * step + (j == 0 ? skip : 0);
-        ml[u] = *reinterpret_cast<const float2*>(from);
-        x[u] = *reinterpret_cast<const f32x4_t*>(from + 4 + c * 4);
-      }
-      float most = top;
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u) most = fmaxf(most, ml[u].x);
-      float f = fast_exp2(top - most);
-      sum *= f;
-      acc *= f;
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u)
-        if (s + u * share < n) {
-          f = fast_exp2(ml[u].x - most);
-          sum += ml[u].y * f;
-          acc += x[u] * f;
-        }
-      top = most;
+    for (int u = 0; u < kDeep; ++u) {
+      const int j = min(s + u * kShare, n - 1);
+      const float* from = parts + j * 2 * step + (j == 0 ? skip : 0);
+      ml[u] = *reinterpret_cast<const float2*>(from);
+      x[u] = *reinterpret_cast<const f32x4_t*>(from + 4 + c * 4);
     }
-    if (share > 1) {   // (then the columns are done at once)
-      float* to = lds + threadIdx.x * 8;
-      to[0] = top;
-      to[1] = sum;
-      *reinterpret_cast<f32x4_t*>(to + 4) = acc;
-      __syncthreads();
-      if (mine != 0) return;
-      for (int w = 1; w < min(share, n); ++w) {
-        const float* from = lds + (w * columns + column) * 8;
-        const float most = fmaxf(top, from[0]);
-        const float f = fast_exp2(top - most), h = fast_exp2(from[0] - most);
-        sum = sum * f + from[1] * h;
-        acc = acc * f + *reinterpret_cast<const f32x4_t*>(from + 4) * h;
-        top = most;
+    float most = top;
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) most = fmaxf(most, ml[u].x);
+    float f = fast_exp2(top - most);
+    sum *= f;
+    acc *= f;
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+      if (s + u * kShare < n) {
+        f = fast_exp2(ml[u].x - most);
+        sum += ml[u].y * f;
+        acc += x[u] * f;
       }
-    }
-    if (active) write_out<D, kHalf>(a, b, head * a.group + r, c, top, sum, acc);
+    top = most;
   }
+  auto join = [](float v, auto f) {
+    if constexpr (kShare >= 2) v = f(v, dpp<kDppQuadSwap1>(v));
+    if constexpr (kShare >= 4) v = f(v, dpp<kDppQuadSwap2>(v));
+    if constexpr (kShare >= 8) v = f(v, dpp<kDppRowHalfMirror>(v));
+    if constexpr (kShare >= 16) v = f(v, dpp<kDppRowRor8>(v));
+    if constexpr (kShare >= 64) v = across(v, f);
+    return v;
+  };
+  const float mine = top;
+  top = join(top, [](float x, float y) { return fmaxf(x, y); });
+  const float f = fast_exp2(mine - top);
+  sum = join(sum * f, [](float x, float y) { return x + y; });
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc[e] = join(acc[e] * f, [](float x, float y) { return x + y; });
+  if (threadIdx.x % kShare == 0 && column < a.group * (D / 4))
+    write_out<D, kHalf>(a, b, head * a.group + r, c, top, sum, acc);
 }
 
 // Segments per KV head.
@@ -710,6 +720,12 @@ extern "C" int kvc_quantized_decode(
   a.hkv = num_kv_heads;
   a.group = group;
   a.segments = segments_of(num_kv_heads, head_dim);
+  a.in_all = Divisor(uint32_t(a.segments));
+  a.in_cus = Divisor(uint32_t(std::max(1, 256 / num_kv_heads)));
+  // One request alone, whose segments are a piece each, is always faster with one per CU if that one
+  // loads enough (8 KV heads of 128: 100000 tokens 37.9 -> 36.6 us, 10^6 307 -> 304; of 64, half the
+  // bytes per token, 23.1 -> 25.5).
+  a.even_from = batch == 1 && head_dim >= 128 ? INT32_MAX : 4 * kWaves;
   a.scale_log2 = sm_scale * kLog2e;
   a.parts = static_cast<float*>(workspace);
   a.out = static_cast<uint16_t*>(out);
@@ -733,9 +749,28 @@ extern "C" int kvc_quantized_decode(
     kernel<<<grid, kWaves * 64, lds, s>>>(a);
     if (cut) {
       const int joins = std::min(batch, a.segments - 1) * num_kv_heads;
-      // Few joins: a query row per workgroup.
-      const int rows = joins * group <= 512 ? 1 : group;
-      quant_merge_kernel<D, H><<<dim3(unsigned(joins), unsigned(group / rows)), 256, 0, s>>>(a, rows);
+      const unsigned columns = unsigned(group * (D / 4));
+      // Lanes per column: as many as make up to 512 workgroups.  (3 requests of 2000 to 12000 tokens, 2 KV
+      // heads of 256: 17.9 us with 4 lanes, 15.7 with 8, 14.6 with 16, 14.2 with 64; 64 of 512 to 4096, 8 of
+      // 128: 57.6 with 2, 58.0 with 4, 59.3 with 8.)
+      auto join = [&](auto lanes) {
+        constexpr int S = decltype(lanes)::value;
+        quant_merge_kernel<D, H, S>
+            <<<dim3(unsigned(joins), (columns * S + 255) / 256), 256, 0, s>>>(a);
+      };
+      const int64_t room = 512 * 256 / (int64_t(joins) * columns);
+      if (room >= 64)
+        join(std::integral_constant<int, 64>{});
+      else if (room >= 16)
+        join(std::integral_constant<int, 16>{});
+      else if (room >= 8)
+        join(std::integral_constant<int, 8>{});
+      else if (room >= 4)
+        join(std::integral_constant<int, 4>{});
+      else if (room >= 2)
+        join(std::integral_constant<int, 2>{});
+      else
+        join(std::integral_constant<int, 1>{});
     }
   };
   auto by_type = [&](auto d, auto c) {

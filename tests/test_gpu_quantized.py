@@ -371,6 +371,34 @@ def test_decode_of_large_batches(gpu, batch, long):
     check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
 
 
+@pytest.mark.parametrize("batch,hkv,group,d", [(3, 2, 4, 128), (6, 8, 4, 128), (12, 8, 4, 128),
+                                               (30, 8, 4, 128), (64, 8, 4, 128), (40, 8, 16, 256)])
+def test_decode_joins(gpu, batch, hkv, group, d):
+    """Few requests to many with cut ones among them: 64 lanes to one per column of the join."""
+    lens = np.random.default_rng(batch).integers(0, 100, batch)
+    lens[1], lens[-1] = 3000, 1100
+    lens = lens.tolist()
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, batch)
+    ip, idx, lpl = pages(table, lens)
+    q = rows((batch, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True)
+    check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
+
+
+@pytest.mark.parametrize("hkv,group,d", [(8, 4, 128), (3, 1, 128), (8, 2, 64), (2, 2, 256), (300, 1, 64)])
+@pytest.mark.parametrize("n", [800, 5000, 18000])
+def test_decode_of_one_long_request(gpu, hkv, group, d, n):
+    """A segment per CU, or two, or (more KV heads than CUs) one for all."""
+    n = n if hkv < 300 else n // 10
+    cache, table, held = random_cache([n], hkv, d, ref.INT8, gpu, n)
+    ip, idx, lpl = pages(table, [n])
+    q = rows((1, hkv * group, d), 5, torch.float16, 0.3).to(gpu)
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), ints(idx, gpu),
+                                        ints(lpl, gpu), return_lse=True)
+    check_decode(*got, q, held, [n], d ** -0.5, torch.float16)
+
+
 def test_decode_of_queries_that_are_not_finite(gpu):
     """A NaN or an infinity in a query head's row stays in that head."""
     lens, hkv, group, d = [40, 2000], 2, 4, 128
