@@ -191,11 +191,12 @@ __device__ __forceinline__ uint32_t word(typename VWord<D>::type v, int i) {
 
 // Whether no request has more pages than one workgroup streams in about the time that cutting
 // and joining it costs: then each is a workgroup's (per KV head) and none is cut.  64 pages where the
-// requests alone fill the GPU (64 requests of 600 to 1000 tokens, 8 KV heads: 26.2 -> 23.2 us),
-// else 48 (8 of 300: 10.2 -> 8.0; but one of 1000: 8.7 cut, 10.1 whole).  Every wave looks through
+// requests alone fill the GPU (64 requests of 600 to 1000 tokens, 8 KV heads: 26.0 cut, 23.5 us whole),
+// 32 where they are few (one of 700: 7.6 and 9.2; 4 of 100 to 700: 10.0 and 10.9; 16 of 200 to 500, whole,
+// 9.7, cut 11.2), else 48 (24 of 100 to 700: 13.8 and 11.5).  Every wave looks through
 // indptr by itself, beside loads that it waits for anyway; batches too large for that are cut.
 __host__ __device__ inline int whole_pages(int batch, int hkv) {
-  return int64_t(batch) * hkv >= 256 ? 64 : 48;
+  return int64_t(batch) * hkv >= 256 ? 64 : batch <= 16 ? 32 : 48;
 }
 // Where the requests are more than the workgroups and shorter still, a wave takes one by itself: no
 // round with idle waves, no join (256 requests of 10 to 180 tokens, 8 KV heads: 20.6 -> 17.5 us, of 16
