@@ -4,9 +4,8 @@
 // with codes kc, vc and their rows' scales ks, vs.
 //
 // What bounds it: every code is read once and used by the `group` query heads of its KV
-// head, 4 * group flop per byte of codes, so HBM.  The products run on MFMA 16x16x32 with
-// the query heads as one side (group <= 16, the rest zero), which leaves the VALU the
-// conversion of the codes.
+// head, 2 * group flop per byte of codes, so HBM.  The products run on MFMA 16x16x32 with
+// the query heads as one side (group <= 16), which leaves the VALU the conversion of the codes.
 //
 // A wave takes 32 tokens (two pages) of one KV head at a time, K and V straight from
 // memory into registers, no LDS:
@@ -19,12 +18,21 @@
 // A row's running maximum is only raised (and O rescaled) where a score exceeds it by 2^8:
 // the maximum needs no cross-lane step per tile.
 //
-// Split: the batch's pages, laid end to end, are cut into equal segments, one per workgroup
-// and KV head; each finds its first request in indptr by itself.  The launch depends on the
-// batch size alone, so a captured one serves other lengths and pages.  The part of a
-// request in one segment is a piece, whose tiles the workgroup's waves take in turn and join in
-// LDS.  A piece that is a whole request is written out; the others leave (m, l, O) in the
-// workspace, which quant_merge_kernel joins, in the order of the pieces.
+// K, V and scales are loaded a tile ahead, each part into the registers that the tile at hand has
+// just freed; page ids and lengths go through the scalar cache.
+//
+// Split, decided on the device from indptr (so a captured launch serves other lengths and pages):
+//   cut        the batch's pages, laid end to end, are cut into equal segments, one per workgroup
+//              and KV head; each finds its first request in indptr by itself.  The part of a request
+//              in a segment is a piece, whose tiles the workgroup's waves take in turn and join in
+//              LDS.  A piece that is a whole request is written out; the others leave (m, l, O) in
+//              the workspace, which quant_merge_kernel joins.
+//   workgroup  each request is a workgroup's (per KV head) where none is long,
+//   wave       or a wave's where they are many and short.
+//
+// 64 requests of 512 to 4096 tokens, 8 KV heads of 128, 4 query heads each: 54.0 us (the kernel 49.7, its
+// join 4.6), 300 MB at 5.5 TB/s; 16 of 32767: 166 us (162), 6.7 TB/s, where the same loads alone take 161.
+// Before the first loads lie 2.4 us: the launch, indptr, a page id.
 #include "quant.h"
 
 #include <algorithm>
@@ -91,18 +99,20 @@ __device__ __forceinline__ int pages_in_all(const QuantDecodeArgs& a, int base, 
   return max(int(min(int64_t(end) - base, a.num_indices - max(base, 0))), 0);
 }
 
-// Pages per segment; the kernels agree on it.  Segments of few pages are one per CU, and not below
-// one round of the waves, or two where a request might then be in more than 64 pieces: more
-// pieces cost more to join than shorter segments save, and a number between one and two per CU
-// leaves some CUs twice the others' work (one request of 8192 tokens, 8 KV heads: 9.0 us in 256
-// segments, 9.7 in 512, 10.7 in 344; 16 of 1000 to 5000, 2 KV heads: 14.5, 15.6 and 16.1).
+// Pages per segment; the kernels agree on it.  Segments of few pages are one per CU, not one and a
+// half, which leaves some CUs twice the others' work (one request of 8192 tokens, 8 KV heads: 9.0 us
+// in 256 segments, 9.7 in 512, 10.7 in 344; 16 of 1000 to 5000, 2 KV heads: 14.5, 15.6 and 16.1).  Nor are
+// they below one round of the waves, or two where requests would on average be in more pieces than the
+// 64 that the join takes at a time (4 of 3000, 2 KV heads: 9.9 us with one round, 10.9 with two; one of
+// 18000, 11.9 and 10.9).
 __device__ __forceinline__ int segment_pages(const QuantDecodeArgs& a, int total) {
   auto ceil_div = [&](Divisor d) {
     return int(uint64_t(uint32_t(total) + d.by - 1) * d.inverse >> 32);
   };
   const int even = ceil_div(a.in_all);
   if (even >= a.even_from) return even;
-  return max(ceil_div(a.in_cus), total <= 64 * 2 * kWaves ? 2 * kWaves : 4 * kWaves);
+  const bool few = int64_t(total) <= int64_t(a.batch) * (64 * 2 * kWaves);
+  return max(ceil_div(a.in_cus), (few ? 2 : 4) * kWaves);
 }
 
 // Index arrays are read through the scalar cache, ahead of use: a vector load of a page id
