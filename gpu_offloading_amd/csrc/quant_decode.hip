@@ -22,11 +22,11 @@
 // just freed; page ids and lengths go through the scalar cache.
 //
 // Split, decided on the device from indptr (so a captured launch serves other lengths and pages):
-//   cut        the batch's pages, laid end to end, are cut into equal segments, one per workgroup
-//              and KV head; each finds its first request in indptr by itself.  The part of a request
-//              in a segment is a piece, whose tiles the workgroup's waves take in turn and join in
-//              LDS.  A piece that is a whole request is written out; the others leave (m, l, O) in
-//              the workspace, which quant_merge_kernel joins.
+//   cut        the batch's requests, laid end to end, are cut into segments of equal work, one per
+//              workgroup and KV head; each finds its first request in indptr by itself.  The part of
+//              a request in a segment is a piece, whose tiles the workgroup's waves take in turn and
+//              join in LDS (a very short request is a wave's).  A piece that is a whole request is
+//              written out; the others leave (m, l, O) in the workspace, which quant_merge_kernel joins.
 //   workgroup  each request is a workgroup's (per KV head) where none is long,
 //   wave       or a wave's where they are many and short.
 //
@@ -86,7 +86,7 @@ struct QuantDecodeArgs {
   int32_t segments;          // per KV head
   int32_t groups;            // workgroups per KV head, at least as many
   Divisor in_all, in_cus;    // by the segments, by the CUs per KV head
-  int32_t even_from;         // pages per segment from which all segments are used
+  int32_t even_from;         // units per segment from which all segments are used
   float scale_log2;
   float* parts;              // [hkv][segments][2][group][D + 4]: m, l, -, -, O
   uint16_t* out;
@@ -99,19 +99,28 @@ __device__ __forceinline__ int pages_in_all(const QuantDecodeArgs& a, int base, 
   return max(int(min(int64_t(end) - base, a.num_indices - max(base, 0))), 0);
 }
 
-// Pages per segment; the kernels agree on it.  Segments of few pages are one per CU, not one and a
-// half, which leaves some CUs twice the others' work (one request of 8192 tokens, 8 KV heads: 9.0 us
+// Segments are equal in units: a page is one, and so are `each` in front of each request's pages, for the
+// piece's start and end (about 3 us, eight pages' time).  Fewer where requests are short or missing, as
+// empty ones count too (a quarter of the pages or so in all), and none where they are so long that it
+// does not matter: then segments may end with requests.  (100 requests of 10 to 1100 tokens 32.0 -> 28.4 us,
+// 64 of 100 to 1200 23.2 -> 22.3, 60 of 1 to 40 and 4 of 8000 24.1 -> 20.2.)
+__device__ __forceinline__ int each_of(int batch, int total) {
+  const int64_t t = total, b = batch;
+  return b == 1 || t >= b * 512 ? 0 : t >= b * 32 ? 8 : t >= b * 16 ? 4 : t >= b * 8 ? 2 : 1;
+}
+
+// Units per segment; the kernels agree on it.  Segments of few are one per CU, not one and a half, which leaves some CUs twice the others' work (one request of 8192 tokens, 8 KV heads: 9.0 us
 // in 256 segments, 9.7 in 512, 10.7 in 344; 16 of 1000 to 5000, 2 KV heads: 14.5, 15.6 and 16.1).  Nor are
 // they below one round of the waves, or two where requests would on average be in more pieces than the
 // 64 that the join takes at a time (4 of 3000, 2 KV heads: 9.9 us with one round, 10.9 with two; one of
 // 18000, 11.9 and 10.9).
-__device__ __forceinline__ int segment_pages(const QuantDecodeArgs& a, int total) {
+__device__ __forceinline__ int segment_units(const QuantDecodeArgs& a, int all) {
   auto ceil_div = [&](Divisor d) {
-    return int(uint64_t(uint32_t(total) + d.by - 1) * d.inverse >> 32);
+    return int(uint64_t(uint32_t(all) + d.by - 1) * d.inverse >> 32);
   };
   const int even = ceil_div(a.in_all);
   if (even >= a.even_from) return even;
-  const bool few = int64_t(total) <= int64_t(a.batch) * (64 * 2 * kWaves);
+  const bool few = int64_t(all) <= int64_t(a.batch) * (64 * 2 * kWaves);
   return max(ceil_div(a.in_cus), (few ? 2 : 4) * kWaves);
 }
 
@@ -145,8 +154,8 @@ __device__ __forceinline__ float across(float v, F f) {
   return f(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
-// First request whose pages reach past a page (pages counted from indptr[0]; the last one if
-// none does), and where it begins and ends.  64 entries of indptr are compared at a time; the
+// First request whose end reaches past a place (in pages from indptr[0], `each` more per request; the
+// last one if none does), and its first page and the one behind its last.  64 entries of indptr are compared at a time; the
 // first 64 are loaded before the page is known, beside what it depends on.
 struct Search {
   int entry, step;
@@ -156,11 +165,12 @@ struct Search {
     step = (batch + 63) / 64;
     entry = indptr[min((lane + 1) * step, batch)];
   }
-  __device__ __forceinline__ int find(const int32_t* indptr, int batch, int base, int page,
+  __device__ __forceinline__ int find(const int32_t* indptr, int batch, int base, int at, int each,
                                       int& first, int& last) const {
     const int lane = threadIdx.x & 63;
-    // blocks of `step` requests before the one looked for end at or below `page`
-    int c = __popcll(__ballot(lane * step < batch && entry - base <= page));
+    // blocks of `step` requests before the one looked for end at or below `at`
+    int c = __popcll(__ballot(lane * step < batch &&
+                              entry - base + each * min((lane + 1) * step, batch) <= at));
     if (step == 1) {
       c = uniform(min(c, batch - 1));
       last = __builtin_amdgcn_readlane(entry, c) - base;
@@ -170,8 +180,9 @@ struct Search {
     int lo = uniform(min(c * step, batch - 1)), n = min(step, batch - lo);
     while (n > 1) {
       const int s = (n + 63) / 64;
-      const int e = indptr[lo + min((lane + 1) * s, n)];
-      c = __popcll(__ballot(lane * s < n && e - base <= page));
+      const int i = lo + min((lane + 1) * s, n);
+      const int e = indptr[i];
+      c = __popcll(__ballot(lane * s < n && e - base + each * i <= at));
       const int skip = min(c * s, n - 1);
       lo = uniform(lo + skip);
       n = s == 1 ? 1 : min(s, n - skip);
@@ -214,6 +225,10 @@ __host__ __device__ inline int whole_pages(int batch, int hkv) {
 // tokens 21.6 and 23.7).
 enum class Share { cut, workgroup, wave };
 constexpr int kWavePages = 20, kWaveRequests = 768;
+// In a segment, whole requests of so few pages are a wave's each, too (300 requests of 1 to 16 tokens and one
+// of 1100 31.1 -> 14.9 us, 1000 of 1 to 40 and 4 of 8000 104 -> 46; up to 8 or 20 pages a wave that has one
+// holds up the others' next piece: 200 of 10 to 1500 63.8, 65.3 and 69.5).
+constexpr int kSoloPages = 4;
 __device__ __forceinline__ Share share_of(const QuantDecodeArgs& a) {
   if (a.batch > kScan) return Share::cut;
   const int most = whole_pages(a.batch, a.hkv);
@@ -269,15 +284,14 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
   Search search;
   search.start(a.indptr, a.batch);
   const int base = indptr[0], total = pages_in_all(a, base, indptr[a.batch]);
-  const int pages = segment_pages(a, total);
+  const int each = each_of(a.batch, total), all = total + each * a.batch;
+  const int units = segment_units(a, all);
   const int group = a.group;
   const Share share = share_of(a);
   const bool whole_requests = share != Share::cut, alone = share == Share::wave;
   if (!whole_requests && segment >= a.segments) return;
-  const int round = alone ? 2 : 2 * kWaves;   // pages that are taken at a time
-  const int64_t begin64 = int64_t(segment) * pages;
-  int end = int(min(begin64 + pages, int64_t(total)));
-  int begin = int(min(begin64, int64_t(end)));
+  const int64_t lo64 = int64_t(segment) * units;
+  const int lo = int(min(lo64, int64_t(all))), hi = int(min(lo64 + units, int64_t(all)));
 
   // The query rows of the head's group, as the B operand.  (Rows past the group are copies
   // of its last: nothing reads what comes of them.)
@@ -450,37 +464,47 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
 
   int first = 0, last = 0, b = alone ? segment * kWaves + wave : segment;
   const int stride = alone ? a.groups * kWaves : a.groups;
-  if (!whole_requests && begin < end)
-    b = search.find(a.indptr, a.batch, base, begin, first, last);
-  for (int at = begin;;) {
+  if (!whole_requests) {
+    if (lo < hi)
+      b = search.find(a.indptr, a.batch, base, lo, each, first, last);
+    else
+      b = a.batch;
+  }
+  auto next = [&] {
     if (whole_requests) {
-      if (b >= a.batch) break;
+      b += stride;
+      return;
+    }
+    first = last;
+    if (++b < a.batch) last = indptr[b + 1] - base;
+    if (last <= first && b < a.batch - 1)   // (requests without pages)
+      b = search.find(a.indptr, a.batch, base, first, 0, first, last);
+  };
+  for (; b < a.batch; next()) {
+    int begin, end;
+    if (whole_requests) {
       first = max(indptr[b] - base, 0);
       last = indptr[b + 1] - base;
-      at = begin = first;
+      begin = first;
       end = min(last, total);
-      if (end <= first) {
-        b += stride;
-        continue;
-      }
     } else {
-      if (at >= end) break;
-      if (last <= at && b < a.batch - 1) {
-        first = last;
-        last = indptr[++b + 1] - base;
-        // (behind requests without pages)
-        if (last <= at) b = search.find(a.indptr, a.batch, base, at, first, last);
-      }
-      if (last <= at) break;   // (an indptr that goes down)
+      begin = lo - each * (b + 1);
+      end = min(hi - each * (b + 1), total);
+      if (first >= end) break;
     }
-    const int stop = min(last, end);
+    const int at = max(max(first, begin), 0), stop = min(last, end);
+    if (at >= stop) continue;
+    const bool whole = first >= begin && min(last, total) <= end;
+    const bool solo = alone || (!whole_requests && whole && stop - at <= kSoloPages);
+    if (solo && !alone && b % kWaves != wave) continue;
+    const int round = solo ? 2 : 2 * kWaves;   // pages that are taken at a time
     const int tail = min(max(lengths[b], 0), kQuantPage);
     m = kLowest;
     l = 0.f;
 #pragma unroll
     for (int e = 0; e < kDims; ++e) o[e] = f32x4_t{};
 
-    int p = alone ? at : at + 2 * wave;
+    int p = solo ? at : at + 2 * wave;
     if (p < stop) {
       fetch(p);
       const uint16_t* from =
@@ -511,7 +535,7 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     }
 
     l = across(l, [](float s, float t) { return s + t; });
-    if (alone) {
+    if (solo) {
       if (row < group) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -520,7 +544,6 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
             write_out<D, kHalf>(a, b, head * group + row, (g * 4 + i) * (kDims / 4) + e / 4, m, l,
                                 f32x4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]});
       }
-      b += stride;
       continue;
     }
     // The waves' parts of the piece, joined in LDS.
@@ -538,7 +561,6 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
               f32x4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
     }
     lds_barrier();
-    const bool whole = first >= begin && min(last, total) <= end;
     float* part = a.parts + ((int64_t(head) * a.segments + segment) * 2 + (first > begin ? 1 : 0)) *
                                 (int64_t(group) * (D + 4));
     for (int i = threadIdx.x; i < group * (D / 4); i += kWaves * 64) {
@@ -563,8 +585,6 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
       }
     }
     lds_barrier();
-    at = stop;
-    if (whole_requests) b += stride;
   }
 
   // Requests without pages, or without any that are listed: zeros, and -inf.
@@ -594,20 +614,22 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(QuantDecodeArgs a) {
   Search search;
   search.start(a.indptr, a.batch);
   if (share_of(a) != Share::cut) return;
-  const int pages = segment_pages(a, total);
+  const int each = each_of(a.batch, total), all = total + each * a.batch;
+  const int units = segment_units(a, all);
+  const int64_t cut = int64_t(i + 1) * units;
   if (!by_request) {
-    const int64_t cut = int64_t(i + 1) * pages;
-    if (cut >= total) return;
-    b = search.find(a.indptr, a.batch, base, int(cut), first, last);
-    if (first >= cut || first < cut - pages) return;
+    if (cut >= all) return;
+    b = search.find(a.indptr, a.batch, base, int(cut), each, first, last);
   }
-  last = min(last, total);
-  if (first < 0 || last <= first) return;
-  const int s0 = uint32_t(first) / uint32_t(pages);
-  const int n = int(uint32_t(last - 1) / uint32_t(pages)) - s0 + 1;
+  if (first < 0) return;
+  last = min(last, total) + each * (b + 1);
+  first += each * (b + 1);
+  if (last <= first || (!by_request && (first >= cut || first < cut - units))) return;
+  const int s0 = uint32_t(first) / uint32_t(units);
+  const int n = int(uint32_t(last - 1) / uint32_t(units)) - s0 + 1;
   if (n == 1) return;
   const int64_t step = int64_t(a.group) * (D + 4);
-  const int64_t skip = first > int64_t(s0) * pages ? step : 0;   // of the first piece's slot
+  const int64_t skip = first > int64_t(s0) * units ? step : 0;   // of the first piece's slot
   const int column = blockIdx.y * (256 / kShare) + threadIdx.x / kShare;
   const int r = min(column / (D / 4), a.group - 1), c = column % (D / 4);
   const float* parts = a.parts + (int64_t(head) * a.segments + s0) * 2 * step + r * (D + 4);
@@ -684,6 +706,7 @@ extern "C" int kvc_quantized_decode(
                   (indices || num_indices == 0),
               KVC_ERR_INVALID_ARG, "null pointer");
   KVC_REQUIRE(batch <= 65535, KVC_ERR_INVALID_ARG, "batch > 65535");
+  KVC_REQUIRE(num_indices <= INT32_MAX - 8 * 65536, KVC_ERR_INVALID_ARG, "too many indices");
   KVC_REQUIRE(code == KVC_CODE_E4M3 || code == KVC_CODE_INT8, KVC_ERR_UNSUPPORTED,
               "code must be KVC_CODE_E4M3 or KVC_CODE_INT8");
   KVC_REQUIRE(dtype == KVC_DTYPE_FP16 || dtype == KVC_DTYPE_BF16, KVC_ERR_UNSUPPORTED,

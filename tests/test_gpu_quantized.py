@@ -386,6 +386,25 @@ def test_decode_joins(gpu, batch, hkv, group, d):
     check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
 
 
+@pytest.mark.parametrize("short,most,long", [(300, 16, [1100]), (60, 40, [3000] * 4), (90, 100, [1500, 0, 5000]),
+                                             (1000, 16, [40000]), (20, 64, [1030] * 20)])
+@pytest.mark.parametrize("hkv,group,d", [(2, 4, 128), (1, 2, 64)])
+def test_decode_of_few_long_requests_among_short_ones(gpu, short, most, long, hkv, group, d):
+    """Very short requests are a wave's; long ones begin in front of, between and behind them."""
+    rng = np.random.default_rng(short)
+    lens = rng.integers(0, most + 1, short).tolist()
+    for i, n in enumerate(long):
+        lens.insert([0, len(lens), len(lens) // 2, 7][i % 4], n)
+    cache, table, held = random_cache(lens, hkv, d, ref.E4M3, gpu, short)
+    ip, idx, lpl = pages(table, lens, first=3)
+    q = rows((len(lens), hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    args = q, *cache[:3], ints(ip, gpu), ints(idx, gpu), ints(lpl, gpu)
+    got = qz.quantized_decode_attention(*args, return_lse=True)
+    check_decode(*got, q, held, lens, d ** -0.5, torch.bfloat16)
+    again = qz.quantized_decode_attention(*args, return_lse=True)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
 @pytest.mark.parametrize("hkv,group,d", [(8, 4, 128), (3, 1, 128), (8, 2, 64), (2, 2, 256), (300, 1, 64)])
 @pytest.mark.parametrize("n", [800, 5000, 18000])
 def test_decode_of_one_long_request(gpu, hkv, group, d, n):

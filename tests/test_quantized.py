@@ -131,7 +131,7 @@ INVALID, UNSUPPORTED, ALIGNMENT, WORKSPACE = 1, 2, 3, 4
     (read, INVALID, dict(batch=65536)), (read, INVALID, dict(width=0)), (read, INVALID, dict(os=255)),
     (read, INVALID, dict(cs=0)), (read, UNSUPPORTED, dict(d=32)), (read, UNSUPPORTED, dict(code=-1)),
     (read, ALIGNMENT, dict(value_cache=A + 8)), (read, ALIGNMENT, dict(ov=A + 1)),
-    (decode, INVALID, dict(batch=-1)), (decode, INVALID, dict(ni=-1)), (decode, INVALID, dict(q=None)),
+    (decode, INVALID, dict(batch=-1)), (decode, INVALID, dict(ni=-1)), (decode, INVALID, dict(ni=(1 << 31) - 1)), (decode, INVALID, dict(q=None)),
     (decode, INVALID, dict(indices=None)), (decode, INVALID, dict(lpl=None)),
     (decode, INVALID, dict(batch=65536)), (decode, INVALID, dict(hq=9)), (decode, INVALID, dict(hkv=0)),
     (decode, INVALID, dict(nb=0)), (decode, INVALID, dict(qs=1023)), (decode, INVALID, dict(os=0)),
