@@ -477,8 +477,10 @@ __global__ __launch_bounds__(kWaves * 64, per_simd(D)) void quant_decode_kernel(
     }
     first = last;
     if (++b < a.batch) last = indptr[b + 1] - base;
-    if (last <= first && b < a.batch - 1)   // (requests without pages)
-      b = search.find(a.indptr, a.batch, base, first, 0, first, last);
+    if (last <= first && b < a.batch - 1) {   // (requests without pages)
+      const int to = search.find(a.indptr, a.batch, base, first, 0, first, last);
+      b = to > b ? to : a.batch;              // (never back, where an indptr goes down)
+    }
   };
   for (; b < a.batch; next()) {
     int begin, end;

@@ -493,6 +493,29 @@ def test_decode_pages_that_are_missing(gpu):
     check_decode(*got, q, kept, [len(t) for t in left], d ** -0.5, torch.bfloat16)
 
 
+@pytest.mark.parametrize("batch", [6, 200])
+def test_decode_ends_whatever_indptr_holds(gpu, batch):
+    """An indptr that goes down or below zero: the call ends, what it gives means nothing, and the next
+    call is right."""
+    hkv, group, d = 2, 4, 128
+    cache, table, held = random_cache([3000] * 2, hkv, d, ref.E4M3, gpu, 4)
+    idx = ints(np.concatenate([table[0, :188], table[1, :188]]), gpu)
+    q = rows((batch, hkv * group, d), 5, torch.bfloat16, 0.3).to(gpu)
+    lpl = ints([16] * batch, gpu)
+    rng = np.random.default_rng(batch)
+    bad = [np.resize([0, 300, 100, 50, 60, 55, 70], batch + 1), np.arange(batch + 1)[::-1] * 2,
+           rng.integers(-400, 400, batch + 1), np.resize([5, 0, 3, -9, 376], batch + 1)]
+    for ip in bad:
+        for n in (376, 40, 0):
+            qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), idx[:n], lpl)
+            torch.cuda.synchronize()
+    ip = np.minimum(np.arange(batch + 1), 2) * 188
+    got = qz.quantized_decode_attention(q, *cache[:3], ints(ip, gpu), idx,
+                                        ints([8, 8] + [0] * (batch - 2), gpu), return_lse=True)
+    lens = [3000] * 2 + [0] * (batch - 2)
+    check_decode(*got, q, held + [held[0]] * (batch - 2), lens, d ** -0.5, torch.bfloat16)
+
+
 @pytest.mark.parametrize("batch,span,have", [(1, 100, 20), (2, 70, 30), (3, 70, 0), (4097, 70, 30),
                                              (4097, 70, 0), (2, 300, 100)])
 def test_decode_of_requests_past_the_index_list(gpu, batch, span, have):
