@@ -543,6 +543,7 @@ class PagedKVCache:
         if (clen < 0).any() or (clen > lens).any():
             raise ValueError("a chunk must be part of its sequence's cached tokens")
         if self.kv_dtype is not None:
+            self._wait_step_users()
             self._plan_quant_chunks(ids, clen, lens)
             return
         nblk = (lens + self.page_size - 1) // self.page_size
@@ -602,7 +603,11 @@ class PagedKVCache:
                 raise RuntimeError("prefill needs plan_prefill first")
             rows, cu, total, longest = self._quant_chunks
             w = self._chunk_wrapper
-            w._run_stream(None)        # (behind the plan's uploads, which the read needs, too)
+            self._step_stream_for_call()
+            sh = w._run_stream(None)   # (behind the plan's uploads, which the read needs, too)
+            if sh != w._plan_stream and not torch.cuda.is_current_stream_capturing():
+                # (also where no step is set up, or the step's stream is this one)
+                self._step_users[sh] = torch.cuda.current_stream(self.device)
             k, v = (torch.empty((total, self.num_kv_heads, self.head_dim), dtype=self.dtype,
                                 device=self.device) for _ in range(2))
             quantized.gather_quantized_kv(self.k_cache[layer], self.v_cache[layer],
@@ -739,15 +744,21 @@ class PagedKVCache:
         step buffer since its last upload, before it is rewritten; return the
         current stream's handle, now the step's stream.  (Stream objects are
         only made on the rare path where another stream was involved.)"""
+        sh = self._wait_step_users()
+        self._step_users = {}
+        self._step_handle = sh
+        self._step_stream_obj = None
+        return sh
+
+    def _wait_step_users(self) -> int:
+        """Order the current stream after the other streams that used the step buffer (or, of a
+        quantised cache, read planned chunks' pages); return its handle."""
         sh = _lib.current_stream_handle(self.device)
         if self._step_users:
             cur = torch.cuda.current_stream(self.device)
             for h, st in self._step_users.items():
                 if h != sh:
                     cur.wait_stream(st)
-            self._step_users = {}
-        self._step_handle = sh
-        self._step_stream_obj = None
         return sh
 
     def _step_stream_for_call(self) -> int:
