@@ -246,7 +246,7 @@ class PagedKVCache:
         self._prompt_wrapper = BatchPromptAttentionWrapper(self._workspace_buf)
         self._weights_wrapper = BatchAttentionWeightsWrapper(self._workspace_buf)
         if self.kv_dtype is not None:
-            self._chunk_wrapper = BatchPromptAttentionWrapper(self._workspace_buf)
+            self._chunk_wrapper: Optional[BatchPromptAttentionWrapper] = None
             self._quant_workspace = quantized.decode_workspace(
                 self.max_seqs, self.num_heads, self.num_kv_heads, self.head_dim, self.device)
 
@@ -565,21 +565,32 @@ class PagedKVCache:
             q_data_type=self.dtype)
 
     def _plan_quant_chunks(self, ids: np.ndarray, clen: np.ndarray, lens: np.ndarray) -> None:
+        w, cu = self._quant_chunk_plan(clen, lens)
+        rows = self.block_table.index_select(0, self._to_device(ids))
+        self._set_quant_chunks(w, cu, rows, self._to_device(cu))
+
+    def _quant_chunk_plan(self, clen: np.ndarray, lens: np.ndarray) -> tuple:
         """Plan chunks of a quantised cache: their sequences' K/V, read back into contiguous
-        rows, are the keys of the prompt attention."""
+        rows, are the keys of the prompt attention.  Returns (wrapper, token index pointers) for
+        ``_set_quant_chunks``; the cache stays as it was, also where this raises."""
         self._check_page_counts((lens + self.page_size - 1) // self.page_size)
         cu, qo = (np.concatenate([[0], np.cumsum(x)]) for x in (lens, clen))
         if cu[-1] > np.iinfo(np.int32).max:
             raise RuntimeError(f"the chunks' sequences hold {int(cu[-1])} tokens, more than one "
                                "plan takes; split the batch")
         cu, qo = cu.astype(np.int32), qo.astype(np.int32)
-        rows = self.block_table.index_select(0, self._to_device(ids))
-        self._chunk_wrapper.plan(torch.from_numpy(qo), torch.from_numpy(cu),
-                                 num_qo_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
-                                 head_dim=self.head_dim, causal=True, q_data_type=self.dtype)
-        cu_d = self._to_device(cu)
-        self._chunk_wrapper._set_staged(*self._chunk_wrapper._staged, rows, cu_d)
-        self._quant_chunks = (rows, cu_d, int(cu[-1]), int(lens.max()) if len(lens) else 0)
+        w = BatchPromptAttentionWrapper(self._workspace_buf)
+        w.plan(torch.from_numpy(qo), torch.from_numpy(cu), num_qo_heads=self.num_heads,
+               num_kv_heads=self.num_kv_heads, head_dim=self.head_dim, causal=True,
+               q_data_type=self.dtype)
+        return w, cu
+
+    def _set_quant_chunks(self, w: BatchPromptAttentionWrapper, cu: np.ndarray,
+                          rows: torch.Tensor, cu_d: torch.Tensor) -> None:
+        """Make a plan, with the sequences' table rows and ``cu`` on the device, the current one."""
+        w._set_staged(*w._staged, rows, cu_d)
+        self._chunk_wrapper = w
+        self._quant_chunks = (rows, cu_d, int(cu[-1]), int(np.diff(cu).max(initial=0)))
 
     def prepare_prefill_chunk(self, seq_ids: Sequence[int], chunk_lens: Sequence[int]) -> torch.Tensor:
         """Setup of a continuation-prefill step (moe_engine.py:1678-1751):
@@ -822,7 +833,9 @@ class PagedKVCache:
                      graph_n: Optional[int] = None) -> torch.Tensor:
         """Setup of a mixed step, the engine's ``step()`` (moe_engine.py:2555-2742,
         piecewise setup :3475-3556, continuation plan :3649-3728), with one
-        host-to-device copy of all its metadata.
+        host-to-device copy of all its metadata (and one of the prompt
+        attention's work list for continuations of a quantised cache).  A step
+        that cannot be planned raises before any length or plan changes.
 
         Tokens are laid out ``[decode | new prefill | continuation]``: one per
         decode request (at its current length), ``prefill_lens[i]`` from
@@ -883,7 +896,8 @@ class PagedKVCache:
         # One pinned int32 image:
         #   ids[R] | qsl[R+1] | lens_before[ms] | lens_after[ms]
         #   | decode kv_indptr[D+1] | decode last_page_len[D]
-        #   | continuation qo_indptr[C+1] | kv_indptr[C+1] | last_page_len[C]
+        #   | continuation qo_indptr[C+1] | kv_indptr[C+1] (quantised: in tokens)
+        #   | last_page_len[C]
         #   | block-table positions (int64) | page ids
         #   | decode schedule | prefill schedule (16-byte aligned each)
         pend = self._peek_bt_pending()
@@ -941,6 +955,11 @@ class PagedKVCache:
                                        True, hs[o_pplan:])
         self._check_page_counts(np.concatenate([(d_after + ps - 1) // ps,
                                                 (c_after + ps - 1) // ps]))
+        if C and quant:
+            chunks, cu = self._quant_chunk_plan(np.asarray(clen, np.int64), c_after)
+            chunk_rows = torch.empty((C, self.max_pages_per_seq), dtype=torch.int32,
+                                     device=self.device)
+            h[o_cip:o_clpl] = cu
 
         # The step's one upload; the plans' unused capacity is not sent.
         self._claim_step_buffer()
@@ -978,7 +997,8 @@ class PagedKVCache:
                         dm[o_dlpl:o_cqo], self._plan_indices_gpu[:total], self.num_heads,
                         self.num_kv_heads, self.head_dim, ps)
         if C and quant:
-            self._plan_quant_chunks(ids[D + P:], np.asarray(clen, np.int64), c_after)
+            torch.index_select(self._bt, 0, ids_d[D + P:], out=chunk_rows)
+            self._set_quant_chunks(chunks, cu, chunk_rows, dm[o_cip:o_clpl])
         elif C:
             total = int(cip[-1])
             ops.copy_page_indices(self._bt, dm[o_cip:o_clpl], self._prefill_indices_gpu,
