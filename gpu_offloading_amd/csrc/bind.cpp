@@ -110,6 +110,17 @@ bool stream_of(PyObject* given, int64_t device, void*& stream) {
   return here && !PyErr_Occurred();
 }
 
+// A C entry's status.  Other Python threads run meanwhile, as during a ctypes call: a launch
+// waits while the stream's queue is full.
+template <typename... P, typename... A>
+int call(int (*entry)(P...), A... args) {
+  struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+  } unlocked;
+  return entry(args...);
+}
+
 // Runs f; what it cannot do, and every exception in it, is None.
 template <typename F>
 PyObject* attempt(F f) {
@@ -141,8 +152,8 @@ PyObject* write(PyObject*, PyObject* const* o, Py_ssize_t n) {
         key->size(0) < slots->numel() || value->size(0) < slots->numel() ||
         !counter(o[6], device, oob) || !stream_of(o[7], device, stream))
       return nullptr;
-    return PyLong_FromLong(write_entry(
-        key->data_ptr(), value->data_ptr(), c.key->data_ptr(), c.value->data_ptr(),
+    return PyLong_FromLong(call(
+        write_entry, key->data_ptr(), value->data_ptr(), c.key->data_ptr(), c.value->data_ptr(),
         static_cast<float*>(c.scales->data_ptr()), static_cast<const int64_t*>(slots->data_ptr()),
         slots->numel(), int32_t(c.heads), int32_t(c.dim), kPage, c.blocks, dtype, c.code, ks, vs,
         c.stride, c.scales_stride, oob, stream));
@@ -171,8 +182,8 @@ PyObject* read(PyObject*, PyObject* const* o, Py_ssize_t n) {
         key->size(0) < 1 || value->size(0) < 1 || ks != vs || !counter(o[9], device, oob) ||
         !stream_of(o[10], device, stream))
       return nullptr;
-    return PyLong_FromLong(read_entry(
-        c.key->data_ptr(), c.value->data_ptr(), static_cast<const float*>(c.scales->data_ptr()),
+    return PyLong_FromLong(call(
+        read_entry, c.key->data_ptr(), c.value->data_ptr(), static_cast<const float*>(c.scales->data_ptr()),
         static_cast<const int32_t*>(table->data_ptr()), table->stride(0), int32_t(table->size(1)),
         static_cast<const int32_t*>(cu->data_ptr()),
         starts ? static_cast<const int32_t*>(starts->data_ptr()) : nullptr, int32_t(batch),
@@ -223,8 +234,8 @@ PyObject* decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
       os = hq * c.dim;
     }
     if (wants && !lse.defined()) lse = at::empty({batch, hq}, q->options().dtype(at::kFloat));
-    const int status = decode_entry(
-        q->data_ptr(), qs, c.key->data_ptr(), c.value->data_ptr(),
+    const int status = call(
+        decode_entry, q->data_ptr(), qs, c.key->data_ptr(), c.value->data_ptr(),
         static_cast<const float*>(c.scales->data_ptr()), c.stride, c.scales_stride, c.blocks,
         static_cast<const int32_t*>(indptr->data_ptr()),
         static_cast<const int32_t*>(indices->data_ptr()), indices->numel(),

@@ -833,3 +833,65 @@ def test_binding_and_python_agree(gpu, monkeypatch):
             qz.gather_quantized_kv(*c, tab, cu, 700, *pair)
     with pytest.raises(RuntimeError):
         qz.gather_quantized_kv(*c, tab, cu, 700, *outs, ints([0, 0], gpu))
+
+
+# ------------------------------------------------------------------ threads
+WAITS_FOR_A_THREAD = r"""
+#include <unistd.h>
+volatile int entered, seen;
+// 0 once another thread has set `seen`, 1 if none does in two seconds
+extern "C" int entry(...) {
+  entered = 1;
+  for (int i = 0; i < 2000; ++i) {
+    if (seen) return 0;
+    usleep(1000);
+  }
+  return 1;
+}
+"""
+
+
+def test_python_threads_run_while_a_launch_waits(gpu, tmp_path):
+    """A C entry that waits (as a launch into a full queue does) holds up no other Python thread.
+    (The binding, over entries that wait until a thread sets a flag.)"""
+    import ctypes
+    import importlib.util
+    import subprocess
+    import threading
+    import time
+
+    from gpu_offloading_amd.build import BIND_PATH
+
+    src, lib = tmp_path / "entry.cpp", str(tmp_path / "entry.so")
+    src.write_text(WAITS_FOR_A_THREAD)
+    subprocess.run(["g++", "-shared", "-fPIC", str(src), "-o", lib], check=True)
+    waits = ctypes.CDLL(lib)
+    entered, seen = (ctypes.c_int.in_dll(waits, name) for name in ("entered", "seen"))
+    # (a module of its own, from a copy: the loaded one stays bound to the library)
+    copy = tmp_path / "kvc_bind.so"
+    copy.write_bytes(open(BIND_PATH, "rb").read())
+    spec = importlib.util.spec_from_file_location("kvc_bind", copy)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    at = ctypes.cast(waits.entry, ctypes.c_void_p).value
+    m.bind(at, at, at, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    c = qz.quantized_cache(4, 2, 64, ref.INT8, gpu)[:3]
+    k = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=gpu)
+    q = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=gpu)
+    ip = ints([0, 1, 2, 3], gpu)
+    calls = {m.write: [k, k, *c, torch.arange(3, device=gpu), None, None],
+             m.read: [*c, ip.view(1, 4), ip[:2], 3, k, k, None, None, None],
+             m.decode: [q, *c, ip, ip, ip[:3], None, None, None, True, ip, None]}
+    for f, args in calls.items():
+        entered.value = seen.value = 0
+
+        def other():
+            while not entered.value:
+                time.sleep(1e-3)
+            seen.value = 1
+
+        t = threading.Thread(target=other)
+        t.start()
+        got = f(*args)
+        t.join()
+        assert got.__class__ is tuple if f is m.decode else got == 0, f.__name__
