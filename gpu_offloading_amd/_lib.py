@@ -309,33 +309,61 @@ def load(path: str | None = None) -> ctypes.CDLL:
         return lib
 
 
+class _NoBinding:
+    """Stands in for the binding: leaves every call to Python."""
+
+    @staticmethod
+    def write(*args):
+        return None
+
+    read = decode = write
+
+
 def binding():
     """The module of csrc/bind.cpp, bound to the loaded library: the quantised ops'
-    short way to their C entries."""
+    short way to their C entries.  Where it is missing, does not load or was built against
+    another torch, a warning says so and the ops call the entries by ctypes."""
     global _bind
     if _bind is None:
-        import importlib.machinery
-        import importlib.util
-
-        import torch
-
-        from .build import BIND_PATH
         lib = load()
-        if not os.path.exists(BIND_PATH):
-            raise RuntimeError(f"{BIND_PATH} is not built. Build it with "
-                               "`python -c 'import __graft_entry__ as g; g.build()'`")
-        loader = importlib.machinery.ExtensionFileLoader("kvc_bind", BIND_PATH)
-        mod = importlib.util.module_from_spec(
-            importlib.util.spec_from_file_location("kvc_bind", BIND_PATH, loader=loader))
-        loader.exec_module(mod)
-        mod.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value
-                   for name in ("kvc_reshape_and_cache_quantized", "kvc_gather_quantized_kv",
-                                "kvc_quantized_decode")),
-                 getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
-                 getattr(torch._C, "_cuda_getCurrentRawStream", None) or
-                 (lambda i: torch.cuda.current_stream(i).cuda_stream))
-        _bind = mod
+        try:
+            _bind = _load_binding(lib)
+        except (OSError, RuntimeError, ImportError) as e:
+            import warnings
+
+            warnings.warn(f"the quantised ops do without their binding: {e}", RuntimeWarning,
+                          stacklevel=3)
+            _bind = _NoBinding()
     return _bind
+
+
+def _load_binding(lib: ctypes.CDLL):
+    import importlib.machinery
+    import importlib.util
+
+    import torch
+
+    from . import build
+    path = build.BIND_PATH
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is not built. Build it with "
+                           "`python -c 'import __graft_entry__ as g; g.build()'`")
+    with open(build.BIND_STAMP_PATH) as f:
+        if f.read().strip() != build.binding_hash():
+            raise RuntimeError(f"{path} was built from other sources or against another torch "
+                               "or Python; rebuild it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
+    loader = importlib.machinery.ExtensionFileLoader("kvc_bind", path)
+    mod = importlib.util.module_from_spec(
+        importlib.util.spec_from_file_location("kvc_bind", path, loader=loader))
+    loader.exec_module(mod)
+    mod.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value
+               for name in ("kvc_reshape_and_cache_quantized", "kvc_gather_quantized_kv",
+                            "kvc_quantized_decode")),
+             getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+             getattr(torch._C, "_cuda_getCurrentRawStream", None) or
+             (lambda i: torch.cuda.current_stream(i).cuda_stream))
+    return mod
 
 
 _bind = None

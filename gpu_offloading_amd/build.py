@@ -1,5 +1,6 @@
 """Build libkvc.so (all HIP sources of csrc/) for gfx950 with hipcc, and the Python
-binding of some of its entries (csrc/bind.cpp) with g++ against torch's headers.
+binding of some of its entries (csrc/bind.cpp) with g++ against torch's headers.  The library
+needs neither torch nor g++; without the binding the ops that use it take a longer way.
 
 Compiled in-tree so that they travel with the repository:
     gpu_offloading_amd/lib/libkvc.so
@@ -46,6 +47,7 @@ STAMP_PATH = LIB_PATH + ".srchash"
 
 BIND_SRC = os.path.join(CSRC, "bind.cpp")
 BIND_PATH = os.path.join(LIB_DIR, "kvc_bind.so")
+BIND_STAMP_PATH = BIND_PATH + ".srchash"
 BIND_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall"]
 
 
@@ -55,7 +57,10 @@ def _bind_command(out: str) -> list[str]:
     import importlib.util
     import sysconfig
 
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch is not installed")
+    torch_dir = os.path.dirname(spec.origin)
     includes = [sysconfig.get_paths()["include"], INCLUDE, os.path.join(torch_dir, "include"),
                 os.path.join(torch_dir, "include", "torch", "csrc", "api", "include")]
     return ["g++", *BIND_FLAGS, *(f"-I{p}" for p in includes), BIND_SRC, "-o", out,
@@ -66,20 +71,32 @@ def sources() -> list[str]:
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
 
 
-def source_hash() -> str:
-    """SHA-256 of everything libkvc.so and its binding are built from (sources,
-    headers, flags): a library whose stamp differs was built from other sources."""
+def _hash(files: list[str], *words: str) -> str:
     import hashlib
 
     h = hashlib.sha256()
-    files = sources() + sorted(glob.glob(os.path.join(CSRC, "*.h"))) + \
-        [os.path.join(INCLUDE, "kvc.h"), BIND_SRC]
     for path in files:
         h.update(os.path.basename(path).encode())
         with open(path, "rb") as f:
             h.update(f.read())
-    h.update(" ".join(HIP_FLAGS + BIND_FLAGS).encode())
+    h.update(" ".join(words).encode())
     return h.hexdigest()
+
+
+def source_hash() -> str:
+    """SHA-256 of everything libkvc.so is built from (sources, headers,
+    flags): a library whose stamp differs was built from other sources."""
+    return _hash(sources() + sorted(glob.glob(os.path.join(CSRC, "*.h"))) +
+                 [os.path.join(INCLUDE, "kvc.h")], *HIP_FLAGS)
+
+
+def binding_hash() -> str:
+    """The binding's own: its source, the C ABI that it calls, and the torch and the Python whose
+    C++ and C interfaces it was built against."""
+    import torch
+
+    return _hash([BIND_SRC, os.path.join(INCLUDE, "kvc.h")], *BIND_FLAGS, torch.__version__,
+                 str(torch.version.git_version), sys.version)
 
 
 def _run(cmd: list[str]) -> tuple[int, list[str]]:
@@ -89,9 +106,35 @@ def _run(cmd: list[str]) -> tuple[int, list[str]]:
                             if noise not in ln]
 
 
+def _build_binding(verbose: bool) -> str | None:
+    """Compile the binding (always recompiles); returns why that failed, or None."""
+    tmp = BIND_PATH + ".tmp"
+    for path in (BIND_PATH, BIND_STAMP_PATH):
+        if os.path.exists(path):
+            os.remove(path)
+    try:
+        cmd = _bind_command(tmp)
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        rc, msgs = _run(cmd)
+        if rc != 0:
+            return "\n".join(msgs)
+        if verbose and msgs:
+            print("\n".join(msgs), file=sys.stderr)
+        stamp = binding_hash()
+    except (OSError, RuntimeError, ImportError) as e:      # no g++, no torch
+        return str(e)
+    os.replace(tmp, BIND_PATH)
+    with open(BIND_STAMP_PATH, "w") as f:
+        f.write(stamp + "\n")
+    return None
+
+
 def build_library(verbose: bool = False, jobs: int | None = None) -> str:
-    """Compile every csrc/*.hip into libkvc.so, and the binding (always
-    recompiles): one process per source file, in parallel, then one link."""
+    """Compile every csrc/*.hip into libkvc.so (always recompiles): one hipcc
+    process per source file, in parallel, then one link.  The binding is compiled behind them;
+    where it cannot be (no torch, no g++), the library is built all the same and stderr
+    says why."""
     from concurrent.futures import ThreadPoolExecutor
 
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -101,9 +144,6 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
     objs = [os.path.join(obj_dir, os.path.basename(s)[:-4] + ".o") for s in srcs]
     cmds = [[hipcc(), *HIP_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o]
             for s, o in zip(srcs, objs)]
-    bind_tmp = BIND_PATH + ".tmp"
-    srcs.append(BIND_SRC)
-    cmds.append(_bind_command(bind_tmp))
     jobs = jobs or min(len(cmds), max(1, min(os.cpu_count() or 1, 16)))
     if verbose:
         for c in cmds:
@@ -112,7 +152,7 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
         results = list(ex.map(_run, cmds))
     failed = [(s, m) for s, (rc, m) in zip(srcs, results) if rc != 0]
     if failed:
-        raise RuntimeError("compilation failed:\n" + "\n".join(
+        raise RuntimeError("hipcc failed:\n" + "\n".join(
             f"{s}:\n" + "\n".join(m) for s, m in failed))
     msgs = [ln for _, m in results for ln in m]
     tmp = LIB_PATH + ".tmp"
@@ -126,9 +166,11 @@ def build_library(verbose: bool = False, jobs: int | None = None) -> str:
     if verbose and msgs:
         print("\n".join(msgs), file=sys.stderr)
     os.replace(tmp, LIB_PATH)
-    os.replace(bind_tmp, BIND_PATH)
     with open(STAMP_PATH, "w") as f:
         f.write(source_hash() + "\n")
+    why = _build_binding(verbose)
+    if why is not None:
+        print(f"{BIND_SRC} is not built, the quantised ops do without it: {why}", file=sys.stderr)
     return LIB_PATH
 
 
