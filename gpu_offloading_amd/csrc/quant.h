@@ -3,8 +3,10 @@
 //   e4m3  scale 2^e, the least with amax / 2^e <= 448; code = x / scale rounded to e4m3
 //         (OCP).  Floating codes gain nothing from a scale between powers of two, and
 //         with a power of two both steps are exact but for the one rounding: a value
-//         read back in bf16 is exact, and quantising it again gives the same code.  Where
-//         256 * scale would be beyond the rows' type, its largest values take the code 240.
+//         read back in bf16 is exact, and quantising the read-back row again keeps its values.
+//         (Not always its codes: a row whose amax is rounded down to 1.75 * 2^k gets half the
+//         scale the next time, and codes of twice the size.)  Where 256 * scale would be
+//         beyond the rows' type, its largest values take the code 240.
 //   int8  scale amax / 127; code = x * (127 / amax) rounded to a whole number.
 // Roundings are to nearest, ties to even.  amax counts as 2^-100 at least, so that scales
 // and their inverses are normal numbers.  A row that holds an infinity or a NaN gets the

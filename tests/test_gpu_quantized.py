@@ -283,6 +283,35 @@ def test_e4m3_values_are_fixed_points(gpu, dtype, d):
     assert torch.equal(gk[slots], rk[slots]) and torch.equal(gv[slots], rv[slots])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_e4m3_rows_written_again_may_change_codes_but_not_values(gpu, dtype, d):
+    """A row whose largest value is rounded down to 1.75 * 2^k is held with half the scale when what
+    was read back is written again: other codes, as the definition has them, and the same values."""
+    tops = torch.tensor([225.0, 231.0, 232.0, 233.0, 1.78125, 0.2197265625, 500.0, 300.0, 224.0])
+    x = torch.rand(len(tops), 1, d, generator=torch.Generator().manual_seed(d)) * 2 - 1
+    x = (x * 0.9 * tops[:, None, None]).to(dtype)
+    x[:, 0, 5] = tops.to(dtype)
+    halved = [True, True, True, False, True, True, False, False, False]   # (232 is a tie: 224 is even)
+    n = len(tops)
+    a, b = (poisoned(1, 1, d, ref.E4M3, gpu) for _ in "ab")
+    table, cu, slots = ints([[0]], gpu), ints([0, n], gpu), torch.arange(n, device=gpu)
+    qz.reshape_and_cache_quantized(x.to(gpu), x.to(gpu), *a[:3], slots)
+    once, _ = qz.gather_quantized_kv(*a[:3], table, cu, n, dtype=dtype)
+    qz.reshape_and_cache_quantized(once, once, *b[:3], slots)
+    twice, _ = qz.gather_quantized_kv(*b[:3], table, cu, n, dtype=dtype)
+    assert torch.equal(once, twice)
+    held = []
+    for c, rows_ in ((a, x), (b, once)):
+        codes, scale = ref.encode(rows_[:, 0], ref.E4M3)
+        assert np.array_equal(bits(c.key_cache)[0, 0, :n], codes)
+        assert np.array_equal(c.scales[0, 0, 0, :n].cpu().numpy(), scale)
+        held.append((codes, scale))
+    (c0, s0), (c1, s1) = held
+    assert (s1 == np.where(halved, s0 / 2, s0)).all()
+    assert [(i != j).any() for i, j in zip(c0, c1)] == halved
+
+
 # ------------------------------------------------------------------ decode
 def pages(table, lens, first=0):
     need = [(n + 15) // 16 for n in lens]
