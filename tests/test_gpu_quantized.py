@@ -924,3 +924,78 @@ def test_python_threads_run_while_a_launch_waits(gpu, tmp_path):
         got = f(*args)
         t.join()
         assert got.__class__ is tuple if f is m.decode else got == 0, f.__name__
+
+
+# --------------------------------------- one captured launch, every way of sharing out requests
+def lengths_of(way, batch, rng):
+    """Lengths for which the kernels take each request with a wave, with a workgroup, or cut."""
+    if way == "wave":
+        return rng.integers(1, 300, batch)
+    if way == "workgroup":
+        return np.r_[rng.integers(330, 500, 1), rng.integers(0, 500, batch - 1)]
+    if way == "cut":
+        n = rng.integers(0, 60, batch)
+        n[::3] = rng.integers(700, 1400, len(n[::3]))
+        n[batch // 2] = 2400
+        return n
+    return np.zeros(batch, np.int64)
+
+
+@pytest.mark.parametrize("dtype,codec,batch,hkv,group,d", [
+    (torch.bfloat16, ref.E4M3, 48, 16, 2, 64), (torch.float16, ref.INT8, 100, 8, 4, 128),
+    (torch.bfloat16, ref.INT8, 3, 2, 3, 256), (torch.float16, ref.E4M3, 1, 8, 4, 128)])
+@pytest.mark.parametrize("first", ["wave", "cut", "none"])
+def test_a_captured_decode_serves_every_length(gpu, dtype, codec, batch, hkv, group, d, first):
+    """One launch, captured over lengths of one kind, replayed over all kinds and back, with eager
+    work between: bit for bit the eager call's result, within the bounds of 64 bits."""
+    pool = 157
+    cache, where, seq = random_cache([pool * 16], hkv, d, codec, gpu, 7)
+    rng = np.random.default_rng(batch)
+    room = batch * 90 + 150
+    ip, lpl, idx = (ints(np.zeros(n), gpu) for n in (batch + 1, batch, room))
+    q = torch.empty(batch, hkv * group, d, dtype=dtype, device=gpu)
+    out = torch.empty_like(q)
+    lse = torch.empty(batch, hkv * group, device=gpu)
+    ws = qz.decode_workspace(batch, hkv * group, hkv, d, gpu)
+
+    def decode():
+        qz.quantized_decode_attention(q, *cache[:3], ip, idx, lpl, out=out, lse=lse, workspace=ws)
+
+    def plan(way, seed):
+        lens = lengths_of(way, batch, rng)
+        need = (lens + 15) // 16
+        places = [rng.integers(0, pool, m) for m in need]      # (pages may be shared)
+        ip.copy_(ints(np.r_[0, np.cumsum(need)], gpu))
+        lpl.copy_(ints((lens - 1) % 16 + (lens > 0), gpu))
+        idx.fill_(1 << 20)
+        if need.sum():
+            idx[:need.sum()] = ints(where[0][np.concatenate(places)], gpu)
+        q.copy_(rows(tuple(q.shape), seed, dtype, 0.3))
+        return lens, places
+
+    def check(lens, places):
+        held = []
+        for n, p in zip(lens, places):
+            t = (p[:, None] * 16 + np.arange(16)).reshape(-1)[:n]
+            held.append([(x[t], s[t]) for x, s in seq[0]])
+        check_decode(out, lse, q, held, lens.tolist(), d ** -0.5, dtype)
+
+    plan(first, 1)
+    decode()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        decode()
+    for i, way in enumerate(["cut", "wave", "cut", "workgroup", "none", "cut", "wave", "wave"]):
+        lens, places = plan(way, 10 + i)
+        out.fill_(math.nan)
+        lse.fill_(math.nan)
+        ws.fill_(0xff)                     # (nothing that an earlier launch left is used)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), lse.clone()
+        out.fill_(math.nan)
+        lse.fill_(math.nan)
+        decode()
+        assert torch.equal(out, got[0]) and torch.equal(lse, got[1]), (i, way)
+        check(lens, places)
