@@ -7,7 +7,8 @@
 // entry.  It returns None for whatever is not an ordinary call (wrong or unusual arguments, a
 // stream of its own, another device than the current one): the op then goes on in Python, which
 // says what is wrong or does the unusual.  Otherwise it returns the entry's status (0 is KVC_OK),
-// or the decode's result.
+// or the decode's result.  The checks here and in quantized.py are two copies of the same ones: a
+// change of either side changes both.
 #include <Python.h>
 
 #include <ATen/ops/empty.h>

@@ -4,18 +4,19 @@
 // is contiguous (2 KB at D = 128), scales fp32 [blocks][heads][2][16], K's and V's of a tile in
 // one 128-byte line: the decode reads both with the tile.
 //
-// Both kernels move bytes (two to three per value) and are bound by them.  The unit is a
+// Both kernels move bytes (three per value, and the scales) and are bound by them.  The unit is a
 // row, one token's D values of one head: D / 8 lanes with 8 values each, 16 bytes of the
 // model's type and 8 of codes, so that both sides are whole lines.  Rows are dealt tile by
 // tile (16 tokens of a head, K and V in turn): 16 neighbouring tokens' codes are one
 // contiguous piece of the cache, and their scales one line that a workgroup completes.
 // Rows of the model's type move with the non-temporal hint (32768 tokens written 40.4 -> 38.8 us,
-// read back 42.4 -> 38.9), codes without: what is written is read next, by the chunk's read-back or the
-// step's attention (16384 tokens written and read back 40.0 -> 35.6 us by stores that stay in the
-// caches, though the write alone takes 42.0 for 38.9 us at 32768), and histories that fit the 256 MB
-// cache in front of the memory are read from there (8 x 4096 tokens 38.6 -> 30.8 us; 41.5 for 40.5
-// where they do not).  A large device copy reaches 5.1 TB/s; these 4.9 and 4.9, from memory, and
-// 4.7 and 6.6 from the cache.
+// read back 42.4 -> 38.9), codes without: a chunk's are read back in the same step, and 16384 tokens
+// written and read back take 35.6 us in place of 40.0 by stores that stay in the caches.  The write
+// alone takes longer by them, 42.0 us for 38.9 at 32768 tokens: a new prompt, whose codes no one reads in
+// its step, pays that.  (A decode step's write is too small to show either; write and attention were not
+// timed together both ways.)  Histories that fit the 256 MB cache in front of the memory are read from
+// there (8 x 4096 tokens 38.6 -> 30.8 us; 41.5 for 40.5 where they do not).  A large device copy reaches
+// 5.1 TB/s; these 4.9 and 4.9, from memory, and 4.7 and 6.6 from the cache.
 #include "quant.h"
 
 #include <algorithm>

@@ -47,9 +47,10 @@ constexpr int kScan = 4096;            // requests that are looked through for l
 
 // Waves per SIMD, which bounds their registers, ...
 constexpr int per_simd(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2; }
-// ... and workgroups per CU that a batch is cut for: these keep 34 KB of loads in flight, and
-// more only compete (16 x 32767 tokens at head_dim 128: 166 us with 2, 169 with 3; 16 of 20000 to
-// 32000 at head_dim 64: 79 with 2, 81 with 4) and leave more to join.
+// ... and workgroups per CU that a batch is cut for: these keep a tile per wave in flight, 34 KB per CU
+// at head_dim 64 and 67 KB at 128 and 256, and more only compete (16 x 32767 tokens at head_dim 128:
+// 166 us with 2, 169 with 3; 16 of 20000 to 32000 at head_dim 64: 79 with 2, 81 with 4) and leave
+// more to join.
 constexpr int cut_for(int head_dim) { return head_dim == 256 ? 1 : 2; }
 
 constexpr float kRaise = 8.f;         // log2: how far a score may exceed the running maximum
@@ -101,9 +102,12 @@ __device__ __forceinline__ int pages_in_all(const QuantDecodeArgs& a, int base, 
 
 // Segments are equal in units: a page is one, and so are `each` in front of each request's pages, for the
 // piece's start and end (about 3 us, eight pages' time).  Fewer where requests are short or missing, as
-// empty ones count too (a quarter of the pages or so in all), and none where they are so long that it
-// does not matter: then segments may end with requests.  (100 requests of 10 to 1100 tokens 32.0 -> 28.4 us,
-// 64 of 100 to 1200 23.2 -> 22.3, 60 of 1 to 40 and 4 of 8000 24.1 -> 20.2.)
+// empty ones count too: an eighth to a quarter of the pages in all for 8 to 64 pages per request, less for
+// longer ones (2% at 512), and more only below 8 (as much as the pages at one per request).  None where
+// they are so long that it does not matter: then segments may end with requests.  (100 requests of 10
+// to 1100 tokens 32.0 -> 28.4 us, 64 of 100 to 1200 23.2 -> 22.3, 60 of 1 to 40 and 4 of 8000 24.1 -> 20.2;
+// in another run at head_dim 64 22.0 -> 19.8, 18.0 -> 16.3, 19.2 -> 14.2, at 256 47.1 -> 44.2, 39.6 -> 36.4,
+// 45.2 -> 28.3.)
 __device__ __forceinline__ int each_of(int batch, int total) {
   const int64_t t = total, b = batch;
   return b == 1 || t >= b * 512 ? 0 : t >= b * 32 ? 8 : t >= b * 16 ? 4 : t >= b * 8 ? 2 : 1;
@@ -216,18 +220,24 @@ __device__ __forceinline__ uint32_t word(typename VWord<D>::type v, int i) {
 // 32 where they are few (one of 700: 7.6 and 9.2; 4 of 100 to 700: 10.0 and 10.9; 16 of 200 to 500, whole,
 // 9.7, cut 11.2), else 48 (24 of 100 to 700: 13.8 and 11.5).  Every wave looks through
 // indptr by itself, beside loads that it waits for anyway; batches too large for that are cut.
+// (These figures are for 8 KV heads of 128.  The limits count pages, whatever a page weighs; cut and
+// whole at 64: 24 of 100 to 700 11.5 and 9.4, 64 of 600 to 1000 17.2 and 14.6, 16 of 200 to 500 9.1 and
+// 8.3; at 256: 16.5 and 14.8, 39.7 and 38.2, 12.3 and 11.8.  Left whole, and
+// without the join's launch, somewhat longer ones would be faster at 64: 4 of 100 to 700 8.8 and 7.6.)
 __host__ __device__ inline int whole_pages(int batch, int hkv) {
   return int64_t(batch) * hkv >= 256 ? 64 : batch <= 16 ? 32 : 48;
 }
 // Where the requests are more than the workgroups and shorter still, a wave takes one by itself: no
 // round with idle waves, no join (256 requests of 10 to 180 tokens, 8 KV heads: 20.6 -> 17.5 us, of 16
 // to 300 25.3 -> 23.7; but 64 of these, a workgroup each 11.3, a wave each 14.3, and 128 of up to 600
-// tokens 21.6 and 23.7).
+// tokens 21.6 and 23.7.  At head_dim 64 the four are 13.7 -> 11.7, 16.1 -> 14.7, 8.1 and 9.3, 13.8 and
+// 18.0; at 256 32.3 -> 25.7, 39.4 -> 36.3, 12.6 and 13.6, 35.4 both).
 enum class Share { cut, workgroup, wave };
 constexpr int kWavePages = 20, kWaveRequests = 768;
 // In a segment, whole requests of so few pages are a wave's each, too (300 requests of 1 to 16 tokens and one
 // of 1100 31.1 -> 14.9 us, 1000 of 1 to 40 and 4 of 8000 104 -> 46; up to 8 or 20 pages a wave that has one
-// holds up the others' next piece: 200 of 10 to 1500 63.8, 65.3 and 69.5).
+// holds up the others' next piece: 200 of 10 to 1500 63.8, 65.3 and 69.5; the first two at head_dim 64
+// 24.9 -> 12.6 and 70.7 -> 33.6, at 256 38.2 -> 17.8 and 180.7 -> 77.7).
 constexpr int kSoloPages = 4;
 __device__ __forceinline__ Share share_of(const QuantDecodeArgs& a) {
   if (a.batch > kScan) return Share::cut;
